@@ -226,6 +226,184 @@ cudaError_t af_mul_f32(float* d_y, const float* d_a, const float* d_b, int n, cu
 cudaError_t af_rope_f32(float* d_q, int n_heads, int head_dim, int pos, float theta,
                         cudaStream_t stream);
 
+/* ------------------------------------- several hypotheses over one cache */
+
+/* A key/value cache in pages, for sequences that share a past: the drafted
+ * trees of speculative decoding, the beams of a search, the requests of a
+ * batch.  (The reference declares a PagedKvCache, include/axonforge/kv_cache.hpp,
+ * whose body is a stub, src/engine.cpp:334-347.)  A pool holds
+ * [n_layers][n_pages][page_size][n_kv_heads][head_dim] values of `type` for K
+ * and as many for V; an engine's own cache is such a pool too (type
+ * AF_KV_F32, pages of consecutive positions, layer_stride = n_ctx rows).
+ * page_size is a power of two, head_dim a multiple of 8 up to 256, k and v are
+ * 16-byte aligned, layer_stride (values from one layer to the next; 0 = the
+ * dense n_pages*page_size*n_kv_heads*head_dim) is a multiple of 8. */
+#define AF_KV_F32 0
+#define AF_KV_F16 1
+#define AF_KV_BF16 2
+typedef struct {
+    void* k;
+    void* v;
+    int64_t layer_stride;
+    int type;
+    int n_layers, n_pages, page_size, n_kv_heads, head_dim;
+} af_kv_cache;
+
+/* The sequences of a call, all pointers to device memory.  Sequence s holds
+ * position p in row p % page_size of page block_table[s*max_blocks +
+ * p/page_size] (-1 where it holds none); block_table NULL: pages
+ * s*max_blocks, s*max_blocks + 1, ... .  len[s] positions are cached; its new
+ * tokens, the nodes, are rows first[s] .. first[s+1]-1 of the call's row
+ * arrays (first NULL: rows s*max_nodes .. (s+1)*max_nodes-1), and node i is
+ * kept at position len[s] + i whatever its depth in a tree.  No sequence has
+ * more than max_nodes nodes.  Lengths, tables and counts are read on the
+ * device, so a captured graph follows them.  A page id or length outside its
+ * range sets the device error word (af_device_error) and is neither read nor
+ * written. */
+typedef struct {
+    const int32_t* block_table;
+    const int32_t* len;
+    const int32_t* first;
+    int n_seq, max_blocks, max_nodes;
+} af_kv_batch;
+
+/* Queries, keys and values of new tokens, on their way into the cache: per
+ * head an optional RMSNorm (qk_norm_order 1 before / 2 after the rotation,
+ * weights q_norm / k_norm [head_dim]), the half-split rotation at position
+ * len[s] + depth[row] (depth NULL: the node's number, a chain) by the tables
+ * cos / sin [n_ctx][head_dim/2], the rotated query to q_out (may be q) and the
+ * rotated key and the value, rounded to the cache's type, to the node's
+ * position of layer `layer`.  q, q_out [n_rows][n_heads][head_dim], k, v
+ * [n_rows][n_kv_heads][head_dim], with the given values from row to row (0 =
+ * dense); rows behind the last sequence stay as they are.  The per-token form
+ * is the first half of af_attention_decode_f32 (llama_model.cpp:1236-1251). */
+typedef struct {
+    af_kv_cache kv;
+    af_kv_batch batch;
+    int layer, n_rows;
+    const float* q;
+    const float* k;
+    const float* v;
+    float* q_out;
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    const int32_t* depth;
+    const float* cos;
+    const float* sin;
+    int n_ctx, n_heads, qk_norm_order;
+    const float* q_norm;
+    const float* k_norm;
+    float eps;
+} af_kv_store_args;
+cudaError_t af_kv_store_f32(const af_kv_store_args* args, cudaStream_t stream);
+
+/* Attention of the nodes of every sequence over its cached positions and, of
+ * the nodes, those that bit j of mask[row*mask_words + j/64] marks for node j
+ * (a node marks itself and its ancestors; any mask is taken).  mask NULL: node
+ * i sees nodes 0..i, a chain — a decode step, a drafted chain, or a chunk of
+ * a prompt.  K and V of the nodes are in the cache already (af_kv_store_f32).
+ * out[row][h] = softmax over what the row sees of q·k·scale, times v; scale 0
+ * = 1/sqrt(head_dim); a row that sees nothing gives zeros; what no row may see
+ * may hold anything, infinities and NaN too.  q, out [n_rows][n_heads]
+ * [head_dim] f32 (strides as above), fp32 accuracy for every cache type.
+ * max_len: no sequence has more positions, cached and new (it sizes the
+ * launch; 0 = max_blocks*page_size).  ws: af_attention_tree_f32_workspace
+ * bytes, zeroed before its first use and left ready for the next; calls that
+ * may overlap on the GPU need workspaces of their own. */
+typedef struct {
+    af_kv_cache kv;
+    af_kv_batch batch;
+    int layer, n_rows, n_heads;
+    const float* q;
+    float* out;
+    int64_t q_stride, out_stride;
+    const uint64_t* mask;
+    int mask_words;
+    float scale;
+    int max_len;
+    void* ws;
+    size_t ws_bytes;
+} af_attention_tree_args;
+size_t af_attention_tree_f32_workspace(const af_attention_tree_args* args);
+cudaError_t af_attention_tree_f32(const af_attention_tree_args* args, cudaStream_t stream);
+
+/* One step of a beam search: of the n_beams beams of each sequence, row
+ * s*n_beams + b of logits [n_seq*n_beams][vocab] (logits_stride values from
+ * row to row, 0 = vocab), the n_out best continuations by
+ * scores[row] + logit - log Σ exp logits, best first, ties to the lowest beam
+ * and then the lowest token.  out_score / out_beam / out_token [n_seq][n_out];
+ * out_beam is the logits row, so that it serves as af_kv_fork's parent.  A
+ * beam whose score is -inf or NaN, or whose logits hold NaN or +inf or nothing
+ * above -inf, scores -inf throughout.  n_out <= 64 and <= n_beams*vocab,
+ * n_beams <= 64.  ws: af_beam_select_f32_workspace bytes, zeroed before its
+ * first use; calls that may overlap need workspaces of their own. */
+typedef struct {
+    const float* logits;
+    int64_t logits_stride;
+    const float* scores;
+    int n_seq, n_beams, vocab, n_out;
+    float* out_score;
+    int32_t* out_beam;
+    int32_t* out_token;
+    void* ws;
+    size_t ws_bytes;
+} af_beam_select_args;
+size_t af_beam_select_f32_workspace(const af_beam_select_args* args);
+cudaError_t af_beam_select_f32(const af_beam_select_args* args, cudaStream_t stream);
+
+/* New sequences from old ones: output sequence i continues input sequence
+ * parent[i] (reordered beams, forks of one prompt, requests that go on) or, with
+ * parent[i] outside 0..n_in-1, starts empty; inputs that no output continues
+ * are freed.  len_out[i] is its parent's length and table_out[i] holds pages for
+ * len_out[i] + n_new[i] positions (n_new NULL: none beyond the length):
+ *  - pages full of cached positions are shared;
+ *  - of the pages behind those, the parent's first child keeps the ones that
+ *    nobody else holds (ref_in 1); every other output takes pages of its own,
+ *    and the rows of a partly filled page are copied, in all layers, K and V;
+ *  - pages taken are those with ref_in 0, lowest id first, in the order of the
+ *    outputs and their positions, so the result is the same on every run.
+ * ref_in / ref_out [n_pages] count the table entries that hold a page (0 =
+ * free); ref_out may be ref_in.  Entries of other tables that share the pool
+ * count too and stay.  table_out and len_out may not overlap the inputs.
+ * Where pages run out, or max_blocks would be passed, entries stay -1,
+ * len_out[i] falls to the last whole page if its partly filled page is
+ * missing, and *n_short (device) is the number of pages missing, else 0.
+ * n_in, n_out <= 4096.  ws: af_kv_fork_workspace bytes, zeroed before its
+ * first use; calls that may overlap need workspaces of their own. */
+typedef struct {
+    af_kv_cache kv;
+    const int32_t* table_in;
+    const int32_t* len_in;
+    const int32_t* ref_in;
+    int32_t* table_out;
+    int32_t* len_out;
+    int32_t* ref_out;
+    const int32_t* parent;
+    const int32_t* n_new;
+    int32_t* n_short;
+    int n_in, n_out, max_blocks;
+    void* ws;
+    size_t ws_bytes;
+} af_kv_fork_args;
+size_t af_kv_fork_workspace(const af_kv_fork_args* args);
+cudaError_t af_kv_fork(const af_kv_fork_args* args, cudaStream_t stream);
+
+/* After a verified tree: the rows of the accepted nodes path[s*max_path + i],
+ * i < n_path[s], move to positions len[s] + i in all layers, K and V, and
+ * len_out[s] = len[s] + n_path[s] (len_out may be len; batch.first and
+ * batch.max_nodes are not read).  A path rises strictly from >= 0; one that
+ * does not, or that leaves the sequence's pages, sets the device error word
+ * and leaves the sequence and its length as they were.  The pages moved in
+ * belong to one sequence alone, as af_kv_fork leaves them. */
+typedef struct {
+    af_kv_cache kv;
+    af_kv_batch batch;
+    const int32_t* path;
+    const int32_t* n_path;
+    int max_path;
+    int32_t* len_out;
+} af_kv_compact_args;
+cudaError_t af_kv_compact(const af_kv_compact_args* args, cudaStream_t stream);
+
 /* --------------------------------------------------------- decode engine */
 
 typedef struct af_engine af_engine;

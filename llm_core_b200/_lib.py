@@ -42,6 +42,60 @@ class GemvFusedArgs(C.Structure):
                 ("epi", C.c_int), ("resid", C.c_void_p), ("argmax", C.c_void_p), ("argmax_base", C.c_int)]
 
 
+class KvCache(C.Structure):
+    """af_kv_cache (include/af_b200.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("layer_stride", C.c_int64), ("type", C.c_int)] + \
+               [(n, C.c_int) for n in ("n_layers", "n_pages", "page_size", "n_kv_heads", "head_dim")]
+
+
+class KvBatch(C.Structure):
+    """af_kv_batch (include/af_b200.h)."""
+    _fields_ = [("block_table", C.c_void_p), ("len", C.c_void_p), ("first", C.c_void_p),
+                ("n_seq", C.c_int), ("max_blocks", C.c_int), ("max_nodes", C.c_int)]
+
+
+class KvStoreArgs(C.Structure):
+    """af_kv_store_args (include/af_b200.h)."""
+    _fields_ = [("kv", KvCache), ("batch", KvBatch), ("layer", C.c_int), ("n_rows", C.c_int), ("q", C.c_void_p),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p), ("q_stride", C.c_int64),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("q_out_stride", C.c_int64),
+                ("depth", C.c_void_p), ("cos", C.c_void_p), ("sin", C.c_void_p), ("n_ctx", C.c_int),
+                ("n_heads", C.c_int), ("qk_norm_order", C.c_int), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p),
+                ("eps", C.c_float)]
+
+
+class AttentionTreeArgs(C.Structure):
+    """af_attention_tree_args (include/af_b200.h)."""
+    _fields_ = [("kv", KvCache), ("batch", KvBatch), ("layer", C.c_int), ("n_rows", C.c_int), ("n_heads", C.c_int),
+                ("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("mask", C.c_void_p), ("mask_words", C.c_int), ("scale", C.c_float), ("max_len", C.c_int),
+                ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
+
+
+class BeamSelectArgs(C.Structure):
+    """af_beam_select_args (include/af_b200.h)."""
+    _fields_ = [("logits", C.c_void_p), ("logits_stride", C.c_int64), ("scores", C.c_void_p)] + \
+               [(n, C.c_int) for n in ("n_seq", "n_beams", "vocab", "n_out")] + \
+               [("out_score", C.c_void_p), ("out_beam", C.c_void_p), ("out_token", C.c_void_p),
+                ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
+
+
+class KvForkArgs(C.Structure):
+    """af_kv_fork_args (include/af_b200.h)."""
+    _fields_ = [("kv", KvCache)] + \
+               [(n, C.c_void_p) for n in ("table_in", "len_in", "ref_in", "table_out", "len_out", "ref_out", "parent",
+                                          "n_new", "n_short")] + \
+               [("n_in", C.c_int), ("n_out", C.c_int), ("max_blocks", C.c_int), ("ws", C.c_void_p),
+                ("ws_bytes", C.c_size_t)]
+
+
+class KvCompactArgs(C.Structure):
+    """af_kv_compact_args (include/af_b200.h)."""
+    _fields_ = [("kv", KvCache), ("batch", KvBatch), ("path", C.c_void_p), ("n_path", C.c_void_p),
+                ("max_path", C.c_int), ("len_out", C.c_void_p)]
+
+
+KV_F32, KV_F16, KV_BF16 = 0, 1, 2
 EPI_STORE, EPI_SWIGLU, EPI_RESID, EPI_ARGMAX = 0, 1, 2, 3
 
 
@@ -101,6 +155,14 @@ def load() -> C.CDLL:
         "af_engine_decode_greedy": (i, [vp, C.c_int32, C.c_int32, i, ip]),
         "af_engine_generate": (i, [vp, ip, i, i, ip, C.POINTER(C.c_int)]),
         "af_sample_f32": (i, [vp, i, vp, i, C.POINTER(Sampling), f, vp, vp]),
+        "af_kv_store_f32": (i, [C.POINTER(KvStoreArgs), vp]),
+        "af_attention_tree_f32_workspace": (sz, [C.POINTER(AttentionTreeArgs)]),
+        "af_attention_tree_f32": (i, [C.POINTER(AttentionTreeArgs), vp]),
+        "af_beam_select_f32_workspace": (sz, [C.POINTER(BeamSelectArgs)]),
+        "af_beam_select_f32": (i, [C.POINTER(BeamSelectArgs), vp]),
+        "af_kv_fork_workspace": (sz, [C.POINTER(KvForkArgs)]),
+        "af_kv_fork": (i, [C.POINTER(KvForkArgs), vp]),
+        "af_kv_compact": (i, [C.POINTER(KvCompactArgs), vp]),
         "af_mt19937_uniform": (i, [C.c_uint32, i, fp]),
         "af_engine_sample": (i, [vp, C.POINTER(Sampling), ip, i, f, ip]),
         "af_engine_generate_sampled": (i, [vp, ip, i, i, C.POINTER(Sampling), fp, i, ip, C.POINTER(C.c_int)]),

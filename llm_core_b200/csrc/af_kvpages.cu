@@ -1,0 +1,534 @@
+// af_kvpages.cu — the paged key/value cache: new tokens written into pages
+// (af_kv_store_f32), sequences forked, reordered, extended and freed
+// (af_kv_fork), accepted rows moved together (af_kv_compact).
+#include <climits>
+#include <cstdint>
+
+#include "af_kvpages.cuh"
+#include "af_ops.cuh"
+
+namespace af {
+
+std::string kv_cache_wrong(const af_kv_cache& c) {
+    if (c.type != AF_KV_F32 && c.type != AF_KV_F16 && c.type != AF_KV_BF16) return "unknown cache type";
+    if (c.n_layers <= 0 || c.n_pages <= 0 || c.n_kv_heads <= 0) return "n_layers, n_pages and n_kv_heads must be positive";
+    if (c.page_size <= 0 || c.page_size > (1 << 20) || (c.page_size & (c.page_size - 1)))
+        return "page_size must be a power of two up to 2^20";
+    if (c.head_dim <= 0 || c.head_dim > 256 || c.head_dim % 8) return "head_dim must be a multiple of 8 up to 256";
+    if (c.n_kv_heads > (1 << 16)) return "n_kv_heads must be at most 65536";
+    const long long dense = (long long)c.n_pages * c.page_size * c.n_kv_heads * c.head_dim;
+    if (c.layer_stride < 0 || c.layer_stride % 8 || (c.layer_stride && c.n_layers > 1 && c.layer_stride < dense))
+        return "layer_stride must be 0 or a multiple of 8 that holds a layer";
+    if (!c.k || !c.v) return "null cache";
+    if ((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & 15) return "k and v must be 16-byte aligned";
+    return "";
+}
+
+std::string kv_batch_wrong(const af_kv_batch& b, const af_kv_cache& c, bool nodes) {
+    if (b.n_seq < 0 || b.n_seq > 65535) return "n_seq must be in 0..65535";
+    if (b.max_blocks <= 0 || (long long)b.max_blocks * c.page_size > (1ll << 30))
+        return "max_blocks must be positive and max_blocks * page_size at most 2^30";
+    if (nodes && b.max_nodes <= 0) return "max_nodes must be positive";
+    if (nodes && !b.first && (long long)b.n_seq * b.max_nodes > INT_MAX) return "too many rows";
+    if (b.n_seq > 0 && !b.len) return "null len";
+    return "";
+}
+
+namespace {
+
+// ------------------------------------------------------------------- store
+
+constexpr int kStoreThreads = 256;
+
+struct StoreParams {
+    KvView kv;
+    KvBatch b;
+    int layer, n_rows, n_ctx, H, order;
+    const float *q, *k, *v;
+    float* q_out;
+    long long qs, ks, vs, os;
+    const int* depth;
+    const float *cos_t, *sin_t, *q_norm, *k_norm;
+    float eps;
+};
+
+// One block per row: its warps take the row's query, key and value heads in
+// turn, a lane the pairs (i, i + hd/2) for i = lane, lane + 32, ...
+template <int TYPE>
+__global__ void __launch_bounds__(kStoreThreads) kv_store_kernel(StoreParams p) {
+    using E = KvElem<TYPE>;
+    __shared__ int s_seq, s_node;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) s_seq = -1;
+    __syncthreads();
+    if (p.b.first) {
+        for (int s = tid; s < p.b.n_seq; s += kStoreThreads) {
+            const int f = p.b.first[s];
+            if (f <= row && row < p.b.first[s + 1]) {
+                s_seq = s;
+                s_node = row - f;
+            }
+        }
+    } else if (tid == 0 && row / p.b.max_nodes < p.b.n_seq) {
+        s_seq = row / p.b.max_nodes;
+        s_node = row % p.b.max_nodes;
+    }
+    __syncthreads();
+    const int seq = s_seq, node = s_node, hd = p.kv.hd, half = hd / 2;
+    if (seq < 0) return;  // a row behind the last sequence
+    const int len = kv_len(p.kv, p.b, seq, 0);
+    if (len < 0) return;
+    const long long at = (long long)len + (p.depth ? p.depth[row] : node);
+    if (at < 0 || at >= p.n_ctx || node >= p.b.max_nodes) {
+        if (tid == 0) set_err(kErrBadArgs);
+        return;
+    }
+    const long long slot = kv_row(p.kv, p.b, seq, len + node);
+    if (slot < 0 && tid == 0) set_err(kErrBadArgs);
+    const float* c = p.cos_t + at * half;
+    const float* sn = p.sin_t + at * half;
+    for (int h = warp; h < p.H + 2 * p.kv.kv_heads; h += kStoreThreads / 32) {
+        const bool isq = h < p.H, isv = h >= p.H + p.kv.kv_heads;
+        const int kvh = isv ? h - p.H - p.kv.kv_heads : h - p.H;
+        const float* src = isq ? p.q + (long long)row * p.qs + (long long)h * hd
+                               : (isv ? p.v + (long long)row * p.vs : p.k + (long long)row * p.ks) + (long long)kvh * hd;
+        float a[4], b[4];
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = lane + 32 * j;
+            a[j] = i < half ? src[i] : 0.f;
+            b[j] = i < half ? src[i + half] : 0.f;
+            ss += a[j] * a[j] + b[j] * b[j];
+        }
+        const float* nw = isv ? nullptr : (isq ? p.q_norm : p.k_norm);
+        if (nw && p.order == 1) {
+            const float sc = 1.f / sqrtf(warp_sum(ss) / (float)hd + p.eps);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = lane + 32 * j;
+                if (i < half) {
+                    a[j] = nw[i] * (a[j] * sc);
+                    b[j] = nw[i + half] * (b[j] * sc);
+                }
+            }
+        }
+        if (!isv) {
+            ss = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = lane + 32 * j;
+                if (i < half) {
+                    const float x = a[j], y = b[j], cc = c[i], s1 = sn[i];
+                    a[j] = x * cc - y * s1;
+                    b[j] = x * s1 + y * cc;
+                    ss += a[j] * a[j] + b[j] * b[j];
+                }
+            }
+        }
+        if (nw && p.order == 2) {
+            const float sc = 1.f / sqrtf(warp_sum(ss) / (float)hd + p.eps);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = lane + 32 * j;
+                if (i < half) {
+                    a[j] = nw[i] * (a[j] * sc);
+                    b[j] = nw[i + half] * (b[j] * sc);
+                }
+            }
+        }
+        if (isq) {
+            float* dst = p.q_out + (long long)row * p.os + (long long)h * hd;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = lane + 32 * j;
+                if (i < half) {
+                    dst[i] = a[j];
+                    dst[i + half] = b[j];
+                }
+            }
+        } else if (slot >= 0) {
+            uint8_t* pool = (isv ? p.kv.v : p.kv.k) + (long long)p.layer * p.kv.layer_bytes + slot;
+            auto* dst = reinterpret_cast<typename E::T*>(pool) + (long long)kvh * hd;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = lane + 32 * j;
+                if (i < half) {
+                    dst[i] = E::round(a[j]);
+                    dst[i + half] = E::round(b[j]);
+                }
+            }
+        }
+    }
+}
+
+// -------------------------------------------------------------------- fork
+
+constexpr int kForkThreads = 1024;
+constexpr int kForkMax = 4096;  // sequences of a call
+
+struct ForkParams {
+    KvView kv;
+    KvBatch in;  // table_in, len_in; n_seq = n_in
+    const int *ref_in, *parent, *n_new;
+    int *table_out, *len_out, *ref_out, *n_short;
+    int n_out;
+    int4* copies;  // [n_out] source page, destination page, rows
+    int* fresh;    // [n_pages] the free pages taken, in order
+};
+
+// What output i needs: its length, and pages behind its `full` whole ones up to `need`.
+struct ForkNeed {
+    int parent, len, full, need, over;
+};
+__device__ __forceinline__ ForkNeed fork_need(const ForkParams& p, int i) {
+    ForkNeed n = {};
+    const int j = p.parent[i];
+    n.parent = j >= 0 && j < p.in.n_seq ? j : -1;
+    n.len = n.parent >= 0 ? kv_len(p.kv, p.in, n.parent, 0) : 0;
+    if (n.len < 0) {
+        n.parent = -1;
+        n.len = 0;
+    }
+    n.full = n.len >> p.kv.ps_shift;
+    const long long want = (long long)n.len + (p.n_new ? max(0, p.n_new[i]) : 0);
+    const long long blocks = (want + (1 << p.kv.ps_shift) - 1) >> p.kv.ps_shift;
+    n.need = (int)min(blocks, (long long)p.in.max_blocks);
+    n.over = (int)min(blocks - n.need, (long long)INT_MAX);
+    return n;
+}
+
+// Whether the first child of `parent` keeps its page of block b.
+__device__ __forceinline__ bool fork_keeps(const ForkParams& p, int parent, int b) {
+    const int page = kv_page(p.in, p.kv.n_pages, parent, b);
+    return page >= 0 && p.ref_in[page] == 1;
+}
+
+// The bookkeeping of a fork, one block: which output is a parent's first
+// child, how many pages each output takes, which pages are free, and then
+// tables, reference counts and the list of pages to copy.
+__global__ void __launch_bounds__(kForkThreads) kv_fork_kernel(ForkParams p) {
+    __shared__ int eldest[kForkMax];
+    __shared__ int base[kForkMax];
+    __shared__ int wsum[32];
+    __shared__ int s_total, s_found;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int j = tid; j < p.in.n_seq; j += kForkThreads) eldest[j] = INT_MAX;
+    __syncthreads();
+    for (int i = tid; i < p.n_out; i += kForkThreads) {
+        const int j = p.parent[i];
+        if (j >= 0 && j < p.in.n_seq) atomicMin(&eldest[j], i);
+    }
+    __syncthreads();
+    // pages that each output takes
+    for (int i = warp; i < p.n_out; i += kForkThreads / 32) {
+        const ForkNeed n = fork_need(p, i);
+        const bool first = n.parent >= 0 && eldest[n.parent] == i;
+        int cnt = 0;
+        for (int b = n.full + lane; b < n.need; b += 32) cnt += !(first && fork_keeps(p, n.parent, b));
+        cnt = __reduce_add_sync(0xffffffffu, cnt);
+        if (lane == 0) base[i] = cnt;
+    }
+    if (tid == 0) s_found = 0;
+    __syncthreads();
+    // exclusive prefix sum of base[]
+    {
+        constexpr int per = kForkMax / kForkThreads;
+        int v[per], sum = 0;
+#pragma unroll
+        for (int e = 0; e < per; ++e) {
+            const int i = tid * per + e;
+            v[e] = i < p.n_out ? base[i] : 0;
+            sum += v[e];
+        }
+        int inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
+        }
+        if (lane == 31) wsum[warp] = inc;
+        __syncthreads();
+        int before = 0;
+        for (int w = 0; w < warp; ++w) before += wsum[w];
+        int at = before + inc - sum;
+#pragma unroll
+        for (int e = 0; e < per; ++e) {
+            const int i = tid * per + e;
+            if (i < p.n_out) base[i] = at;
+            at += v[e];
+        }
+        if (tid == kForkThreads - 1) s_total = at;
+    }
+    __syncthreads();
+    // the lowest s_total pages that nobody holds, in order
+    const int total = s_total;
+    for (int p0 = 0; p0 < p.kv.n_pages; p0 += kForkThreads) {
+        const int found = s_found;
+        if (found >= total) break;
+        const int page = p0 + tid;
+        const bool is = page < p.kv.n_pages && p.ref_in[page] == 0;
+        const unsigned m = __ballot_sync(0xffffffffu, is);
+        if (lane == 0) wsum[warp] = __popc(m);
+        __syncthreads();
+        int before = found, all = 0;
+        for (int w = 0; w < kForkThreads / 32; ++w) {
+            before += w < warp ? wsum[w] : 0;
+            all += wsum[w];
+        }
+        const int rank = before + __popc(m & ((1u << lane) - 1));
+        if (is && rank < total) p.fresh[rank] = page;
+        __syncthreads();
+        if (tid == 0) s_found = found + all;
+        __syncthreads();
+    }
+    const int avail = min(s_found, total);
+    if (p.ref_out != p.ref_in)
+        for (int i = tid; i < p.kv.n_pages; i += kForkThreads) p.ref_out[i] = p.ref_in[i];
+    if (tid == 0) wsum[0] = 0;
+    // Which of its pages a first child keeps depends on ref_in, which may be
+    // ref_out: they are marked in table_out before any count changes.
+    const int nb = p.in.max_blocks;
+    __syncthreads();
+    int missing = 0;
+    for (int i = warp; i < p.n_out; i += kForkThreads / 32) {
+        const ForkNeed n = fork_need(p, i);
+        const bool first = n.parent >= 0 && eldest[n.parent] == i;
+        int taken = base[i], len = n.len;
+        for (int b0 = 0; b0 < nb; b0 += 32) {
+            const int b = b0 + lane;
+            const int old = n.parent >= 0 && b < nb ? kv_page(p.in, p.kv.n_pages, n.parent, b) : -1;
+            const bool shared = b < n.full;
+            const bool keep = !shared && b < n.need && first && fork_keeps(p, n.parent, b);
+            const bool take = !shared && !keep && b < n.need;
+            const unsigned m = __ballot_sync(0xffffffffu, take);
+            int page = shared || keep ? old : -1;
+            if (take) {
+                const int rank = taken + __popc(m & ((1u << lane) - 1));
+                if (rank < avail) page = p.fresh[rank];
+                else ++missing;
+            }
+            taken += __popc(m);
+            if (b < nb) p.table_out[(long long)i * nb + b] = page;
+            // the partly filled page
+            const int rows = n.len & ((1 << p.kv.ps_shift) - 1);
+            if (b == n.full && b < nb) p.copies[i] = make_int4(old, page, take && page >= 0 && old >= 0 ? rows : 0, 0);
+            const bool lost = b == n.full && rows > 0 && page < 0;
+            if (__any_sync(0xffffffffu, lost)) len = n.full << p.kv.ps_shift;
+        }
+        if (n.full >= nb && lane == 0) p.copies[i] = make_int4(-1, -1, 0, 0);
+        if (lane == 0) {
+            p.len_out[i] = len;
+            missing += n.over;
+        }
+    }
+    missing = __reduce_add_sync(0xffffffffu, missing);
+    if (lane == 0 && missing) atomicAdd(&wsum[0], missing);
+    __syncthreads();
+    if (tid == 0) *p.n_short = wsum[0];
+    // counts: one off for every entry of the inputs, one on for every entry of the outputs
+    for (long long e = tid; e < (long long)p.in.n_seq * nb; e += kForkThreads) {
+        const int page = kv_page(p.in, p.kv.n_pages, (int)(e / nb), (int)(e % nb));
+        if (page >= 0) atomicSub(&p.ref_out[page], 1);
+    }
+    for (long long e = tid; e < (long long)p.n_out * nb; e += kForkThreads) {
+        const int page = p.table_out[e];
+        if (page >= 0) atomicAdd(&p.ref_out[page], 1);
+    }
+}
+
+constexpr int kCopyThreads = 256;
+
+// Block (i, layer, K or V): the rows of output i's partly filled page.
+__global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(KvView kv, const int4* copies) {
+    const int4 c = copies[blockIdx.x];
+    if (c.z <= 0) return;
+    uint8_t* pool = (blockIdx.z ? kv.v : kv.k) + (long long)blockIdx.y * kv.layer_bytes;
+    const uint4* src = reinterpret_cast<const uint4*>(pool + ((long long)c.x << kv.ps_shift) * kv.row_bytes);
+    uint4* dst = reinterpret_cast<uint4*>(pool + ((long long)c.y << kv.ps_shift) * kv.row_bytes);
+    const long long n = (long long)c.z * kv.row_bytes / 16;
+    for (long long i = threadIdx.x; i < n; i += kCopyThreads) dst[i] = src[i];
+}
+
+// ----------------------------------------------------------------- compact
+
+constexpr int kCompactThreads = 128;
+
+// Block (columns, layer and K or V, sequence): a thread moves 16 bytes of
+// every row of the path, in path order.  A row's source is never in front of
+// its destination and destinations rise, so a row is read before it is
+// written over: dst i = len + i <= len + path[i'] for every i' >= i.
+__global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(KvView kv, KvBatch b, const int* path,
+                                                                     const int* n_path, int max_path, int* len_out,
+                                                                     const int* len_in) {
+    const int s = blockIdx.z, layer = blockIdx.y >> 1, tid = threadIdx.x;
+    const int col = blockIdx.x * kCompactThreads + tid;
+    const int n = n_path[s];
+    const int* pa = path + (long long)s * max_path;
+    const int len = len_in[s];
+    bool bad = len < 0 || n < 0 || n > max_path;
+    for (int i = 0; i < n && !bad; ++i) {
+        const int x = pa[i];
+        bad = x < 0 || (i && x <= pa[i - 1]) || (long long)len + x >= ((long long)b.max_blocks << kv.ps_shift) ||
+              kv_row(kv, b, s, len + x) < 0 || kv_row(kv, b, s, len + i) < 0;
+    }
+    if (bad) {
+        if (tid == 0) set_err(kErrBadArgs);
+        return;
+    }
+    if (col * 16 >= kv.row_bytes) return;
+    uint8_t* pool = ((blockIdx.y & 1) ? kv.v : kv.k) + (long long)layer * kv.layer_bytes + (long long)col * 16;
+    for (int i = 0; i < n; ++i) {
+        if (pa[i] == i) continue;
+        const uint4 x = *reinterpret_cast<const uint4*>(pool + kv_row(kv, b, s, len + pa[i]));
+        *reinterpret_cast<uint4*>(pool + kv_row(kv, b, s, len + i)) = x;
+    }
+}
+
+// The new lengths, after the rows: len_out may be len, which the rows' blocks read.
+__global__ void kv_compact_len_kernel(KvView kv, KvBatch b, const int* path, const int* n_path, int max_path,
+                                      int* len_out) {
+    const int s = blockIdx.x * blockDim.x + threadIdx.x;
+    if (s >= b.n_seq) return;
+    const int n = n_path[s], len = b.len[s];
+    const int* pa = path + (long long)s * max_path;
+    bool bad = len < 0 || n < 0 || n > max_path;
+    for (int i = 0; i < n && !bad; ++i) {
+        const int x = pa[i];
+        bad = x < 0 || (i && x <= pa[i - 1]) || (long long)len + x >= ((long long)b.max_blocks << kv.ps_shift) ||
+              kv_row(kv, b, s, len + x) < 0 || kv_row(kv, b, s, len + i) < 0;
+    }
+    len_out[s] = bad ? len : len + n;
+}
+
+cudaError_t refuse(const char* what, const std::string& why) {
+    set_last_error(std::string(what) + ": " + why);
+    return cudaErrorInvalidValue;
+}
+
+size_t fork_ws(const af_kv_fork_args& a) {
+    return (size_t)a.n_out * sizeof(int4) + (size_t)a.kv.n_pages * sizeof(int);
+}
+
+std::string fork_wrong(const af_kv_fork_args& a) {
+    const std::string why = kv_cache_wrong(a.kv);
+    if (!why.empty()) return why;
+    if (a.n_in < 0 || a.n_in > kForkMax || a.n_out < 0 || a.n_out > kForkMax) return "n_in and n_out must be in 0..4096";
+    if (a.max_blocks <= 0 || (long long)a.max_blocks * a.kv.page_size > (1ll << 30))
+        return "max_blocks must be positive and max_blocks * page_size at most 2^30";
+    if (!a.ref_in || !a.ref_out || !a.n_short) return "null ref_in, ref_out or n_short";
+    if (a.n_in > 0 && (!a.table_in || !a.len_in)) return "null table_in or len_in";
+    if (a.n_out > 0 && (!a.table_out || !a.len_out || !a.parent)) return "null table_out, len_out or parent";
+    auto over = [](const void* x, size_t nx, const void* y, size_t ny) {
+        const uintptr_t p = reinterpret_cast<uintptr_t>(x), q = reinterpret_cast<uintptr_t>(y);
+        return nx && ny && p < q + ny && q < p + nx;
+    };
+    const size_t ti = (size_t)a.n_in * a.max_blocks * 4, to = (size_t)a.n_out * a.max_blocks * 4;
+    if (over(a.table_in, ti, a.table_out, to) || over(a.len_in, (size_t)a.n_in * 4, a.len_out, (size_t)a.n_out * 4))
+        return "table_out and len_out may not overlap the inputs";
+    if (a.ref_in != a.ref_out && over(a.ref_in, (size_t)a.kv.n_pages * 4, a.ref_out, (size_t)a.kv.n_pages * 4))
+        return "ref_out must be ref_in or apart from it";
+    return "";
+}
+
+}  // namespace
+}  // namespace af
+
+using namespace af;
+
+extern "C" cudaError_t af_kv_store_f32(const af_kv_store_args* a, cudaStream_t stream) {
+    const char* me = "af_kv_store_f32";
+    if (!a) return refuse(me, "null arguments");
+    std::string why = kv_cache_wrong(a->kv);
+    if (why.empty()) why = kv_batch_wrong(a->batch, a->kv, true);
+    if (!why.empty()) return refuse(me, why);
+    if (a->layer < 0 || a->layer >= a->kv.n_layers) return refuse(me, "layer outside the cache");
+    if (a->n_rows < 0 || a->n_heads <= 0 || a->n_ctx <= 0) return refuse(me, "need n_rows >= 0, n_heads > 0, n_ctx > 0");
+    if (a->qk_norm_order < 0 || a->qk_norm_order > 2) return refuse(me, "qk_norm_order must be 0, 1 or 2");
+    if (a->n_rows == 0 || a->batch.n_seq == 0) return cudaSuccess;
+    if (!a->q || !a->k || !a->v || !a->q_out || !a->cos || !a->sin) return refuse(me, "null q, k, v, q_out, cos or sin");
+    const long long qd = (long long)a->n_heads * a->kv.head_dim, kd = (long long)a->kv.n_kv_heads * a->kv.head_dim;
+    if ((a->q_stride && a->q_stride < qd) || (a->q_out_stride && a->q_out_stride < qd) ||
+        (a->k_stride && a->k_stride < kd) || (a->v_stride && a->v_stride < kd))
+        return refuse(me, "a row stride is shorter than a row");
+    StoreParams p = {};
+    p.kv = kv_view(a->kv);
+    p.b = kv_batch(a->batch);
+    p.layer = a->layer;
+    p.n_rows = a->n_rows;
+    p.n_ctx = a->n_ctx;
+    p.H = a->n_heads;
+    p.order = a->qk_norm_order;
+    p.q = a->q;
+    p.k = a->k;
+    p.v = a->v;
+    p.q_out = a->q_out;
+    p.qs = a->q_stride ? a->q_stride : qd;
+    p.os = a->q_out_stride ? a->q_out_stride : qd;
+    p.ks = a->k_stride ? a->k_stride : kd;
+    p.vs = a->v_stride ? a->v_stride : kd;
+    p.depth = a->depth;
+    p.cos_t = a->cos;
+    p.sin_t = a->sin;
+    p.q_norm = a->q_norm;
+    p.k_norm = a->k_norm;
+    p.eps = a->eps;
+    if (a->q_out == a->q && p.os != p.qs) return refuse(me, "q_out in place needs q's stride");
+    switch (a->kv.type) {
+        case AF_KV_F32: kv_store_kernel<AF_KV_F32><<<a->n_rows, kStoreThreads, 0, stream>>>(p); break;
+        case AF_KV_F16: kv_store_kernel<AF_KV_F16><<<a->n_rows, kStoreThreads, 0, stream>>>(p); break;
+        default: kv_store_kernel<AF_KV_BF16><<<a->n_rows, kStoreThreads, 0, stream>>>(p); break;
+    }
+    return cudaGetLastError();
+}
+
+extern "C" size_t af_kv_fork_workspace(const af_kv_fork_args* a) {
+    if (!a || a->n_out < 0 || a->kv.n_pages < 0) return 0;
+    return fork_ws(*a);
+}
+
+extern "C" cudaError_t af_kv_fork(const af_kv_fork_args* a, cudaStream_t stream) {
+    const char* me = "af_kv_fork";
+    if (!a) return refuse(me, "null arguments");
+    const std::string why = fork_wrong(*a);
+    if (!why.empty()) return refuse(me, why);
+    if (!a->ws || a->ws_bytes < fork_ws(*a) || (reinterpret_cast<uintptr_t>(a->ws) & 15))
+        return refuse(me, "ws must hold af_kv_fork_workspace bytes, 16-byte aligned");
+    ForkParams p = {};
+    p.kv = kv_view(a->kv);
+    p.in = {a->table_in, a->len_in, nullptr, a->n_in, a->max_blocks, 0};
+    p.ref_in = a->ref_in;
+    p.parent = a->parent;
+    p.n_new = a->n_new;
+    p.table_out = a->table_out;
+    p.len_out = a->len_out;
+    p.ref_out = a->ref_out;
+    p.n_short = a->n_short;
+    p.n_out = a->n_out;
+    p.copies = static_cast<int4*>(a->ws);
+    p.fresh = reinterpret_cast<int*>(p.copies + a->n_out);
+    kv_fork_kernel<<<1, kForkThreads, 0, stream>>>(p);
+    AF_CUDA_TRY(cudaGetLastError());
+    if (a->n_out == 0) return cudaSuccess;
+    kv_copy_kernel<<<dim3(a->n_out, a->kv.n_layers, 2), kCopyThreads, 0, stream>>>(p.kv, p.copies);
+    return cudaGetLastError();
+}
+
+extern "C" cudaError_t af_kv_compact(const af_kv_compact_args* a, cudaStream_t stream) {
+    const char* me = "af_kv_compact";
+    if (!a) return refuse(me, "null arguments");
+    std::string why = kv_cache_wrong(a->kv);
+    if (why.empty()) why = kv_batch_wrong(a->batch, a->kv, false);
+    if (!why.empty()) return refuse(me, why);
+    if (a->max_path < 0) return refuse(me, "max_path must not be negative");
+    if (a->batch.n_seq == 0) return cudaSuccess;
+    if (!a->len_out || !a->n_path || (a->max_path > 0 && !a->path)) return refuse(me, "null path, n_path or len_out");
+    if (a->kv.n_layers > 32767) return refuse(me, "n_layers must be at most 32767");
+    const KvView kv = kv_view(a->kv);
+    const KvBatch b = kv_batch(a->batch);
+    const dim3 grid((kv.row_bytes / 16 + kCompactThreads - 1) / kCompactThreads, 2 * kv.n_layers, b.n_seq);
+    kv_compact_kernel<<<grid, kCompactThreads, 0, stream>>>(kv, b, a->path, a->n_path, a->max_path, a->len_out, b.len);
+    AF_CUDA_TRY(cudaGetLastError());
+    kv_compact_len_kernel<<<(b.n_seq + 127) / 128, 128, 0, stream>>>(kv, b, a->path, a->n_path, a->max_path, a->len_out);
+    return cudaGetLastError();
+}
