@@ -16,6 +16,8 @@ SOURCES = ["af_gemv.cu", "af_ops.cu", "af_attention.cu", "af_step.cu", "af_prefi
            "af_kvpages.cu", "af_tree.cu", "af_beam.cu", "af_engine.cu",
            "af_gguf.cpp"]
 HEADERS = ["af_common.cuh", "af_gemv.cuh", "af_gemv_dev.cuh", "af_ops.cuh", "af_step.cuh", "af_kvpages.cuh", "af_gguf.h"]
+# Compiled as whole programs, not for device linking: setmaxnreg is ignored in separate compilation.
+WHOLE = {"af_tree.cu"}
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
@@ -39,7 +41,7 @@ def build(verbose: bool = False, jobs: int = 8) -> str:
         obj = os.path.join(objdir, src + ".o")
         objs.append(obj)
         if _stale(obj, [sp] + hdrs):
-            cmd = [NVCC, *GENCODE, *FLAGS, "-dc" if src.endswith(".cu") else "-c", sp, "-o", obj]
+            cmd = [NVCC, *GENCODE, *FLAGS, "-dc" if src not in WHOLE else "-c", sp, "-o", obj]
             if src.endswith(".cpp"):
                 cmd = [NVCC, *FLAGS, "-x", "c++", "-c", sp, "-o", obj]
             if verbose:

@@ -12,7 +12,12 @@ namespace af {
 
 // Device-side error word.  Kernels never trap: a wait that runs out sets a
 // code here and the kernel returns; the host reads it with af_device_error().
+// A file compiled as a whole program (AF_WHOLE_PROGRAM; setmaxnreg needs
+// that) cannot name it: its kernels get the word's address
+// (device_error_word()) as an argument.
+#ifndef AF_WHOLE_PROGRAM
 extern __device__ int g_err;
+#endif
 
 constexpr int kErrMbarTimeout = 1;     // an mbarrier wait exceeded its limit
 constexpr int kErrBadArgs = 2;         // launch arguments failed a device check
@@ -22,7 +27,10 @@ constexpr int kErrBadToken = 3;        // a step saw a token id outside the voca
 // up to the hardware time limit, so this is seconds of wall time at most.
 constexpr uint32_t kSpinLimit = 1u << 26;
 
-__device__ __forceinline__ void set_err(int code) { atomicCAS(&g_err, 0, code); }
+__device__ __forceinline__ void set_err_at(int* err, int code) { atomicCAS(err, 0, code); }
+#ifndef AF_WHOLE_PROGRAM
+__device__ __forceinline__ void set_err(int code) { set_err_at(&g_err, code); }
+#endif
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -78,15 +86,20 @@ __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
 
 // With `abort`, the wait also gives up (without an error code) once *abort
 // is set by another thread of the CTA.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const volatile int* abort = nullptr) {
+__device__ __forceinline__ bool mbar_wait_at(uint64_t* bar, uint32_t parity, int* err, const volatile int* abort) {
     if (mbar_test_wait(bar, parity)) return true;  // already complete: no suspend
     for (uint32_t i = 0; i < kSpinLimit; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if (abort && (i & 15) == 15 && *abort) return false;
     }
-    set_err(kErrMbarTimeout);
+    set_err_at(err, kErrMbarTimeout);
     return false;
 }
+#ifndef AF_WHOLE_PROGRAM
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const volatile int* abort = nullptr) {
+    return mbar_wait_at(bar, parity, &g_err, abort);
+}
+#endif
 
 // ---- bulk copy global -> shared (TMA engine, no tensor map, no multicast) --
 

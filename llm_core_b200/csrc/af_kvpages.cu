@@ -15,7 +15,8 @@ std::string kv_cache_wrong(const af_kv_cache& c) {
     if (c.page_size <= 0 || c.page_size > (1 << 20) || (c.page_size & (c.page_size - 1)))
         return "page_size must be a power of two up to 2^20";
     if (c.head_dim <= 0 || c.head_dim > 256 || c.head_dim % 8) return "head_dim must be a multiple of 8 up to 256";
-    if (c.n_kv_heads > (1 << 16)) return "n_kv_heads must be at most 65536";
+    if (c.n_kv_heads > 65535) return "n_kv_heads must be at most 65535";
+    if ((long long)c.n_pages * c.page_size > INT_MAX) return "n_pages * page_size must be below 2^31";
     const long long dense = (long long)c.n_pages * c.page_size * c.n_kv_heads * c.head_dim;
     if (c.layer_stride < 0 || c.layer_stride % 8 || (c.layer_stride && c.n_layers > 1 && c.layer_stride < dense))
         return "layer_stride must be 0 or a multiple of 8 that holds a layer";
@@ -80,11 +81,11 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_kernel(StoreParams p) 
     if (len < 0) return;
     const long long at = (long long)len + (p.depth ? p.depth[row] : node);
     if (at < 0 || at >= p.n_ctx || node >= p.b.max_nodes) {
-        if (tid == 0) set_err(kErrBadArgs);
+        if (tid == 0) set_err_at(p.b.err, kErrBadArgs);
         return;
     }
     const long long slot = kv_row(p.kv, p.b, seq, len + node);
-    if (slot < 0 && tid == 0) set_err(kErrBadArgs);
+    if (slot < 0 && tid == 0) set_err_at(p.b.err, kErrBadArgs);
     const float* c = p.cos_t + at * half;
     const float* sn = p.sin_t + at * half;
     for (int h = warp; h < p.H + 2 * p.kv.kv_heads; h += kStoreThreads / 32) {
@@ -373,7 +374,7 @@ __global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(KvView kv, 
               kv_row(kv, b, s, len + x) < 0 || kv_row(kv, b, s, len + i) < 0;
     }
     if (bad) {
-        if (tid == 0) set_err(kErrBadArgs);
+        if (tid == 0) set_err_at(b.err, kErrBadArgs);
         return;
     }
     if (col * 16 >= kv.row_bytes) return;
@@ -451,9 +452,13 @@ extern "C" cudaError_t af_kv_store_f32(const af_kv_store_args* a, cudaStream_t s
     if ((a->q_stride && a->q_stride < qd) || (a->q_out_stride && a->q_out_stride < qd) ||
         (a->k_stride && a->k_stride < kd) || (a->v_stride && a->v_stride < kd))
         return refuse(me, "a row stride is shorter than a row");
+    if (a->q_out == a->q && (a->q_out_stride ? a->q_out_stride : qd) != (a->q_stride ? a->q_stride : qd))
+        return refuse(me, "q_out in place needs q's stride");
     StoreParams p = {};
+    int* err = nullptr;
+    AF_CUDA_TRY(device_error_word(&err));
     p.kv = kv_view(a->kv);
-    p.b = kv_batch(a->batch);
+    p.b = kv_batch(a->batch, err);
     p.layer = a->layer;
     p.n_rows = a->n_rows;
     p.n_ctx = a->n_ctx;
@@ -473,7 +478,6 @@ extern "C" cudaError_t af_kv_store_f32(const af_kv_store_args* a, cudaStream_t s
     p.q_norm = a->q_norm;
     p.k_norm = a->k_norm;
     p.eps = a->eps;
-    if (a->q_out == a->q && p.os != p.qs) return refuse(me, "q_out in place needs q's stride");
     switch (a->kv.type) {
         case AF_KV_F32: kv_store_kernel<AF_KV_F32><<<a->n_rows, kStoreThreads, 0, stream>>>(p); break;
         case AF_KV_F16: kv_store_kernel<AF_KV_F16><<<a->n_rows, kStoreThreads, 0, stream>>>(p); break;
@@ -496,7 +500,9 @@ extern "C" cudaError_t af_kv_fork(const af_kv_fork_args* a, cudaStream_t stream)
         return refuse(me, "ws must hold af_kv_fork_workspace bytes, 16-byte aligned");
     ForkParams p = {};
     p.kv = kv_view(a->kv);
-    p.in = {a->table_in, a->len_in, nullptr, a->n_in, a->max_blocks, 0};
+    int* err = nullptr;
+    AF_CUDA_TRY(device_error_word(&err));
+    p.in = {a->table_in, a->len_in, nullptr, a->n_in, a->max_blocks, 0, err};
     p.ref_in = a->ref_in;
     p.parent = a->parent;
     p.n_new = a->n_new;
@@ -525,7 +531,9 @@ extern "C" cudaError_t af_kv_compact(const af_kv_compact_args* a, cudaStream_t s
     if (!a->len_out || !a->n_path || (a->max_path > 0 && !a->path)) return refuse(me, "null path, n_path or len_out");
     if (a->kv.n_layers > 32767) return refuse(me, "n_layers must be at most 32767");
     const KvView kv = kv_view(a->kv);
-    const KvBatch b = kv_batch(a->batch);
+    int* err = nullptr;
+    AF_CUDA_TRY(device_error_word(&err));
+    const KvBatch b = kv_batch(a->batch, err);
     const dim3 grid((kv.row_bytes / 16 + kCompactThreads - 1) / kCompactThreads, 2 * kv.n_layers, b.n_seq);
     kv_compact_kernel<<<grid, kCompactThreads, 0, stream>>>(kv, b, a->path, a->n_path, a->max_path, a->len_out, b.len);
     AF_CUDA_TRY(cudaGetLastError());

@@ -22,6 +22,7 @@ struct KvView {
 struct KvBatch {
     const int *table, *len, *first;
     int n_seq, max_blocks, max_nodes;
+    int* err;  // the device error word
 };
 
 inline int kv_type_bytes(int type) { return type == AF_KV_F32 ? 4 : 2; }
@@ -42,8 +43,8 @@ inline KvView kv_view(const af_kv_cache& c) {
     return v;
 }
 
-inline KvBatch kv_batch(const af_kv_batch& b) {
-    return {b.block_table, b.len, b.first, b.n_seq, b.max_blocks, b.max_nodes};
+inline KvBatch kv_batch(const af_kv_batch& b, int* err) {
+    return {b.block_table, b.len, b.first, b.n_seq, b.max_blocks, b.max_nodes, err};
 }
 
 // "" if the cache's shape and pointers can be served, else what is wrong.
@@ -74,7 +75,7 @@ __device__ __forceinline__ void kv_nodes(const KvBatch& b, int n_rows, int s, in
         r0 = b.first[s];
         n = b.first[s + 1] - r0;
         if (r0 < 0 || n < 0 || n > b.max_nodes || r0 > n_rows - n) {
-            set_err(kErrBadArgs);
+            set_err_at(b.err, kErrBadArgs);
             n = 0;
         }
     } else {
@@ -88,7 +89,7 @@ __device__ __forceinline__ void kv_nodes(const KvBatch& b, int n_rows, int s, in
 __device__ __forceinline__ int kv_len(const KvView& v, const KvBatch& b, int s, int n) {
     const int len = b.len[s];
     if (len < 0 || (long long)len + n > ((long long)b.max_blocks << v.ps_shift)) {
-        set_err(kErrBadArgs);
+        set_err_at(b.err, kErrBadArgs);
         return -1;
     }
     return len;

@@ -24,6 +24,13 @@ int gemv_grid() {
     return num_sms() * per_sm;
 }
 
+cudaError_t device_error_word(int** out) {
+    void* p = nullptr;
+    AF_CUDA_TRY(cudaGetSymbolAddress(&p, g_err));
+    *out = static_cast<int*>(p);
+    return cudaSuccess;
+}
+
 int num_sms() {
     int dev = 0, n = 0;
     cudaGetDevice(&dev);

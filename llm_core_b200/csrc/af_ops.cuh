@@ -9,6 +9,8 @@ namespace af {
 
 void set_last_error(const std::string& s);
 int num_sms();
+// Address of the current device's error word, for kernels that get it as an argument.
+cudaError_t device_error_word(int** out);
 int gemv_grid();
 
 // Byte offset, inside a 512-byte fragment block of a unit, of byte i of
