@@ -137,11 +137,14 @@ __global__ void __launch_bounds__(kTreeThreads) tree_row_kernel(TreeParams p) {
 // first, then the hi·hi ones, and the softmax warps add each tile's P·V to
 // sums in registers, which round to nearest.
 //
-// Warps 0-3 (one query row a thread) run the softmax; warps 4-11 load K and V
-// rows, page by page, straight into registers (16 loads of 16 bytes a lane
-// in flight, 64 KB an SM), split them and store them in the layout that
-// tcgen05 reads; warp 12 issues the products.  registers: 232 / 120 / 40 a
-// thread (setmaxnreg; 232·128 + 120·256 + 40·128 = 65,536, the launch's 128·512).
+// Warps (20): 0-3 turn scores into weights, one query row a thread; 4-7 bring
+// the queries in, add up the tiles' P·V and write the rows out; 8-15 load K
+// and V, page by page, with cp.async (48-64 KB an SM in flight for f32, 96 KB
+// otherwise) and put them into the form that the products take: a lane works
+// on the 16 bytes that it copied itself; 16 issues the products.  Registers a
+// thread: 112 / 184 / 72 / 40 (setmaxnreg; 128 threads of the first two kinds,
+// 256 and 128: 61,440, the launch's 640·96; head_dim 64 has tiles of 128
+// positions and half the sums, so the first two change places).
 //
 // Shared-memory tiles: 8-row × 16-byte core matrices without swizzle, 144
 // bytes apart along the row (16 bytes of padding: the stores of a warp then
@@ -152,19 +155,73 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// d (+)= A · B: A in tensor memory, B by descriptor.
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+// d (+)= A · B: A in tensor memory, B by descriptor.  The whole warp comes
+// here, its leader's instruction runs: the operands then stay in uniform
+// registers (issued by one diverged thread, each product cost 130 cycles).
+__device__ __forceinline__ void tc_mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(leader)
         : "memory");
 }
 
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
+__device__ __forceinline__ void tc_commit(uint32_t leader, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+        "r"(leader)
+        : "memory");
+}
+
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r;
+}
+
+// Two f32 operations an instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(f32x2 x, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// The largest |x|, NaN if one is NaN.
+__device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
+    return r;
 }
 
 // No-swizzle descriptor: strides in bytes, version 1.
@@ -173,23 +230,28 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lbo, uint3
 }
 
 // 32 consecutive columns of this thread's lane.
-__device__ __forceinline__ void tc_ld32(uint32_t t, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tc_ld32(uint32_t t, float* r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
         "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+          "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+          "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
         : "r"(t));
 }
-__device__ __forceinline__ void tc_st16(uint32_t t, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tc_ld16(uint32_t t, float* r) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-        "%14, %15};" ::"r"(r[0]),
-        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(t)
-        : "memory");
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+        : "r"(t));
+}
+__device__ __forceinline__ void tc_st8(uint32_t t, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(t)
+                 : "memory");
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -199,10 +261,13 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // a, b -> packed f16 hi and, of what is left, lo.
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+__device__ __forceinline__ void split2(f32x2 x, uint32_t& hi, uint32_t& lo) {
+    float a, b;
+    unpair(x, a, b);
     const __half2 h = __floats2half2_rn(a, b);
     const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    unpair(fma2(pair(f.x, f.y), pair(-1.f, -1.f), x), a, b);
+    const __half2 l = __floats2half2_rn(a, b);
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
@@ -219,35 +284,68 @@ __device__ __forceinline__ int scale_of(uint32_t max_bits, int top) {
 }
 __device__ __forceinline__ float pow2(int a) { return __int_as_float((a + 127) << 23); }
 
-constexpr int kMmaThreads = 512;
+constexpr int kMmaThreads = 640;
 constexpr int kMmaRows = 128;
 constexpr int kMmaBadWords = 512;  // tiles of a split whose V holds something non-finite, a bit each
 
 template <int TYPE, int HD>
 struct MmaShape {
-    static constexpr int SIZE = TYPE == AF_KV_F32 ? 4 : 2;
+    static constexpr bool F32 = TYPE == AF_KV_F32;
+    static constexpr int SIZE = F32 ? 4 : 2;
     static constexpr int T = HD == 128 ? 64 : 128;      // positions of a tile
-    static constexpr int TERMS = TYPE == AF_KV_F32 ? 2 : 1;  // hi, lo of K and V
+    static constexpr int TERMS = F32 ? 2 : 1;           // hi, lo of K and V
     static constexpr int CS = 144;                      // between 16-byte columns of a tile
     static constexpr int RS = HD / 8 * CS;              // between groups of 8 rows
     static constexpr int TILE = T / 8 * RS;             // 18,432
-    static constexpr int STAGE = 2 * TERMS * TILE;      // K hi, K lo, V hi, V lo
-    static constexpr int NB = TYPE == AF_KV_F32 ? 3 : HD == 128 ? 6 : 5;
+    static constexpr int HALF = TERMS * TILE;           // K or V of a tile: hi, lo
+    static constexpr int NB = F32 ? 2 : 5;              // tiles in shared memory: K V K V ...
+    static constexpr int AHEAD = NB - 2;                // 16-bit caches: tiles whose copies are in flight
     static constexpr int RPW = T / 8;                   // rows of a loading warp in a tile
     static constexpr int LPR = HD * SIZE / 16;          // lanes of a row
-    static constexpr int RPC = 32 / LPR;                // rows of one load
-    static constexpr int NCK = RPW / RPC;               // loads of a lane for K (and for V)
-    static constexpr int RING = 16 / (2 * NCK);         // tiles in flight in registers
+    static constexpr int RPC = 32 / LPR;                // rows of one copy of a warp (512 bytes)
+    static constexpr int NCK = RPW / RPC;               // copies of a lane for K (and for V): 8 or 4
+    // queries in, rows out: 128 rows with 16 bytes of padding, over the last tiles' place
+    static constexpr int QROW = HD * 4 + 16;
+    static constexpr int QTILE = NB - (kMmaRows * QROW + 2 * HALF - 1) / (2 * HALF);
+    static_assert(QTILE >= (F32 ? 1 : AHEAD), "the first copies do not wait for the queries");
+    // registers
+    static constexpr int REG_S = HD == 128 ? 112 : 184, REG_O = HD == 128 ? 184 : 112;
     // tensor memory columns
-    static constexpr int QH = 0, QL = HD / 2, S0 = HD, O0 = HD + 2 * T;
-    static_assert(O0 + 2 * HD <= 512, "tensor memory");
-    // shared memory
-    static constexpr int BAD = 256;                     // behind the mbarriers: kMmaBadWords words
-    static constexpr int SCALE = BAD + kMmaBadWords * 4;  // [NB][3][T] floats
-    static constexpr int TILES = (SCALE + NB * 3 * T * 4 + 127) / 128 * 128;
-    static constexpr int BYTES = TILES + NB * STAGE;
+    static constexpr int NS = 3;                          // score tiles (each becomes its weights)
+    static constexpr int QH = 0, QL = HD / 2, S0 = HD, O0 = HD + NS * T;
+    static_assert(O0 + HD <= 512, "tensor memory");
+    // shared memory, behind 512 bytes of mbarriers
+    static constexpr int BAD = 512;                       // kMmaBadWords words
+    static constexpr int ROWS = BAD + kMmaBadWords * 4;   // [128] query scales, [NS][128] corrections, [128] tops, [128] sums
+    static constexpr int GROUPS = 8;                      // a loading warp's rows share their powers of two
+    static constexpr int SCALE = ROWS + (3 + NS) * kMmaRows * 4; // [2 NB][3][GROUPS] floats
+    static constexpr int TILES = (SCALE + (TYPE == AF_KV_F16 ? 0 : 2 * NB * 3 * GROUPS * 4) + 127) / 128 * 128;
+    static constexpr int RAW = TILES + NB * 2 * HALF;     // f32: 8 warps x 16 copies x 512 bytes as they are
+    static constexpr int BYTES = RAW + (F32 ? 65536 : 0);
     static_assert(BYTES <= 227 * 1024, "shared memory");
 };
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Zeros for what is not finite; the largest of the rest, over the warp.
+__device__ __noinline__ uint32_t clean(float4 (&x)[8]) {
+    uint32_t b = 0;
+    for (int i = 0; i < 8; ++i) {
+        float* e = &x[i].x;
+        for (int j = 0; j < 4; ++j) {
+            if (!(fabsf(e[j]) < INFINITY)) e[j] = 0.f;
+            b = max(b, __float_as_uint(e[j]) & 0x7fffffffu);
+        }
+    }
+    return __reduce_max_sync(0xffffffffu, b);
+}
 
 struct MmaParams {
     TreeParams t;
@@ -276,29 +374,37 @@ template <int TYPE, int HD>
 __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) {
     using SH = MmaShape<TYPE, HD>;
     using E = KvElem<TYPE>;
-    constexpr int T = SH::T, NB = SH::NB, RING = SH::RING, NCK = SH::NCK;
+    constexpr int T = SH::T, NB = SH::NB, NCK = SH::NCK, NS = SH::NS;
     extern __shared__ __align__(1024) uint8_t sm[];
     const TreeParams& p = mp.t;
-    uint64_t* full = reinterpret_cast<uint64_t*>(sm);  // [NB] 8 loading warps
-    uint64_t* empty = full + NB;                       // [NB] P·V done
-    uint64_t* s_full = empty + NB;                     // [2] scores done
-    uint64_t* p_full = s_full + 2;                     // [2] 4 softmax warps: weights written
-    uint64_t* o_full = p_full + 2;                     // [2] P·V done
-    uint64_t* o_free = o_full + 2;                     // [2] 4 softmax warps: P·V taken
-    uint64_t* q_full = o_free + 2;                     // 4 softmax warps: queries written
-    uint64_t* done = q_full + 1;                       // every product done
+    // A waiter never falls a whole ring behind: K of t + NB may be there before the softmax looks for K of t, so
+    // its barriers (and the scales) are 2 NB; every other one's next phase needs what the waiter of this one does.
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(sm);  // [2 NB] 8 loading warps: K of a tile is there
+    uint64_t* v_full = k_full + 2 * NB;                  // [NB] V
+    uint64_t* k_empty = v_full + NB;                     // [NB] scores done
+    uint64_t* v_empty = k_empty + NB;                    // [NB] P·V done
+    uint64_t* s_full = v_empty + NB;                     // [NS] scores done
+    uint64_t* p_full = s_full + NS;                      // [NS] softmax warps: weights written
+    uint64_t* c_full = p_full + NS;                      // [NS] softmax warps: correction written
+    uint64_t* o_full = c_full + NS;                      // P·V done
+    uint64_t* o_free = o_full + 1;                       // output warps: P·V and correction taken
+    uint64_t* q_full = o_free + 1;                       // 8 softmax and output warps: queries written
+    uint64_t* fin = q_full + 1;                          // softmax warps: tops and sums written
+    uint64_t* done = fin + 1;                            // every product done
+    static_assert((5 * NB + 3 * NS + 5) * 8 + 8 <= SH::BAD, "barriers");
     uint32_t* tslot = reinterpret_cast<uint32_t*>(done + 1);
     volatile int* flag = reinterpret_cast<volatile int*>(tslot + 1);
     uint32_t* bad = reinterpret_cast<uint32_t*>(sm + SH::BAD);
+    float* s_rs = reinterpret_cast<float*>(sm + SH::ROWS);
+    float* s_corr = s_rs + kMmaRows;
+    float* s_top = s_corr + NS * kMmaRows;
+    float* s_sum = s_top + kMmaRows;
     float* scales = reinterpret_cast<float*>(sm + SH::SCALE);
     uint8_t* tiles = sm + SH::TILES;
-    auto wait = [&](uint64_t* bar, uint32_t parity, const volatile int* abort) -> bool {
-        return mbar_wait_at(bar, parity, p.b.err, abort);
-    };
+    uint8_t* staged = tiles + SH::QTILE * 2 * SH::HALF;
+    auto wait = [&](uint64_t* bar, int phase) -> bool { return mbar_wait_at(bar, (uint32_t)phase & 1u, p.b.err, flag); };
     // the same for a whole warp, which stays together
-    auto wait_warp = [&](uint64_t* bar, uint32_t parity) -> bool {
-        return __all_sync(0xffffffffu, mbar_wait_at(bar, parity, p.b.err, flag));
-    };
+    auto wait_warp = [&](uint64_t* bar, int phase) -> bool { return __all_sync(0xffffffffu, wait(bar, phase)); };
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.x % mp.nsplit, rt = blockIdx.x / mp.nsplit, kvh = blockIdx.y, seq = blockIdx.z;
 
@@ -312,28 +418,34 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
     const int nt_all = (end + T - 1) / T;
     const int t0 = (int)((long long)nt_all * split / mp.nsplit), t1 = (int)((long long)nt_all * (split + 1) / mp.nsplit);
     const int nt = t1 - t0;
+    const int live_warps = (row_hi - row_lo + 31) / 32;  // of the 4 + 4 that work on rows; the others have none
     int bs = 0;  // tiles of a bit of bad[]: 1 << bs
     while (nt > (kMmaBadWords * 32) << bs) ++bs;
     pdl_launch_dependents();
 
     if (tid == 0) {
         for (int i = 0; i < NB; ++i) {
-            mbar_init(&full[i], 8);
-            mbar_init(&empty[i], 1);
+            mbar_init(&k_full[i], 8);
+            mbar_init(&k_full[NB + i], 8);
+            mbar_init(&v_full[i], 8);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < NS; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
-            mbar_init(&o_full[i], 1);
-            mbar_init(&o_free[i], 4);
+            mbar_init(&p_full[i], live_warps);
+            mbar_init(&c_full[i], live_warps);
         }
-        mbar_init(q_full, 4);
+        mbar_init(o_full, 1);
+        mbar_init(o_free, live_warps);
+        mbar_init(q_full, 8);
+        mbar_init(fin, live_warps);
         mbar_init(done, 1);
         *flag = 0;
         fence_mbar_init();
     }
     for (int i = tid; i < kMmaBadWords; i += kMmaThreads) bad[i] = 0;
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(512u)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -343,98 +455,102 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
     tc_fence_after();
     const uint32_t tmem = *tslot;
 
+    // Queries, by the softmax and output warps: a row a warp in turn — its largest value, hi and lo — into the staging
+    // place, from there a row a thread (hi by one kind of warps, lo by the other) into tensor memory.  Rows that are
+    // none keep what is there: what comes of them stays in their own row.
+    auto queries = [&]() {
+        constexpr int Q4 = HD / 4, QR = 32 / Q4;  // lanes of a row at 16 bytes each, rows of a warp's load
+        const int sub = lane / Q4, col = lane % Q4, rows = row_hi - row_lo;
+        const bool wide = ((reinterpret_cast<uintptr_t>(p.q) & 15) | (p.qs & 3)) == 0;
+#pragma unroll 1
+        for (int i0 = warp * QR; i0 < rows; i0 += 4 * 8 * QR) {
+            float4 f[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int x = row_lo + min(i0 + j * 8 * QR + sub, rows - 1);
+                const float* q = p.q + (long long)(r0 + x / p.G) * p.qs + (long long)(kvh * p.G + x % p.G) * HD + 4 * col;
+                if (wide) f[j] = __ldg(reinterpret_cast<const float4*>(q));
+                else f[j] = make_float4(q[0], q[1], q[2], q[3]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = i0 + j * 8 * QR + sub;
+                float big = max3_abs_nan(max3_abs_nan(0.f, f[j].x, f[j].y), f[j].z, f[j].w);
+                uint32_t mx = __float_as_uint(big);
+#pragma unroll
+                for (int o = 1; o < Q4; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                const int a = scale_of(mx, 100);
+                const f32x2 s = pair(pow2(a), pow2(a));
+                uint2 hi, lo;
+                split2(mul2(pair(f[j].x, f[j].y), s), hi.x, lo.x);
+                split2(mul2(pair(f[j].z, f[j].w), s), hi.y, lo.y);
+                if (i < rows) {
+                    *reinterpret_cast<uint2*>(staged + i * SH::QROW + 8 * col) = hi;
+                    *reinterpret_cast<uint2*>(staged + i * SH::QROW + 2 * HD + 8 * col) = lo;
+                    if (col == 0) s_rs[i] = p.scale * pow2(-a);
+                }
+            }
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const int mine = tid & 127;
+        if ((mine & ~31) < rows) {
+            const uint8_t* from = staged + mine * SH::QROW + (warp < 4 ? 0 : 2 * HD);
+            const uint32_t to = tmem + ((uint32_t)(mine & ~31) << 16) + (warp < 4 ? SH::QH : SH::QL);
+#pragma unroll 2
+            for (int c = 0; c < HD / 16; ++c) {
+                const uint4 x = *reinterpret_cast<const uint4*>(from + 32 * c), y = *reinterpret_cast<const uint4*>(from + 32 * c + 16);
+                const uint32_t v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                tc_st8(to + 8 * c, v);
+            }
+            tc_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+    };
+
     if (warp < 4) {
         // ------------------------------------------------------- softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH::REG_S));
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
         const int r = row_lo + tid;
         const bool live = r < row_hi;
-        const int node = live ? r / p.G : 0, row = r0 + node, head = kvh * p.G + (live ? r % p.G : 0);
-        float rs;  // what a raw score is times, but for K's power of two
-        {
-            const float* q = p.q + (long long)row * p.qs + (long long)head * HD;
-            float x[HD];
-            uint32_t mx = 0;
-            if ((reinterpret_cast<uintptr_t>(q) & 15) == 0) {
-#pragma unroll
-                for (int i = 0; i < HD; i += 4) {
-                    const float4 f = live ? __ldg(reinterpret_cast<const float4*>(q + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    x[i] = f.x, x[i + 1] = f.y, x[i + 2] = f.z, x[i + 3] = f.w;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < HD; ++i) x[i] = live ? q[i] : 0.f;
-            }
-#pragma unroll
-            for (int i = 0; i < HD; ++i) mx = max(mx, __float_as_uint(x[i]) & 0x7fffffffu);
-            const int a = scale_of(mx, 100);
-            const float s = pow2(a);
-            rs = p.scale * pow2(-a);
-#pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
-                uint32_t hi[16], lo[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) split2(x[32 * c + 2 * i] * s, x[32 * c + 2 * i + 1] * s, hi[i], lo[i]);
-                tc_st16(tmem + lanes + SH::QH + 16 * c, hi);
-                tc_st16(tmem + lanes + SH::QL + 16 * c, lo);
-            }
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
-        }
-        float acc[HD];
-#pragma unroll
-        for (int i = 0; i < HD; ++i) acc[i] = 0.f;
-        float m = -INFINITY, l = 0.f, corr = 0.f;  // corr: of the sums, for the tile whose P·V is due
+        const int node = live ? r / p.G : 0, row = r0 + node;
+        queries();
+        float m = -INFINITY, l = 0.f;
         bool ok = true;
-        auto take = [&](int t) -> bool {           // acc = acc·corr + (P·V)(t)
-            if (!wait_warp(&o_full[t & 1], (uint32_t)(t >> 1) & 1u)) return false;
+        const float rs = s_rs[tid];  // what a raw score is times, but for K's power of two
+        for (int t = 0; ok && t < nt && warp < live_warps; ++t) {
+            const int st = t % NB, sl = t % NS;
+            ok = wait_warp(&k_full[t % (2 * NB)], t / (2 * NB)) && wait_warp(&s_full[sl], t / NS);
+            if (!ok) break;
             tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
-                uint32_t o[32];
-                tc_ld32(tmem + lanes + SH::O0 + (t & 1) * HD + 32 * c, o);
-                tc_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(acc[32 * c + i], corr, __uint_as_float(o[i]));
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&o_free[t & 1]);
-            return true;
-        };
-        for (int t = 0; t < nt; ++t) {
-            const int st = t % NB;
-            if (!wait_warp(&full[st], (uint32_t)(t / NB) & 1u) || !wait_warp(&s_full[t & 1], (uint32_t)(t >> 1) & 1u)) {
-                ok = false;
-                break;
-            }
-            tc_fence_after();
-            const uint32_t sb = tmem + lanes + SH::S0 + (t & 1) * T;
+            const uint32_t sb = tmem + lanes + SH::S0 + sl * T;
             float v[T];
 #pragma unroll
-            for (int c = 0; c < T / 32; ++c) {
-                uint32_t x[32];
-                tc_ld32(sb + 32 * c, x);
-                tc_wait_ld();
+            for (int c = 0; c < T / 32; ++c) tc_ld32(sb + 32 * c, v + 32 * c);
+            tc_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[32 * c + i] = __uint_as_float(x[i]);
-            }
-            const float4* kc = reinterpret_cast<const float4*>(scales + (st * 3 + 0) * T);  // 2^-a of K
-            const float4* vf = reinterpret_cast<const float4*>(scales + (st * 3 + 1) * T);  // -a of V
-            const float4* vg = reinterpret_cast<const float4*>(scales + (st * 3 + 2) * T);  // 2^a of V
-            if (TYPE == AF_KV_F16) {
+            for (int i = 0; i < T; ++i) asm volatile("" : "+f"(v[i]));  // no use may move above the wait
+            const float4* kc = reinterpret_cast<const float4*>(scales + (t % (2 * NB)) * 3 * SH::GROUPS);  // 2^-a of K
+            const float4* vf = kc + SH::GROUPS / 4;                                                        // -a of V
+            const float4* vg = vf + SH::GROUPS / 4;                                                        // 2^a of V
+            ok = wait_warp(&v_full[st], t / NB);
+            if (!ok) break;
+            {
+                float c[8], f[8];
 #pragma unroll
-                for (int i = 0; i < T; ++i) v[i] *= rs;
-            } else {
+                for (int i = 0; i < 8; ++i) c[i] = rs, f[i] = 0.f;
+                if (TYPE != AF_KV_F16) {
+                    const float4 x = kc[0], y = kc[1], z = vf[0], w = vf[1];
+                    c[0] *= x.x, c[1] *= x.y, c[2] *= x.z, c[3] *= x.w, c[4] *= y.x, c[5] *= y.y, c[6] *= y.z, c[7] *= y.w;
+                    f[0] = z.x, f[1] = z.y, f[2] = z.z, f[3] = z.w, f[4] = w.x, f[5] = w.y, f[6] = w.z, f[7] = w.w;
+                }
 #pragma unroll
-                for (int i = 0; i < T; i += 4) {
-                    const float4 c = kc[i / 4], f = vf[i / 4];
-                    v[i] = fmaf(v[i] * rs, c.x, f.x);
-                    v[i + 1] = fmaf(v[i + 1] * rs, c.y, f.y);
-                    v[i + 2] = fmaf(v[i + 2] * rs, c.z, f.z);
-                    v[i + 3] = fmaf(v[i + 3] * rs, c.w, f.w);
+                for (int e = 0; e < T; e += 2) {
+                    const int g = e / SH::RPW;
+                    const f32x2 x = pair(v[e], v[e + 1]), cc = pair(c[g], c[g]);
+                    unpair(TYPE == AF_KV_F16 ? mul2(x, cc) : fma2(x, cc, pair(f[g], f[g])), v[e], v[e + 1]);
                 }
             }
             const int p0 = (t0 + t) * T;
@@ -447,57 +563,112 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
                         if (!((see >> i) & 1)) v[64 * w + i] = -INFINITY;
                 }
             }
-            float top = v[0];
+            float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-            for (int i = 1; i < T; ++i) top = fmaxf(top, v[i]);
-            const float mn = fmaxf(m, top);
+            for (int i = 4; i + 1 < T; i += 2) top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], v[i], v[i + 1]);
+            const float mn = max3(m, fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
             const float ms = mn == -INFINITY ? 0.f : mn - 14.f;  // weights times 2^14
-            const float c_new = ex2(m - (mn == -INFINITY ? 0.f : mn));
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < T / 32; ++c) {
-                uint32_t hi[16], lo[16];
-#pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    const int e = 32 * c + i;
-                    float w[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) w[j] = ex2(v[e + j] - ms);
-                    if (TYPE == AF_KV_F16) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) sum[j] += w[j];
-                    } else {
-                        const float4 g = vg[e / 4];
-                        sum[0] = fmaf(w[0], g.x, sum[0]);
-                        sum[1] = fmaf(w[1], g.y, sum[1]);
-                        sum[2] = fmaf(w[2], g.z, sum[2]);
-                        sum[3] = fmaf(w[3], g.w, sum[3]);
-                    }
-                    split2(w[0], w[1], hi[i / 2], lo[i / 2]);
-                    split2(w[2], w[3], hi[i / 2 + 1], lo[i / 2 + 1]);
-                }
-                tc_st16(sb + 16 * c, hi);
-                tc_st16(sb + T / 2 + 16 * c, lo);
-            }
-            l = fmaf(l, c_new, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+            const float corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
             m = mn;
+            // its place is free: these scores were issued behind P·V of t - 2, which waited until t - NS was taken
+            s_corr[sl * kMmaRows + tid] = corr;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&c_full[sl]);
+            f32x2 sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+            const f32x2 ms2 = pair(-ms, -ms);
+            float g8[8];
+            if (TYPE != AF_KV_F16) {
+                const float4 x = vg[0], y = vg[1];
+                g8[0] = x.x, g8[1] = x.y, g8[2] = x.z, g8[3] = x.w, g8[4] = y.x, g8[5] = y.y, g8[6] = y.z, g8[7] = y.w;
+            }
+#pragma unroll
+            for (int c = 0; c < T / 16; ++c) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const int e = 16 * c + i;
+                    float w[4];
+                    unpair(add2(pair(v[e], v[e + 1]), ms2), w[0], w[1]);
+                    unpair(add2(pair(v[e + 2], v[e + 3]), ms2), w[2], w[3]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[j] = ex2(w[j]);
+                    const f32x2 x = pair(w[0], w[1]), y = pair(w[2], w[3]);
+                    if (TYPE == AF_KV_F16) {
+                        sum[0] = add2(sum[0], x);
+                        sum[1] = add2(sum[1], y);
+                    } else {
+                        const float g = g8[e / SH::RPW];
+                        sum[0] = fma2(x, pair(g, g), sum[0]);
+                        sum[1] = fma2(y, pair(g, g), sum[1]);
+                    }
+                    split2(x, hi[i / 2], lo[i / 2]);
+                    split2(y, hi[i / 2 + 1], lo[i / 2 + 1]);
+                }
+                tc_st8(sb + 16 * c, hi);  // over the 16 scores that they came from
+                tc_st8(sb + 16 * c + 8, lo);
+            }
+            {
+                float a, b;
+                unpair(add2(sum[0], sum[1]), a, b);
+                l = fmaf(l, corr, a + b);
+            }
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t & 1]);
-            if (t > 0 && !take(t - 1)) {
-                ok = false;
-                break;
-            }
-            corr = c_new;
+            if (lane == 0) mbar_arrive(&p_full[sl]);
         }
-        if (ok && nt > 0) ok = take(nt - 1);
         if (!ok) *flag = 1;
+        s_top[tid] = m;
+        s_sum[tid] = l;
+        __syncwarp();
+        if (lane == 0 && warp < live_warps) mbar_arrive(fin);
+    } else if (warp < 8) {
+        // ------------------------------------------- queries in, sums, rows out
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH::REG_O));
+        queries();
+        constexpr int Q4 = HD / 4, QR = 32 / Q4;  // lanes of a row at 16 bytes each, rows of a warp's store
+        const int w = warp - 4, ti = tid - 128;
+        const uint32_t lanes = (uint32_t)(w * 32) << 16;
+        const int sub = lane / Q4, col = lane % Q4;
+        uint8_t* wrow = staged + w * 32 * SH::QROW;
+        float* mine = reinterpret_cast<float*>(staged + ti * SH::QROW);
+        const int r = row_lo + ti;
+        const bool live = r < row_hi;
+        const int node = live ? r / p.G : 0, row = r0 + node, head = kvh * p.G + (live ? r % p.G : 0);
+        float acc[HD];
+#pragma unroll
+        for (int i = 0; i < HD; ++i) acc[i] = 0.f;
+        bool ok = true;
+        for (int t = 0; t < nt && w < live_warps; ++t) {  // acc = acc·corr + (P·V)(t)
+            ok = wait_warp(&c_full[t % NS], t / NS) && wait_warp(o_full, t);
+            if (!ok) break;
+            tc_fence_after();
+            const float corr = s_corr[(t % NS) * kMmaRows + ti];
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) {
+                float o[16];
+                tc_ld16(tmem + lanes + SH::O0 + 16 * c, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(o[i]));  // no use may move above the wait
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    float& x = acc[16 * c + i];
+                    float& y = acc[16 * c + i + 1];
+                    unpair(fma2(pair(x, y), pair(corr, corr), pair(o[i], o[i + 1])), x, y);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_free);
+        }
+        ok = ok && w < live_warps && wait_warp(fin, 0);
+        if (!ok && w < live_warps) *flag = 1;
         // non-finite values of V were taken out of the products: the rows that see them get them back
-        for (int w = 0; ok && w < kMmaBadWords && (32 * w) << bs < nt; ++w) {
-            uint32_t b = bad[w];
+        for (int wd = 0; ok && wd < kMmaBadWords && (32 * wd) << bs < nt; ++wd) {
+            uint32_t b = bad[wd];
             while (b) {
-                const int t = (32 * w + __ffs(b) - 1) << bs;
+                const int t = (32 * wd + __ffs(b) - 1) << bs;
                 b &= b - 1;
                 for (int pos = (t0 + t) * T; pos < min((t0 + min(t + (1 << bs), nt)) * T, end); ++pos) {
                     if (!live || !(tree_window(p, row, node, n, len, pos) & 1)) continue;
@@ -512,238 +683,323 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
                 }
             }
         }
-        if (live && ok) {
-            if (mp.nsplit == 1) {
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                float* o = p.out + (long long)row * p.os + (long long)head * HD;
-                if ((reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+        if (ok) {
+            const float l = s_sum[ti], inv = mp.nsplit > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-                    for (int i = 0; i < HD; i += 4)
-                        *reinterpret_cast<float4*>(o + i) =
-                            make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < HD; ++i) o[i] = acc[i] * inv;
+            for (int i = 0; i < HD; i += 4)
+                *reinterpret_cast<float4*>(mine + i) =
+                    make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
+            __syncwarp();
+            // out, or the split's place in the workspace: rows of HD values either way
+            const long long at = ((long long)split * p.n_rows + row) * p.H + head;
+            float* orow = !live ? nullptr : mp.nsplit == 1 ? p.out + (long long)row * p.os + (long long)head * HD : mp.part + at * HD;
+            const bool wide_out = mp.nsplit > 1 || ((reinterpret_cast<uintptr_t>(p.out) & 15) | (p.os & 3)) == 0;
+            if (live && mp.nsplit > 1)
+                *reinterpret_cast<float2*>(mp.part + (long long)mp.nsplit * p.n_rows * p.H * HD + at * 2) = make_float2(s_top[ti], l);
+            const int mine_rows = min(32, row_hi - row_lo - w * 32);
+#pragma unroll 4
+            for (int i = 0; i < mine_rows; i += QR) {
+                float* o = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), i + sub));
+                const float4 f = *reinterpret_cast<const float4*>(wrow + (i + sub) * SH::QROW + 16 * col);
+                if (o) {
+                    o += 4 * col;
+                    if (wide_out) *reinterpret_cast<float4*>(o) = f;
+                    else o[0] = f.x, o[1] = f.y, o[2] = f.z, o[3] = f.w;
                 }
-            } else {
-                const long long at = ((long long)split * p.n_rows + row) * p.H + head;
-                float* o = mp.part + at * HD;
-#pragma unroll
-                for (int i = 0; i < HD; i += 4)
-                    *reinterpret_cast<float4*>(o + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-                float* ml = mp.part + (long long)mp.nsplit * p.n_rows * p.H * HD + at * 2;
-                *reinterpret_cast<float2*>(ml) = make_float2(m, l);
             }
         }
-    } else if (warp < 12) {
+    } else if (warp < 16) {
         // ------------------------------------------------------- K and V
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
-        const int w = warp - 4, sub = lane / SH::LPR, col = lane % SH::LPR;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        const int w = warp - 8, sub = lane / SH::LPR, col = lane % SH::LPR;
         const long long hoff = p.layer * p.kv.layer_bytes + (long long)kvh * HD * SH::SIZE + col * 16;
         const uint8_t* kb = p.kv.k + hoff;
         const uint8_t* vb = p.kv.v + hoff;
-        const int mine = w * SH::RPW + lane;  // lane < RPW: the row that this lane looks up
-        auto lookup = [&](int t) -> int {     // pool row of the lane's position, -1: none
-            const int pos = (t0 + t) * T + mine;
-            if (t >= nt || lane >= SH::RPW || pos >= end) return -1;
-            const int page = kv_page(p.b, p.kv.n_pages, seq, pos >> p.kv.ps_shift);
-            if (page < 0) {
+        // Rows of a tile for the warp, one a lane (lane < RPW).  fetch() asks for the page early; row() makes it a
+        // pool row when it is needed: behind the last position the last one again (no weight reaches it), for a
+        // page that is none row 0 and the error word.
+        const int off = w * SH::RPW + min(lane, SH::RPW - 1);
+        const int* table = p.b.table ? p.b.table + (long long)seq * p.b.max_blocks : nullptr;
+        const int page0 = (int)min((long long)seq * p.b.max_blocks, (long long)p.kv.n_pages);  // no table: pages in order
+        auto position = [&](int t) { return min((t0 + min(t, max(nt - 1, 0))) * T + off, end - 1); };
+        auto fetch = [&](int t) -> int {
+            const int blk = position(t) >> p.kv.ps_shift;
+            return table ? __ldg(table + blk) : page0 + blk;
+        };
+        auto row_of = [&](int t, int page) -> int {
+            if ((unsigned)page >= (unsigned)p.kv.n_pages) {
                 set_err_at(p.b.err, kErrBadArgs);
-                return -1;
+                page = 0;
             }
-            return (page << p.kv.ps_shift) + (pos & ((1 << p.kv.ps_shift) - 1));
+            return (page << p.kv.ps_shift) + (position(t) & ((1 << p.kv.ps_shift) - 1));
         };
-        uint4 ring[RING][2 * NCK];
-        auto load = [&](int idx, int c) -> uint4 {  // chunk c: K rows first, then V
-            const int at = __shfl_sync(0xffffffffu, idx, (c % NCK) * SH::RPC + sub);
-            if (at < 0) return make_uint4(0u, 0u, 0u, 0u);
-            return __ldg(reinterpret_cast<const uint4*>((c < NCK ? kb : vb) + (long long)at * p.kv.row_bytes));
+        auto copy = [&](uint32_t dst, const uint8_t* base, int idx, int chunk) {
+            const uint32_t at = (uint32_t)__shfl_sync(0xffffffffu, idx, chunk * SH::RPC + sub);
+            cp_async16(dst, base + (unsigned long long)at * (uint32_t)p.kv.row_bytes);
         };
-        int idx = lookup(0);
-#pragma unroll
-        for (int s = 0; s < RING; ++s) {
-#pragma unroll
-            for (int c = 0; c < 2 * NCK; ++c) ring[s][c] = load(idx, c);
-            idx = lookup(s + 1);
-        }
+        auto hand_over = [&](uint64_t* bar) {
+            fence_proxy_async_smem();  // these stores, before the products read them
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
         bool ok = true;
-        for (int tb = 0; tb < nt && ok; tb += RING) {
+        if (SH::F32) {
+            // Halves of a tile in the order K0 K1 V0 K2 V1 K3 ..., so that no K waits for the products of a V before
+            // it: 8 copies (4,096 bytes of a warp) in two groups; two halves are in flight.
+            uint8_t* raw = sm + SH::RAW + w * 8192 + lane * 16;
+            const uint32_t raw_s = smem_u32(raw);
+            const int halves = nt > 0 ? 2 * nt + 1 : 0;
+            auto is_v = [](int h) { return h > 0 && !(h & 1); };
+            auto tile_of = [](int h) { return h > 0 && !(h & 1) ? h / 2 - 1 : (h + 1) / 2; };
+            // rows of the next V, of the K before the next, of the next K, the page of the one after
+            int idx_v = row_of(0, fetch(0)), idx_m = row_of(1, fetch(1)), idx_k = idx_v, page = fetch(2);
+            auto issue = [&](int h) {  // nothing behind the last V; K of a tile that is none is not used
+                if (h < halves) {
+                    const bool v = is_v(h);
+                    const int idx = v ? idx_v : idx_k;
+                    const uint8_t* base = v ? vb : kb;
 #pragma unroll
-            for (int s = 0; s < RING; ++s) {
-                const int t = tb + s, st = t % NB;
-                if (t >= nt) break;
-                if (t >= NB && !wait_warp(&empty[st], (uint32_t)(t / NB - 1) & 1u)) {
-                    ok = false;
-                    break;
+                    for (int i = 0; i < 8; ++i) copy(raw_s + (h & 1) * 4096 + i * 512, base, idx, i);
                 }
-                uint8_t* stage = tiles + st * SH::STAGE;
-                float* sc = scales + st * 3 * T;
+                cp_async_commit();
+            };
+            // the lane's first row and column in a tile; a copy lies RPC rows on
+            uint8_t* home = tiles + w * (SH::RPW / 8) * SH::RS + sub * 16 + (col >> 1) * SH::CS + (col & 1) * 8;
+            issue(0);
+            idx_k = idx_m;
+            issue(1);
+            idx_k = row_of(2, page);
+            page = fetch(3);
+            uint64_t* due = nullptr;  // a half that is stored and not yet handed over
+#pragma unroll 1
+            for (int h = 0; ok && h < halves; ++h) {
+                const int t = tile_of(h), st = t % NB;
+                const bool isv = is_v(h), real = t < nt;
+                cp_async_wait<1>();
+                const uint8_t* src = raw + (h & 1) * 4096;
+                float4 x[8];
+                float big[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int c = 0; c < 2 * NCK; ++c) {
-                    const bool isv = c >= NCK;
-                    const int trow = w * SH::RPW + (c % NCK) * SH::RPC + sub;  // row of the tile
-                    uint8_t* dst = stage + (isv ? SH::TERMS * SH::TILE : 0) + (trow >> 3) * SH::RS + (trow & 7) * 16;
-                    uint4 x = ring[s][c];
-                    ring[s][c] = load(idx, c);
-                    if (TYPE == AF_KV_F32) {
-                        uint32_t b = max(max(x.x & 0x7fffffffu, x.y & 0x7fffffffu), max(x.z & 0x7fffffffu, x.w & 0x7fffffffu));
-                        uint32_t mx = __reduce_max_sync(0xffffffffu, b);
-                        if (isv && mx >= 0x7f800000u) {  // rare: take what is not finite out, and remember the tile
-                            uint32_t* e = &x.x;
-                            b = 0;
+                for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const float4*>(src + i * 512);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                if ((e[i] & 0x7fffffffu) >= 0x7f800000u) e[i] = 0u;
-                                b = max(b, e[i] & 0x7fffffffu);
-                            }
-                            mx = __reduce_max_sync(0xffffffffu, b);
-                            if (lane == 0) atomicOr(&bad[(t >> bs) >> 5], 1u << ((t >> bs) & 31));
+                for (int i = 0; i < 8; ++i) {
+                    big[(2 * i) & 3] = max3_abs_nan(big[(2 * i) & 3], x[i].x, x[i].y);
+                    big[(2 * i + 1) & 3] = max3_abs_nan(big[(2 * i + 1) & 3], x[i].z, x[i].w);
+                }
+                uint32_t mx = __reduce_max_sync(
+                    0xffffffffu, __float_as_uint(max3_abs_nan(max3_abs_nan(big[0], big[1], big[2]), big[3], 0.f)));
+                issue(h + 2);  // over what is in registers now
+                if (due) hand_over(due);  // the half before: its stores are through by now
+                due = nullptr;
+                if (!real) continue;
+                if (h == 2 * SH::QTILE - 1) ok = wait_warp(q_full, 0);  // the first K over the staged queries' place
+                if (ok && t >= NB) ok = wait_warp(isv ? &v_empty[st] : &k_empty[st], t / NB - 1);
+                if (!ok) break;
+                if (isv && mx >= 0x7f800000u) {  // rare: take what is not finite out, and remember the tile
+                    float4 y[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = x[i];
+                    mx = clean(y);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = y[i];
+                    if (lane == 0) atomicOr(&bad[(t >> bs) >> 5], 1u << ((t >> bs) & 31));
+                }
+                const int a = scale_of(mx, isv ? 60 : 100);
+                const float f = pow2(a);
+                const f32x2 f2 = pair(f, f);
+                uint8_t* dst = home + (st * 2 + (isv ? 1 : 0)) * SH::HALF;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    uint2 hi, lo;
+                    split2(mul2(pair(x[i].x, x[i].y), f2), hi.x, lo.x);
+                    split2(mul2(pair(x[i].z, x[i].w), f2), hi.y, lo.y);
+                    uint8_t* d = dst + (i * SH::RPC / 8) * SH::RS + (i * SH::RPC % 8) * 16;
+                    *reinterpret_cast<uint2*>(d) = hi;
+                    *reinterpret_cast<uint2*>(d + SH::TILE) = lo;
+                }
+                if (lane == 0) {
+                    float* sc = scales + ((t % (2 * NB)) * 3 + (isv ? 1 : 0)) * SH::GROUPS + w;
+                    sc[0] = isv ? (float)-a : pow2(-a);
+                    if (isv) sc[SH::GROUPS] = f;
+                }
+                due = isv ? &v_full[st] : &k_full[t % (2 * NB)];
+                if (h & 1) {  // K of tile (h + 3) / 2 went out
+                    idx_v = idx_m, idx_m = idx_k;
+                    idx_k = row_of((h + 5) / 2, page);
+                    page = fetch((h + 7) / 2);
+                }
+            }
+            if (due) hand_over(due);
+        } else {
+            // 4 copies of K and 4 of V a tile, straight to their place, AHEAD tiles early
+            auto place = [&](int t, int isv, int i) -> uint8_t* {
+                const int trow = w * SH::RPW + i * SH::RPC + sub;
+                return tiles + ((t % NB) * 2 + isv) * SH::HALF + (trow >> 3) * SH::RS + (trow & 7) * 16 + col * SH::CS;
+            };
+            int page = fetch(0);
+            auto issue = [&](int t) -> bool {
+                bool good = true;
+                if (t < nt) {
+                    const int idx = row_of(t, page);
+                    page = fetch(t + 1);
+                    if (t == SH::QTILE) good = wait_warp(q_full, 0);
+                    if (good && t >= NB) good = wait_warp(&k_empty[t % NB], t / NB - 1);
+                    if (good) {
+#pragma unroll
+                        for (int i = 0; i < NCK; ++i) copy(smem_u32(place(t, 0, i)), kb, idx, i);
+                    }
+                    cp_async_commit();
+                    if (good && t >= NB) good = wait_warp(&v_empty[t % NB], t / NB - 1);
+                    if (good) {
+#pragma unroll
+                        for (int i = 0; i < NCK; ++i) copy(smem_u32(place(t, 1, i)), vb, idx, i);
+                    }
+                    cp_async_commit();
+                } else {
+                    cp_async_commit();
+                    cp_async_commit();
+                }
+                return good;
+            };
+            // what a lane copied, in bf16 -> f16 times a power of two; non-finite values of V out
+            auto fix = [&](int t, int isv) {
+                if (TYPE == AF_KV_F16 && !isv) return;
+                uint4 x[NCK];
+                uint32_t* e = &x[0].x;
+#pragma unroll
+                for (int i = 0; i < NCK; ++i) x[i] = *reinterpret_cast<const uint4*>(place(t, isv, i));
+                if (TYPE == AF_KV_F16) {
+                    __half2 z = __float2half2_rn(0.f);  // x·0 is 0 for what is finite, NaN otherwise
+#pragma unroll
+                    for (int i = 0; i < 4 * NCK; ++i)
+                        z = __hfma2(*reinterpret_cast<const __half2*>(&e[i]), __float2half2_rn(0.f), z);
+                    const uint32_t zz = *reinterpret_cast<const uint32_t*>(&z) & 0x7fff7fffu;
+                    if (__any_sync(0xffffffffu, zz != 0)) {
+#pragma unroll
+                        for (int i = 0; i < 4 * NCK; ++i) {
+                            if ((e[i] & 0x7c00u) == 0x7c00u) e[i] &= 0xffff0000u;
+                            if ((e[i] & 0x7c000000u) == 0x7c000000u) e[i] &= 0x0000ffffu;
                         }
-                        const int a = scale_of(mx, isv ? 60 : 100);
-                        const float f = pow2(a);
-                        uint2 hi, lo;
-                        split2(__uint_as_float(x.x) * f, __uint_as_float(x.y) * f, hi.x, lo.x);
-                        split2(__uint_as_float(x.z) * f, __uint_as_float(x.w) * f, hi.y, lo.y);
-                        dst += (col >> 1) * SH::CS + (col & 1) * 8;
-                        *reinterpret_cast<uint2*>(dst) = hi;
-                        *reinterpret_cast<uint2*>(dst + SH::TILE) = lo;
-                        if (col == 0) {
-                            if (isv) {
-                                sc[T + trow] = (float)-a;
-                                sc[2 * T + trow] = f;
-                            } else {
-                                sc[trow] = pow2(-a);
-                            }
+#pragma unroll
+                        for (int i = 0; i < NCK; ++i) *reinterpret_cast<uint4*>(place(t, isv, i)) = x[i];
+                        if (lane == 0) atomicOr(&bad[(t >> bs) >> 5], 1u << ((t >> bs) & 31));
+                    }
+                } else {
+                    uint32_t b = 0;
+#pragma unroll
+                    for (int i = 0; i < 4 * NCK; ++i) b = max(b, max((e[i] << 16) & 0x7fff0000u, e[i] & 0x7fff0000u));
+                    uint32_t mx = __reduce_max_sync(0xffffffffu, b);
+                    if (isv && mx >= 0x7f800000u) {
+                        b = 0;
+#pragma unroll
+                        for (int i = 0; i < 4 * NCK; ++i) {
+                            if (((e[i] << 16) & 0x7fff0000u) >= 0x7f800000u) e[i] &= 0xffff0000u;
+                            if ((e[i] & 0x7fff0000u) >= 0x7f800000u) e[i] &= 0x0000ffffu;
+                            b = max(b, max((e[i] << 16) & 0x7fff0000u, e[i] & 0x7fff0000u));
                         }
-                    } else if (TYPE == AF_KV_BF16) {
-                        uint32_t* e = &x.x;
-                        uint32_t b = 0;
+                        mx = __reduce_max_sync(0xffffffffu, b);
+                        if (lane == 0) atomicOr(&bad[(t >> bs) >> 5], 1u << ((t >> bs) & 31));
+                    }
+                    const int a = scale_of(mx, isv ? 60 : 100);
+                    const float f = pow2(a);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) b = max(b, max((e[i] << 16) & 0x7fff0000u, e[i] & 0x7fff0000u));
-                        uint32_t mx = __reduce_max_sync(0xffffffffu, b);
-                        if (isv && mx >= 0x7f800000u) {
-                            b = 0;
+                    for (int i = 0; i < 4 * NCK; ++i)
+                        e[i] = pack2(__uint_as_float(e[i] << 16) * f, __uint_as_float(e[i] & 0xffff0000u) * f);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                if (((e[i] << 16) & 0x7fff0000u) >= 0x7f800000u) e[i] &= 0xffff0000u;
-                                if ((e[i] & 0x7fff0000u) >= 0x7f800000u) e[i] &= 0x0000ffffu;
-                                b = max(b, max((e[i] << 16) & 0x7fff0000u, e[i] & 0x7fff0000u));
-                            }
-                            mx = __reduce_max_sync(0xffffffffu, b);
-                            if (lane == 0) atomicOr(&bad[(t >> bs) >> 5], 1u << ((t >> bs) & 31));
-                        }
-                        const int a = scale_of(mx, isv ? 60 : 100);
-                        const float f = pow2(a);
-                        uint4 h;
-                        uint32_t* o = &h.x;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            o[i] = pack2(__uint_as_float(e[i] << 16) * f, __uint_as_float(e[i] & 0xffff0000u) * f);
-                        *reinterpret_cast<uint4*>(dst + col * SH::CS) = h;
-                        if (col == 0) {
-                            if (isv) {
-                                sc[T + trow] = (float)-a;
-                                sc[2 * T + trow] = f;
-                            } else {
-                                sc[trow] = pow2(-a);
-                            }
-                        }
-                    } else {
-                        if (isv) {
-                            uint32_t* e = &x.x;
-                            __half2 z = __float2half2_rn(0.f);  // x·0 is 0 for what is finite, NaN otherwise
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                z = __hfma2(*reinterpret_cast<const __half2*>(&e[i]), __float2half2_rn(0.f), z);
-                            const uint32_t zz = *reinterpret_cast<const uint32_t*>(&z) & 0x7fff7fffu;
-                            if (__any_sync(0xffffffffu, zz != 0)) {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    if ((e[i] & 0x7c00u) == 0x7c00u) e[i] &= 0xffff0000u;
-                                    if ((e[i] & 0x7c000000u) == 0x7c000000u) e[i] &= 0x0000ffffu;
-                                }
-                                if (lane == 0) atomicOr(&bad[(t >> bs) >> 5], 1u << ((t >> bs) & 31));
-                            }
-                        }
-                        *reinterpret_cast<uint4*>(dst + col * SH::CS) = x;
+                    for (int i = 0; i < NCK; ++i) *reinterpret_cast<uint4*>(place(t, isv, i)) = x[i];
+                    if (lane == 0) {
+                        float* sc = scales + ((t % (2 * NB)) * 3 + isv) * SH::GROUPS + w;
+                        sc[0] = isv ? (float)-a : pow2(-a);
+                        if (isv) sc[SH::GROUPS] = f;
                     }
                 }
-                idx = lookup(t + RING + 1);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&full[st]);
+            };
+#pragma unroll 1
+            for (int t = 0; ok && t < SH::AHEAD; ++t) ok = issue(t);
+#pragma unroll 1
+            for (int t = 0; ok && t < nt; ++t) {
+                cp_async_wait<2 * SH::AHEAD - 1>();
+                fix(t, 0);
+                hand_over(&k_full[t % (2 * NB)]);
+                cp_async_wait<2 * SH::AHEAD - 2>();
+                fix(t, 1);
+                hand_over(&v_full[t % NB]);
+                ok = issue(t + SH::AHEAD);
             }
         }
         if (!ok) *flag = 1;
+        cp_async_wait<0>();
     } else {
         // ------------------------------------------------------- products
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp == 12 && lane == 0 && nt > 0) {
+        if (warp == 16 && nt > 0) {
             constexpr uint32_t base = (1u << 4) | ((uint32_t)(kMmaRows >> 4) << 24);  // f32 accumulators, f16 operands
             constexpr uint32_t ids = base | ((uint32_t)(T >> 3) << 17);
             constexpr uint32_t ido = base | ((uint32_t)(HD >> 3) << 17) | (1u << 16);  // B MN-major
-            auto scores = [&](int t) {
-                const uint32_t k0 = smem_u32(tiles + (t % NB) * SH::STAGE), d = tmem + SH::S0 + (t & 1) * T;
-                bool acc = false;
-                auto pass = [&](uint32_t q, uint32_t k) {
+            const uint32_t leader = elect_one();
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const int n_tiles = __shfl_sync(0xffffffffu, nt, 0);
+            const uint64_t kd = tile_desc(smem_u32(tiles), SH::CS, SH::RS), vd = tile_desc(smem_u32(tiles) + SH::HALF, SH::RS, SH::CS);
+            auto scores = [&](int st, int sl) {
+                const uint64_t k = kd + (uint32_t)(st * (2 * SH::HALF >> 4));
+                const uint32_t d = tm + SH::S0 + sl * T;
 #pragma unroll
-                    for (int ks = 0; ks < HD / 16; ++ks) {
-                        tc_mma_ts(d, tmem + q + 8 * ks, tile_desc(k + 2 * ks * SH::CS, SH::CS, SH::RS), ids, acc);
-                        acc = true;
-                    }
-                };
-                pass(SH::QL, k0);
-                if (SH::TERMS == 2) pass(SH::QH, k0 + SH::TILE);
-                pass(SH::QH, k0);
-                tc_commit(&s_full[t & 1]);
-            };
-            auto values = [&](int t) {
-                const uint32_t v0 = smem_u32(tiles + (t % NB) * SH::STAGE + SH::TERMS * SH::TILE);
-                const uint32_t w = tmem + SH::S0 + (t & 1) * T, d = tmem + SH::O0 + (t & 1) * HD;
-                bool acc = false;
-                auto pass = [&](uint32_t a, uint32_t v) {
+                for (int ks = 0; ks < HD / 16; ++ks) tc_mma_ts(leader, d, tm + SH::QL + 8 * ks, k + (2 * ks * SH::CS >> 4), ids, ks > 0);
+                if (SH::TERMS == 2) {
 #pragma unroll
-                    for (int ks = 0; ks < T / 16; ++ks) {
-                        tc_mma_ts(d, a + 8 * ks, tile_desc(v + 2 * ks * SH::RS, SH::RS, SH::CS), ido, acc);
-                        acc = true;
-                    }
-                };
-                pass(w + T / 2, v0);
-                if (SH::TERMS == 2) pass(w, v0 + SH::TILE);
-                pass(w, v0);
-                tc_commit(&empty[t % NB]);
-                tc_commit(&o_full[t & 1]);
+                    for (int ks = 0; ks < HD / 16; ++ks)
+                        tc_mma_ts(leader, d, tm + SH::QH + 8 * ks, k + ((SH::TILE + 2 * ks * SH::CS) >> 4), ids, true);
+                }
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ++ks) tc_mma_ts(leader, d, tm + SH::QH + 8 * ks, k + (2 * ks * SH::CS >> 4), ids, true);
+                tc_commit(leader, &s_full[sl]);
+                tc_commit(leader, &k_empty[st]);
             };
-            bool ok = wait(q_full, 0u, flag) && wait(&full[0], 0u, flag);
+            auto values = [&](int st, int sl) {
+                const uint64_t v = vd + (uint32_t)(st * (2 * SH::HALF >> 4));
+                const uint32_t w = tm + SH::S0 + sl * T, d = tm + SH::O0;
+#pragma unroll
+                for (int ks = 0; ks < T / 16; ++ks) tc_mma_ts(leader, d, w + 8 + 16 * ks, v + (2 * ks * SH::RS >> 4), ido, ks > 0);
+                if (SH::TERMS == 2) {
+#pragma unroll
+                    for (int ks = 0; ks < T / 16; ++ks)
+                        tc_mma_ts(leader, d, w + 16 * ks, v + ((SH::TILE + 2 * ks * SH::RS) >> 4), ido, true);
+                }
+#pragma unroll
+                for (int ks = 0; ks < T / 16; ++ks) tc_mma_ts(leader, d, w + 16 * ks, v + (2 * ks * SH::RS >> 4), ido, true);
+                tc_commit(leader, o_full);
+                tc_commit(leader, &v_empty[st]);
+            };
+            bool ok = wait_warp(q_full, 0) && wait_warp(&k_full[0], 0);
             if (ok) {
                 tc_fence_after();
-                scores(0);
+                scores(0, 0);
             }
-            for (int t = 0; ok && t < nt; ++t) {
-                if (t + 1 < nt) {  // the next tile's scores, over the weights of the tile before this one
-                    ok = wait(&full[(t + 1) % NB], (uint32_t)((t + 1) / NB) & 1u, flag) &&
-                         (t < 1 || wait(&o_full[(t + 1) & 1], (uint32_t)((t - 1) >> 1) & 1u, flag));
+            for (int t = 0; ok && t < n_tiles; ++t) {
+                if (t + 1 < n_tiles) {  // the next tile's scores, over the weights of t - 2
+                    // (whose P·V is over: that of t - 1 waited until it was taken)
+                    ok = wait_warp(&k_full[(t + 1) % (2 * NB)], (t + 1) / (2 * NB));
                     if (!ok) break;
                     tc_fence_after();
-                    scores(t + 1);
+                    scores((t + 1) % NB, (t + 1) % NS);
                 }
-                ok = wait(&p_full[t & 1], (uint32_t)(t >> 1) & 1u, flag) &&
-                     (t < 2 || wait(&o_free[t & 1], (uint32_t)((t >> 1) - 1) & 1u, flag));
+                ok = wait_warp(&p_full[t % NS], t / NS) && wait_warp(&v_full[t % NB], t / NB) && (t < 1 || wait_warp(o_free, t - 1));
                 if (!ok) break;
                 tc_fence_after();
-                values(t);
+                values(t % NB, t % NS);
             }
             if (!ok) *flag = 1;
             // whatever was issued ends before tensor memory is given back
-            tc_commit(done);
-            wait(done, 0u, nullptr);
+            tc_commit(leader, done);
+            __syncwarp();
+            mbar_wait_at(done, 0u, p.b.err, nullptr);
         }
         __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
 }
