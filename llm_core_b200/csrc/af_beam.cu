@@ -3,19 +3,24 @@
 //     score(b, t) = scores[b] + x[b][t] - log Σ_t' exp x[b][t'],
 // in one pass over the logits.
 //
-//  * Chunk kernel: a block holds up to 8192 logits of a row in registers
-//    (32 a thread): their maximum, Σ exp(x - max), and their K = n_out largest
-//    in order.  Within a beam scores are ordered as logits, so the K best of a
-//    chunk are its K largest logits, ties to the lower token: 64-bit keys
-//    (ordered value, ~token) are distinct.  The K-th largest of the threads'
-//    own largest keys is a threshold with at least K keys at or above it and
-//    at most K·32 (those of K threads), so what passes it fits a fixed buffer
-//    whatever the logits (all equal, say), and its order is found by counting.
-//  * Merge kernel, a block per sequence: the chunks' sums to one base
+//  * Segment kernel: a block streams a segment of a row, 2048 logits a step
+//    (two 16-byte loads a thread, the next step's in flight): the running
+//    maximum, Σ exp(x - max), and a buffer of what may be among the segment's
+//    K = n_out largest.  Within a beam scores are ordered as logits, so the K
+//    best of a segment are its K largest, ties to the lower token: 64-bit
+//    keys (ordered value, ~token) are distinct.  The first step's threshold:
+//    each warp sorts its threads' largest values, and the smallest of the
+//    warps' ceil(K/8)-th has at least K values at or above it.  Later logits
+//    have higher tokens, so one that only equals the threshold has K better
+//    ones in front of it and is passed over: what enters the buffer is rare,
+//    and where it is not (rising or equal logits) the buffer is cut back to its
+//    K best, which raises the threshold.
+//  * Merge kernel, a block per sequence: the segments' sums to one base
 //    scores[b] - log Σ per beam in 64 bits, so that scores of different beams
-//    compare as their definition does, and the K best of the chunk lists: the
+//    compare as their definition does, and the K best of the segment lists: the
 //    K-th best list head is again a threshold, which at most K lists of K pass.
 //  * A beam that is dead before the call (score -inf or NaN) is not read.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -29,8 +34,9 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kBeamThreads = 256;
-constexpr int kBeamPer = 32;                            // logits of a thread
-constexpr int kBeamChunk = kBeamThreads * kBeamPer;     // 8192
+constexpr int kBeamStep = kBeamThreads * 8;             // logits of a step
+constexpr int kBeamBuffer = 2 * kBeamStep;              // keys kept: cut back when more than a step's are there
+constexpr int kBeamChunk = 8192;                        // shortest segment
 constexpr int kBeamMaxK = 64;
 constexpr int kBeamLists = 1024;                        // chunk lists of a sequence
 constexpr int kMergeThreads = 1024;
@@ -38,10 +44,10 @@ constexpr int kMergeThreads = 1024;
 struct BeamParams {
     const float *logits, *scores;
     long long stride;
-    int n_seq, beams, vocab, K, chunks, vec;
+    int n_seq, beams, vocab, K, chunks, seg, vec;  // chunks: segments of a row, of seg logits
     float* out_score;
     int *out_beam, *out_token;
-    u64* keys;      // [rows][chunks][K] the chunks' largest, in order; 0: none
+    u64* keys;      // [rows][chunks][K] the segments' largest, in order; 0: none
     double* sums;   // [rows][chunks]
     float* tops;    // [rows][chunks]
 };
@@ -56,95 +62,165 @@ __device__ __forceinline__ double warp_sum_d(double v) {
 
 __device__ __forceinline__ bool dead_score(float s) { return !(s > -INFINITY); }  // -inf and NaN
 
-__global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(BeamParams p) {
-    constexpr int W = kBeamThreads / 32;
-    __shared__ u64 tmax[kBeamThreads];
-    __shared__ u64 cand[kBeamMaxK * kBeamPer];
-    __shared__ float wtop[W];
-    __shared__ double wsum[W];
-    __shared__ u64 s_thr;
-    __shared__ int s_cnt;
-    const int chunk = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (dead_score(p.scores[row])) return;
-    const int t0 = chunk * kBeamChunk, n = min(kBeamChunk, p.vocab - t0);
-    const float* x = p.logits + (long long)row * p.stride + t0;
-    float v[kBeamPer];
-    // thread's element e is token t0 + 4*(tid + 256*(e/4)) + e%4 (16-byte loads where the rows allow them)
+// This lane's value of the warp's 32 in descending order.
+template <typename T>
+__device__ __forceinline__ T warp_sort_desc(T v, int lane) {
 #pragma unroll
-    for (int e = 0; e < kBeamPer; e += 4) {
-        const int i = 4 * (tid + kBeamThreads * (e / 4));
-        if (p.vec && i + 4 <= n) {
-            const float4 f = *reinterpret_cast<const float4*>(x + i);
-            v[e] = f.x;
-            v[e + 1] = f.y;
-            v[e + 2] = f.z;
-            v[e + 3] = f.w;
+    for (int k = 2; k <= 32; k <<= 1) {
+#pragma unroll
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            const T o = __shfl_xor_sync(0xffffffffu, v, j);
+            const bool up = (lane & k) != 0, low = (lane & j) == 0;  // ascending run; lower partner
+            v = (low != up) == (v > o) ? v : o;
+        }
+    }
+    return v;
+}
+
+struct BeamShared {
+    u64 key[kBeamBuffer];
+    u64 out[kBeamMaxK];
+    u64 wkey[kBeamThreads / 32];
+    float wval[kBeamThreads / 32];
+    double wsum[kBeamThreads / 32];
+    int count, kept;
+};
+
+// The buffer's K best keys, in order, to its front (fewer where it has fewer).
+__device__ void beam_cut(BeamShared& sh, int K) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = sh.count;
+    u64 best = 0;
+    for (int i = tid; i < n; i += kBeamThreads) best = max(best, sh.key[i]);
+    best = warp_sort_desc(best, lane);
+    if (lane == (K + 7) / 8 - 1) sh.wkey[warp] = best;  // 0 where the warp has fewer: everything passes
+    if (tid == 0) sh.kept = 0;
+    __syncthreads();
+    u64 thr = sh.wkey[0];
+#pragma unroll
+    for (int w = 1; w < kBeamThreads / 32; ++w) thr = min(thr, sh.wkey[w]);
+    // what passes, to the front (read before it is written over)
+    u64 mine[kBeamBuffer / kBeamThreads];
+    int at[kBeamBuffer / kBeamThreads];
+#pragma unroll
+    for (int e = 0; e < kBeamBuffer / kBeamThreads; ++e) {
+        const int i = tid + e * kBeamThreads;
+        at[e] = -1;
+        if (i < n) {
+            mine[e] = sh.key[i];
+            if (mine[e] >= thr) at[e] = atomicAdd(&sh.kept, 1);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kBeamBuffer / kBeamThreads; ++e)
+        if (at[e] >= 0) sh.key[at[e]] = mine[e];
+    __syncthreads();
+    const int kept = sh.kept;
+    for (int c = tid; c < kept; c += kBeamThreads) {
+        const u64 k = sh.key[c];
+        int rank = 0;
+        for (int i = 0; i < kept; ++i) rank += sh.key[i] > k;
+        if (rank < K) sh.out[rank] = k;
+    }
+    __syncthreads();
+    const int have = min(K, kept);
+    if (tid < have) sh.key[tid] = sh.out[tid];
+    if (tid == 0) sh.count = have;
+    __syncthreads();
+}
+
+__global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParams p) {
+    constexpr int W = kBeamThreads / 32;
+    __shared__ BeamShared sh;
+    pdl_launch_dependents();  // the merge kernel may start launching
+    const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (dead_score(p.scores[row])) return;
+    const int lo = blockIdx.x * p.seg, hi = min(lo + p.seg, p.vocab), K = p.K;
+    const float* x = p.logits + (long long)row * p.stride;
+    auto load = [&](int t0, float (&v)[8]) {  // tokens t0 + 4·tid .. +3 and 1024 on
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int t = t0 + h * (kBeamStep / 2) + 4 * tid;
+            if (p.vec && t + 4 <= hi) {
+                const float4 f = __ldcs(reinterpret_cast<const float4*>(x + t));
+                v[4 * h] = f.x, v[4 * h + 1] = f.y, v[4 * h + 2] = f.z, v[4 * h + 3] = f.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[4 * h + j] = t + j < hi ? x[t + j] : -INFINITY;
+            }
+        }
+    };
+    float next[8];
+    load(lo, next);
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    float top = -INFINITY, thr = 0.f;
+    double sum = 0.;
+    constexpr float kLog2e = 1.4426950408889634f;
+    for (int t0 = lo; t0 < hi; t0 += kBeamStep) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = next[j];
+        if (t0 + kBeamStep < hi) load(t0 + kBeamStep, next);
+        float big = v[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) big = fmaxf(big, v[j]);
+        if (big > top) {
+            sum *= (double)exp2f((top - big) * kLog2e);
+            top = big;
+        }
+        // 8 terms in 32 bits, the rest in 64; NaN stays NaN (and -inf - -inf is left out)
+        float part = 0.f;
+        if (top > -INFINITY) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) part += exp2f((v[j] - top) * kLog2e);
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[e + j] = i + j < n ? x[i + j] : -INFINITY;
+            for (int j = 0; j < 8; ++j) part += v[j] != v[j] ? v[j] : 0.f;
+        }
+        sum += (double)part;
+        const bool begin = t0 == lo;
+        if (begin) {  // the threshold
+            const float s = warp_sort_desc(big, lane);
+            if (lane == (K + 7) / 8 - 1) sh.wval[warp] = s;
+            __syncthreads();
+            thr = sh.wval[0];
+#pragma unroll
+            for (int w = 1; w < W; ++w) thr = fminf(thr, sh.wval[w]);
+        }
+        if (begin ? big >= thr : big > thr) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int t = t0 + (j >> 2) * (kBeamStep / 2) + 4 * tid + (j & 3);
+                if (t < hi && (begin ? v[j] >= thr : v[j] > thr)) sh.key[atomicAdd(&sh.count, 1)] = logit_key(v[j], t);
+            }
+        }
+        // at most a step's keys came on top of at most a step's
+        if (__syncthreads_or(tid == 0 && sh.count > kBeamStep)) {
+            beam_cut(sh, K);
+            thr = ordered_to_float((uint32_t)(sh.key[K - 1] >> 32));
+            __syncthreads();
         }
     }
-    float top = -INFINITY;
-    bool nan = false;
-    u64 best = 0;
-#pragma unroll
-    for (int e = 0; e < kBeamPer; ++e) {
-        const int i = 4 * (tid + kBeamThreads * (e / 4)) + (e & 3);
-        nan |= v[e] != v[e];
-        top = fmaxf(top, v[e]);
-        if (i < n) best = max(best, logit_key(v[e], t0 + i));
-    }
-    if (tid == 0) {
-        s_cnt = 0;
-        s_thr = 0;
-    }
-    tmax[tid] = best;
-    top = warp_max(top);
-    if (lane == 0) wtop[warp] = top;
+    beam_cut(sh, K);
+    const long long list = (long long)row * p.chunks + blockIdx.x;
+    const int have = sh.count;
+    if (tid < K) p.keys[list * K + tid] = tid < have ? sh.key[tid] : 0;
+    // one maximum and one sum
+    const float wtop = warp_max(top);
+    if (lane == 0) sh.wval[warp] = wtop;
     __syncthreads();
-    top = wtop[0];
+    float all = sh.wval[0];
 #pragma unroll
-    for (int w = 1; w < W; ++w) top = fmaxf(top, wtop[w]);
-    // Σ exp(x - top): 32 terms a thread in 32 bits, the rest in 64
-    float part = 0.f;
-    if (top > -INFINITY) {
-#pragma unroll
-        for (int e = 0; e < kBeamPer; ++e) part += expf(v[e] - top);
-    }
-    double sum = warp_sum_d(nan ? (double)NAN : (double)part);
-    if (lane == 0) wsum[warp] = sum;
-    // the K-th largest of the threads' largest
-    const int K = min(p.K, n);
-    if (best) {
-        int rank = 0;
-        for (int i = 0; i < kBeamThreads; ++i) rank += tmax[i] > best;
-        if (rank == K - 1) s_thr = best;  // fewer than K threads with logits: 0, everything passes
-    }
+    for (int w = 1; w < W; ++w) all = fmaxf(all, sh.wval[w]);
+    sum = warp_sum_d(top == all ? sum : sum * exp((double)top - (double)all));  // 0·exp(-inf) = 0
+    if (lane == 0) sh.wsum[warp] = sum;
     __syncthreads();
-    const u64 thr = s_thr;
-#pragma unroll
-    for (int e = 0; e < kBeamPer; ++e) {
-        const int i = 4 * (tid + kBeamThreads * (e / 4)) + (e & 3);
-        if (i < n) {
-            const u64 k = logit_key(v[e], t0 + i);
-            if (k >= thr) cand[atomicAdd(&s_cnt, 1)] = k;
-        }
-    }
-    __syncthreads();
-    const int cnt = s_cnt;
-    const long long list = (long long)row * p.chunks + chunk;
-    for (int c = tid; c < cnt; c += kBeamThreads) {
-        const u64 k = cand[c];
-        int rank = 0;
-        for (int i = 0; i < cnt; ++i) rank += cand[i] > k;
-        if (rank < K) p.keys[list * p.K + rank] = k;
-    }
-    for (int c = K + tid; c < p.K; c += kBeamThreads) p.keys[list * p.K + c] = 0;
     if (tid == 0) {
         sum = 0.;
-        for (int w = 0; w < W; ++w) sum += wsum[w];
+        for (int w = 0; w < W; ++w) sum += sh.wsum[w];
         p.sums[list] = sum;
-        p.tops[list] = top;
+        p.tops[list] = all;
     }
 }
 
@@ -176,6 +252,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamParams p)
     int* ctl = reinterpret_cast<int*>(cf + kBeamMaxK * kBeamMaxK);  // [0] candidates
     const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row0 = seq * p.beams, K = p.K;
+    pdl_wait();
     // a beam's base: scores[b] - log Σ exp, -inf for a dead one
     for (int b = warp; b < p.beams; b += kMergeThreads / 32) {
         const float s = p.scores[row0 + b];
@@ -272,8 +349,15 @@ std::string beam_wrong(const af_beam_select_args& a) {
     return "";
 }
 
+// Segments of a row: enough blocks to fill the SMs four times, none below kBeamChunk logits.
+int beam_segments(const af_beam_select_args& a) {
+    const int most = (a.vocab + kBeamChunk - 1) / kBeamChunk;
+    const long long rows = std::max(1ll, (long long)a.n_seq * a.n_beams);
+    return (int)std::min((long long)most, std::max(1ll, 4 * 148 / rows));
+}
+
 size_t beam_ws(const af_beam_select_args& a) {
-    const size_t lists = (size_t)a.n_seq * a.n_beams * ((a.vocab + kBeamChunk - 1) / kBeamChunk);
+    const size_t lists = (size_t)a.n_seq * a.n_beams * beam_segments(a);
     return lists * ((size_t)a.n_out * 8 + 16);
 }
 
@@ -302,7 +386,9 @@ extern "C" cudaError_t af_beam_select_f32(const af_beam_select_args* a, cudaStre
     p.beams = a->n_beams;
     p.vocab = a->vocab;
     p.K = a->n_out;
-    p.chunks = (a->vocab + kBeamChunk - 1) / kBeamChunk;
+    p.chunks = beam_segments(*a);
+    p.seg = ((a->vocab + p.chunks - 1) / p.chunks + kBeamStep - 1) / kBeamStep * kBeamStep;
+    p.chunks = (a->vocab + p.seg - 1) / p.seg;
     p.vec = !(reinterpret_cast<uintptr_t>(a->logits) & 15) && p.stride % 4 == 0;
     p.out_score = a->out_score;
     p.out_beam = a->out_beam;
@@ -311,9 +397,18 @@ extern "C" cudaError_t af_beam_select_f32(const af_beam_select_args* a, cudaStre
     p.keys = static_cast<u64*>(a->ws);
     p.sums = reinterpret_cast<double*>(p.keys + lists * p.K);
     p.tops = reinterpret_cast<float*>(p.sums + lists);
-    beam_chunk_kernel<<<dim3(p.chunks, p.n_seq * p.beams), kBeamThreads, 0, stream>>>(p);
+    beam_segment_kernel<<<dim3(p.chunks, p.n_seq * p.beams), kBeamThreads, 0, stream>>>(p);
     AF_CUDA_TRY(cudaGetLastError());
     AF_CUDA_TRY(cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMergeSmem));
-    beam_merge_kernel<<<p.n_seq, kMergeThreads, kMergeSmem, stream>>>(p);
-    return cudaGetLastError();
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.n_seq);
+    cfg.blockDim = dim3(kMergeThreads);
+    cfg.dynamicSmemBytes = kMergeSmem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, beam_merge_kernel, p);
 }

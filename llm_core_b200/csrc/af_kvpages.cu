@@ -3,6 +3,7 @@
 // (af_kv_fork), accepted rows moved together (af_kv_compact).
 #include <climits>
 #include <cstdint>
+#include <type_traits>
 
 #include "af_kvpages.cuh"
 #include "af_ops.cuh"
@@ -53,39 +54,131 @@ struct StoreParams {
     float eps;
 };
 
-// One block per row: its warps take the row's query, key and value heads in
-// turn, a lane the pairs (i, i + hd/2) for i = lane, lane + 32, ...
-template <int TYPE>
-__global__ void __launch_bounds__(kStoreThreads) kv_store_kernel(StoreParams p) {
-    using E = KvElem<TYPE>;
-    __shared__ int s_seq, s_node;
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) s_seq = -1;
+// The block's row: its sequence and node, -1 for a row behind the last sequence.
+__device__ __forceinline__ void store_row(const StoreParams& p, int row, int* s_seq, int* s_node) {
+    const int tid = threadIdx.x;
+    if (tid == 0) *s_seq = -1;
     __syncthreads();
     if (p.b.first) {
         for (int s = tid; s < p.b.n_seq; s += kStoreThreads) {
             const int f = p.b.first[s];
             if (f <= row && row < p.b.first[s + 1]) {
-                s_seq = s;
-                s_node = row - f;
+                *s_seq = s;
+                *s_node = row - f;
             }
         }
     } else if (tid == 0 && row / p.b.max_nodes < p.b.n_seq) {
-        s_seq = row / p.b.max_nodes;
-        s_node = row % p.b.max_nodes;
+        *s_seq = row / p.b.max_nodes;
+        *s_node = row % p.b.max_nodes;
     }
     __syncthreads();
-    const int seq = s_seq, node = s_node, hd = p.kv.hd, half = hd / 2;
-    if (seq < 0) return;  // a row behind the last sequence
+}
+
+// Where the row's rotation and cache position are; false (and the error word) where it has none.
+__device__ __forceinline__ bool store_place(const StoreParams& p, int row, int seq, int node, long long& at, long long& slot) {
     const int len = kv_len(p.kv, p.b, seq, 0);
-    if (len < 0) return;
-    const long long at = (long long)len + (p.depth ? p.depth[row] : node);
+    if (len < 0) return false;
+    at = (long long)len + (p.depth ? p.depth[row] : node);
     if (at < 0 || at >= p.n_ctx || node >= p.b.max_nodes) {
-        if (tid == 0) set_err_at(p.b.err, kErrBadArgs);
-        return;
+        if (threadIdx.x == 0) set_err_at(p.b.err, kErrBadArgs);
+        return false;
     }
-    const long long slot = kv_row(p.kv, p.b, seq, len + node);
-    if (slot < 0 && tid == 0) set_err_at(p.b.err, kErrBadArgs);
+    slot = kv_row(p.kv, p.b, seq, len + node);
+    if (slot < 0 && threadIdx.x == 0) set_err_at(p.b.err, kErrBadArgs);
+    return true;
+}
+
+// A block per row, its heads (queries, keys, values) over the warps.  HD 64
+// and 128 with 16-byte rows: a lane holds 4 values, HD/4 lanes a head, the
+// partner of a rotation sits HD/8 lanes away; up to 4 heads a warp are loaded
+// before the first is worked on.  Bound by memory: q, k, v once in, once out.
+template <int TYPE, int HD>
+__global__ void __launch_bounds__(kStoreThreads) kv_store_vec_kernel(StoreParams p) {
+    constexpr int LH = HD / 4, HPW = 32 / LH, W = kStoreThreads / 32, U = 4;
+    __shared__ int s_seq, s_node;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int sub = lane / LH, col = lane % LH, heads = p.H + 2 * p.kv.kv_heads;
+    const long long kvd = (long long)p.kv.kv_heads * HD;
+    auto load = [&](int h) -> float4 {
+        const float* src = h < p.H ? p.q + (long long)row * p.qs + (long long)h * HD
+                           : h < p.H + p.kv.kv_heads ? p.k + (long long)row * p.ks + (long long)h * HD - (long long)p.H * HD
+                                                     : p.v + (long long)row * p.vs + (long long)h * HD - (long long)p.H * HD - kvd;
+        return *reinterpret_cast<const float4*>(src + 4 * col);
+    };
+    float4 x[U];
+    // the first heads' loads do not wait for the row's place
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int h = (u * W + warp) * HPW + sub;
+        x[u] = h < heads ? load(h) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    store_row(p, row, &s_seq, &s_node);
+    if (s_seq < 0) return;
+    long long at, slot;
+    if (!store_place(p, row, s_seq, s_node, at, slot)) return;
+    const float4 c = *reinterpret_cast<const float4*>(p.cos_t + at * (HD / 2) + 4 * (col % (LH / 2)));
+    const float4 sn = *reinterpret_cast<const float4*>(p.sin_t + at * (HD / 2) + 4 * (col % (LH / 2)));
+    const float sign = col < LH / 2 ? -1.f : 1.f;
+    for (int h0 = 0; h0 < heads; h0 += U * W * HPW) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int h = h0 + (u * W + warp) * HPW + sub;
+            if (h0) x[u] = h < heads ? load(h) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int h = h0 + (u * W + warp) * HPW + sub;
+            const bool isq = h < p.H, isv = h >= p.H + p.kv.kv_heads;
+            float4 v = x[u];
+            const float* nw = isv ? nullptr : isq ? p.q_norm : p.k_norm;
+            auto norm = [&]() {  // the heads of a warp may differ in kind: all lanes add up
+                float ss = v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
+#pragma unroll
+                for (int o = 1; o < LH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                if (nw) {
+                    const float sc = 1.f / sqrtf(ss / (float)HD + p.eps);
+                    const float4 w = *reinterpret_cast<const float4*>(nw + 4 * col);
+                    v.x = w.x * (v.x * sc), v.y = w.y * (v.y * sc), v.z = w.z * (v.z * sc), v.w = w.w * (v.w * sc);
+                }
+            };
+            if (p.order == 1) norm();
+            float4 o;
+            o.x = __shfl_xor_sync(0xffffffffu, v.x, LH / 2), o.y = __shfl_xor_sync(0xffffffffu, v.y, LH / 2);
+            o.z = __shfl_xor_sync(0xffffffffu, v.z, LH / 2), o.w = __shfl_xor_sync(0xffffffffu, v.w, LH / 2);
+            if (!isv) {  // x0·cos - x1·sin in the first half, x0·sin + x1·cos in the second
+                v.x = fmaf(v.x, c.x, sign * (o.x * sn.x)), v.y = fmaf(v.y, c.y, sign * (o.y * sn.y));
+                v.z = fmaf(v.z, c.z, sign * (o.z * sn.z)), v.w = fmaf(v.w, c.w, sign * (o.w * sn.w));
+            }
+            if (p.order == 2) norm();
+            if (h >= heads) continue;
+            if (isq) {
+                *reinterpret_cast<float4*>(p.q_out + (long long)row * p.os + (long long)h * HD + 4 * col) = v;
+            } else if (slot >= 0) {
+                const int kvh = isv ? h - p.H - p.kv.kv_heads : h - p.H;
+                uint8_t* dst = (isv ? p.kv.v : p.kv.k) + (long long)p.layer * p.kv.layer_bytes + slot;
+                if (TYPE == AF_KV_F32) {
+                    reinterpret_cast<float4*>(dst)[kvh * LH + col] = v;
+                } else {
+                    using E = KvElem<TYPE>;
+                    typename E::T r[4] = {E::round(v.x), E::round(v.y), E::round(v.z), E::round(v.w)};
+                    reinterpret_cast<uint2*>(dst)[kvh * LH + col] = *reinterpret_cast<const uint2*>(r);
+                }
+            }
+        }
+    }
+}
+
+// Any head size and alignment: a warp per head, a lane the pairs (i, i + hd/2) for i = lane, lane + 32, ...
+template <int TYPE>
+__global__ void __launch_bounds__(kStoreThreads) kv_store_kernel(StoreParams p) {
+    using E = KvElem<TYPE>;
+    __shared__ int s_seq, s_node;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    store_row(p, row, &s_seq, &s_node);
+    if (s_seq < 0) return;
+    long long at, slot;
+    if (!store_place(p, row, s_seq, s_node, at, slot)) return;
+    const int hd = p.kv.hd, half = hd / 2;
     const float* c = p.cos_t + at * half;
     const float* sn = p.sin_t + at * half;
     for (int h = warp; h < p.H + 2 * p.kv.kv_heads; h += kStoreThreads / 32) {
@@ -214,6 +307,7 @@ __global__ void __launch_bounds__(kForkThreads) kv_fork_kernel(ForkParams p) {
     __shared__ int wsum[32];
     __shared__ int s_total, s_found;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_launch_dependents();  // the copies may start launching
     for (int j = tid; j < p.in.n_seq; j += kForkThreads) eldest[j] = INT_MAX;
     __syncthreads();
     for (int i = tid; i < p.n_out; i += kForkThreads) {
@@ -340,66 +434,96 @@ __global__ void __launch_bounds__(kForkThreads) kv_fork_kernel(ForkParams p) {
 
 constexpr int kCopyThreads = 256;
 
-// Block (i, layer, K or V): the rows of output i's partly filled page.
+// Block (i, layer, K or V): the rows of output i's partly filled page, one
+// contiguous range.  Bound by memory; 4 loads of 16 bytes a thread in flight.
 __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(KvView kv, const int4* copies) {
+    pdl_wait();
     const int4 c = copies[blockIdx.x];
     if (c.z <= 0) return;
     uint8_t* pool = (blockIdx.z ? kv.v : kv.k) + (long long)blockIdx.y * kv.layer_bytes;
     const uint4* src = reinterpret_cast<const uint4*>(pool + ((long long)c.x << kv.ps_shift) * kv.row_bytes);
     uint4* dst = reinterpret_cast<uint4*>(pool + ((long long)c.y << kv.ps_shift) * kv.row_bytes);
     const long long n = (long long)c.z * kv.row_bytes / 16;
-    for (long long i = threadIdx.x; i < n; i += kCopyThreads) dst[i] = src[i];
+    for (long long i = threadIdx.x; i < n; i += 4 * kCopyThreads) {
+        uint4 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i + j * kCopyThreads < n) x[j] = __ldcs(src + i + j * kCopyThreads);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i + j * kCopyThreads < n) dst[i + j * kCopyThreads] = x[j];
+    }
 }
 
 // ----------------------------------------------------------------- compact
 
 constexpr int kCompactThreads = 128;
+constexpr int kCompactVec = 2;    // 16-byte columns of a thread
+constexpr int kCompactRows = 8;   // rows read before the first is written
+constexpr int kCompactPath = 128; // of a path at a time
 
-// Block (columns, layer and K or V, sequence): a thread moves 16 bytes of
-// every row of the path, in path order.  A row's source is never in front of
-// its destination and destinations rise, so a row is read before it is
-// written over: dst i = len + i <= len + path[i'] for every i' >= i.
-__global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(KvView kv, KvBatch b, const int* path,
-                                                                     const int* n_path, int max_path, int* len_out,
-                                                                     const int* len_in) {
-    const int s = blockIdx.z, layer = blockIdx.y >> 1, tid = threadIdx.x;
-    const int col = blockIdx.x * kCompactThreads + tid;
-    const int n = n_path[s];
-    const int* pa = path + (long long)s * max_path;
-    const int len = len_in[s];
+// A sequence's path, checked by the whole block.
+__device__ __forceinline__ bool path_bad(const KvView& kv, const KvBatch& b, const int* pa, int s, int n, int max_path, int len) {
     bool bad = len < 0 || n < 0 || n > max_path;
-    for (int i = 0; i < n && !bad; ++i) {
+    for (int i = threadIdx.x; i < n && !bad; i += blockDim.x) {
         const int x = pa[i];
         bad = x < 0 || (i && x <= pa[i - 1]) || (long long)len + x >= ((long long)b.max_blocks << kv.ps_shift) ||
               kv_row(kv, b, s, len + x) < 0 || kv_row(kv, b, s, len + i) < 0;
     }
-    if (bad) {
-        if (tid == 0) set_err_at(b.err, kErrBadArgs);
-        return;
+    return __syncthreads_or(bad);
+}
+
+// Block (columns, layer and K or V, sequence): a thread moves its columns of
+// every row of the path, in path order.  A row's source is never in front of
+// its destination and destinations rise, so a row is read before it is
+// written over: dst i = len + i <= len + path[i'] for every i' >= i.  Bound by
+// memory; each block first turns the path into row offsets, side by side.
+__global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(KvView kv, KvBatch b, const int* path,
+                                                                     const int* n_path, int max_path, int* len_out) {
+    __shared__ long long from[kCompactPath], to[kCompactPath];
+    const int s = blockIdx.z, layer = blockIdx.y >> 1, tid = threadIdx.x;
+    const int* pa = path + (long long)s * max_path;
+    const int n = n_path[s], len = b.len[s];
+    const bool bad = path_bad(kv, b, pa, s, n, max_path, len);
+    if (tid == 0 && blockIdx.x == 0 && blockIdx.y == 0) {
+        if (bad) set_err_at(b.err, kErrBadArgs);
+        if (len_out) len_out[s] = bad ? len : len + n;
     }
-    if (col * 16 >= kv.row_bytes) return;
-    uint8_t* pool = ((blockIdx.y & 1) ? kv.v : kv.k) + (long long)layer * kv.layer_bytes + (long long)col * 16;
-    for (int i = 0; i < n; ++i) {
-        if (pa[i] == i) continue;
-        const uint4 x = *reinterpret_cast<const uint4*>(pool + kv_row(kv, b, s, len + pa[i]));
-        *reinterpret_cast<uint4*>(pool + kv_row(kv, b, s, len + i)) = x;
+    if (bad) return;
+    const int col = (blockIdx.x * kCompactThreads + tid) * 16, step = gridDim.x * kCompactThreads * 16;
+    uint8_t* pool = ((blockIdx.y & 1) ? kv.v : kv.k) + (long long)layer * kv.layer_bytes;
+    for (int i0 = 0; i0 < n; i0 += kCompactPath) {
+        const int m = min(kCompactPath, n - i0);
+        __syncthreads();
+        if (tid < m) {
+            from[tid] = pa[i0 + tid] == i0 + tid ? -1 : kv_row(kv, b, s, len + pa[i0 + tid]);  // -1: in its place
+            to[tid] = kv_row(kv, b, s, len + i0 + tid);
+        }
+        __syncthreads();
+        for (int j0 = 0; j0 < m; j0 += kCompactRows) {
+            uint4 x[kCompactRows][kCompactVec];
+#pragma unroll
+            for (int j = 0; j < kCompactRows; ++j)
+#pragma unroll
+                for (int v = 0; v < kCompactVec; ++v)
+                    if (j0 + j < m && from[j0 + j] >= 0 && col + v * step < kv.row_bytes)
+                        x[j][v] = *reinterpret_cast<const uint4*>(pool + from[j0 + j] + col + v * step);
+#pragma unroll
+            for (int j = 0; j < kCompactRows; ++j)
+#pragma unroll
+                for (int v = 0; v < kCompactVec; ++v)
+                    if (j0 + j < m && from[j0 + j] >= 0 && col + v * step < kv.row_bytes)
+                        *reinterpret_cast<uint4*>(pool + to[j0 + j] + col + v * step) = x[j][v];
+        }
     }
 }
 
-// The new lengths, after the rows: len_out may be len, which the rows' blocks read.
+// The new lengths where they replace the old, which the rows' blocks read.
 __global__ void kv_compact_len_kernel(KvView kv, KvBatch b, const int* path, const int* n_path, int max_path,
                                       int* len_out) {
-    const int s = blockIdx.x * blockDim.x + threadIdx.x;
-    if (s >= b.n_seq) return;
-    const int n = n_path[s], len = b.len[s];
-    const int* pa = path + (long long)s * max_path;
-    bool bad = len < 0 || n < 0 || n > max_path;
-    for (int i = 0; i < n && !bad; ++i) {
-        const int x = pa[i];
-        bad = x < 0 || (i && x <= pa[i - 1]) || (long long)len + x >= ((long long)b.max_blocks << kv.ps_shift) ||
-              kv_row(kv, b, s, len + x) < 0 || kv_row(kv, b, s, len + i) < 0;
-    }
-    len_out[s] = bad ? len : len + n;
+    const int s = blockIdx.x, n = n_path[s], len = b.len[s];
+    const bool bad = path_bad(kv, b, path + (long long)s * max_path, s, n, max_path, len);
+    if (threadIdx.x == 0) len_out[s] = bad ? len : len + n;
 }
 
 cudaError_t refuse(const char* what, const std::string& why) {
@@ -478,10 +602,20 @@ extern "C" cudaError_t af_kv_store_f32(const af_kv_store_args* a, cudaStream_t s
     p.q_norm = a->q_norm;
     p.k_norm = a->k_norm;
     p.eps = a->eps;
+    const int hd = a->kv.head_dim;
+    auto vec = [](const void* x) { return !(reinterpret_cast<uintptr_t>(x) & 15); };
+    const bool wide = (hd == 64 || hd == 128) && vec(p.q) && vec(p.k) && vec(p.v) && vec(p.q_out) && vec(p.cos_t) &&
+                      vec(p.sin_t) && vec(p.q_norm) && vec(p.k_norm) && !((p.qs | p.ks | p.vs | p.os) & 3);
+    auto go = [&](auto type) {
+        constexpr int TYPE = decltype(type)::value;
+        if (wide && hd == 64) kv_store_vec_kernel<TYPE, 64><<<p.n_rows, kStoreThreads, 0, stream>>>(p);
+        else if (wide) kv_store_vec_kernel<TYPE, 128><<<p.n_rows, kStoreThreads, 0, stream>>>(p);
+        else kv_store_kernel<TYPE><<<p.n_rows, kStoreThreads, 0, stream>>>(p);
+    };
     switch (a->kv.type) {
-        case AF_KV_F32: kv_store_kernel<AF_KV_F32><<<a->n_rows, kStoreThreads, 0, stream>>>(p); break;
-        case AF_KV_F16: kv_store_kernel<AF_KV_F16><<<a->n_rows, kStoreThreads, 0, stream>>>(p); break;
-        default: kv_store_kernel<AF_KV_BF16><<<a->n_rows, kStoreThreads, 0, stream>>>(p); break;
+        case AF_KV_F32: go(std::integral_constant<int, AF_KV_F32>()); break;
+        case AF_KV_F16: go(std::integral_constant<int, AF_KV_F16>()); break;
+        default: go(std::integral_constant<int, AF_KV_BF16>()); break;
     }
     return cudaGetLastError();
 }
@@ -516,8 +650,16 @@ extern "C" cudaError_t af_kv_fork(const af_kv_fork_args* a, cudaStream_t stream)
     kv_fork_kernel<<<1, kForkThreads, 0, stream>>>(p);
     AF_CUDA_TRY(cudaGetLastError());
     if (a->n_out == 0) return cudaSuccess;
-    kv_copy_kernel<<<dim3(a->n_out, a->kv.n_layers, 2), kCopyThreads, 0, stream>>>(p.kv, p.copies);
-    return cudaGetLastError();
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a->n_out, a->kv.n_layers, 2);
+    cfg.blockDim = dim3(kCopyThreads);
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kv_copy_kernel, p.kv, (const int4*)p.copies);
 }
 
 extern "C" cudaError_t af_kv_compact(const af_kv_compact_args* a, cudaStream_t stream) {
@@ -534,9 +676,13 @@ extern "C" cudaError_t af_kv_compact(const af_kv_compact_args* a, cudaStream_t s
     int* err = nullptr;
     AF_CUDA_TRY(device_error_word(&err));
     const KvBatch b = kv_batch(a->batch, err);
-    const dim3 grid((kv.row_bytes / 16 + kCompactThreads - 1) / kCompactThreads, 2 * kv.n_layers, b.n_seq);
-    kv_compact_kernel<<<grid, kCompactThreads, 0, stream>>>(kv, b, a->path, a->n_path, a->max_path, a->len_out, b.len);
+    const int per = kCompactThreads * kCompactVec * 16;
+    const dim3 grid((kv.row_bytes + per - 1) / per, 2 * kv.n_layers, b.n_seq);
+    const bool in_place = a->len_out == a->batch.len;
+    kv_compact_kernel<<<grid, kCompactThreads, 0, stream>>>(kv, b, a->path, a->n_path, a->max_path,
+                                                           in_place ? nullptr : a->len_out);
     AF_CUDA_TRY(cudaGetLastError());
-    kv_compact_len_kernel<<<(b.n_seq + 127) / 128, 128, 0, stream>>>(kv, b, a->path, a->n_path, a->max_path, a->len_out);
+    if (in_place)
+        kv_compact_len_kernel<<<b.n_seq, 32, 0, stream>>>(kv, b, a->path, a->n_path, a->max_path, a->len_out);
     return cudaGetLastError();
 }
