@@ -3,8 +3,8 @@
 //     score(b, t) = scores[b] + x[b][t] - log Σ_t' exp x[b][t'],
 // in one pass over the logits.
 //
-//  * Segment kernel: a block streams a segment of a row, 2048 logits a step
-//    (two 16-byte loads a thread, the next step's in flight): the running
+//  * Segment kernel: a block streams a segment of a row, 4096 logits a step
+//    (four 16-byte loads a thread, the next step's in flight): the running
 //    maximum, Σ exp(x - max), and a buffer of what may be among the segment's
 //    K = n_out largest.  Within a beam scores are ordered as logits, so the K
 //    best of a segment are its K largest, ties to the lower token: 64-bit
@@ -34,8 +34,11 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kBeamThreads = 256;
-constexpr int kBeamStep = kBeamThreads * 8;             // logits of a step
-constexpr int kBeamBuffer = 2 * kBeamStep;              // keys kept: cut back when more than a step's are there
+constexpr int kBeamPer = 16;                            // logits of a thread in a step
+constexpr int kBeamStep = kBeamThreads * kBeamPer;      // 4096
+constexpr int kBeamFull = 2048;                         // keys kept: cut back when more are there
+constexpr int kBeamBuffer = kBeamFull + kBeamStep;
+constexpr int kBeamSelect = 512;                        // of those, near the best
 constexpr int kBeamChunk = 8192;                        // shortest segment
 constexpr int kBeamMaxK = 64;
 constexpr int kBeamLists = 1024;                        // chunk lists of a sequence
@@ -79,6 +82,7 @@ __device__ __forceinline__ T warp_sort_desc(T v, int lane) {
 
 struct BeamShared {
     u64 key[kBeamBuffer];
+    u64 sel[kBeamSelect];
     u64 out[kBeamMaxK];
     u64 wkey[kBeamThreads / 32];
     float wval[kBeamThreads / 32];
@@ -98,28 +102,26 @@ __device__ void beam_cut(BeamShared& sh, int K) {
     u64 thr = sh.wkey[0];
 #pragma unroll
     for (int w = 1; w < kBeamThreads / 32; ++w) thr = min(thr, sh.wkey[w]);
-    // what passes, to the front (read before it is written over)
-    u64 mine[kBeamBuffer / kBeamThreads];
-    int at[kBeamBuffer / kBeamThreads];
-#pragma unroll
-    for (int e = 0; e < kBeamBuffer / kBeamThreads; ++e) {
-        const int i = tid + e * kBeamThreads;
-        at[e] = -1;
-        if (i < n) {
-            mine[e] = sh.key[i];
-            if (mine[e] >= thr) at[e] = atomicAdd(&sh.kept, 1);
+    // their order among what passes (where that is more than sel holds, as equal keys' neighbours never are but
+    // rising ones may be, among all)
+    for (int i = tid; i < n; i += kBeamThreads) {
+        const u64 k = sh.key[i];
+        if (k >= thr) {
+            const int at = atomicAdd(&sh.kept, 1);
+            if (at < kBeamSelect) sh.sel[at] = k;
         }
     }
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < kBeamBuffer / kBeamThreads; ++e)
-        if (at[e] >= 0) sh.key[at[e]] = mine[e];
-    __syncthreads();
     const int kept = sh.kept;
-    for (int c = tid; c < kept; c += kBeamThreads) {
-        const u64 k = sh.key[c];
+    const bool few = kept <= kBeamSelect;
+    const u64* from = few ? sh.sel : sh.key;
+    const int m = few ? kept : n;
+    for (int c = tid; c < m; c += kBeamThreads) {
+        const u64 k = from[c];
+        if (k < thr) continue;
         int rank = 0;
-        for (int i = 0; i < kept; ++i) rank += sh.key[i] > k;
+#pragma unroll 8
+        for (int i = 0; i < m; ++i) rank += from[i] > k;
         if (rank < K) sh.out[rank] = k;
     }
     __syncthreads();
@@ -131,16 +133,18 @@ __device__ void beam_cut(BeamShared& sh, int K) {
 
 __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParams p) {
     constexpr int W = kBeamThreads / 32;
-    __shared__ BeamShared sh;
+    extern __shared__ __align__(16) uint8_t sm[];
+    BeamShared& sh = *reinterpret_cast<BeamShared*>(sm);
     pdl_launch_dependents();  // the merge kernel may start launching
     const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (dead_score(p.scores[row])) return;
     const int lo = blockIdx.x * p.seg, hi = min(lo + p.seg, p.vocab), K = p.K;
     const float* x = p.logits + (long long)row * p.stride;
-    auto load = [&](int t0, float (&v)[8]) {  // tokens t0 + 4·tid .. +3 and 1024 on
+    auto token = [&](int t0, int j) { return t0 + (j >> 2) * (4 * kBeamThreads) + 4 * tid + (j & 3); };
+    auto load = [&](int t0, float (&v)[kBeamPer]) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int t = t0 + h * (kBeamStep / 2) + 4 * tid;
+        for (int h = 0; h < kBeamPer / 4; ++h) {
+            const int t = token(t0, 4 * h);
             if (p.vec && t + 4 <= hi) {
                 const float4 f = __ldcs(reinterpret_cast<const float4*>(x + t));
                 v[4 * h] = f.x, v[4 * h + 1] = f.y, v[4 * h + 2] = f.z, v[4 * h + 3] = f.w;
@@ -150,7 +154,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParam
             }
         }
     };
-    float next[8];
+    float next[kBeamPer];
     load(lo, next);
     if (tid == 0) sh.count = 0;
     __syncthreads();
@@ -158,25 +162,25 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParam
     double sum = 0.;
     constexpr float kLog2e = 1.4426950408889634f;
     for (int t0 = lo; t0 < hi; t0 += kBeamStep) {
-        float v[8];
+        float v[kBeamPer];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = next[j];
+        for (int j = 0; j < kBeamPer; ++j) v[j] = next[j];
         if (t0 + kBeamStep < hi) load(t0 + kBeamStep, next);
         float big = v[0];
 #pragma unroll
-        for (int j = 1; j < 8; ++j) big = fmaxf(big, v[j]);
+        for (int j = 1; j < kBeamPer; ++j) big = fmaxf(big, v[j]);
         if (big > top) {
             sum *= (double)exp2f((top - big) * kLog2e);
             top = big;
         }
-        // 8 terms in 32 bits, the rest in 64; NaN stays NaN (and -inf - -inf is left out)
+        // a step's terms in 32 bits, the rest in 64; NaN stays NaN (and -inf - -inf is left out)
         float part = 0.f;
         if (top > -INFINITY) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) part += exp2f((v[j] - top) * kLog2e);
+            for (int j = 0; j < kBeamPer; ++j) part += exp2f((v[j] - top) * kLog2e);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) part += v[j] != v[j] ? v[j] : 0.f;
+            for (int j = 0; j < kBeamPer; ++j) part += v[j] != v[j] ? v[j] : 0.f;
         }
         sum += (double)part;
         const bool begin = t0 == lo;
@@ -190,13 +194,13 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParam
         }
         if (begin ? big >= thr : big > thr) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int t = t0 + (j >> 2) * (kBeamStep / 2) + 4 * tid + (j & 3);
+            for (int j = 0; j < kBeamPer; ++j) {
+                const int t = token(t0, j);
                 if (t < hi && (begin ? v[j] >= thr : v[j] > thr)) sh.key[atomicAdd(&sh.count, 1)] = logit_key(v[j], t);
             }
         }
-        // at most a step's keys came on top of at most a step's
-        if (__syncthreads_or(tid == 0 && sh.count > kBeamStep)) {
+        // at most a step's keys came on top of at most kBeamFull
+        if (__syncthreads_or(tid == 0 && sh.count > kBeamFull)) {
             beam_cut(sh, K);
             thr = ordered_to_float((uint32_t)(sh.key[K - 1] >> 32));
             __syncthreads();
@@ -240,7 +244,7 @@ struct Cand {
 };
 __device__ __forceinline__ bool better(u64 s, unsigned f, u64 s2, unsigned f2) { return s > s2 || (s == s2 && f < f2); }
 
-constexpr int kMergeSmem = kBeamLists * 12 + kBeamMaxK * kBeamMaxK * 12 + 64 * 8 + 64;
+constexpr int kMergeSmem = kBeamLists * 12 + kBeamMaxK * kBeamMaxK * 12 + 64 * 8 + (2 + kBeamMaxK) * 4;
 
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamParams p) {
     extern __shared__ __align__(16) uint8_t sm[];
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamParams p)
     double* base = reinterpret_cast<double*>(cs + kBeamMaxK * kBeamMaxK);  // [beams]
     unsigned* hf = reinterpret_cast<unsigned*>(base + 64);
     unsigned* cf = hf + kBeamLists;
-    int* ctl = reinterpret_cast<int*>(cf + kBeamMaxK * kBeamMaxK);  // [0] candidates
+    int* ctl = reinterpret_cast<int*>(cf + kBeamMaxK * kBeamMaxK);  // candidates, lists, the lists with the best heads
     const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row0 = seq * p.beams, K = p.K;
     pdl_wait();
@@ -258,14 +262,15 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamParams p)
         const float s = p.scores[row0 + b];
         double d = -INFINITY;
         if (!dead_score(s)) {
-            float top = -INFINITY;
-            for (int c = lane; c < p.chunks; c += 32) top = fmaxf(top, p.tops[(long long)(row0 + b) * p.chunks + c]);
+            const long long l0 = (long long)(row0 + b) * p.chunks;
+            float t = lane < p.chunks ? p.tops[l0 + lane] : -INFINITY, top = t;
+            double sum = lane < p.chunks ? p.sums[l0 + lane] : 0.;
+            for (int c = lane + 32; c < p.chunks; c += 32) top = fmaxf(top, p.tops[l0 + c]);
             top = warp_max(top);
-            double sum = 0.;
-            for (int c = lane; c < p.chunks; c += 32) {
-                const long long l = (long long)(row0 + b) * p.chunks + c;
-                const float t = p.tops[l];
-                sum += p.sums[l] * (t == top ? 1. : exp((double)t - (double)top));
+            if (lane < p.chunks && t != top) sum *= exp((double)t - (double)top);
+            for (int c = lane + 32; c < p.chunks; c += 32) {
+                t = p.tops[l0 + c];
+                sum += p.sums[l0 + c] * (t == top ? 1. : exp((double)t - (double)top));
             }
             sum = warp_sum_d(sum);
             d = (double)s - ((double)top + log(sum));
@@ -302,28 +307,61 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamParams p)
         hf[tid] = have ? mf : UINT_MAX;
     }
     __syncthreads();
+    // only the K lists with the best heads can hold the K best, and of the one of rank r only its first K - r entries
     if (have) {
         int rank = 0;
+#pragma unroll 4
         for (int i = 0; i < lists; ++i) rank += better(hs[i], hf[i], ms, mf);
-        // only the K lists with the best heads can hold the K best
-        if (rank < K) {
-            for (int c = 0; c < K; ++c) {
-                u64 s;
-                unsigned f;
-                if (!entry(tid, c, s, f)) break;
-                const int at = atomicAdd(&ctl[0], 1);
-                cs[at] = s;
-                cf[at] = f;
-            }
-        }
+        if (rank < K) ctl[2 + rank] = tid;
+    }
+    if (tid < 32) {  // how many lists have a head at all
+        int any = 0;
+        for (int i = tid; i < lists; i += 32) any += hf[i] != UINT_MAX;
+        any = __reduce_add_sync(0xffffffffu, any);
+        if (tid == 0) ctl[1] = min(any, K);
     }
     __syncthreads();
+    const int good = ctl[1];
+    u64 best = 0;
+    for (int i = tid; i < good * K; i += kMergeThreads) {
+        const int r = i / K, c = i % K;
+        u64 s;
+        unsigned f;
+        if (r + c < K && entry(ctl[2 + r], c, s, f)) {
+            const int at = atomicAdd(&ctl[0], 1);
+            cs[at] = s;
+            cf[at] = f;
+            best = max(best, s);
+        }
+    }
+    // a score that at least K reach: the smallest of the warps' ceil(K/32)-th best
+    best = warp_sort_desc(best, lane);
+    if (lane == (K + 31) / 32 - 1) hs[warp] = best;
+    if (tid == 0) ctl[1] = 0;
+    __syncthreads();
+    u64 thr = hs[0];
+    for (int w = 1; w < kMergeThreads / 32; ++w) thr = min(thr, hs[w]);
+    __syncthreads();
     const int cnt = ctl[0];
-    for (int c = tid; c < cnt; c += kMergeThreads) {
+    unsigned* sel = hf;  // the candidates that reach it, up to kBeamLists
+    for (int c = tid; c < cnt; c += kMergeThreads)
+        if (cs[c] >= thr) {
+            const int at = atomicAdd(&ctl[1], 1);
+            if (at < kBeamLists) sel[at] = c;
+        }
+    __syncthreads();
+    const bool few = ctl[1] <= kBeamLists;
+    const int m = few ? ctl[1] : cnt;
+    for (int i = tid; i < m; i += kMergeThreads) {
+        const int c = few ? sel[i] : i;
         const u64 s = cs[c];
         const unsigned f = cf[c];
         int rank = 0;
-        for (int i = 0; i < cnt; ++i) rank += better(cs[i], cf[i], s, f);
+#pragma unroll 4
+        for (int j = 0; j < m; ++j) {
+            const int o = few ? sel[j] : j;
+            rank += better(cs[o], cf[o], s, f);
+        }
         if (rank < K) {
             const long long at = (long long)seq * K + rank;
             p.out_score[at] = (float)ordered_double(s);
@@ -397,7 +435,8 @@ extern "C" cudaError_t af_beam_select_f32(const af_beam_select_args* a, cudaStre
     p.keys = static_cast<u64*>(a->ws);
     p.sums = reinterpret_cast<double*>(p.keys + lists * p.K);
     p.tops = reinterpret_cast<float*>(p.sums + lists);
-    beam_segment_kernel<<<dim3(p.chunks, p.n_seq * p.beams), kBeamThreads, 0, stream>>>(p);
+    AF_CUDA_TRY(cudaFuncSetAttribute(beam_segment_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(BeamShared)));
+    beam_segment_kernel<<<dim3(p.chunks, p.n_seq * p.beams), kBeamThreads, sizeof(BeamShared), stream>>>(p);
     AF_CUDA_TRY(cudaGetLastError());
     AF_CUDA_TRY(cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMergeSmem));
     cudaLaunchAttribute attr[1];

@@ -54,37 +54,36 @@ struct StoreParams {
     float eps;
 };
 
-// The block's row: its sequence and node, -1 for a row behind the last sequence.
-__device__ __forceinline__ void store_row(const StoreParams& p, int row, int* s_seq, int* s_node) {
+// A row's sequence (-1: a row behind the last), node and cached length, found
+// by the whole block: every load that does not need another's result goes out
+// with it.
+struct StorePlace {
+    int seq, node, len;
+};
+__device__ __forceinline__ void store_row(const StoreParams& p, int row, StorePlace* out) {
     const int tid = threadIdx.x;
-    if (tid == 0) *s_seq = -1;
+    if (tid == 0) out->seq = -1;
     __syncthreads();
     if (p.b.first) {
         for (int s = tid; s < p.b.n_seq; s += kStoreThreads) {
-            const int f = p.b.first[s];
-            if (f <= row && row < p.b.first[s + 1]) {
-                *s_seq = s;
-                *s_node = row - f;
-            }
+            const int f = p.b.first[s], e = p.b.first[s + 1], len = p.b.len[s];
+            if (f <= row && row < e) *out = {s, row - f, len};
         }
     } else if (tid == 0 && row / p.b.max_nodes < p.b.n_seq) {
-        *s_seq = row / p.b.max_nodes;
-        *s_node = row % p.b.max_nodes;
+        *out = {row / p.b.max_nodes, row % p.b.max_nodes, p.b.len[row / p.b.max_nodes]};
     }
     __syncthreads();
 }
 
 // Where the row's rotation and cache position are; false (and the error word) where it has none.
-__device__ __forceinline__ bool store_place(const StoreParams& p, int row, int seq, int node, long long& at, long long& slot) {
-    const int len = kv_len(p.kv, p.b, seq, 0);
-    if (len < 0) return false;
-    at = (long long)len + (p.depth ? p.depth[row] : node);
-    if (at < 0 || at >= p.n_ctx || node >= p.b.max_nodes) {
+__device__ __forceinline__ bool store_place(const StoreParams& p, const StorePlace& w, int depth, long long& at, long long& slot) {
+    at = (long long)w.len + (p.depth ? depth : w.node);
+    if (w.len < 0 || at < 0 || at >= p.n_ctx || w.node < 0 || w.node >= p.b.max_nodes) {
         if (threadIdx.x == 0) set_err_at(p.b.err, kErrBadArgs);
         return false;
     }
-    slot = kv_row(p.kv, p.b, seq, len + node);
-    if (slot < 0 && threadIdx.x == 0) set_err_at(p.b.err, kErrBadArgs);
+    const long long pos = (long long)w.len + w.node;
+    slot = pos < ((long long)p.b.max_blocks << p.kv.ps_shift) ? kv_row(p.kv, p.b, w.seq, (int)pos) : -1;
     return true;
 }
 
@@ -95,7 +94,7 @@ __device__ __forceinline__ bool store_place(const StoreParams& p, int row, int s
 template <int TYPE, int HD>
 __global__ void __launch_bounds__(kStoreThreads) kv_store_vec_kernel(StoreParams p) {
     constexpr int LH = HD / 4, HPW = 32 / LH, W = kStoreThreads / 32, U = 4;
-    __shared__ int s_seq, s_node;
+    __shared__ StorePlace where;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int sub = lane / LH, col = lane % LH, heads = p.H + 2 * p.kv.kv_heads;
     const long long kvd = (long long)p.kv.kv_heads * HD;
@@ -112,13 +111,15 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_vec_kernel(StoreParams
         const int h = (u * W + warp) * HPW + sub;
         x[u] = h < heads ? load(h) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    store_row(p, row, &s_seq, &s_node);
-    if (s_seq < 0) return;
+    const int depth = p.depth ? p.depth[row] : 0;
+    store_row(p, row, &where);
+    if (where.seq < 0) return;
     long long at, slot;
-    if (!store_place(p, row, s_seq, s_node, at, slot)) return;
+    if (!store_place(p, where, depth, at, slot)) return;
     const float4 c = *reinterpret_cast<const float4*>(p.cos_t + at * (HD / 2) + 4 * (col % (LH / 2)));
     const float4 sn = *reinterpret_cast<const float4*>(p.sin_t + at * (HD / 2) + 4 * (col % (LH / 2)));
     const float sign = col < LH / 2 ? -1.f : 1.f;
+    if (slot < 0 && tid == 0) set_err_at(p.b.err, kErrBadArgs);
     for (int h0 = 0; h0 < heads; h0 += U * W * HPW) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -172,12 +173,14 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_vec_kernel(StoreParams
 template <int TYPE>
 __global__ void __launch_bounds__(kStoreThreads) kv_store_kernel(StoreParams p) {
     using E = KvElem<TYPE>;
-    __shared__ int s_seq, s_node;
+    __shared__ StorePlace where;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    store_row(p, row, &s_seq, &s_node);
-    if (s_seq < 0) return;
+    const int depth = p.depth ? p.depth[row] : 0;
+    store_row(p, row, &where);
+    if (where.seq < 0) return;
     long long at, slot;
-    if (!store_place(p, row, s_seq, s_node, at, slot)) return;
+    if (!store_place(p, where, depth, at, slot)) return;
+    if (slot < 0 && tid == 0) set_err_at(p.b.err, kErrBadArgs);
     const int hd = p.kv.hd, half = hd / 2;
     const float* c = p.cos_t + at * half;
     const float* sn = p.sin_t + at * half;
@@ -261,6 +264,8 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_kernel(StoreParams p) 
 constexpr int kForkThreads = 1024;
 constexpr int kForkMax = 4096;  // sequences of a call
 
+constexpr int kForkAhead = 4;   // reference counts a thread loads before anything else
+
 struct ForkParams {
     KvView kv;
     KvBatch in;  // table_in, len_in; n_seq = n_in
@@ -269,71 +274,87 @@ struct ForkParams {
     int n_out;
     int4* copies;  // [n_out] source page, destination page, rows
     int* fresh;    // [n_pages] the free pages taken, in order
+    int* before;   // [n_pages] the counts as they came, where ref_out is ref_in
 };
 
-// What output i needs: its length, and pages behind its `full` whole ones up to `need`.
+// What an output needs: pages behind its `full` whole ones up to `need`.
 struct ForkNeed {
-    int parent, len, full, need, over;
+    int parent, len, need, base;  // base: its first page among those taken
 };
-__device__ __forceinline__ ForkNeed fork_need(const ForkParams& p, int i) {
-    ForkNeed n = {};
-    const int j = p.parent[i];
-    n.parent = j >= 0 && j < p.in.n_seq ? j : -1;
-    n.len = n.parent >= 0 ? kv_len(p.kv, p.in, n.parent, 0) : 0;
-    if (n.len < 0) {
-        n.parent = -1;
-        n.len = 0;
-    }
-    n.full = n.len >> p.kv.ps_shift;
-    const long long want = (long long)n.len + (p.n_new ? max(0, p.n_new[i]) : 0);
-    const long long blocks = (want + (1 << p.kv.ps_shift) - 1) >> p.kv.ps_shift;
-    n.need = (int)min(blocks, (long long)p.in.max_blocks);
-    n.over = (int)min(blocks - n.need, (long long)INT_MAX);
-    return n;
-}
 
-// Whether the first child of `parent` keeps its page of block b.
-__device__ __forceinline__ bool fork_keeps(const ForkParams& p, int parent, int b) {
-    const int page = kv_page(p.in, p.kv.n_pages, parent, b);
-    return page >= 0 && p.ref_in[page] == 1;
-}
+constexpr int kForkSmem = kForkMax * (4 + 16);
 
 // The bookkeeping of a fork, one block: which output is a parent's first
 // child, how many pages each output takes, which pages are free, and then
-// tables, reference counts and the list of pages to copy.
+// tables, reference counts and the list of pages to copy.  Bound by latency: a
+// chain of dependent loads (parent, length; page, count; page again), so what
+// does not hang on it is loaded first and the counts go out as reductions.
 __global__ void __launch_bounds__(kForkThreads) kv_fork_kernel(ForkParams p) {
-    __shared__ int eldest[kForkMax];
-    __shared__ int base[kForkMax];
+    extern __shared__ __align__(16) uint8_t sm[];
+    ForkNeed* needs = reinterpret_cast<ForkNeed*>(sm);        // [n_out]
+    int* eldest = reinterpret_cast<int*>(needs + kForkMax);  // [n_in]
     __shared__ int wsum[32];
-    __shared__ int s_total, s_found;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    pdl_launch_dependents();  // the copies may start launching
+    __shared__ int s_total, s_missing;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_pages = p.kv.n_pages, nb = p.in.max_blocks;
+    const bool in_place = p.ref_out == p.ref_in;
+    const int* ref = in_place ? p.before : p.ref_in;  // the counts as they came
+    pdl_launch_dependents();                          // the copies may start launching
+    int held[kForkAhead];
+#pragma unroll
+    for (int e = 0; e < kForkAhead; ++e) {
+        const int page = e * kForkThreads + tid;
+        held[e] = page < n_pages ? p.ref_in[page] : 1;
+    }
     for (int j = tid; j < p.in.n_seq; j += kForkThreads) eldest[j] = INT_MAX;
+    if (tid == 0) s_missing = 0;
     __syncthreads();
     for (int i = tid; i < p.n_out; i += kForkThreads) {
-        const int j = p.parent[i];
-        if (j >= 0 && j < p.in.n_seq) atomicMin(&eldest[j], i);
+        const int j = p.parent[i], more = p.n_new ? max(0, p.n_new[i]) : 0;
+        ForkNeed n = {j >= 0 && j < p.in.n_seq ? j : -1, 0, 0, 0};
+        if (n.parent >= 0) {
+            n.len = kv_len(p.kv, p.in, j, 0);
+            if (n.len < 0) n.parent = -1, n.len = 0;
+        }
+        if (n.parent >= 0) atomicMin(&eldest[j], i);
+        const long long blocks = ((long long)n.len + more + (1 << p.kv.ps_shift) - 1) >> p.kv.ps_shift;
+        n.need = (int)min(blocks, (long long)nb);
+        if (blocks > n.need) atomicAdd(&s_missing, (int)min(blocks - n.need, (long long)INT_MAX));
+        needs[i] = n;
     }
+    // the counts, where they go
+#pragma unroll
+    for (int e = 0; e < kForkAhead; ++e) {
+        const int page = e * kForkThreads + tid;
+        if (page < n_pages) (in_place ? p.before : p.ref_out)[page] = held[e];
+    }
+    for (int page = kForkAhead * kForkThreads + tid; page < n_pages; page += kForkThreads)
+        (in_place ? p.before : p.ref_out)[page] = p.ref_in[page];
     __syncthreads();
+    auto keeps = [&](int parent, int b) {  // whether the first child of `parent` keeps its page of block b
+        const int page = kv_page(p.in, n_pages, parent, b);
+        return page >= 0 && ref[page] == 1;
+    };
     // pages that each output takes
     for (int i = warp; i < p.n_out; i += kForkThreads / 32) {
-        const ForkNeed n = fork_need(p, i);
-        const bool first = n.parent >= 0 && eldest[n.parent] == i;
-        int cnt = 0;
-        for (int b = n.full + lane; b < n.need; b += 32) cnt += !(first && fork_keeps(p, n.parent, b));
-        cnt = __reduce_add_sync(0xffffffffu, cnt);
-        if (lane == 0) base[i] = cnt;
+        const ForkNeed n = needs[i];
+        const int full = n.len >> p.kv.ps_shift;
+        int cnt = max(0, n.need - full);
+        if (n.parent >= 0 && eldest[n.parent] == i) {
+            cnt = 0;
+            for (int b = full + lane; b < n.need; b += 32) cnt += !keeps(n.parent, b);
+            cnt = __reduce_add_sync(0xffffffffu, cnt);
+        }
+        __syncwarp();
+        if (lane == 0) needs[i].base = cnt;
     }
-    if (tid == 0) s_found = 0;
     __syncthreads();
-    // exclusive prefix sum of base[]
-    {
+    {  // exclusive prefix sum of base
         constexpr int per = kForkMax / kForkThreads;
         int v[per], sum = 0;
 #pragma unroll
         for (int e = 0; e < per; ++e) {
             const int i = tid * per + e;
-            v[e] = i < p.n_out ? base[i] : 0;
+            v[e] = i < p.n_out ? needs[i].base : 0;
             sum += v[e];
         }
         int inc = sum;
@@ -344,13 +365,13 @@ __global__ void __launch_bounds__(kForkThreads) kv_fork_kernel(ForkParams p) {
         }
         if (lane == 31) wsum[warp] = inc;
         __syncthreads();
-        int before = 0;
-        for (int w = 0; w < warp; ++w) before += wsum[w];
-        int at = before + inc - sum;
+        int front = 0;
+        for (int w = 0; w < warp; ++w) front += wsum[w];
+        int at = front + inc - sum;
 #pragma unroll
         for (int e = 0; e < per; ++e) {
             const int i = tid * per + e;
-            if (i < p.n_out) base[i] = at;
+            if (i < p.n_out) needs[i].base = at;
             at += v[e];
         }
         if (tid == kForkThreads - 1) s_total = at;
@@ -358,43 +379,44 @@ __global__ void __launch_bounds__(kForkThreads) kv_fork_kernel(ForkParams p) {
     __syncthreads();
     // the lowest s_total pages that nobody holds, in order
     const int total = s_total;
-    for (int p0 = 0; p0 < p.kv.n_pages; p0 += kForkThreads) {
-        const int found = s_found;
-        if (found >= total) break;
-        const int page = p0 + tid;
-        const bool is = page < p.kv.n_pages && p.ref_in[page] == 0;
-        const unsigned m = __ballot_sync(0xffffffffu, is);
+    int found = 0;
+    for (int e = 0; e * kForkThreads < n_pages && found < total; ++e) {
+        const int page = e * kForkThreads + tid;
+        int count = 1;
+        if (e < kForkAhead) {
+#pragma unroll
+            for (int k = 0; k < kForkAhead; ++k)
+                if (k == e) count = held[k];
+        } else if (page < n_pages) {
+            count = ref[page];
+        }
+        const unsigned m = __ballot_sync(0xffffffffu, count == 0);
         if (lane == 0) wsum[warp] = __popc(m);
         __syncthreads();
-        int before = found, all = 0;
-        for (int w = 0; w < kForkThreads / 32; ++w) {
-            before += w < warp ? wsum[w] : 0;
-            all += wsum[w];
-        }
-        const int rank = before + __popc(m & ((1u << lane) - 1));
-        if (is && rank < total) p.fresh[rank] = page;
-        __syncthreads();
-        if (tid == 0) s_found = found + all;
+        const int mine = wsum[lane];
+        const int front = __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0);
+        const int rank = found + front + __popc(m & ((1u << lane) - 1));
+        if (count == 0 && rank < total) p.fresh[rank] = page;
+        found += __reduce_add_sync(0xffffffffu, mine);
         __syncthreads();
     }
-    const int avail = min(s_found, total);
-    if (p.ref_out != p.ref_in)
-        for (int i = tid; i < p.kv.n_pages; i += kForkThreads) p.ref_out[i] = p.ref_in[i];
-    if (tid == 0) wsum[0] = 0;
-    // Which of its pages a first child keeps depends on ref_in, which may be
-    // ref_out: they are marked in table_out before any count changes.
-    const int nb = p.in.max_blocks;
-    __syncthreads();
+    const int avail = min(found, total);
+    // one off for every entry of the inputs
+    for (long long e = tid; e < (long long)p.in.n_seq * nb; e += kForkThreads) {
+        const int page = kv_page(p.in, n_pages, (int)(e / nb), (int)(e % nb));
+        if (page >= 0) atomicSub(&p.ref_out[page], 1);
+    }
     int missing = 0;
     for (int i = warp; i < p.n_out; i += kForkThreads / 32) {
-        const ForkNeed n = fork_need(p, i);
+        const ForkNeed n = needs[i];
         const bool first = n.parent >= 0 && eldest[n.parent] == i;
-        int taken = base[i], len = n.len;
+        const int full = n.len >> p.kv.ps_shift, rows = n.len & ((1 << p.kv.ps_shift) - 1);
+        int taken = n.base, len = n.len;
         for (int b0 = 0; b0 < nb; b0 += 32) {
             const int b = b0 + lane;
-            const int old = n.parent >= 0 && b < nb ? kv_page(p.in, p.kv.n_pages, n.parent, b) : -1;
-            const bool shared = b < n.full;
-            const bool keep = !shared && b < n.need && first && fork_keeps(p, n.parent, b);
+            const int old = n.parent >= 0 && b < n.need ? kv_page(p.in, n_pages, n.parent, b) : -1;
+            const bool shared = b < full;
+            const bool keep = !shared && b < n.need && first && old >= 0 && ref[old] == 1;
             const bool take = !shared && !keep && b < n.need;
             const unsigned m = __ballot_sync(0xffffffffu, take);
             int page = shared || keep ? old : -1;
@@ -405,31 +427,20 @@ __global__ void __launch_bounds__(kForkThreads) kv_fork_kernel(ForkParams p) {
             }
             taken += __popc(m);
             if (b < nb) p.table_out[(long long)i * nb + b] = page;
+            if (page >= 0) atomicAdd(&p.ref_out[page], 1);
             // the partly filled page
-            const int rows = n.len & ((1 << p.kv.ps_shift) - 1);
-            if (b == n.full && b < nb) p.copies[i] = make_int4(old, page, take && page >= 0 && old >= 0 ? rows : 0, 0);
-            const bool lost = b == n.full && rows > 0 && page < 0;
-            if (__any_sync(0xffffffffu, lost)) len = n.full << p.kv.ps_shift;
+            if (b == full && b < nb) p.copies[i] = make_int4(old, page, take && page >= 0 && old >= 0 ? rows : 0, 0);
+            if (__any_sync(0xffffffffu, b == full && rows > 0 && page < 0)) len = full << p.kv.ps_shift;
         }
-        if (n.full >= nb && lane == 0) p.copies[i] = make_int4(-1, -1, 0, 0);
         if (lane == 0) {
+            if (full >= nb) p.copies[i] = make_int4(-1, -1, 0, 0);
             p.len_out[i] = len;
-            missing += n.over;
         }
     }
     missing = __reduce_add_sync(0xffffffffu, missing);
-    if (lane == 0 && missing) atomicAdd(&wsum[0], missing);
+    if (lane == 0 && missing) atomicAdd(&s_missing, missing);
     __syncthreads();
-    if (tid == 0) *p.n_short = wsum[0];
-    // counts: one off for every entry of the inputs, one on for every entry of the outputs
-    for (long long e = tid; e < (long long)p.in.n_seq * nb; e += kForkThreads) {
-        const int page = kv_page(p.in, p.kv.n_pages, (int)(e / nb), (int)(e % nb));
-        if (page >= 0) atomicSub(&p.ref_out[page], 1);
-    }
-    for (long long e = tid; e < (long long)p.n_out * nb; e += kForkThreads) {
-        const int page = p.table_out[e];
-        if (page >= 0) atomicAdd(&p.ref_out[page], 1);
-    }
+    if (tid == 0) *p.n_short = s_missing;
 }
 
 constexpr int kCopyThreads = 256;
@@ -532,7 +543,7 @@ cudaError_t refuse(const char* what, const std::string& why) {
 }
 
 size_t fork_ws(const af_kv_fork_args& a) {
-    return (size_t)a.n_out * sizeof(int4) + (size_t)a.kv.n_pages * sizeof(int);
+    return (size_t)a.n_out * sizeof(int4) + 2 * (size_t)a.kv.n_pages * sizeof(int);
 }
 
 std::string fork_wrong(const af_kv_fork_args& a) {
@@ -647,7 +658,9 @@ extern "C" cudaError_t af_kv_fork(const af_kv_fork_args* a, cudaStream_t stream)
     p.n_out = a->n_out;
     p.copies = static_cast<int4*>(a->ws);
     p.fresh = reinterpret_cast<int*>(p.copies + a->n_out);
-    kv_fork_kernel<<<1, kForkThreads, 0, stream>>>(p);
+    p.before = p.fresh + a->kv.n_pages;
+    AF_CUDA_TRY(cudaFuncSetAttribute(kv_fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kForkSmem));
+    kv_fork_kernel<<<1, kForkThreads, kForkSmem, stream>>>(p);
     AF_CUDA_TRY(cudaGetLastError());
     if (a->n_out == 0) return cudaSuccess;
     cudaLaunchAttribute attr[1];
