@@ -42,7 +42,7 @@ constexpr int kBeamSelect = 512;                        // of those, near the be
 constexpr int kBeamChunk = 8192;                        // shortest segment
 constexpr int kBeamMaxK = 64;
 constexpr int kBeamLists = 1024;                        // chunk lists of a sequence
-constexpr int kMergeThreads = 1024;
+constexpr int kMergeThreads = 256;
 
 struct BeamParams {
     const float *logits, *scores;
@@ -78,6 +78,12 @@ __device__ __forceinline__ T warp_sort_desc(T v, int lane) {
         }
     }
     return v;
+}
+
+__device__ __forceinline__ float beam_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 struct BeamShared {
@@ -142,6 +148,14 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParam
     const float* x = p.logits + (long long)row * p.stride;
     auto token = [&](int t0, int j) { return t0 + (j >> 2) * (4 * kBeamThreads) + 4 * tid + (j & 3); };
     auto load = [&](int t0, float (&v)[kBeamPer]) {
+        if (p.vec && t0 + kBeamStep <= hi) {
+#pragma unroll
+            for (int h = 0; h < kBeamPer / 4; ++h) {
+                const float4 f = __ldcs(reinterpret_cast<const float4*>(x + token(t0, 4 * h)));
+                v[4 * h] = f.x, v[4 * h + 1] = f.y, v[4 * h + 2] = f.z, v[4 * h + 3] = f.w;
+            }
+            return;
+        }
 #pragma unroll
         for (int h = 0; h < kBeamPer / 4; ++h) {
             const int t = token(t0, 4 * h);
@@ -161,48 +175,68 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParam
     float top = -INFINITY, thr = 0.f;
     double sum = 0.;
     constexpr float kLog2e = 1.4426950408889634f;
+    auto lowest = [&]() {
+        float m = sh.wval[0];
+#pragma unroll
+        for (int w = 1; w < W; ++w) m = fminf(m, sh.wval[w]);
+        return m;
+    };
     for (int t0 = lo; t0 < hi; t0 += kBeamStep) {
         float v[kBeamPer];
 #pragma unroll
         for (int j = 0; j < kBeamPer; ++j) v[j] = next[j];
         if (t0 + kBeamStep < hi) load(t0 + kBeamStep, next);
-        float big = v[0];
+        float m[4];
 #pragma unroll
-        for (int j = 1; j < kBeamPer; ++j) big = fmaxf(big, v[j]);
+        for (int j = 0; j < 4; ++j) m[j] = fmaxf(fmaxf(v[4 * j], v[4 * j + 1]), fmaxf(v[4 * j + 2], v[4 * j + 3]));
+        const float big = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
         if (big > top) {
-            sum *= (double)exp2f((top - big) * kLog2e);
+            sum *= (double)beam_exp2((top - big) * kLog2e);
             top = big;
         }
-        // a step's terms in 32 bits, the rest in 64; NaN stays NaN (and -inf - -inf is left out)
-        float part = 0.f;
-        if (top > -INFINITY) {
+        // a step's terms in 32 bits, the rest in 64; NaN stays NaN, and where all is -inf, nothing is added
+        const float off = top > -INFINITY ? top : 0.f;
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < kBeamPer; ++j) part += exp2f((v[j] - top) * kLog2e);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kBeamPer; ++j) part += v[j] != v[j] ? v[j] : 0.f;
-        }
-        sum += (double)part;
+        for (int j = 0; j < kBeamPer; ++j) part[j & 3] += beam_exp2((v[j] - off) * kLog2e);
+        sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
         const bool begin = t0 == lo;
-        if (begin) {  // the threshold
-            const float s = warp_sort_desc(big, lane);
+        // The threshold, of the first step before anything is kept; of all steps so far behind steps 1, 2, 4, 8, ...,
+        // which halves how many pass each time (top is the thread's largest so far).
+        const int step = (t0 - lo) / kBeamStep + 1;
+        const bool raise = (step & (step - 1)) == 0;
+        if (raise) {
+            const float s = warp_sort_desc(top, lane);
             if (lane == (K + 7) / 8 - 1) sh.wval[warp] = s;
-            __syncthreads();
-            thr = sh.wval[0];
-#pragma unroll
-            for (int w = 1; w < W; ++w) thr = fminf(thr, sh.wval[w]);
         }
-        if (begin ? big >= thr : big > thr) {
+        if (begin) {
+            __syncthreads();
+            thr = lowest();
+        }
+        auto keep = [&](int j) { sh.key[atomicAdd(&sh.count, 1)] = logit_key(v[j], token(t0, j)); };
+        if (begin) {
+            if (big >= thr) {
 #pragma unroll
-            for (int j = 0; j < kBeamPer; ++j) {
-                const int t = token(t0, j);
-                if (t < hi && (begin ? v[j] >= thr : v[j] > thr)) sh.key[atomicAdd(&sh.count, 1)] = logit_key(v[j], t);
+                for (int j = 0; j < kBeamPer; ++j)
+                    if (v[j] >= thr && token(t0, j) < hi) keep(j);
+            }
+        } else if (big > thr) {  // what lies behind the segment is -inf
+#pragma unroll
+            for (int j = 0; j < kBeamPer; j += 4) {
+                if (m[(j >> 2) & 3] <= thr) continue;
+#pragma unroll
+                for (int i = j; i < j + 4; ++i)
+                    if (v[i] > thr) keep(i);
             }
         }
         // at most a step's keys came on top of at most kBeamFull
         if (__syncthreads_or(tid == 0 && sh.count > kBeamFull)) {
             beam_cut(sh, K);
-            thr = ordered_to_float((uint32_t)(sh.key[K - 1] >> 32));
+            thr = fmaxf(thr, ordered_to_float((uint32_t)(sh.key[K - 1] >> 32)));
+            __syncthreads();
+        }
+        if (raise && !begin) {
+            thr = fmaxf(thr, lowest());
             __syncthreads();
         }
     }
@@ -217,7 +251,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParam
     float all = sh.wval[0];
 #pragma unroll
     for (int w = 1; w < W; ++w) all = fmaxf(all, sh.wval[w]);
-    sum = warp_sum_d(top == all ? sum : sum * exp((double)top - (double)all));  // 0·exp(-inf) = 0
+    sum = warp_sum_d(top == all ? sum : sum * (double)expf(top - all));  // 0·exp(-inf) = 0
     if (lane == 0) sh.wsum[warp] = sum;
     __syncthreads();
     if (tid == 0) {
@@ -267,10 +301,10 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamParams p)
             double sum = lane < p.chunks ? p.sums[l0 + lane] : 0.;
             for (int c = lane + 32; c < p.chunks; c += 32) top = fmaxf(top, p.tops[l0 + c]);
             top = warp_max(top);
-            if (lane < p.chunks && t != top) sum *= exp((double)t - (double)top);
+            if (lane < p.chunks && t != top) sum *= (double)expf(t - top);  // NaN sums stay
             for (int c = lane + 32; c < p.chunks; c += 32) {
                 t = p.tops[l0 + c];
-                sum += p.sums[l0 + c] * (t == top ? 1. : exp((double)t - (double)top));
+                sum += p.sums[l0 + c] * (t == top ? 1. : (double)expf(t - top));
             }
             sum = warp_sum_d(sum);
             d = (double)s - ((double)top + log(sum));
@@ -298,21 +332,23 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamParams p)
         return true;
     };
     const int lists = p.beams * p.chunks;
-    u64 ms = 0;
-    unsigned mf = 0;
-    bool have = false;
-    if (tid < lists) {
-        have = entry(tid, 0, ms, mf);
-        hs[tid] = have ? ms : 0;
-        hf[tid] = have ? mf : UINT_MAX;
+    for (int l = tid; l < lists; l += kMergeThreads) {
+        u64 ms = 0;
+        unsigned mf = UINT_MAX;  // no entry at all
+        if (!entry(l, 0, ms, mf)) ms = 0, mf = UINT_MAX;
+        hs[l] = ms;
+        hf[l] = mf;
     }
     __syncthreads();
     // only the K lists with the best heads can hold the K best, and of the one of rank r only its first K - r entries
-    if (have) {
+    for (int l = tid; l < lists; l += kMergeThreads) {
+        const u64 ms = hs[l];
+        const unsigned mf = hf[l];
+        if (mf == UINT_MAX) continue;
         int rank = 0;
 #pragma unroll 4
         for (int i = 0; i < lists; ++i) rank += better(hs[i], hf[i], ms, mf);
-        if (rank < K) ctl[2 + rank] = tid;
+        if (rank < K) ctl[2 + rank] = l;
     }
     if (tid < 32) {  // how many lists have a head at all
         int any = 0;
@@ -334,9 +370,9 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamParams p)
             best = max(best, s);
         }
     }
-    // a score that at least K reach: the smallest of the warps' ceil(K/32)-th best
+    // a score that at least K reach: the smallest of the warps' ceil(K/8)-th best
     best = warp_sort_desc(best, lane);
-    if (lane == (K + 31) / 32 - 1) hs[warp] = best;
+    if (lane == (K + 7) / 8 - 1) hs[warp] = best;
     if (tid == 0) ctl[1] = 0;
     __syncthreads();
     u64 thr = hs[0];

@@ -89,27 +89,27 @@ __device__ __forceinline__ bool store_place(const StoreParams& p, const StorePla
 
 // A block per row, its heads (queries, keys, values) over the warps.  HD 64
 // and 128 with 16-byte rows: a lane holds 4 values, HD/4 lanes a head, the
-// partner of a rotation sits HD/8 lanes away; up to 4 heads a warp are loaded
-// before the first is worked on.  Bound by memory: q, k, v once in, once out.
+// partner of a rotation sits HD/8 lanes away; a warp's first heads (up to 3)
+// are loaded before the row's place is known.  Bound by memory: q, k, v once
+// in, once out.
 template <int TYPE, int HD>
-__global__ void __launch_bounds__(kStoreThreads) kv_store_vec_kernel(StoreParams p) {
-    constexpr int LH = HD / 4, HPW = 32 / LH, W = kStoreThreads / 32, U = 4;
+__global__ void __launch_bounds__(kStoreThreads, 5) kv_store_vec_kernel(StoreParams p) {
+    constexpr int LH = HD / 4, HPW = 32 / LH, W = kStoreThreads / 32, U = 3;
+    using E = KvElem<TYPE>;
     __shared__ StorePlace where;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int sub = lane / LH, col = lane % LH, heads = p.H + 2 * p.kv.kv_heads;
-    const long long kvd = (long long)p.kv.kv_heads * HD;
+    const int sub = lane / LH, col = lane % LH, KV = p.kv.kv_heads, heads = p.H + 2 * KV;
+    const float* q = p.q + (long long)row * p.qs + 4 * col;
+    const float* k = p.k + (long long)row * p.ks + 4 * col - p.H * HD;         // by the head's number
+    const float* v = p.v + (long long)row * p.vs + 4 * col - (p.H + KV) * HD;
     auto load = [&](int h) -> float4 {
-        const float* src = h < p.H ? p.q + (long long)row * p.qs + (long long)h * HD
-                           : h < p.H + p.kv.kv_heads ? p.k + (long long)row * p.ks + (long long)h * HD - (long long)p.H * HD
-                                                     : p.v + (long long)row * p.vs + (long long)h * HD - (long long)p.H * HD - kvd;
-        return *reinterpret_cast<const float4*>(src + 4 * col);
+        return __ldcs(reinterpret_cast<const float4*>((h < p.H ? q : h < p.H + KV ? k : v) + h * HD));
     };
     float4 x[U];
-    // the first heads' loads do not wait for the row's place
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int h = (u * W + warp) * HPW + sub;
-        x[u] = h < heads ? load(h) : make_float4(0.f, 0.f, 0.f, 0.f);
+        if (h < heads) x[u] = load(h);
     }
     const int depth = p.depth ? p.depth[row] : 0;
     store_row(p, row, &where);
@@ -117,52 +117,56 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_vec_kernel(StoreParams
     long long at, slot;
     if (!store_place(p, where, depth, at, slot)) return;
     const float4 c = *reinterpret_cast<const float4*>(p.cos_t + at * (HD / 2) + 4 * (col % (LH / 2)));
-    const float4 sn = *reinterpret_cast<const float4*>(p.sin_t + at * (HD / 2) + 4 * (col % (LH / 2)));
-    const float sign = col < LH / 2 ? -1.f : 1.f;
+    float4 sn = *reinterpret_cast<const float4*>(p.sin_t + at * (HD / 2) + 4 * (col % (LH / 2)));
+    if (col < LH / 2) sn = make_float4(-sn.x, -sn.y, -sn.z, -sn.w);
     if (slot < 0 && tid == 0) set_err_at(p.b.err, kErrBadArgs);
+    float* qo = p.q_out + (long long)row * p.os + 4 * col;
+    typename E::T* ko = reinterpret_cast<typename E::T*>(p.kv.k + (long long)p.layer * p.kv.layer_bytes + slot) + 4 * col - p.H * HD;
+    typename E::T* vo = reinterpret_cast<typename E::T*>(p.kv.v + (long long)p.layer * p.kv.layer_bytes + slot) + 4 * col - (p.H + KV) * HD;
     for (int h0 = 0; h0 < heads; h0 += U * W * HPW) {
+        if (h0) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int h = h0 + (u * W + warp) * HPW + sub;
-            if (h0) x[u] = h < heads ? load(h) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int u = 0; u < U; ++u) {
+                const int h = h0 + (u * W + warp) * HPW + sub;
+                if (h < heads) x[u] = load(h);
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            if (h0 + (u * W + warp) * HPW >= heads) break;  // the same in the whole warp
             const int h = h0 + (u * W + warp) * HPW + sub;
-            const bool isq = h < p.H, isv = h >= p.H + p.kv.kv_heads;
-            float4 v = x[u];
-            const float* nw = isv ? nullptr : isq ? p.q_norm : p.k_norm;
+            const bool isv = h >= p.H + KV;
+            float4 y = x[u];
             auto norm = [&]() {  // the heads of a warp may differ in kind: all lanes add up
-                float ss = v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
+                const float* nw = isv ? nullptr : h < p.H ? p.q_norm : p.k_norm;
+                float ss = y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
 #pragma unroll
                 for (int o = 1; o < LH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
                 if (nw) {
-                    const float sc = 1.f / sqrtf(ss / (float)HD + p.eps);
+                    const float sc = rsqrtf(ss * (1.f / HD) + p.eps);
                     const float4 w = *reinterpret_cast<const float4*>(nw + 4 * col);
-                    v.x = w.x * (v.x * sc), v.y = w.y * (v.y * sc), v.z = w.z * (v.z * sc), v.w = w.w * (v.w * sc);
+                    y.x = w.x * (y.x * sc), y.y = w.y * (y.y * sc), y.z = w.z * (y.z * sc), y.w = w.w * (y.w * sc);
                 }
             };
             if (p.order == 1) norm();
             float4 o;
-            o.x = __shfl_xor_sync(0xffffffffu, v.x, LH / 2), o.y = __shfl_xor_sync(0xffffffffu, v.y, LH / 2);
-            o.z = __shfl_xor_sync(0xffffffffu, v.z, LH / 2), o.w = __shfl_xor_sync(0xffffffffu, v.w, LH / 2);
-            if (!isv) {  // x0·cos - x1·sin in the first half, x0·sin + x1·cos in the second
-                v.x = fmaf(v.x, c.x, sign * (o.x * sn.x)), v.y = fmaf(v.y, c.y, sign * (o.y * sn.y));
-                v.z = fmaf(v.z, c.z, sign * (o.z * sn.z)), v.w = fmaf(v.w, c.w, sign * (o.w * sn.w));
+            o.x = __shfl_xor_sync(0xffffffffu, y.x, LH / 2), o.y = __shfl_xor_sync(0xffffffffu, y.y, LH / 2);
+            o.z = __shfl_xor_sync(0xffffffffu, y.z, LH / 2), o.w = __shfl_xor_sync(0xffffffffu, y.w, LH / 2);
+            if (!isv) {  // x0·cos - x1·sin in the first half, x1·cos + x0·sin in the second
+                y.x = fmaf(y.x, c.x, o.x * sn.x), y.y = fmaf(y.y, c.y, o.y * sn.y);
+                y.z = fmaf(y.z, c.z, o.z * sn.z), y.w = fmaf(y.w, c.w, o.w * sn.w);
             }
             if (p.order == 2) norm();
             if (h >= heads) continue;
-            if (isq) {
-                *reinterpret_cast<float4*>(p.q_out + (long long)row * p.os + (long long)h * HD + 4 * col) = v;
+            if (h < p.H) {
+                *reinterpret_cast<float4*>(qo + h * HD) = y;
             } else if (slot >= 0) {
-                const int kvh = isv ? h - p.H - p.kv.kv_heads : h - p.H;
-                uint8_t* dst = (isv ? p.kv.v : p.kv.k) + (long long)p.layer * p.kv.layer_bytes + slot;
+                typename E::T* dst = (isv ? vo : ko) + h * HD;
                 if (TYPE == AF_KV_F32) {
-                    reinterpret_cast<float4*>(dst)[kvh * LH + col] = v;
+                    *reinterpret_cast<float4*>(dst) = y;
                 } else {
-                    using E = KvElem<TYPE>;
-                    typename E::T r[4] = {E::round(v.x), E::round(v.y), E::round(v.z), E::round(v.w)};
-                    reinterpret_cast<uint2*>(dst)[kvh * LH + col] = *reinterpret_cast<const uint2*>(r);
+                    typename E::T r[4] = {E::round(y.x), E::round(y.y), E::round(y.z), E::round(y.w)};
+                    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(r);
                 }
             }
         }
