@@ -322,7 +322,7 @@ struct MmaShape {
     static constexpr int TILES = (SCALE + (TYPE == AF_KV_F16 ? 0 : 2 * NB * 3 * GROUPS * 4) + 127) / 128 * 128;
     static constexpr int RAW = TILES + NB * 2 * HALF;     // f32: 8 warps x 16 copies x 512 bytes as they are
     static constexpr int BYTES = RAW + (F32 ? 65536 : 0);
-    static_assert(BYTES <= 227 * 1024, "shared memory");
+    static_assert(BYTES <= 227 * 1024 - 64, "shared memory");
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -347,11 +347,109 @@ __device__ __noinline__ uint32_t clean(float4 (&x)[8]) {
     return __reduce_max_sync(0xffffffffu, b);
 }
 
+// Work: an item is 128 rows of a sequence with one kv head, its tiles split
+// over blocks of at most t tiles.  How many tiles there are is known on the
+// device alone (lengths, counts), so every block finds its place itself: the
+// smallest t for which the blocks fit the waves that the items need anyway.  A
+// ragged batch then costs its average and not its longest: 16 sequences of
+// 8190 to 0 positions, 120 -> 75 us.
+constexpr int kTreeSms = 148;
+constexpr int kTreeWaves = 4;                                // beyond so many the items balance one another
+constexpr int kTreeItems = kTreeSms * kTreeWaves;
+constexpr int kTreeMinTiles = 3;                             // a shorter split costs more than it saves
+
 struct MmaParams {
     TreeParams t;
-    int nsplit, row_tiles;
-    float* part;  // [nsplit][n_rows][H][HD], then [nsplit][n_rows][H][2]: top, sum (nsplit > 1)
+    int blocks, slots;  // blocks launched; rooms for the sums of a split item
+    float* part;        // [slots][128][HD], then [slots][128][2]: top, sum
+    int2* plan;         // [n_seq] first slot, splits of an item; null where no item can be split
 };
+
+struct TreeSpot {
+    int seq, rt, kvh, split, splits, slot, first_slot;
+};
+
+// Items and tiles of sequence s.
+__device__ __forceinline__ void tree_items(const MmaParams& mp, int T, int s, int& items, int& tiles) {
+    items = tiles = 0;
+    if (s >= mp.t.b.n_seq) return;
+    int r0, n;
+    kv_nodes(mp.t.b, mp.t.n_rows, s, r0, n);
+    const int len = kv_len(mp.t.kv, mp.t.b, s, n);
+    if (len < 0 || n == 0) return;
+    items = (n * mp.t.G + 127) / 128 * mp.t.kv.kv_heads;
+    tiles = (len + n + T - 1) / T;
+}
+
+__device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += y;
+    }
+    return v;
+}
+
+// Where block b works (by a whole warp); seq -1: nowhere.
+__device__ __forceinline__ TreeSpot tree_spot(const MmaParams& mp, int T, int b) {
+    const int lane = threadIdx.x & 31, n_seq = mp.t.b.n_seq;
+    int items0, tiles0;  // of sequence `lane`; of later ones again each time
+    tree_items(mp, T, lane, items0, tiles0);
+    auto of = [&](int s0, int& items, int& tiles) {
+        if (s0) tree_items(mp, T, s0 + lane, items, tiles);
+        else items = items0, tiles = tiles0;
+    };
+    unsigned all = 0, longest = 0;
+    float work = 0.f;
+    for (int s0 = 0; s0 < n_seq; s0 += 32) {
+        int items, tiles;
+        of(s0, items, tiles);
+        all += __reduce_add_sync(0xffffffffu, (unsigned)items);
+        longest = max(longest, __reduce_max_sync(0xffffffffu, (unsigned)tiles));
+        work += warp_sum((float)items * (float)tiles);
+    }
+    const int waves = min(max((int)((all + kTreeSms - 1) / kTreeSms), 1), kTreeWaves);
+    const int cap = all <= kTreeItems ? min((int)((all + kTreeSms - 1) / kTreeSms) * kTreeSms, mp.blocks) : mp.blocks;
+    int t = max(kTreeMinTiles, (int)ceilf(work / (float)(waves * kTreeSms)));
+    while (t < (int)longest) {
+        int blocks = 0, slots = 0;
+        for (int s0 = 0; s0 < n_seq; s0 += 32) {
+            int items, tiles;
+            of(s0, items, tiles);
+            const int k = (tiles + t - 1) / t;
+            blocks += __reduce_add_sync(0xffffffffu, items * k);
+            slots += __reduce_add_sync(0xffffffffu, k > 1 ? items * k : 0);
+        }
+        if (blocks <= cap && slots <= mp.slots) break;
+        t += max(1, t >> 4);
+    }
+    TreeSpot w = {-1, 0, 0, 0, 1, 0, 0};
+    int front = 0, slots = 0;
+    for (int s0 = 0; s0 < n_seq; s0 += 32) {
+        int items, tiles;
+        of(s0, items, tiles);
+        const int k = max(1, (tiles + t - 1) / t), mine = items * k;
+        const int end = warp_scan(mine, lane), send = warp_scan(k > 1 ? mine : 0, lane);
+        const unsigned hit = __ballot_sync(0xffffffffu, b < front + end);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            const int r = b - front - __shfl_sync(0xffffffffu, end - mine, src);
+            w.splits = __shfl_sync(0xffffffffu, k, src);
+            w.slot = slots + __shfl_sync(0xffffffffu, send - (k > 1 ? mine : 0), src);
+            w.seq = s0 + src;
+            w.split = r % w.splits;
+            const int item = r / w.splits;
+            w.kvh = item % mp.t.kv.kv_heads;
+            w.rt = item / mp.t.kv.kv_heads;
+            w.first_slot = w.slot;
+            w.slot += r;       // items in order, an item's splits side by side
+            break;
+        }
+        front += __shfl_sync(0xffffffffu, end, 31);
+        slots += __shfl_sync(0xffffffffu, send, 31);
+    }
+    return w;
+}
 
 // Which of positions p0 .. p0+63 the row sees, bit by bit.
 __device__ __forceinline__ unsigned long long tree_window(const TreeParams& p, int row, int node, int n, int len, int p0) {
@@ -406,17 +504,28 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
     // the same for a whole warp, which stays together
     auto wait_warp = [&](uint64_t* bar, int phase) -> bool { return __all_sync(0xffffffffu, wait(bar, phase)); };
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = blockIdx.x % mp.nsplit, rt = blockIdx.x / mp.nsplit, kvh = blockIdx.y, seq = blockIdx.z;
+    __shared__ TreeSpot spot;
+    if (warp == 0) {
+        const TreeSpot w = tree_spot(mp, T, blockIdx.x);
+        if (lane == 0) {
+            spot = w;
+            if (w.seq >= 0 && mp.plan && w.split == 0 && w.rt == 0 && w.kvh == 0) mp.plan[w.seq] = make_int2(w.first_slot, w.splits);
+        }
+    }
+    __syncthreads();
+    if (spot.seq < 0) return;
+    const int kvh = spot.kvh, seq = spot.seq;
 
     // the block's rows and tiles (the same in every thread)
     int r0, n;
     kv_nodes(p.b, p.n_rows, seq, r0, n);
     const int len = kv_len(p.kv, p.b, seq, n);
-    const int row_lo = rt * kMmaRows, row_hi = min(row_lo + kMmaRows, n * p.G);
+    const int row_lo = spot.rt * kMmaRows, row_hi = min(row_lo + kMmaRows, n * p.G);
     if (len < 0 || row_lo >= row_hi) return;
     const int end = p.mask ? len + n : len + (row_hi - 1) / p.G + 1;  // positions that some row may see
     const int nt_all = (end + T - 1) / T;
-    const int t0 = (int)((long long)nt_all * split / mp.nsplit), t1 = (int)((long long)nt_all * (split + 1) / mp.nsplit);
+    const int t0 = (int)((long long)nt_all * spot.split / spot.splits),
+              t1 = (int)((long long)nt_all * (spot.split + 1) / spot.splits);
     const int nt = t1 - t0;
     const int live_warps = (row_hi - row_lo + 31) / 32;  // of the 4 + 4 that work on rows; the others have none
     int bs = 0;  // tiles of a bit of bad[]: 1 << bs
@@ -684,18 +793,19 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
             }
         }
         if (ok) {
-            const float l = s_sum[ti], inv = mp.nsplit > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+            const int splits = spot.splits;
+            const float l = s_sum[ti], inv = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
             for (int i = 0; i < HD; i += 4)
                 *reinterpret_cast<float4*>(mine + i) =
                     make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
             __syncwarp();
             // out, or the split's place in the workspace: rows of HD values either way
-            const long long at = ((long long)split * p.n_rows + row) * p.H + head;
-            float* orow = !live ? nullptr : mp.nsplit == 1 ? p.out + (long long)row * p.os + (long long)head * HD : mp.part + at * HD;
-            const bool wide_out = mp.nsplit > 1 || ((reinterpret_cast<uintptr_t>(p.out) & 15) | (p.os & 3)) == 0;
-            if (live && mp.nsplit > 1)
-                *reinterpret_cast<float2*>(mp.part + (long long)mp.nsplit * p.n_rows * p.H * HD + at * 2) = make_float2(s_top[ti], l);
+            const long long at = (long long)spot.slot * kMmaRows + ti;
+            float* orow = !live ? nullptr : splits == 1 ? p.out + (long long)row * p.os + (long long)head * HD : mp.part + at * HD;
+            const bool wide_out = splits > 1 || ((reinterpret_cast<uintptr_t>(p.out) & 15) | (p.os & 3)) == 0;
+            if (live && splits > 1)
+                *reinterpret_cast<float2*>(mp.part + (long long)mp.slots * kMmaRows * HD + at * 2) = make_float2(s_top[ti], l);
             const int mine_rows = min(32, row_hi - row_lo - w * 32);
 #pragma unroll 4
             for (int i = 0; i < mine_rows; i += QR) {
@@ -1012,32 +1122,35 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(MmaParams mp) {
     const int lane = threadIdx.x & 31, seq = blockIdx.y;
     int r0, n;
     kv_nodes(p.b, p.n_rows, seq, r0, n);
-    if (kv_len(p.kv, p.b, seq, n) < 0) return;
-    const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int len = kv_len(p.kv, p.b, seq, n);
+    const int i = blockIdx.x * 8 + (threadIdx.x >> 5), r = i / p.H * p.G + i % p.H % p.G, kvh = i % p.H / p.G;
     pdl_wait();
-    if (i >= n * p.H) return;
+    if (len < 0 || i >= n * p.H) return;
+    const int2 plan = mp.plan[seq];
+    const int item = (r / kMmaRows) * p.kv.kv_heads + kvh;
+    if (plan.y <= 1 || plan.x < 0 || plan.x + (long long)(item + 1) * plan.y > mp.slots) return;
     const int row = r0 + i / p.H, head = i % p.H;
-    const long long step = (long long)p.n_rows * p.H, at = (long long)row * p.H + head;
+    const long long at = (plan.x + (long long)item * plan.y) * kMmaRows + r % kMmaRows;
     const float* o = mp.part + at * HD + lane * PER;
-    const float* ml = mp.part + mp.nsplit * step * HD + at * 2;
+    const float* ml = mp.part + (long long)mp.slots * kMmaRows * HD + at * 2;
     float top = -INFINITY;
-    for (int s = lane; s < mp.nsplit; s += 32) top = fmaxf(top, ml[s * step * 2]);
+    for (int s = lane; s < plan.y; s += 32) top = fmaxf(top, ml[s * (2 * kMmaRows)]);
     top = warp_max(top);
     float acc[PER], sum = 0.f;
 #pragma unroll
     for (int d = 0; d < PER; ++d) acc[d] = 0.f;
 #pragma unroll 4
-    for (int s = 0; s < mp.nsplit; ++s) {
-        const float2 x = *reinterpret_cast<const float2*>(ml + s * step * 2);
+    for (int s = 0; s < plan.y; ++s) {
+        const float2 x = *reinterpret_cast<const float2*>(ml + s * (2 * kMmaRows));
         if (x.y == 0.f && x.x == -INFINITY) continue;  // a split that the row sees nothing of
         const float c = ex2(x.x - top);
         sum = fmaf(c, x.y, sum);
         float v[PER];
         if (PER == 4) {
-            const float4 f = *reinterpret_cast<const float4*>(o + s * step * HD);
+            const float4 f = *reinterpret_cast<const float4*>(o + (long long)s * kMmaRows * HD);
             v[0] = f.x, v[1] = f.y, v[2 % PER] = f.z, v[3 % PER] = f.w;
         } else {
-            const float2 f = *reinterpret_cast<const float2*>(o + s * step * HD);
+            const float2 f = *reinterpret_cast<const float2*>(o + (long long)s * kMmaRows * HD);
             v[0] = f.x, v[1] = f.y;
         }
 #pragma unroll
@@ -1051,28 +1164,26 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(MmaParams mp) {
 
 // ------------------------------------------------------------------ launch
 
-// Splits of the positions: enough blocks for every SM, none below 4 tiles.
 struct TreePlan {
     bool mma;
-    int row_tiles, nsplit;
+    int blocks, slots;  // slots 0: nothing is split, no second launch
     size_t ws;
 };
 
 TreePlan tree_plan(const af_attention_tree_args& a) {
     TreePlan pl = {};
     const int hd = a.kv.head_dim, G = a.n_heads / a.kv.n_kv_heads;
-    pl.nsplit = 1;
     pl.mma = hd == 64 || hd == 128;
     if (!pl.mma) return pl;
     const long long cap = (long long)a.batch.max_blocks * a.kv.page_size;
     const long long max_len = a.max_len > 0 ? std::min((long long)a.max_len, cap) : cap;
-    pl.row_tiles = (int)(((long long)a.batch.max_nodes * G + kMmaRows - 1) / kMmaRows);
-    const long long base = (long long)pl.row_tiles * a.kv.n_kv_heads * std::max(1, a.batch.n_seq);
     const int T = hd == 128 ? 64 : 128;
-    const long long tiles = (max_len + T - 1) / T;
-    long long want = 148 / base;
-    pl.nsplit = (int)std::max(1ll, std::min({want, tiles / 2, 148ll}));
-    if (pl.nsplit > 1) pl.ws = (size_t)pl.nsplit * a.n_rows * a.n_heads * (hd + 2) * sizeof(float);
+    const long long tiles = (max_len + T - 1) / T, most = (tiles + kTreeMinTiles - 1) / kTreeMinTiles;
+    const long long items = ((long long)a.batch.max_nodes * G + kMmaRows - 1) / kMmaRows * a.kv.n_kv_heads * a.batch.n_seq;
+    const long long split = items <= kTreeItems ? (items + kTreeSms - 1) / kTreeSms * kTreeSms : items + 2 * kTreeItems;
+    pl.blocks = (int)std::min({split, items * std::max(1ll, most), (long long)INT_MAX});
+    if (most > 1) pl.slots = (int)std::min((long long)pl.blocks, 2ll * kTreeItems);
+    if (pl.slots) pl.ws = (size_t)pl.slots * kMmaRows * (hd + 2) * sizeof(float) + (size_t)a.batch.n_seq * sizeof(int2);
     return pl;
 }
 
@@ -1080,9 +1191,9 @@ template <int TYPE, int HD>
 cudaError_t mma_launch(const MmaParams& mp, int n_seq, int max_nodes, cudaStream_t st) {
     constexpr int smem = MmaShape<TYPE, HD>::BYTES;
     AF_CUDA_TRY(cudaFuncSetAttribute(tree_mma_kernel<TYPE, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    tree_mma_kernel<TYPE, HD><<<dim3(mp.nsplit * mp.row_tiles, mp.t.kv.kv_heads, n_seq), kMmaThreads, smem, st>>>(mp);
+    tree_mma_kernel<TYPE, HD><<<mp.blocks, kMmaThreads, smem, st>>>(mp);
     AF_CUDA_TRY(cudaGetLastError());
-    if (mp.nsplit == 1) return cudaSuccess;
+    if (!mp.slots) return cudaSuccess;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -1098,7 +1209,8 @@ cudaError_t mma_launch(const MmaParams& mp, int n_seq, int max_nodes, cudaStream
 template <int TYPE>
 cudaError_t tree_launch(const TreeParams& p, const TreePlan& pl, int max_nodes, void* ws, cudaStream_t st) {
     if (pl.mma) {
-        MmaParams mp = {p, pl.nsplit, pl.row_tiles, static_cast<float*>(ws)};
+        MmaParams mp = {p, pl.blocks, pl.slots, static_cast<float*>(ws), nullptr};
+        if (pl.slots) mp.plan = reinterpret_cast<int2*>(mp.part + (size_t)pl.slots * kMmaRows * (p.kv.hd + 2));
         return p.kv.hd == 64 ? mma_launch<TYPE, 64>(mp, p.b.n_seq, max_nodes, st) : mma_launch<TYPE, 128>(mp, p.b.n_seq, max_nodes, st);
     }
     tree_row_kernel<TYPE><<<dim3(p.n_rows, p.H), kTreeThreads, 0, st>>>(p);
