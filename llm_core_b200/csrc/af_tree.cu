@@ -2,6 +2,8 @@
 // (af_attention_tree_f32): the nodes of every sequence see its cached
 // positions and, by a bit mask, one another.
 #define AF_WHOLE_PROGRAM  // the register split below (setmaxnreg) holds only without separate compilation
+#include <cuda.h>
+
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -137,18 +139,21 @@ __global__ void __launch_bounds__(kTreeThreads) tree_row_kernel(TreeParams p) {
 // first, then the hi·hi ones, and the softmax warps add each tile's P·V to
 // sums in registers, which round to nearest.
 //
-// Warps (20): 0-3 turn scores into weights, one query row a thread; 4-7 bring
-// the queries in, add up the tiles' P·V and write the rows out; 8-15 load K
-// and V, page by page, with cp.async (48-64 KB an SM in flight for f32, 96 KB
-// otherwise) and put them into the form that the products take: a lane works
-// on the 16 bytes that it copied itself; 16 issues the products.  Registers a
-// thread: 112 / 184 / 72 / 40 (setmaxnreg; 128 threads of the first two kinds,
-// 256 and 128: 61,440, the launch's 640·96; head_dim 64 has tiles of 128
-// positions and half the sums, so the first two change places).
+// Warps (20): 0-3 turn scores into weights, one query row a thread; 4-7 add up
+// the tiles' P·V and write the rows out; 8-15 put K and V into the form that the
+// products take (split, scaled; a cache in f16 only has its V looked through);
+// 16 issues the products; 17 the copies: a box of rows per page by the TMA
+// engine (rows of a warp by cp.async cost 60 cycles of issue each and filled
+// the load pipe that every other warp waits for; single rows by bulk copies
+// run at 2.3 TB/s).  Registers a thread: 112 / 184 / 72 / 40 (setmaxnreg; 128
+// threads of the first two kinds, 256 and 128: 61,440, the launch's 640·96;
+// head_dim 64 has tiles of 128 positions and half the sums, so the first two
+// change places).
 //
-// Shared-memory tiles: 8-row × 16-byte core matrices without swizzle, 144
-// bytes apart along the row (16 bytes of padding: the stores of a warp then
-// fall into all banks) — K-major for K, and the same tile MN-major for V.
+// Tiles in shared memory: rows of 64 values (128 bytes) in the 128-byte
+// swizzle, K-major for K, the same tile MN-major for V; for f32 the TMA engine
+// leaves rows as they are in a place of their own (64 KB, half a tile's K and
+// half its V in flight) and the splitting warps write the tiles.
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -224,9 +229,10 @@ __device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
     return r;
 }
 
-// No-swizzle descriptor: strides in bytes, version 1.
+// Descriptor of a tile in the 128-byte swizzle: strides in bytes, version 1.
 __device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | (1ull << 46);
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | (1ull << 46) |
+           (2ull << 61);
 }
 
 // 32 consecutive columns of this thread's lane.
@@ -294,20 +300,19 @@ struct MmaShape {
     static constexpr int SIZE = F32 ? 4 : 2;
     static constexpr int T = HD == 128 ? 64 : 128;      // positions of a tile
     static constexpr int TERMS = F32 ? 2 : 1;           // hi, lo of K and V
-    static constexpr int CS = 144;                      // between 16-byte columns of a tile
-    static constexpr int RS = HD / 8 * CS;              // between groups of 8 rows
-    static constexpr int TILE = T / 8 * RS;             // 18,432
+    static constexpr int COLS = T * 128;                // 64 values of every row
+    static constexpr int TILE = HD / 64 * COLS;         // 16,384
     static constexpr int HALF = TERMS * TILE;           // K or V of a tile: hi, lo
-    static constexpr int NB = F32 ? 2 : 5;              // tiles in shared memory: K V K V ...
-    static constexpr int AHEAD = NB - 2;                // 16-bit caches: tiles whose copies are in flight
-    static constexpr int RPW = T / 8;                   // rows of a loading warp in a tile
-    static constexpr int LPR = HD * SIZE / 16;          // lanes of a row
-    static constexpr int RPC = 32 / LPR;                // rows of one copy of a warp (512 bytes)
-    static constexpr int NCK = RPW / RPC;               // copies of a lane for K (and for V): 8 or 4
-    // queries in, rows out: 128 rows with 16 bytes of padding, over the last tiles' place
-    static constexpr int QROW = HD * 4 + 16;
+    static constexpr int NB = F32 ? 2 : 6;              // tiles in shared memory: K V K V ...
+    static constexpr int RAWS = 2;                      // f32: halves of a tile as they are
+    static constexpr int RAWB = T * HD * 4;             // 32,768
+    static constexpr int RPW = T / 8;                   // rows of a splitting warp in a tile
+    static constexpr int LPR = HD * SIZE / 16;          // lanes of a row (f32)
+    static constexpr int RPC = 32 / LPR;                // rows of a warp's 512 bytes (f32)
+    // queries in, rows out: 128 rows over the last tiles' place, 16-byte columns swizzled by the row
+    static constexpr int QROW = HD * 4;
     static constexpr int QTILE = NB - (kMmaRows * QROW + 2 * HALF - 1) / (2 * HALF);
-    static_assert(QTILE >= (F32 ? 1 : AHEAD), "the first copies do not wait for the queries");
+    static_assert(QTILE >= 1, "the first tile does not wait for the queries");
     // registers
     static constexpr int REG_S = HD == 128 ? 112 : 184, REG_O = HD == 128 ? 184 : 112;
     // tensor memory columns
@@ -317,21 +322,20 @@ struct MmaShape {
     // shared memory, behind 512 bytes of mbarriers
     static constexpr int BAD = 512;                       // kMmaBadWords words
     static constexpr int ROWS = BAD + kMmaBadWords * 4;   // [128] query scales, [NS][128] corrections, [128] tops, [128] sums
-    static constexpr int GROUPS = 8;                      // a loading warp's rows share their powers of two
-    static constexpr int SCALE = ROWS + (3 + NS) * kMmaRows * 4; // [2 NB][3][GROUPS] floats
-    static constexpr int TILES = (SCALE + (TYPE == AF_KV_F16 ? 0 : 2 * NB * 3 * GROUPS * 4) + 127) / 128 * 128;
-    static constexpr int RAW = TILES + NB * 2 * HALF;     // f32: 8 warps x 16 copies x 512 bytes as they are
-    static constexpr int BYTES = RAW + (F32 ? 65536 : 0);
-    static_assert(BYTES <= 227 * 1024 - 64, "shared memory");
+    static constexpr int GROUPS = 8;                      // a splitting warp's rows share their powers of two
+    static constexpr int SCALE = ROWS + (3 + NS) * kMmaRows * 4;  // [2 NB][3][GROUPS] floats
+    static constexpr int TILES = (SCALE + 2 * NB * 3 * GROUPS * 4 + 1023) / 1024 * 1024;
+    static constexpr int RAW = TILES + NB * 2 * HALF;
+    static constexpr int BYTES = RAW + (F32 ? RAWS * RAWB : 0);
+    static_assert(BYTES <= 227 * 1024 - 128, "shared memory");
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// A box of rows of one kv head (TMA engine): x value, y head, z row.
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
 }
 
 // Zeros for what is not finite; the largest of the rest, over the warp.
@@ -359,7 +363,9 @@ constexpr int kTreeItems = kTreeSms * kTreeWaves;
 constexpr int kTreeMinTiles = 3;                             // a shorter split costs more than it saves
 
 struct MmaParams {
+    CUtensorMap k_map, v_map;  // [rows of the layer's pool][kv heads][HD], boxes of box_rows rows
     TreeParams t;
+    int box_rows;
     int blocks, slots;  // blocks launched; rooms for the sums of a split item
     float* part;        // [slots][128][HD], then [slots][128][2]: top, sum
     int2* plan;         // [n_seq] first slot, splits of an item; null where no item can be split
@@ -367,18 +373,28 @@ struct MmaParams {
 
 struct TreeSpot {
     int seq, rt, kvh, split, splits, slot, first_slot;
+    int r0, n, len;  // the sequence's rows and cached positions
 };
 
-// Items and tiles of sequence s.
-__device__ __forceinline__ void tree_items(const MmaParams& mp, int T, int s, int& items, int& tiles) {
-    items = tiles = 0;
-    if (s >= mp.t.b.n_seq) return;
-    int r0, n;
-    kv_nodes(mp.t.b, mp.t.n_rows, s, r0, n);
-    const int len = kv_len(mp.t.kv, mp.t.b, s, n);
-    if (len < 0 || n == 0) return;
-    items = (n * mp.t.G + 127) / 128 * mp.t.kv.kv_heads;
-    tiles = (len + n + T - 1) / T;
+// Rows, items and tiles of sequence s.
+struct TreeSeq {
+    int r0, n, len, items, tiles;
+};
+__device__ __forceinline__ TreeSeq tree_seq(const MmaParams& mp, int T, int s) {
+    TreeSeq q = {};
+    const KvBatch& b = mp.t.b;
+    if (s >= b.n_seq) return q;
+    q.len = b.len[s];  // beside the counts, not behind them
+    kv_nodes(b, mp.t.n_rows, s, q.r0, q.n);
+    if (q.len < 0 || (long long)q.len + q.n > ((long long)b.max_blocks << mp.t.kv.ps_shift)) {
+        set_err_at(b.err, kErrBadArgs);
+        q.n = 0;
+    }
+    if (q.n) {
+        q.items = (q.n * mp.t.G + kMmaRows - 1) / kMmaRows * mp.t.kv.kv_heads;
+        q.tiles = (q.len + q.n + T - 1) / T;
+    }
+    return q;
 }
 
 __device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
@@ -393,62 +409,70 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
 // Where block b works (by a whole warp); seq -1: nowhere.
 __device__ __forceinline__ TreeSpot tree_spot(const MmaParams& mp, int T, int b) {
     const int lane = threadIdx.x & 31, n_seq = mp.t.b.n_seq;
-    int items0, tiles0;  // of sequence `lane`; of later ones again each time
-    tree_items(mp, T, lane, items0, tiles0);
-    auto of = [&](int s0, int& items, int& tiles) {
-        if (s0) tree_items(mp, T, s0 + lane, items, tiles);
-        else items = items0, tiles = tiles0;
-    };
-    unsigned all = 0, longest = 0;
+    const TreeSeq first = tree_seq(mp, T, lane);  // of sequence `lane`; later ones are looked up each time
+    auto of = [&](int s0) { return s0 ? tree_seq(mp, T, s0 + lane) : first; };
+    int all = 0, longest = 0;
     float work = 0.f;
     for (int s0 = 0; s0 < n_seq; s0 += 32) {
-        int items, tiles;
-        of(s0, items, tiles);
-        all += __reduce_add_sync(0xffffffffu, (unsigned)items);
-        longest = max(longest, __reduce_max_sync(0xffffffffu, (unsigned)tiles));
-        work += warp_sum((float)items * (float)tiles);
+        const TreeSeq q = of(s0);
+        all += __reduce_add_sync(0xffffffffu, q.items);
+        longest = max(longest, __reduce_max_sync(0xffffffffu, q.tiles));
+        work += warp_sum((float)q.items * (float)q.tiles);
     }
-    const int waves = min(max((int)((all + kTreeSms - 1) / kTreeSms), 1), kTreeWaves);
-    const int cap = all <= kTreeItems ? min((int)((all + kTreeSms - 1) / kTreeSms) * kTreeSms, mp.blocks) : mp.blocks;
-    int t = max(kTreeMinTiles, (int)ceilf(work / (float)(waves * kTreeSms)));
-    while (t < (int)longest) {
+    const int need = (all + kTreeSms - 1) / kTreeSms, waves = min(max(need, 1), kTreeWaves);
+    const int cap = all <= kTreeItems ? min(need * kTreeSms, mp.blocks) : mp.blocks;
+    // the splits of an item at 1/t tiles each: one rule for everybody, whatever it rounds to
+    auto splits_of = [](int tiles, float inv_t) { return max(1, (int)ceilf((float)tiles * inv_t - 1e-4f)); };
+    const float t_min = fmaxf((float)kTreeMinTiles, work / (float)(waves * kTreeSms));
+    float inv_t = 0.f;  // nothing is split
+    // 32 candidates, a lane each, 1/32 further apart every time: the first that fits
+    for (float base = t_min; base < (float)longest; base *= 2.f) {
+        const float mine = 1.f / (base * (1.f + (float)lane * (1.f / 32.f)));
         int blocks = 0, slots = 0;
         for (int s0 = 0; s0 < n_seq; s0 += 32) {
-            int items, tiles;
-            of(s0, items, tiles);
-            const int k = (tiles + t - 1) / t;
-            blocks += __reduce_add_sync(0xffffffffu, items * k);
-            slots += __reduce_add_sync(0xffffffffu, k > 1 ? items * k : 0);
+            const TreeSeq q = of(s0);
+            const int m = min(32, n_seq - s0);
+            for (int j = 0; j < m; ++j) {
+                const int items = __shfl_sync(0xffffffffu, q.items, j), tiles = __shfl_sync(0xffffffffu, q.tiles, j);
+                const int k = splits_of(tiles, mine);
+                blocks += items * k;
+                slots += k > 1 ? items * k : 0;
+            }
         }
-        if (blocks <= cap && slots <= mp.slots) break;
-        t += max(1, t >> 4);
+        const unsigned fits = __ballot_sync(0xffffffffu, blocks <= cap && slots <= mp.slots);
+        if (fits) {
+            inv_t = __shfl_sync(0xffffffffu, mine, __ffs(fits) - 1);
+            break;
+        }
     }
-    TreeSpot w = {-1, 0, 0, 0, 1, 0, 0};
+    TreeSpot w = {};
+    w.seq = -1;
     int front = 0, slots = 0;
     for (int s0 = 0; s0 < n_seq; s0 += 32) {
-        int items, tiles;
-        of(s0, items, tiles);
-        const int k = max(1, (tiles + t - 1) / t), mine = items * k;
-        const int end = warp_scan(mine, lane), send = warp_scan(k > 1 ? mine : 0, lane);
+        const TreeSeq q = of(s0);
+        const int k = splits_of(q.tiles, inv_t), mine = q.items * k, split = k > 1 ? mine : 0;
+        const int end = warp_scan(mine, lane), send = warp_scan(split, lane);
         const unsigned hit = __ballot_sync(0xffffffffu, b < front + end);
         if (hit) {
             const int src = __ffs(hit) - 1;
-            const int r = b - front - __shfl_sync(0xffffffffu, end - mine, src);
-            w.splits = __shfl_sync(0xffffffffu, k, src);
-            w.slot = slots + __shfl_sync(0xffffffffu, send - (k > 1 ? mine : 0), src);
-            w.seq = s0 + src;
-            w.split = r % w.splits;
-            const int item = r / w.splits;
-            w.kvh = item % mp.t.kv.kv_heads;
-            w.rt = item / mp.t.kv.kv_heads;
-            w.first_slot = w.slot;
-            w.slot += r;       // items in order, an item's splits side by side
+            if (lane == src) {  // items in order, an item's splits side by side
+                const int r = b - front - (end - mine), item = r / k;
+                w.seq = s0 + src;
+                w.splits = k;
+                w.split = r - item * k;
+                w.rt = item / mp.t.kv.kv_heads;
+                w.kvh = item - w.rt * mp.t.kv.kv_heads;
+                w.first_slot = slots + send - split;
+                w.slot = w.first_slot + r;
+                w.r0 = q.r0, w.n = q.n, w.len = q.len;
+            }
+            w.seq = __shfl_sync(0xffffffffu, w.seq, src);
             break;
         }
         front += __shfl_sync(0xffffffffu, end, 31);
         slots += __shfl_sync(0xffffffffu, send, 31);
     }
-    return w;
+    return w;  // whole in the lane whose first_slot, n, ... are set: the one that `src` was
 }
 
 // Which of positions p0 .. p0+63 the row sees, bit by bit.
@@ -469,19 +493,22 @@ __device__ __forceinline__ unsigned long long tree_window(const TreeParams& p, i
 }
 
 template <int TYPE, int HD>
-__global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) {
+__global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_constant__ MmaParams mp) {
     using SH = MmaShape<TYPE, HD>;
     using E = KvElem<TYPE>;
-    constexpr int T = SH::T, NB = SH::NB, NCK = SH::NCK, NS = SH::NS;
+    constexpr int T = SH::T, NB = SH::NB, NS = SH::NS;
     extern __shared__ __align__(1024) uint8_t sm[];
     const TreeParams& p = mp.t;
     // A waiter never falls a whole ring behind: K of t + NB may be there before the softmax looks for K of t, so
     // its barriers (and the scales) are 2 NB; every other one's next phase needs what the waiter of this one does.
-    uint64_t* k_full = reinterpret_cast<uint64_t*>(sm);  // [2 NB] 8 loading warps: K of a tile is there
-    uint64_t* v_full = k_full + 2 * NB;                  // [NB] V
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(sm);  // [2 NB] K of a tile is ready: 8 splitting warps (f16: the copy)
+    uint64_t* v_full = k_full + 2 * NB;                  // [NB] V, 8 splitting warps
     uint64_t* k_empty = v_full + NB;                     // [NB] scores done
     uint64_t* v_empty = k_empty + NB;                    // [NB] P·V done
-    uint64_t* s_full = v_empty + NB;                     // [NS] scores done
+    uint64_t* k_land = v_empty + NB;                     // [NB] copies of K (bf16) or of a half (f32: RAWS) landed
+    uint64_t* v_land = k_land + NB;                      // [NB] copies of V landed
+    uint64_t* raw_free = v_land + NB;                    // [RAWS] f32: 8 splitting warps have a half in registers
+    uint64_t* s_full = raw_free + SH::RAWS;              // [NS] scores done
     uint64_t* p_full = s_full + NS;                      // [NS] softmax warps: weights written
     uint64_t* c_full = p_full + NS;                      // [NS] softmax warps: correction written
     uint64_t* o_full = c_full + NS;                      // P·V done
@@ -489,7 +516,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
     uint64_t* q_full = o_free + 1;                       // 8 softmax and output warps: queries written
     uint64_t* fin = q_full + 1;                          // softmax warps: tops and sums written
     uint64_t* done = fin + 1;                            // every product done
-    static_assert((5 * NB + 3 * NS + 5) * 8 + 8 <= SH::BAD, "barriers");
+    static_assert((7 * NB + 3 * NS + 5 + SH::RAWS) * 8 + 16 <= SH::BAD, "barriers");
     uint32_t* tslot = reinterpret_cast<uint32_t*>(done + 1);
     volatile int* flag = reinterpret_cast<volatile int*>(tslot + 1);
     uint32_t* bad = reinterpret_cast<uint32_t*>(sm + SH::BAD);
@@ -500,120 +527,128 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
     float* scales = reinterpret_cast<float*>(sm + SH::SCALE);
     uint8_t* tiles = sm + SH::TILES;
     uint8_t* staged = tiles + SH::QTILE * 2 * SH::HALF;
+    auto staged_at = [&](int row, int byte) { return staged + row * SH::QROW + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15); };
     auto wait = [&](uint64_t* bar, int phase) -> bool { return mbar_wait_at(bar, (uint32_t)phase & 1u, p.b.err, flag); };
     // the same for a whole warp, which stays together
     auto wait_warp = [&](uint64_t* bar, int phase) -> bool { return __all_sync(0xffffffffu, wait(bar, phase)); };
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     __shared__ TreeSpot spot;
+    pdl_launch_dependents();
     if (warp == 0) {
         const TreeSpot w = tree_spot(mp, T, blockIdx.x);
-        if (lane == 0) {
+        if (w.seq < 0 ? lane == 0 : w.splits > 0) {
             spot = w;
             if (w.seq >= 0 && mp.plan && w.split == 0 && w.rt == 0 && w.kvh == 0) mp.plan[w.seq] = make_int2(w.first_slot, w.splits);
         }
+    } else if (warp == 1 && lane == 0) {
+        for (int i = 0; i < NB; ++i) {
+            mbar_init(&k_full[i], TYPE == AF_KV_F16 ? 1 : 8);
+            mbar_init(&k_full[NB + i], TYPE == AF_KV_F16 ? 1 : 8);
+            mbar_init(&v_full[i], 8);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_empty[i], 1);
+            mbar_init(&k_land[i], 1);
+            mbar_init(&v_land[i], 1);
+        }
+        for (int i = 0; i < SH::RAWS; ++i) mbar_init(&raw_free[i], 8);
+        for (int i = 0; i < NS; ++i) mbar_init(&s_full[i], 1);
+        mbar_init(o_full, 1);
+        mbar_init(q_full, 8);
+        mbar_init(done, 1);
+        *flag = 0;
+    } else if (warp == 16) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else if (warp == 17 && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&mp.k_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&mp.v_map) : "memory");
     }
+    for (int i = tid; i < kMmaBadWords; i += kMmaThreads) bad[i] = 0;
     __syncthreads();
-    if (spot.seq < 0) return;
-    const int kvh = spot.kvh, seq = spot.seq;
-
+    const int seq = spot.seq, kvh = spot.kvh, r0 = spot.r0, n = spot.n, len = spot.len;
     // the block's rows and tiles (the same in every thread)
-    int r0, n;
-    kv_nodes(p.b, p.n_rows, seq, r0, n);
-    const int len = kv_len(p.kv, p.b, seq, n);
     const int row_lo = spot.rt * kMmaRows, row_hi = min(row_lo + kMmaRows, n * p.G);
-    if (len < 0 || row_lo >= row_hi) return;
+    const int live_warps = (row_hi - row_lo + 31) / 32;  // of the 4 + 4 that work on rows; the others have none
+    if (tid == 0 && seq >= 0) {
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&p_full[i], live_warps);
+            mbar_init(&c_full[i], live_warps);
+        }
+        mbar_init(o_free, live_warps);
+        mbar_init(fin, live_warps);
+    }
+    if (tid < 64) fence_mbar_init();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tslot;
+    if (seq < 0) {
+        if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        return;
+    }
     const int end = p.mask ? len + n : len + (row_hi - 1) / p.G + 1;  // positions that some row may see
     const int nt_all = (end + T - 1) / T;
     const int t0 = (int)((long long)nt_all * spot.split / spot.splits),
               t1 = (int)((long long)nt_all * (spot.split + 1) / spot.splits);
     const int nt = t1 - t0;
-    const int live_warps = (row_hi - row_lo + 31) / 32;  // of the 4 + 4 that work on rows; the others have none
     int bs = 0;  // tiles of a bit of bad[]: 1 << bs
     while (nt > (kMmaBadWords * 32) << bs) ++bs;
-    pdl_launch_dependents();
-
-    if (tid == 0) {
-        for (int i = 0; i < NB; ++i) {
-            mbar_init(&k_full[i], 8);
-            mbar_init(&k_full[NB + i], 8);
-            mbar_init(&v_full[i], 8);
-            mbar_init(&k_empty[i], 1);
-            mbar_init(&v_empty[i], 1);
-        }
-        for (int i = 0; i < NS; ++i) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], live_warps);
-            mbar_init(&c_full[i], live_warps);
-        }
-        mbar_init(o_full, 1);
-        mbar_init(o_free, live_warps);
-        mbar_init(q_full, 8);
-        mbar_init(fin, live_warps);
-        mbar_init(done, 1);
-        *flag = 0;
-        fence_mbar_init();
-    }
-    for (int i = tid; i < kMmaBadWords; i += kMmaThreads) bad[i] = 0;
-    if (warp == 16) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(512u)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *tslot;
 
     // Queries, by the softmax and output warps: a row a warp in turn — its largest value, hi and lo — into the staging
     // place, from there a row a thread (hi by one kind of warps, lo by the other) into tensor memory.  Rows that are
     // none keep what is there: what comes of them stays in their own row.
     auto queries = [&]() {
-        constexpr int Q4 = HD / 4, QR = 32 / Q4;  // lanes of a row at 16 bytes each, rows of a warp's load
+        constexpr int Q4 = HD / 4, QR = 32 / Q4, QN = 16 / QR;  // lanes of a row at 16 bytes, rows and number of a warp's loads
         const int sub = lane / Q4, col = lane % Q4, rows = row_hi - row_lo;
         const bool wide = ((reinterpret_cast<uintptr_t>(p.q) & 15) | (p.qs & 3)) == 0;
-#pragma unroll 1
-        for (int i0 = warp * QR; i0 < rows; i0 += 4 * 8 * QR) {
-            float4 f[4];
+        float4 f[QN];  // all in flight
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int x = row_lo + min(i0 + j * 8 * QR + sub, rows - 1);
-                const float* q = p.q + (long long)(r0 + x / p.G) * p.qs + (long long)(kvh * p.G + x % p.G) * HD + 4 * col;
-                if (wide) f[j] = __ldg(reinterpret_cast<const float4*>(q));
-                else f[j] = make_float4(q[0], q[1], q[2], q[3]);
-            }
+        for (int j = 0; j < QN; ++j) {
+            if ((warp + 8 * j) * QR >= rows) break;
+            const int x = row_lo + min((warp + 8 * j) * QR + sub, rows - 1), node = x / p.G;
+            const float* q = p.q + (long long)(r0 + node) * p.qs + (kvh * p.G + x - node * p.G) * HD + 4 * col;
+            if (wide) f[j] = __ldg(reinterpret_cast<const float4*>(q));
+            else f[j] = make_float4(q[0], q[1], q[2], q[3]);
+        }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = i0 + j * 8 * QR + sub;
-                float big = max3_abs_nan(max3_abs_nan(0.f, f[j].x, f[j].y), f[j].z, f[j].w);
-                uint32_t mx = __float_as_uint(big);
+        for (int j = 0; j < QN; ++j) {
+            if ((warp + 8 * j) * QR >= rows) break;
+            const int i = (warp + 8 * j) * QR + sub;
+            uint32_t mx = __float_as_uint(max3_abs_nan(max3_abs_nan(0.f, f[j].x, f[j].y), f[j].z, f[j].w));
+            if (QR == 1) {
+                mx = __reduce_max_sync(0xffffffffu, mx);
+            } else {
 #pragma unroll
                 for (int o = 1; o < Q4; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                const int a = scale_of(mx, 100);
-                const f32x2 s = pair(pow2(a), pow2(a));
-                uint2 hi, lo;
-                split2(mul2(pair(f[j].x, f[j].y), s), hi.x, lo.x);
-                split2(mul2(pair(f[j].z, f[j].w), s), hi.y, lo.y);
-                if (i < rows) {
-                    *reinterpret_cast<uint2*>(staged + i * SH::QROW + 8 * col) = hi;
-                    *reinterpret_cast<uint2*>(staged + i * SH::QROW + 2 * HD + 8 * col) = lo;
-                    if (col == 0) s_rs[i] = p.scale * pow2(-a);
-                }
+            }
+            const int a = scale_of(mx, 100);
+            const f32x2 s = pair(pow2(a), pow2(a));
+            uint2 hi, lo;
+            split2(mul2(pair(f[j].x, f[j].y), s), hi.x, lo.x);
+            split2(mul2(pair(f[j].z, f[j].w), s), hi.y, lo.y);
+            if (i < rows) {
+                *reinterpret_cast<uint2*>(staged_at(i, 8 * col)) = hi;
+                *reinterpret_cast<uint2*>(staged_at(i, 2 * HD + 8 * col)) = lo;
+                if (col == 0) s_rs[i] = p.scale * pow2(-a);
             }
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
         const int mine = tid & 127;
         if ((mine & ~31) < rows) {
-            const uint8_t* from = staged + mine * SH::QROW + (warp < 4 ? 0 : 2 * HD);
+            const int from = warp < 4 ? 0 : 2 * HD;
             const uint32_t to = tmem + ((uint32_t)(mine & ~31) << 16) + (warp < 4 ? SH::QH : SH::QL);
 #pragma unroll 2
             for (int c = 0; c < HD / 16; ++c) {
-                const uint4 x = *reinterpret_cast<const uint4*>(from + 32 * c), y = *reinterpret_cast<const uint4*>(from + 32 * c + 16);
+                const uint4 x = *reinterpret_cast<const uint4*>(staged_at(mine, from + 32 * c));
+                const uint4 y = *reinterpret_cast<const uint4*>(staged_at(mine, from + 32 * c + 16));
                 const uint32_t v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
                 tc_st8(to + 8 * c, v);
             }
             tc_wait_st();
         }
         tc_fence_before();
+        fence_proxy_async_smem();  // the copies may write over the staging place now
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
     };
@@ -629,22 +664,31 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         const float rs = s_rs[tid];  // what a raw score is times, but for K's power of two
-        for (int t = 0; ok && t < nt && warp < live_warps; ++t) {
+        // weights written: said a little late, when the next scores are on their way
+        auto publish = [&](int t) {
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[t % NS]);
+        };
+        const int tiles_mine = warp < live_warps ? nt : 0;
+        for (int t = 0; ok && t < tiles_mine; ++t) {
             const int st = t % NB, sl = t % NS;
-            ok = wait_warp(&k_full[t % (2 * NB)], t / (2 * NB)) && wait_warp(&s_full[sl], t / NS);
+            ok = (TYPE == AF_KV_F16 || wait_warp(&k_full[t % (2 * NB)], t / (2 * NB))) && wait_warp(&s_full[sl], t / NS);
             if (!ok) break;
             tc_fence_after();
             const uint32_t sb = tmem + lanes + SH::S0 + sl * T;
             float v[T];
 #pragma unroll
             for (int c = 0; c < T / 32; ++c) tc_ld32(sb + 32 * c, v + 32 * c);
+            if (t) publish(t - 1);
             tc_wait_ld();
 #pragma unroll
             for (int i = 0; i < T; ++i) asm volatile("" : "+f"(v[i]));  // no use may move above the wait
             const float4* kc = reinterpret_cast<const float4*>(scales + (t % (2 * NB)) * 3 * SH::GROUPS);  // 2^-a of K
             const float4* vf = kc + SH::GROUPS / 4;                                                        // -a of V
             const float4* vg = vf + SH::GROUPS / 4;                                                        // 2^a of V
-            ok = wait_warp(&v_full[st], t / NB);
+            if (TYPE != AF_KV_F16) ok = wait_warp(&v_full[st], t / NB);
             if (!ok) break;
             {
                 float c[8], f[8];
@@ -721,34 +765,26 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
                 unpair(add2(sum[0], sum[1]), a, b);
                 l = fmaf(l, corr, a + b);
             }
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[sl]);
         }
+        if (ok && tiles_mine) publish(tiles_mine - 1);
         if (!ok) *flag = 1;
         s_top[tid] = m;
         s_sum[tid] = l;
         __syncwarp();
         if (lane == 0 && warp < live_warps) mbar_arrive(fin);
     } else if (warp < 8) {
-        // ------------------------------------------- queries in, sums, rows out
+        // ------------------------------------------------ sums, rows out
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH::REG_O));
         queries();
         constexpr int Q4 = HD / 4, QR = 32 / Q4;  // lanes of a row at 16 bytes each, rows of a warp's store
         const int w = warp - 4, ti = tid - 128;
         const uint32_t lanes = (uint32_t)(w * 32) << 16;
         const int sub = lane / Q4, col = lane % Q4;
-        uint8_t* wrow = staged + w * 32 * SH::QROW;
-        float* mine = reinterpret_cast<float*>(staged + ti * SH::QROW);
-        const int r = row_lo + ti;
-        const bool live = r < row_hi;
-        const int node = live ? r / p.G : 0, row = r0 + node, head = kvh * p.G + (live ? r % p.G : 0);
         float acc[HD];
 #pragma unroll
         for (int i = 0; i < HD; ++i) acc[i] = 0.f;
-        bool ok = true;
-        for (int t = 0; t < nt && w < live_warps; ++t) {  // acc = acc·corr + (P·V)(t)
+        bool ok = w < live_warps;
+        for (int t = 0; ok && t < nt; ++t) {  // acc = acc·corr + (P·V)(t)
             ok = wait_warp(&c_full[t % NS], t / NS) && wait_warp(o_full, t);
             if (!ok) break;
             tc_fence_after();
@@ -771,8 +807,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
             __syncwarp();
             if (lane == 0) mbar_arrive(o_free);
         }
-        ok = ok && w < live_warps && wait_warp(fin, 0);
+        ok = ok && wait_warp(fin, 0);
         if (!ok && w < live_warps) *flag = 1;
+        const int r = row_lo + ti;
+        const bool live = r < row_hi;
+        const int node = live ? r / p.G : 0, row = r0 + node, head = kvh * p.G + (live ? r % p.G : 0);
         // non-finite values of V were taken out of the products: the rows that see them get them back
         for (int wd = 0; ok && wd < kMmaBadWords && (32 * wd) << bs < nt; ++wd) {
             uint32_t b = bad[wd];
@@ -793,104 +832,76 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
             }
         }
         if (ok) {
-            const int splits = spot.splits;
+            const int splits = spot.splits, mine_rows = min(32, row_hi - row_lo - w * 32);
             const float l = s_sum[ti], inv = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
             for (int i = 0; i < HD; i += 4)
-                *reinterpret_cast<float4*>(mine + i) =
+                *reinterpret_cast<float4*>(staged_at(ti, 4 * i)) =
                     make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
             __syncwarp();
-            // out, or the split's place in the workspace: rows of HD values either way
-            const long long at = (long long)spot.slot * kMmaRows + ti;
-            float* orow = !live ? nullptr : splits == 1 ? p.out + (long long)row * p.os + (long long)head * HD : mp.part + at * HD;
-            const bool wide_out = splits > 1 || ((reinterpret_cast<uintptr_t>(p.out) & 15) | (p.os & 3)) == 0;
-            if (live && splits > 1)
-                *reinterpret_cast<float2*>(mp.part + (long long)mp.slots * kMmaRows * HD + at * 2) = make_float2(s_top[ti], l);
-            const int mine_rows = min(32, row_hi - row_lo - w * 32);
+            auto from = [&](int i) { return *reinterpret_cast<const float4*>(staged_at(w * 32 + i + sub, 16 * col)); };
+            if (splits > 1) {  // the split's place in the workspace, rows of HD values side by side
+                const long long at = (long long)spot.slot * kMmaRows + w * 32;
+                float* o = mp.part + (at + sub) * HD + 4 * col;
+#pragma unroll 8
+                for (int i = 0; i < mine_rows; i += QR)
+                    if (i + sub < mine_rows)
+                        *reinterpret_cast<float4*>(o + i * HD) = from(i);
+                if (lane < mine_rows)
+                    *reinterpret_cast<float2*>(mp.part + (long long)mp.slots * kMmaRows * HD + (at + lane) * 2) =
+                        make_float2(s_top[ti], l);
+            } else {
+                float* orow = live ? p.out + (long long)row * p.os + (long long)head * HD : nullptr;
+                const bool wide_out = ((reinterpret_cast<uintptr_t>(p.out) & 15) | (p.os & 3)) == 0;
 #pragma unroll 4
-            for (int i = 0; i < mine_rows; i += QR) {
-                float* o = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), i + sub));
-                const float4 f = *reinterpret_cast<const float4*>(wrow + (i + sub) * SH::QROW + 16 * col);
-                if (o) {
-                    o += 4 * col;
-                    if (wide_out) *reinterpret_cast<float4*>(o) = f;
-                    else o[0] = f.x, o[1] = f.y, o[2] = f.z, o[3] = f.w;
+                for (int i = 0; i < mine_rows; i += QR) {
+                    float* o = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), i + sub));
+                    const float4 f = from(i);
+                    if (o) {
+                        o += 4 * col;
+                        if (wide_out) *reinterpret_cast<float4*>(o) = f;
+                        else o[0] = f.x, o[1] = f.y, o[2] = f.z, o[3] = f.w;
+                    }
                 }
             }
         }
     } else if (warp < 16) {
-        // ------------------------------------------------------- K and V
+        // ------------------------------------------------- splitting K and V
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        const int w = warp - 8, sub = lane / SH::LPR, col = lane % SH::LPR;
-        const long long hoff = p.layer * p.kv.layer_bytes + (long long)kvh * HD * SH::SIZE + col * 16;
-        const uint8_t* kb = p.kv.k + hoff;
-        const uint8_t* vb = p.kv.v + hoff;
-        // Rows of a tile for the warp, one a lane (lane < RPW).  fetch() asks for the page early; row() makes it a
-        // pool row when it is needed: behind the last position the last one again (no weight reaches it), for a
-        // page that is none row 0 and the error word.
-        const int off = w * SH::RPW + min(lane, SH::RPW - 1);
-        const int* table = p.b.table ? p.b.table + (long long)seq * p.b.max_blocks : nullptr;
-        const int page0 = (int)min((long long)seq * p.b.max_blocks, (long long)p.kv.n_pages);  // no table: pages in order
-        auto position = [&](int t) { return min((t0 + min(t, max(nt - 1, 0))) * T + off, end - 1); };
-        auto fetch = [&](int t) -> int {
-            const int blk = position(t) >> p.kv.ps_shift;
-            return table ? __ldg(table + blk) : page0 + blk;
-        };
-        auto row_of = [&](int t, int page) -> int {
-            if ((unsigned)page >= (unsigned)p.kv.n_pages) {
-                set_err_at(p.b.err, kErrBadArgs);
-                page = 0;
-            }
-            return (page << p.kv.ps_shift) + (position(t) & ((1 << p.kv.ps_shift) - 1));
-        };
-        auto copy = [&](uint32_t dst, const uint8_t* base, int idx, int chunk) {
-            const uint32_t at = (uint32_t)__shfl_sync(0xffffffffu, idx, chunk * SH::RPC + sub);
-            cp_async16(dst, base + (unsigned long long)at * (uint32_t)p.kv.row_bytes);
-        };
+        const int w = warp - 8;
         auto hand_over = [&](uint64_t* bar) {
             fence_proxy_async_smem();  // these stores, before the products read them
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
+        auto note_bad = [&](int t) {
+            if (lane == 0) atomicOr(&bad[(t >> bs) >> 5], 1u << ((t >> bs) & 31));
+        };
         bool ok = true;
         if (SH::F32) {
-            // Halves of a tile in the order K0 K1 V0 K2 V1 K3 ..., so that no K waits for the products of a V before
-            // it: 8 copies (4,096 bytes of a warp) in two groups; two halves are in flight.
-            uint8_t* raw = sm + SH::RAW + w * 8192 + lane * 16;
-            const uint32_t raw_s = smem_u32(raw);
-            const int halves = nt > 0 ? 2 * nt + 1 : 0;
-            auto is_v = [](int h) { return h > 0 && !(h & 1); };
-            auto tile_of = [](int h) { return h > 0 && !(h & 1) ? h / 2 - 1 : (h + 1) / 2; };
-            // rows of the next V, of the K before the next, of the next K, the page of the one after
-            int idx_v = row_of(0, fetch(0)), idx_m = row_of(1, fetch(1)), idx_k = idx_v, page = fetch(2);
-            auto issue = [&](int h) {  // nothing behind the last V; K of a tile that is none is not used
-                if (h < halves) {
-                    const bool v = is_v(h);
-                    const int idx = v ? idx_v : idx_k;
-                    const uint8_t* base = v ? vb : kb;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) copy(raw_s + (h & 1) * 4096 + i * 512, base, idx, i);
-                }
-                cp_async_commit();
-            };
-            // the lane's first row and column in a tile; a copy lies RPC rows on
-            uint8_t* home = tiles + w * (SH::RPW / 8) * SH::RS + sub * 16 + (col >> 1) * SH::CS + (col & 1) * 8;
-            issue(0);
-            idx_k = idx_m;
-            issue(1);
-            idx_k = row_of(2, page);
-            page = fetch(3);
-            uint64_t* due = nullptr;  // a half that is stored and not yet handed over
+            // Halves of a tile in the order K0 K1 V0 K2 V1 K3 ..., so that no K waits for the products of a V before it.
+            const int sub = lane / SH::LPR, col = lane % SH::LPR, halves = 2 * nt;
+            const uint8_t* raw = sm + SH::RAW + w * SH::RPW * HD * 4 + lane * 16;
+            const int in_half = (4 * col) % 64 * 2;  // byte of the lane's 4 values in a 128-byte row
+            uint8_t* home = tiles + (4 * col) / 64 * SH::COLS + w * SH::RPW * 128 + (in_half & 8);
+            uint64_t* due = nullptr;                 // a half that is stored and not yet handed over
 #pragma unroll 1
             for (int h = 0; ok && h < halves; ++h) {
-                const int t = tile_of(h), st = t % NB;
-                const bool isv = is_v(h), real = t < nt;
-                cp_async_wait<1>();
-                const uint8_t* src = raw + (h & 1) * 4096;
+                const bool isv = nt == 1 ? h == 1 : h == halves - 1 || (h > 0 && !(h & 1));
+                const int t = isv ? (h == halves - 1 ? nt - 1 : h / 2 - 1) : (h + 1) / 2, st = t % NB;
+                ok = wait_warp(&k_land[h % SH::RAWS], h / SH::RAWS);
+                if (!ok) break;
+                const uint8_t* src = raw + (h % SH::RAWS) * SH::RAWB;
                 float4 x[8];
                 float big[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const float4*>(src + i * 512);
+                const int left = end - (t0 + t) * T - w * SH::RPW - sub;  // rows in front of the end
+                if (left < SH::RPW) {                                     // the last tile: what lies behind is nothing
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i * SH::RPC >= left) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     big[(2 * i) & 3] = max3_abs_nan(big[(2 * i) & 3], x[i].x, x[i].y);
@@ -898,11 +909,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
                 }
                 uint32_t mx = __reduce_max_sync(
                     0xffffffffu, __float_as_uint(max3_abs_nan(max3_abs_nan(big[0], big[1], big[2]), big[3], 0.f)));
-                issue(h + 2);  // over what is in registers now
-                if (due) hand_over(due);  // the half before: its stores are through by now
+                if (lane == 0) mbar_arrive(&raw_free[h % SH::RAWS]);  // all lanes hold theirs
+                if (due) hand_over(due);                             // the half before: its stores are through by now
                 due = nullptr;
-                if (!real) continue;
-                if (h == 2 * SH::QTILE - 1) ok = wait_warp(q_full, 0);  // the first K over the staged queries' place
+                if (t == SH::QTILE) ok = wait_warp(q_full, 0);  // the staged queries' place is written over
                 if (ok && t >= NB) ok = wait_warp(isv ? &v_empty[st] : &k_empty[st], t / NB - 1);
                 if (!ok) break;
                 if (isv && mx >= 0x7f800000u) {  // rare: take what is not finite out, and remember the tile
@@ -912,7 +922,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
                     mx = clean(y);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) x[i] = y[i];
-                    if (lane == 0) atomicOr(&bad[(t >> bs) >> 5], 1u << ((t >> bs) & 31));
+                    note_bad(t);
                 }
                 const int a = scale_of(mx, isv ? 60 : 100);
                 const float f = pow2(a);
@@ -923,7 +933,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
                     uint2 hi, lo;
                     split2(mul2(pair(x[i].x, x[i].y), f2), hi.x, lo.x);
                     split2(mul2(pair(x[i].z, x[i].w), f2), hi.y, lo.y);
-                    uint8_t* d = dst + (i * SH::RPC / 8) * SH::RS + (i * SH::RPC % 8) * 16;
+                    const int rr = i * SH::RPC + sub;
+                    uint8_t* d = dst + rr * 128 + (((in_half >> 4) ^ (rr & 7)) << 4);
                     *reinterpret_cast<uint2*>(d) = hi;
                     *reinterpret_cast<uint2*>(d + SH::TILE) = lo;
                 }
@@ -933,90 +944,69 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
                     if (isv) sc[SH::GROUPS] = f;
                 }
                 due = isv ? &v_full[st] : &k_full[t % (2 * NB)];
-                if (h & 1) {  // K of tile (h + 3) / 2 went out
-                    idx_v = idx_m, idx_m = idx_k;
-                    idx_k = row_of((h + 5) / 2, page);
-                    page = fetch((h + 7) / 2);
-                }
             }
             if (due) hand_over(due);
         } else {
-            // 4 copies of K and 4 of V a tile, straight to their place, AHEAD tiles early
+            // 512 bytes of the warp's rows: 4 rows of 64 values; in place
+            const int NC = 4;
             auto place = [&](int t, int isv, int i) -> uint8_t* {
-                const int trow = w * SH::RPW + i * SH::RPC + sub;
-                return tiles + ((t % NB) * 2 + isv) * SH::HALF + (trow >> 3) * SH::RS + (trow & 7) * 16 + col * SH::CS;
+                constexpr int PER = SH::RPW / 4;  // accesses of 64 values of the warp's rows
+                return tiles + ((t % NB) * 2 + isv) * SH::HALF + (i / PER) * SH::COLS + (w * SH::RPW + (i % PER) * 4) * 128 + lane * 16;
             };
-            int page = fetch(0);
-            auto issue = [&](int t) -> bool {
-                bool good = true;
-                if (t < nt) {
-                    const int idx = row_of(t, page);
-                    page = fetch(t + 1);
-                    if (t == SH::QTILE) good = wait_warp(q_full, 0);
-                    if (good && t >= NB) good = wait_warp(&k_empty[t % NB], t / NB - 1);
-                    if (good) {
-#pragma unroll
-                        for (int i = 0; i < NCK; ++i) copy(smem_u32(place(t, 0, i)), kb, idx, i);
-                    }
-                    cp_async_commit();
-                    if (good && t >= NB) good = wait_warp(&v_empty[t % NB], t / NB - 1);
-                    if (good) {
-#pragma unroll
-                        for (int i = 0; i < NCK; ++i) copy(smem_u32(place(t, 1, i)), vb, idx, i);
-                    }
-                    cp_async_commit();
-                } else {
-                    cp_async_commit();
-                    cp_async_commit();
-                }
-                return good;
-            };
-            // what a lane copied, in bf16 -> f16 times a power of two; non-finite values of V out
             auto fix = [&](int t, int isv) {
-                if (TYPE == AF_KV_F16 && !isv) return;
-                uint4 x[NCK];
+                uint4 x[NC];
                 uint32_t* e = &x[0].x;
 #pragma unroll
-                for (int i = 0; i < NCK; ++i) x[i] = *reinterpret_cast<const uint4*>(place(t, isv, i));
+                for (int i = 0; i < NC; ++i) x[i] = *reinterpret_cast<const uint4*>(place(t, isv, i));
                 if (TYPE == AF_KV_F16) {
                     __half2 z = __float2half2_rn(0.f);  // x·0 is 0 for what is finite, NaN otherwise
 #pragma unroll
-                    for (int i = 0; i < 4 * NCK; ++i)
+                    for (int i = 0; i < 4 * NC; ++i)
                         z = __hfma2(*reinterpret_cast<const __half2*>(&e[i]), __float2half2_rn(0.f), z);
                     const uint32_t zz = *reinterpret_cast<const uint32_t*>(&z) & 0x7fff7fffu;
                     if (__any_sync(0xffffffffu, zz != 0)) {
 #pragma unroll
-                        for (int i = 0; i < 4 * NCK; ++i) {
+                        for (int i = 0; i < 4 * NC; ++i) {
                             if ((e[i] & 0x7c00u) == 0x7c00u) e[i] &= 0xffff0000u;
                             if ((e[i] & 0x7c000000u) == 0x7c000000u) e[i] &= 0x0000ffffu;
                         }
 #pragma unroll
-                        for (int i = 0; i < NCK; ++i) *reinterpret_cast<uint4*>(place(t, isv, i)) = x[i];
-                        if (lane == 0) atomicOr(&bad[(t >> bs) >> 5], 1u << ((t >> bs) & 31));
+                        for (int i = 0; i < NC; ++i) *reinterpret_cast<uint4*>(place(t, isv, i)) = x[i];
+                        note_bad(t);
                     }
                 } else {
+                    const int left = end - (t0 + t) * T - w * SH::RPW - lane / 8;  // rows in front of the end
+                    if (left < SH::RPW) {                                          // the last tile: what lies behind is nothing
+#pragma unroll
+                        for (int i = 0; i < NC; ++i)
+                            if (i % (SH::RPW / 4) * 4 >= left) x[i] = make_uint4(0u, 0u, 0u, 0u);
+                    }
                     uint32_t b = 0;
 #pragma unroll
-                    for (int i = 0; i < 4 * NCK; ++i) b = max(b, max((e[i] << 16) & 0x7fff0000u, e[i] & 0x7fff0000u));
+                    for (int i = 0; i < 4 * NC; ++i) b = max(b, max((e[i] << 16) & 0x7fff0000u, e[i] & 0x7fff0000u));
                     uint32_t mx = __reduce_max_sync(0xffffffffu, b);
                     if (isv && mx >= 0x7f800000u) {
                         b = 0;
 #pragma unroll
-                        for (int i = 0; i < 4 * NCK; ++i) {
+                        for (int i = 0; i < 4 * NC; ++i) {
                             if (((e[i] << 16) & 0x7fff0000u) >= 0x7f800000u) e[i] &= 0xffff0000u;
                             if ((e[i] & 0x7fff0000u) >= 0x7f800000u) e[i] &= 0x0000ffffu;
                             b = max(b, max((e[i] << 16) & 0x7fff0000u, e[i] & 0x7fff0000u));
                         }
                         mx = __reduce_max_sync(0xffffffffu, b);
-                        if (lane == 0) atomicOr(&bad[(t >> bs) >> 5], 1u << ((t >> bs) & 31));
+                        note_bad(t);
                     }
                     const int a = scale_of(mx, isv ? 60 : 100);
                     const float f = pow2(a);
+                    const f32x2 f2 = pair(f, f);
 #pragma unroll
-                    for (int i = 0; i < 4 * NCK; ++i)
-                        e[i] = pack2(__uint_as_float(e[i] << 16) * f, __uint_as_float(e[i] & 0xffff0000u) * f);
+                    for (int i = 0; i < 4 * NC; ++i) {
+                        float lo, hi;
+                        unpair(mul2(pair(__uint_as_float(e[i] << 16), __uint_as_float(e[i] & 0xffff0000u)), f2), lo, hi);
+                        e[i] = pack2(lo, hi);
+                    }
 #pragma unroll
-                    for (int i = 0; i < NCK; ++i) *reinterpret_cast<uint4*>(place(t, isv, i)) = x[i];
+                    for (int i = 0; i < NC; ++i) *reinterpret_cast<uint4*>(place(t, isv, i)) = x[i];
                     if (lane == 0) {
                         float* sc = scales + ((t % (2 * NB)) * 3 + isv) * SH::GROUPS + w;
                         sc[0] = isv ? (float)-a : pow2(-a);
@@ -1025,43 +1015,119 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
                 }
             };
 #pragma unroll 1
-            for (int t = 0; ok && t < SH::AHEAD; ++t) ok = issue(t);
-#pragma unroll 1
             for (int t = 0; ok && t < nt; ++t) {
-                cp_async_wait<2 * SH::AHEAD - 1>();
-                fix(t, 0);
-                hand_over(&k_full[t % (2 * NB)]);
-                cp_async_wait<2 * SH::AHEAD - 2>();
+                if (TYPE != AF_KV_F16) {
+                    ok = wait_warp(&k_land[t % NB], t / NB);
+                    if (!ok) break;
+                    fix(t, 0);
+                    hand_over(&k_full[t % (2 * NB)]);
+                }
+                ok = wait_warp(&v_land[t % NB], t / NB);
+                if (!ok) break;
                 fix(t, 1);
                 hand_over(&v_full[t % NB]);
-                ok = issue(t + SH::AHEAD);
             }
         }
         if (!ok) *flag = 1;
-        cp_async_wait<0>();
     } else {
-        // ------------------------------------------------------- products
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp == 16 && nt > 0) {
+        if (warp == 17 && nt > 0) {
+            // --------------------------------------------------- copies
+            const int R = mp.box_rows;  // a box never crosses a page
+            const int* table = p.b.table ? p.b.table + (long long)seq * p.b.max_blocks : nullptr;
+            const int page0 = (int)min((long long)seq * p.b.max_blocks, (long long)p.kv.n_pages);  // no table: pages in order
+            const int in_page = (1 << p.kv.ps_shift) - 1;
+            auto fetch = [&](int t, int box) -> int {  // the page of a box, asked for early
+                const int pos = min((t0 + min(t, nt - 1)) * T + box * R, end - 1);
+                const int blk = pos >> p.kv.ps_shift;
+                return table ? __ldg(table + blk) : page0 + blk;
+            };
+            bool ok = true;
+            // the boxes of K or V of tile t (column halves for 16 bits): a lane a box
+            auto send = [&](int t, bool isv, uint8_t* dst, uint64_t* bar, int page_a) {
+                constexpr int HALVES = SH::F32 ? 1 : HD / 64;
+                const int p0 = (t0 + t) * T, live = (min(T, end - p0) + R - 1) / R;
+                // bytes first: a box of a page that is none does not come
+                int count = 0;
+                for (int b0 = 0; b0 < live; b0 += 32) {
+                    const int page = b0 ? fetch(t, b0 + lane) : page_a;
+                    count += __popc(__ballot_sync(0xffffffffu, b0 + lane < live && (unsigned)page < (unsigned)p.kv.n_pages));
+                }
+                if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(count * R * HD * SH::SIZE));
+                __syncwarp();
+                for (int b0 = 0; b0 < live; b0 += 32) {
+                    const int box = b0 + lane, page = b0 ? fetch(t, box) : page_a;
+                    if (box < live) {
+                        if ((unsigned)page < (unsigned)p.kv.n_pages) {
+                            const int z = (page << p.kv.ps_shift) + ((p0 + box * R) & in_page);
+#pragma unroll
+                            for (int c = 0; c < HALVES; ++c)
+                                tma_rows(smem_u32(dst) + c * SH::COLS + box * R * (SH::F32 ? HD * 4 : 128),
+                                         isv ? &mp.v_map : &mp.k_map, 64 * c, kvh, z, bar);
+                        } else {
+                            set_err_at(p.b.err, kErrBadArgs);
+                        }
+                    }
+                }
+                __syncwarp();
+            };
+            int page = fetch(0, lane);
+            if (SH::F32) {
+                int page_v = page, page_n = fetch(1, lane);  // of the next V's tile; of the next K's
+                const int halves = 2 * nt;
+                for (int h = 0; ok && h < halves; ++h) {
+                    const bool isv = nt == 1 ? h == 1 : h == halves - 1 || (h > 0 && !(h & 1));
+                    const int t = isv ? (h == halves - 1 ? nt - 1 : h / 2 - 1) : (h + 1) / 2;
+                    if (h >= SH::RAWS) ok = wait_warp(&raw_free[h % SH::RAWS], h / SH::RAWS - 1);
+                    if (!ok) break;
+                    send(t, isv, sm + SH::RAW + (h % SH::RAWS) * SH::RAWB, &k_land[h % SH::RAWS], isv ? page_v : page);
+                    if (isv) {
+                        page_v = page;
+                        page = page_n;
+                        page_n = fetch(t + 3, lane);
+                    } else if (t == 0) {
+                        page = page_n;
+                        page_n = fetch(2, lane);
+                    }
+                }
+            } else {
+                for (int t = 0; ok && t < nt; ++t) {
+                    const int next = fetch(t + 1, lane);
+                    if (t == SH::QTILE) ok = wait_warp(q_full, 0);  // the staged queries' place is written over
+                    uint8_t* dst = tiles + (t % NB) * 2 * SH::HALF;
+                    if (ok && t >= NB) ok = wait_warp(&k_empty[t % NB], t / NB - 1);
+                    if (!ok) break;
+                    send(t, false, dst, TYPE == AF_KV_F16 ? &k_full[t % (2 * NB)] : &k_land[t % NB], page);
+                    if (t >= NB) ok = wait_warp(&v_empty[t % NB], t / NB - 1);
+                    if (!ok) break;
+                    send(t, true, dst + SH::HALF, &v_land[t % NB], page);
+                    page = next;
+                }
+            }
+            if (!ok) *flag = 1;
+        } else if (warp == 16 && nt > 0) {
+            // --------------------------------------------------- products
             constexpr uint32_t base = (1u << 4) | ((uint32_t)(kMmaRows >> 4) << 24);  // f32 accumulators, f16 operands
             constexpr uint32_t ids = base | ((uint32_t)(T >> 3) << 17);
             constexpr uint32_t ido = base | ((uint32_t)(HD >> 3) << 17) | (1u << 16);  // B MN-major
             const uint32_t leader = elect_one();
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             const int n_tiles = __shfl_sync(0xffffffffu, nt, 0);
-            const uint64_t kd = tile_desc(smem_u32(tiles), SH::CS, SH::RS), vd = tile_desc(smem_u32(tiles) + SH::HALF, SH::RS, SH::CS);
+            // K: 8-row groups 1,024 bytes apart, 16 values 32 bytes on; V: 64 values COLS bytes apart, 16 positions 2,048 on
+            const uint64_t kd = tile_desc(smem_u32(tiles), 16, 1024), vd = tile_desc(smem_u32(tiles) + SH::HALF, SH::COLS, 1024);
+            auto k_step = [](int ks) { return (uint32_t)((ks >> 2) * SH::COLS + (ks & 3) * 32) >> 4; };
             auto scores = [&](int st, int sl) {
                 const uint64_t k = kd + (uint32_t)(st * (2 * SH::HALF >> 4));
                 const uint32_t d = tm + SH::S0 + sl * T;
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks) tc_mma_ts(leader, d, tm + SH::QL + 8 * ks, k + (2 * ks * SH::CS >> 4), ids, ks > 0);
+                for (int ks = 0; ks < HD / 16; ++ks) tc_mma_ts(leader, d, tm + SH::QL + 8 * ks, k + k_step(ks), ids, ks > 0);
                 if (SH::TERMS == 2) {
 #pragma unroll
                     for (int ks = 0; ks < HD / 16; ++ks)
-                        tc_mma_ts(leader, d, tm + SH::QH + 8 * ks, k + ((SH::TILE + 2 * ks * SH::CS) >> 4), ids, true);
+                        tc_mma_ts(leader, d, tm + SH::QH + 8 * ks, k + (SH::TILE >> 4) + k_step(ks), ids, true);
                 }
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks) tc_mma_ts(leader, d, tm + SH::QH + 8 * ks, k + (2 * ks * SH::CS >> 4), ids, true);
+                for (int ks = 0; ks < HD / 16; ++ks) tc_mma_ts(leader, d, tm + SH::QH + 8 * ks, k + k_step(ks), ids, true);
                 tc_commit(leader, &s_full[sl]);
                 tc_commit(leader, &k_empty[st]);
             };
@@ -1069,14 +1135,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
                 const uint64_t v = vd + (uint32_t)(st * (2 * SH::HALF >> 4));
                 const uint32_t w = tm + SH::S0 + sl * T, d = tm + SH::O0;
 #pragma unroll
-                for (int ks = 0; ks < T / 16; ++ks) tc_mma_ts(leader, d, w + 8 + 16 * ks, v + (2 * ks * SH::RS >> 4), ido, ks > 0);
+                for (int ks = 0; ks < T / 16; ++ks) tc_mma_ts(leader, d, w + 8 + 16 * ks, v + (2048 * ks >> 4), ido, ks > 0);
                 if (SH::TERMS == 2) {
 #pragma unroll
                     for (int ks = 0; ks < T / 16; ++ks)
-                        tc_mma_ts(leader, d, w + 16 * ks, v + ((SH::TILE + 2 * ks * SH::RS) >> 4), ido, true);
+                        tc_mma_ts(leader, d, w + 16 * ks, v + ((SH::TILE + 2048 * ks) >> 4), ido, true);
                 }
 #pragma unroll
-                for (int ks = 0; ks < T / 16; ++ks) tc_mma_ts(leader, d, w + 16 * ks, v + (2 * ks * SH::RS >> 4), ido, true);
+                for (int ks = 0; ks < T / 16; ++ks) tc_mma_ts(leader, d, w + 16 * ks, v + (2048 * ks >> 4), ido, true);
                 tc_commit(leader, o_full);
                 tc_commit(leader, &v_empty[st]);
             };
@@ -1116,7 +1182,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(MmaParams mp) 
 
 // The splits of a row, a warp each: out = Σ 2^(m_s - m)·O_s / Σ 2^(m_s - m)·l_s, in split order.
 template <int HD>
-__global__ void __launch_bounds__(256) tree_merge_kernel(MmaParams mp) {
+__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ MmaParams mp) {
     const TreeParams& p = mp.t;
     constexpr int PER = HD / 32;
     const int lane = threadIdx.x & 31, seq = blockIdx.y;
@@ -1187,6 +1253,35 @@ TreePlan tree_plan(const af_attention_tree_args& a) {
     return pl;
 }
 
+// The driver's cuTensorMapEncodeTiled, through the runtime (the library does not link libcuda).
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess) f = nullptr;
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return fn;
+}
+
+// Rows of a layer's pool as boxes of up to a tile's or a page's rows: f32 rows whole, others 64 values swizzled.
+bool tree_map(CUtensorMap* map, const TreeParams& p, int type, uint8_t* pool, int box_rows) {
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return false;
+    const bool f32 = type == AF_KV_F32;
+    const int size = kv_type_bytes(type);
+    const cuuint64_t dims[3] = {(cuuint64_t)p.kv.hd, (cuuint64_t)p.kv.kv_heads, (cuuint64_t)p.kv.n_pages << p.kv.ps_shift};
+    const cuuint64_t strides[2] = {(cuuint64_t)p.kv.hd * size, (cuuint64_t)p.kv.row_bytes};
+    const cuuint32_t box[3] = {(cuuint32_t)(f32 ? p.kv.hd : 64), 1u, (cuuint32_t)box_rows}, step[3] = {1, 1, 1};
+    return encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3,
+                  pool + (size_t)p.layer * p.kv.layer_bytes, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  f32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int TYPE, int HD>
 cudaError_t mma_launch(const MmaParams& mp, int n_seq, int max_nodes, cudaStream_t st) {
     constexpr int smem = MmaShape<TYPE, HD>::BYTES;
@@ -1209,7 +1304,16 @@ cudaError_t mma_launch(const MmaParams& mp, int n_seq, int max_nodes, cudaStream
 template <int TYPE>
 cudaError_t tree_launch(const TreeParams& p, const TreePlan& pl, int max_nodes, void* ws, cudaStream_t st) {
     if (pl.mma) {
-        MmaParams mp = {p, pl.blocks, pl.slots, static_cast<float*>(ws), nullptr};
+        MmaParams mp = {};
+        mp.t = p;
+        mp.blocks = pl.blocks;
+        mp.slots = pl.slots;
+        mp.part = static_cast<float*>(ws);
+        mp.box_rows = std::min(1 << p.kv.ps_shift, p.kv.hd == 128 ? 64 : 128);
+        if (!tree_map(&mp.k_map, p, TYPE, p.kv.k, mp.box_rows) || !tree_map(&mp.v_map, p, TYPE, p.kv.v, mp.box_rows)) {
+            set_last_error("af_attention_tree_f32: the cache cannot be described to the copy engine");
+            return cudaErrorInvalidValue;
+        }
         if (pl.slots) mp.plan = reinterpret_cast<int2*>(mp.part + (size_t)pl.slots * kMmaRows * (p.kv.hd + 2));
         return p.kv.hd == 64 ? mma_launch<TYPE, 64>(mp, p.b.n_seq, max_nodes, st) : mma_launch<TYPE, 128>(mp, p.b.n_seq, max_nodes, st);
     }
