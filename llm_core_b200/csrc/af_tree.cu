@@ -19,6 +19,7 @@ struct TreeParams {
     KvView kv;
     KvBatch b;
     int layer, n_rows, H, G;
+    uint32_t G_inv;  // 2^32 / G, rounded up
     const float* q;
     float* out;
     long long qs, os;
@@ -139,21 +140,18 @@ __global__ void __launch_bounds__(kTreeThreads) tree_row_kernel(TreeParams p) {
 // first, then the hi·hi ones, and the softmax warps add each tile's P·V to
 // sums in registers, which round to nearest.
 //
-// Warps (20): 0-3 turn scores into weights, one query row a thread; 4-7 add up
-// the tiles' P·V and write the rows out; 8-15 put K and V into the form that the
-// products take (split, scaled; a cache in f16 only has its V looked through);
-// 16 issues the products; 17 the copies: a box of rows per page by the TMA
-// engine (rows of a warp by cp.async cost 60 cycles of issue each and filled
-// the load pipe that every other warp waits for; single rows by bulk copies
-// run at 2.3 TB/s).  Registers a thread: 112 / 184 / 72 / 40 (setmaxnreg; 128
-// threads of the first two kinds, 256 and 128: 61,440, the launch's 640·96;
-// head_dim 64 has tiles of 128 positions and half the sums, so the first two
-// change places).
+// Warps (24): 0-7 turn scores into weights, half a query row a thread; 8-11
+// add up the tiles' P·V and write the rows out; 12-15 put K and 16-19 V into
+// the form that the products take (split, scaled; a cache in f16 only has its V
+// looked through); 20 issues the products; 21 and 22 the copies of K and V, a
+// box of rows per page by the TMA engine (single rows by bulk copies run at 2.3 TB/s).  Registers a
+// thread (setmaxnreg): 72 / 168 / 64 / 40 for head_dim 128, 88 / 128 / 64 / 40
+// for 64, whose tiles have 128 positions, out of the launch's 768·80.
 //
 // Tiles in shared memory: rows of 64 values (128 bytes) in the 128-byte
 // swizzle, K-major for K, the same tile MN-major for V; for f32 the TMA engine
-// leaves rows as they are in a place of their own (64 KB, half a tile's K and
-// half its V in flight) and the splitting warps write the tiles.
+// leaves rows as they are in a place of their own (64 KB, a tile's K and V in
+// halves) and the splitting warps write the tiles.
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -290,7 +288,8 @@ __device__ __forceinline__ int scale_of(uint32_t max_bits, int top) {
 }
 __device__ __forceinline__ float pow2(int a) { return __int_as_float((a + 127) << 23); }
 
-constexpr int kMmaThreads = 640;
+constexpr int kMmaThreads = 768;
+constexpr int kOutWarp = 8, kSplitWarp = 12, kMmaWarp = 20, kCopyWarp = 21;  // softmax 0-7, splitting K 12-15, V 16-19, copies 21, 22
 constexpr int kMmaRows = 128;
 constexpr int kMmaBadWords = 512;  // tiles of a split whose V holds something non-finite, a bit each
 
@@ -304,9 +303,8 @@ struct MmaShape {
     static constexpr int TILE = HD / 64 * COLS;         // 16,384
     static constexpr int HALF = TERMS * TILE;           // K or V of a tile: hi, lo
     static constexpr int NB = F32 ? 2 : 6;              // tiles in shared memory: K V K V ...
-    static constexpr int RAWS = 2;                      // f32: halves of a tile as they are
-    static constexpr int RAWB = T * HD * 4;             // 32,768
-    static constexpr int RPW = T / 8;                   // rows of a splitting warp in a tile
+    static constexpr int RAWB = T / 2 * HD * 4;         // f32: half the rows of K or V as they are, 16,384
+    static constexpr int RPW = T / 8;                   // rows that share a power of two: a splitting warp's, of half a tile
     static constexpr int LPR = HD * SIZE / 16;          // lanes of a row (f32)
     static constexpr int RPC = 32 / LPR;                // rows of a warp's 512 bytes (f32)
     // queries in, rows out: 128 rows over the last tiles' place, 16-byte columns swizzled by the row
@@ -314,27 +312,31 @@ struct MmaShape {
     static constexpr int QTILE = NB - (kMmaRows * QROW + 2 * HALF - 1) / (2 * HALF);
     static_assert(QTILE >= 1, "the first tile does not wait for the queries");
     // registers
-    static constexpr int REG_S = HD == 128 ? 112 : 184, REG_O = HD == 128 ? 184 : 112;
+    static constexpr int REG_S = HD == 128 ? 72 : 88, REG_O = HD == 128 ? 168 : 128, REG_K = 64, REG_M = 40;
+    static_assert(2 * REG_S + REG_O + 2 * REG_K + REG_M <= 6 * 80, "what the launch gives: 768 threads of 80");
     // tensor memory columns
     static constexpr int NS = 3;                          // score tiles (each becomes its weights)
     static constexpr int QH = 0, QL = HD / 2, S0 = HD, O0 = HD + NS * T;
     static_assert(O0 + HD <= 512, "tensor memory");
-    // shared memory, behind 512 bytes of mbarriers
-    static constexpr int BAD = 512;                       // kMmaBadWords words
-    static constexpr int ROWS = BAD + kMmaBadWords * 4;   // [128] query scales, [NS][128] corrections, [128] tops, [128] sums
-    static constexpr int GROUPS = 8;                      // a splitting warp's rows share their powers of two
-    static constexpr int SCALE = ROWS + (3 + NS) * kMmaRows * 4;  // [2 NB][3][GROUPS] floats
+    // shared memory, behind 768 bytes of mbarriers
+    static constexpr int BAD = 768;                       // kMmaBadWords words
+    static constexpr int ROWS = BAD + kMmaBadWords * 4;   // [128] query scales, [NS][128] corrections, [2][2][128] exchange, [128] tops, [2][128] sums
+    static constexpr int GROUPS = 8;                      // of RPW rows
+    static constexpr int SCALE = ROWS + (8 + NS) * kMmaRows * 4;  // [2 NB][3][GROUPS] floats
     static constexpr int TILES = (SCALE + 2 * NB * 3 * GROUPS * 4 + 1023) / 1024 * 1024;
     static constexpr int RAW = TILES + NB * 2 * HALF;
-    static constexpr int BYTES = RAW + (F32 ? RAWS * RAWB : 0);
+    static constexpr int BYTES = RAW + (F32 ? 4 * RAWB : 0);  // K, K, V, V
     static_assert(BYTES <= 227 * 1024 - 128, "shared memory");
 };
 
 // A box of rows of one kv head (TMA engine): x value, y head, z row.
-__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+// The whole warp comes here, its leader's instruction runs (see tc_mma_ts).
+__device__ __forceinline__ void tma_rows(uint32_t leader, uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}\n" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(leader)
         : "memory");
 }
 
@@ -475,6 +477,9 @@ __device__ __forceinline__ TreeSpot tree_spot(const MmaParams& mp, int T, int b)
     return w;  // whole in the lane whose first_slot, n, ... are set: the one that `src` was
 }
 
+// x / G for row x of a sequence's n·G: exact while x·G < 2^32, which the call is checked for.
+__device__ __forceinline__ int node_of(const TreeParams& p, int x) { return p.G == 1 ? x : (int)__umulhi((uint32_t)x, p.G_inv); }
+
 // Which of positions p0 .. p0+63 the row sees, bit by bit.
 __device__ __forceinline__ unsigned long long tree_window(const TreeParams& p, int row, int node, int n, int len, int p0) {
     auto ones = [](int c) -> unsigned long long { return c >= 64 ? ~0ull : c <= 0 ? 0ull : (1ull << c) - 1; };
@@ -501,36 +506,47 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     const TreeParams& p = mp.t;
     // A waiter never falls a whole ring behind: K of t + NB may be there before the softmax looks for K of t, so
     // its barriers (and the scales) are 2 NB; every other one's next phase needs what the waiter of this one does.
-    uint64_t* k_full = reinterpret_cast<uint64_t*>(sm);  // [2 NB] K of a tile is ready: 8 splitting warps (f16: the copy)
-    uint64_t* v_full = k_full + 2 * NB;                  // [NB] V, 8 splitting warps
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(sm);  // [2 NB] K of a tile is ready: 4 splitting warps (f16: the copy)
+    uint64_t* v_full = k_full + 2 * NB;                  // [NB] V, 4 splitting warps
     uint64_t* k_empty = v_full + NB;                     // [NB] scores done
     uint64_t* v_empty = k_empty + NB;                    // [NB] P·V done
-    uint64_t* k_land = v_empty + NB;                     // [NB] copies of K (bf16) or of a half (f32: RAWS) landed
-    uint64_t* v_land = k_land + NB;                      // [NB] copies of V landed
-    uint64_t* raw_free = v_land + NB;                    // [RAWS] f32: 8 splitting warps have a half in registers
-    uint64_t* s_full = raw_free + SH::RAWS;              // [NS] scores done
+    uint64_t* k_land = v_empty + NB;                     // [NB] copies of K landed (f32: [2] halves of its rows)
+    uint64_t* v_land = k_land + NB;                      // [NB] copies of V
+    uint64_t* raw_free = v_land + NB;                    // [2][2] f32: 4 splitting warps have half of K's, V's rows in registers
+    uint64_t* s_full = raw_free + 4;              // [NS] scores done
     uint64_t* p_full = s_full + NS;                      // [NS] softmax warps: weights written
     uint64_t* c_full = p_full + NS;                      // [NS] softmax warps: correction written
     uint64_t* o_full = c_full + NS;                      // P·V done
     uint64_t* o_free = o_full + 1;                       // output warps: P·V and correction taken
-    uint64_t* q_full = o_free + 1;                       // 8 softmax and output warps: queries written
+    uint64_t* q_full = o_free + 1;                       // softmax and output warps: queries written
     uint64_t* fin = q_full + 1;                          // softmax warps: tops and sums written
     uint64_t* done = fin + 1;                            // every product done
-    static_assert((7 * NB + 3 * NS + 5 + SH::RAWS) * 8 + 16 <= SH::BAD, "barriers");
-    uint32_t* tslot = reinterpret_cast<uint32_t*>(done + 1);
+    uint64_t* x_full = done + 1;                         // [4] the two softmax warps of 32 rows: largest scores written
+    static_assert((7 * NB + 3 * NS + 13) * 8 + 16 <= SH::BAD, "barriers");
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(x_full + 4);
     volatile int* flag = reinterpret_cast<volatile int*>(tslot + 1);
     uint32_t* bad = reinterpret_cast<uint32_t*>(sm + SH::BAD);
     float* s_rs = reinterpret_cast<float*>(sm + SH::ROWS);
     float* s_corr = s_rs + kMmaRows;
-    float* s_top = s_corr + NS * kMmaRows;
+    float* s_other = s_corr + NS * kMmaRows;
+    float* s_top = s_other + 4 * kMmaRows;
     float* s_sum = s_top + kMmaRows;
     float* scales = reinterpret_cast<float*>(sm + SH::SCALE);
     uint8_t* tiles = sm + SH::TILES;
     uint8_t* staged = tiles + SH::QTILE * 2 * SH::HALF;
     auto staged_at = [&](int row, int byte) { return staged + row * SH::QROW + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15); };
-    auto wait = [&](uint64_t* bar, int phase) -> bool { return mbar_wait_at(bar, (uint32_t)phase & 1u, p.b.err, flag); };
-    // the same for a whole warp, which stays together
-    auto wait_warp = [&](uint64_t* bar, int phase) -> bool { return __all_sync(0xffffffffu, wait(bar, phase)); };
+    // A whole warp waits and stays together: the first look is cheap, the rest bounded (kSpinLimit, or another's flag).
+    auto wait_warp = [&](uint64_t* bar, int phase) -> bool {
+        bool ok = mbar_try_wait(bar, (uint32_t)phase & 1u);
+        if (__all_sync(0xffffffffu, ok)) return true;
+        for (uint32_t i = 0; i < kSpinLimit; ++i) {
+            ok = ok || mbar_try_wait(bar, (uint32_t)phase & 1u);
+            if (__all_sync(0xffffffffu, ok)) return true;
+            if ((i & 15) == 15 && __any_sync(0xffffffffu, *flag != 0)) return false;
+        }
+        set_err_at(p.b.err, kErrMbarTimeout);
+        return false;
+    };
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     __shared__ TreeSpot spot;
     pdl_launch_dependents();
@@ -542,25 +558,26 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         }
     } else if (warp == 1 && lane == 0) {
         for (int i = 0; i < NB; ++i) {
-            mbar_init(&k_full[i], TYPE == AF_KV_F16 ? 1 : 8);
-            mbar_init(&k_full[NB + i], TYPE == AF_KV_F16 ? 1 : 8);
-            mbar_init(&v_full[i], 8);
+            mbar_init(&k_full[i], TYPE == AF_KV_F16 ? 1 : 4);
+            mbar_init(&k_full[NB + i], TYPE == AF_KV_F16 ? 1 : 4);
+            mbar_init(&v_full[i], 4);
             mbar_init(&k_empty[i], 1);
             mbar_init(&v_empty[i], 1);
             mbar_init(&k_land[i], 1);
             mbar_init(&v_land[i], 1);
         }
-        for (int i = 0; i < SH::RAWS; ++i) mbar_init(&raw_free[i], 8);
+        for (int i = 0; i < 4; ++i) mbar_init(&raw_free[i], 4);
         for (int i = 0; i < NS; ++i) mbar_init(&s_full[i], 1);
         mbar_init(o_full, 1);
-        mbar_init(q_full, 8);
+        mbar_init(q_full, 12);
         mbar_init(done, 1);
+        for (int i = 0; i < 4; ++i) mbar_init(&x_full[i], 2);
         *flag = 0;
-    } else if (warp == 16) {
+    } else if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(512u)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    } else if (warp == 17 && lane == 0) {
+    } else if (warp == kCopyWarp && lane == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&mp.k_map) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&mp.v_map) : "memory");
     }
@@ -569,14 +586,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     const int seq = spot.seq, kvh = spot.kvh, r0 = spot.r0, n = spot.n, len = spot.len;
     // the block's rows and tiles (the same in every thread)
     const int row_lo = spot.rt * kMmaRows, row_hi = min(row_lo + kMmaRows, n * p.G);
-    const int live_warps = (row_hi - row_lo + 31) / 32;  // of the 4 + 4 that work on rows; the others have none
+    const int live_warps = (row_hi - row_lo + 31) / 32;  // of every 4 that work on rows; the others have none
     if (tid == 0 && seq >= 0) {
         for (int i = 0; i < NS; ++i) {
-            mbar_init(&p_full[i], live_warps);
+            mbar_init(&p_full[i], 2 * live_warps);
             mbar_init(&c_full[i], live_warps);
         }
         mbar_init(o_free, live_warps);
-        mbar_init(fin, live_warps);
+        mbar_init(fin, 2 * live_warps);
     }
     if (tid < 64) fence_mbar_init();
     tc_fence_before();
@@ -584,10 +601,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     tc_fence_after();
     const uint32_t tmem = *tslot;
     if (seq < 0) {
-        if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
         return;
     }
-    const int end = p.mask ? len + n : len + (row_hi - 1) / p.G + 1;  // positions that some row may see
+    const int end = p.mask ? len + n : len + node_of(p, row_hi - 1) + 1;  // positions that some row may see
     const int nt_all = (end + T - 1) / T;
     const int t0 = (int)((long long)nt_all * spot.split / spot.splits),
               t1 = (int)((long long)nt_all * (spot.split + 1) / spot.splits);
@@ -596,25 +613,25 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     while (nt > (kMmaBadWords * 32) << bs) ++bs;
 
     // Queries, by the softmax and output warps: a row a warp in turn — its largest value, hi and lo — into the staging
-    // place, from there a row a thread (hi by one kind of warps, lo by the other) into tensor memory.  Rows that are
+    // place, from there a row a thread (hi by softmax warps 0-3, lo by 4-7) into tensor memory.  Rows that are
     // none keep what is there: what comes of them stays in their own row.
     auto queries = [&]() {
-        constexpr int Q4 = HD / 4, QR = 32 / Q4, QN = 16 / QR;  // lanes of a row at 16 bytes, rows and number of a warp's loads
+        constexpr int Q4 = HD / 4, QR = 32 / Q4, QN = (128 / QR + 11) / 12;  // lanes of a row at 16 bytes, rows and number of a warp's loads
         const int sub = lane / Q4, col = lane % Q4, rows = row_hi - row_lo;
         const bool wide = ((reinterpret_cast<uintptr_t>(p.q) & 15) | (p.qs & 3)) == 0;
         float4 f[QN];  // all in flight
 #pragma unroll
         for (int j = 0; j < QN; ++j) {
-            if ((warp + 8 * j) * QR >= rows) break;
-            const int x = row_lo + min((warp + 8 * j) * QR + sub, rows - 1), node = x / p.G;
+            if ((warp + 12 * j) * QR >= rows) break;
+            const int x = row_lo + min((warp + 12 * j) * QR + sub, rows - 1), node = node_of(p, x);
             const float* q = p.q + (long long)(r0 + node) * p.qs + (kvh * p.G + x - node * p.G) * HD + 4 * col;
             if (wide) f[j] = __ldg(reinterpret_cast<const float4*>(q));
             else f[j] = make_float4(q[0], q[1], q[2], q[3]);
         }
 #pragma unroll
         for (int j = 0; j < QN; ++j) {
-            if ((warp + 8 * j) * QR >= rows) break;
-            const int i = (warp + 8 * j) * QR + sub;
+            if ((warp + 12 * j) * QR >= rows) break;
+            const int i = (warp + 12 * j) * QR + sub;
             uint32_t mx = __float_as_uint(max3_abs_nan(max3_abs_nan(0.f, f[j].x, f[j].y), f[j].z, f[j].w));
             if (QR == 1) {
                 mx = __reduce_max_sync(0xffffffffu, mx);
@@ -633,9 +650,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 if (col == 0) s_rs[i] = p.scale * pow2(-a);
             }
         }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        asm volatile("bar.sync 1, 384;" ::: "memory");
         const int mine = tid & 127;
-        if ((mine & ~31) < rows) {
+        if (warp < 8 && (mine & ~31) < rows) {
             const int from = warp < 4 ? 0 : 2 * HD;
             const uint32_t to = tmem + ((uint32_t)(mine & ~31) << 16) + (warp < 4 ? SH::QH : SH::QL);
 #pragma unroll 2
@@ -653,109 +670,114 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         if (lane == 0) mbar_arrive(q_full);
     };
 
-    if (warp < 4) {
+    if (warp < kOutWarp) {
         // ------------------------------------------------------- softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH::REG_S));
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-        const int r = row_lo + tid;
+        // Warps 0-3 have the first half of a tile's columns, 4-7 the second, of the same rows; a row's two threads
+        // tell each other their largest value and keep sums of their own.
+        if constexpr (SH::REG_S > 80) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH::REG_S));
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::REG_S));
+        constexpr int C = T / 2;
+        const int half = warp >> 2, ti = tid & 127, w4 = warp & 3;
+        const uint32_t lanes = (uint32_t)(w4 * 32) << 16;
+        const int r = row_lo + ti;
         const bool live = r < row_hi;
-        const int node = live ? r / p.G : 0, row = r0 + node;
+        const int node = live ? node_of(p, r) : 0, row = r0 + node;
         queries();
         float m = -INFINITY, l = 0.f;
         bool ok = true;
-        const float rs = s_rs[tid];  // what a raw score is times, but for K's power of two
+        const float rs = s_rs[ti];  // what a raw score is times, but for K's power of two
         // weights written: said a little late, when the next scores are on their way
-        auto publish = [&](int t) {
+        auto publish = [&](int sl) {
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t % NS]);
+            if (lane == 0) mbar_arrive(&p_full[sl]);
         };
-        const int tiles_mine = warp < live_warps ? nt : 0;
-        for (int t = 0; ok && t < tiles_mine; ++t) {
-            const int st = t % NB, sl = t % NS;
-            ok = (TYPE == AF_KV_F16 || wait_warp(&k_full[t % (2 * NB)], t / (2 * NB))) && wait_warp(&s_full[sl], t / NS);
+        const int tiles_mine = w4 < live_warps ? nt : 0;
+        int sl = 0, sl_ph = 0, st = 0, st_ph = 0, kt = 0, kt_ph = 0;  // rings of NS, NB, 2 NB and their phases
+        for (int t = 0; t < tiles_mine; ++t) {
+            ok = (TYPE == AF_KV_F16 || wait_warp(&k_full[kt], kt_ph)) && wait_warp(&s_full[sl], sl_ph);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t sb = tmem + lanes + SH::S0 + sl * T;
-            float v[T];
+            const uint32_t sb = tmem + lanes + SH::S0 + sl * T + half * C;
+            float v[C];
 #pragma unroll
-            for (int c = 0; c < T / 32; ++c) tc_ld32(sb + 32 * c, v + 32 * c);
-            if (t) publish(t - 1);
+            for (int c = 0; c < C / 32; ++c) tc_ld32(sb + 32 * c, v + 32 * c);
+            if (t) publish(sl ? sl - 1 : NS - 1);
             tc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < T; ++i) asm volatile("" : "+f"(v[i]));  // no use may move above the wait
-            const float4* kc = reinterpret_cast<const float4*>(scales + (t % (2 * NB)) * 3 * SH::GROUPS);  // 2^-a of K
-            const float4* vf = kc + SH::GROUPS / 4;                                                        // -a of V
-            const float4* vg = vf + SH::GROUPS / 4;                                                        // 2^a of V
-            if (TYPE != AF_KV_F16) ok = wait_warp(&v_full[st], t / NB);
+            for (int i = 0; i < C; ++i) asm volatile("" : "+f"(v[i]));  // no use may move above the wait
+            const float4* kc = reinterpret_cast<const float4*>(scales + kt * 3 * SH::GROUPS) + half;  // 2^-a of K
+            const float4* vf = kc + SH::GROUPS / 4;                                                   // -a of V
+            const float4* vg = vf + SH::GROUPS / 4;                                                   // 2^a of V
+            if (TYPE != AF_KV_F16) ok = wait_warp(&v_full[st], st_ph);
             if (!ok) break;
             {
-                float c[8], f[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) c[i] = rs, f[i] = 0.f;
+                float c[4] = {rs, rs, rs, rs}, f[4] = {0.f, 0.f, 0.f, 0.f};
                 if (TYPE != AF_KV_F16) {
-                    const float4 x = kc[0], y = kc[1], z = vf[0], w = vf[1];
-                    c[0] *= x.x, c[1] *= x.y, c[2] *= x.z, c[3] *= x.w, c[4] *= y.x, c[5] *= y.y, c[6] *= y.z, c[7] *= y.w;
-                    f[0] = z.x, f[1] = z.y, f[2] = z.z, f[3] = z.w, f[4] = w.x, f[5] = w.y, f[6] = w.z, f[7] = w.w;
+                    const float4 x = *kc, z = *vf;
+                    c[0] *= x.x, c[1] *= x.y, c[2] *= x.z, c[3] *= x.w;
+                    f[0] = z.x, f[1] = z.y, f[2] = z.z, f[3] = z.w;
                 }
 #pragma unroll
-                for (int e = 0; e < T; e += 2) {
+                for (int e = 0; e < C; e += 2) {
                     const int g = e / SH::RPW;
                     const f32x2 x = pair(v[e], v[e + 1]), cc = pair(c[g], c[g]);
                     unpair(TYPE == AF_KV_F16 ? mul2(x, cc) : fma2(x, cc, pair(f[g], f[g])), v[e], v[e + 1]);
                 }
             }
-            const int p0 = (t0 + t) * T;
-            if (p0 + T > len) {
+            const int p0 = (t0 + t) * T + half * C;
+            if (p0 + C > len) {
+                unsigned long long see = live ? tree_window(p, row, node, n, len, p0) : 0ull;
 #pragma unroll
-                for (int w = 0; w < T / 64; ++w) {
-                    const unsigned long long see = live ? tree_window(p, row, node, n, len, p0 + 64 * w) : 0ull;
-#pragma unroll
-                    for (int i = 0; i < 64; ++i)
-                        if (!((see >> i) & 1)) v[64 * w + i] = -INFINITY;
-                }
+                for (int i = 0; i < C; ++i)
+                    if (!((see >> i) & 1)) v[i] = -INFINITY;
             }
             float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-            for (int i = 4; i + 1 < T; i += 2) top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], v[i], v[i + 1]);
-            const float mn = max3(m, fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            for (int i = 4; i + 1 < C; i += 2) top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], v[i], v[i + 1]);
+            float mn = max3(m, fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            // the row's other half, in two places in turn: this one is written again when both have read it
+            s_other[((t & 1) * 2 + half) * kMmaRows + ti] = mn;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&x_full[w4]);
+            ok = wait_warp(&x_full[w4], t);
+            if (!ok) break;
+            mn = fmaxf(mn, s_other[((t & 1) * 2 + (half ^ 1)) * kMmaRows + ti]);
             const float ms = mn == -INFINITY ? 0.f : mn - 14.f;  // weights times 2^14
             const float corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
             m = mn;
-            // its place is free: these scores were issued behind P·V of t - 2, which waited until t - NS was taken
-            s_corr[sl * kMmaRows + tid] = corr;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&c_full[sl]);
+            if (half == 0) {
+                // its place is free: these scores were issued behind P·V of t - 2, which waited until t - NS was taken
+                s_corr[sl * kMmaRows + ti] = corr;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&c_full[sl]);
+            }
             f32x2 sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
             const f32x2 ms2 = pair(-ms, -ms);
-            float g8[8];
+            float g4[4];
             if (TYPE != AF_KV_F16) {
-                const float4 x = vg[0], y = vg[1];
-                g8[0] = x.x, g8[1] = x.y, g8[2] = x.z, g8[3] = x.w, g8[4] = y.x, g8[5] = y.y, g8[6] = y.z, g8[7] = y.w;
+                const float4 x = *vg;
+                g4[0] = x.x, g4[1] = x.y, g4[2] = x.z, g4[3] = x.w;
             }
 #pragma unroll
-            for (int c = 0; c < T / 16; ++c) {
+            for (int c = 0; c < C / 16; ++c) {
                 uint32_t hi[8], lo[8];
+                float w[16];
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const int e = 16 * c + i;
-                    float w[4];
-                    unpair(add2(pair(v[e], v[e + 1]), ms2), w[0], w[1]);
-                    unpair(add2(pair(v[e + 2], v[e + 3]), ms2), w[2], w[3]);
+                for (int i = 0; i < 16; i += 2) unpair(add2(pair(v[16 * c + i], v[16 * c + i + 1]), ms2), w[i], w[i + 1]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) w[j] = ex2(w[j]);
-                    const f32x2 x = pair(w[0], w[1]), y = pair(w[2], w[3]);
+                for (int i = 0; i < 16; ++i) w[i] = ex2(w[i]);
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const f32x2 x = pair(w[i], w[i + 1]);
                     if (TYPE == AF_KV_F16) {
-                        sum[0] = add2(sum[0], x);
-                        sum[1] = add2(sum[1], y);
+                        sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], x);
                     } else {
-                        const float g = g8[e / SH::RPW];
-                        sum[0] = fma2(x, pair(g, g), sum[0]);
-                        sum[1] = fma2(y, pair(g, g), sum[1]);
+                        const float g = g4[(16 * c + i) / SH::RPW];
+                        sum[(i >> 1) & 1] = fma2(x, pair(g, g), sum[(i >> 1) & 1]);
                     }
                     split2(x, hi[i / 2], lo[i / 2]);
-                    split2(y, hi[i / 2 + 1], lo[i / 2 + 1]);
                 }
                 tc_st8(sb + 16 * c, hi);  // over the 16 scores that they came from
                 tc_st8(sb + 16 * c + 8, lo);
@@ -765,30 +787,35 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 unpair(add2(sum[0], sum[1]), a, b);
                 l = fmaf(l, corr, a + b);
             }
+            if (++sl == NS) sl = 0, sl_ph ^= 1;
+            if (++st == NB) st = 0, st_ph ^= 1;
+            if (++kt == 2 * NB) kt = 0, kt_ph ^= 1;
         }
-        if (ok && tiles_mine) publish(tiles_mine - 1);
+        if (ok && tiles_mine) publish(sl ? sl - 1 : NS - 1);
         if (!ok) *flag = 1;
-        s_top[tid] = m;
-        s_sum[tid] = l;
+        if (half == 0) s_top[ti] = m;
+        s_sum[half * kMmaRows + ti] = l;
         __syncwarp();
-        if (lane == 0 && warp < live_warps) mbar_arrive(fin);
-    } else if (warp < 8) {
+        if (lane == 0 && w4 < live_warps) mbar_arrive(fin);
+    } else if (warp < kSplitWarp) {
         // ------------------------------------------------ sums, rows out
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH::REG_O));
         queries();
         constexpr int Q4 = HD / 4, QR = 32 / Q4;  // lanes of a row at 16 bytes each, rows of a warp's store
-        const int w = warp - 4, ti = tid - 128;
+        const int w = warp - kOutWarp, ti = tid - kOutWarp * 32;
         const uint32_t lanes = (uint32_t)(w * 32) << 16;
         const int sub = lane / Q4, col = lane % Q4;
         float acc[HD];
 #pragma unroll
         for (int i = 0; i < HD; ++i) acc[i] = 0.f;
         bool ok = w < live_warps;
+        int sl = 0, sl_ph = 0;
         for (int t = 0; ok && t < nt; ++t) {  // acc = acc·corr + (P·V)(t)
-            ok = wait_warp(&c_full[t % NS], t / NS) && wait_warp(o_full, t);
+            ok = wait_warp(&c_full[sl], sl_ph) && wait_warp(o_full, t);
             if (!ok) break;
             tc_fence_after();
-            const float corr = s_corr[(t % NS) * kMmaRows + ti];
+            const float corr = s_corr[sl * kMmaRows + ti];
+            if (++sl == NS) sl = 0, sl_ph ^= 1;
 #pragma unroll
             for (int c = 0; c < HD / 16; ++c) {
                 float o[16];
@@ -811,7 +838,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         if (!ok && w < live_warps) *flag = 1;
         const int r = row_lo + ti;
         const bool live = r < row_hi;
-        const int node = live ? r / p.G : 0, row = r0 + node, head = kvh * p.G + (live ? r % p.G : 0);
+        const int node = live ? node_of(p, r) : 0, row = r0 + node, head = kvh * p.G + (live ? r - node * p.G : 0);
         // non-finite values of V were taken out of the products: the rows that see them get them back
         for (int wd = 0; ok && wd < kMmaBadWords && (32 * wd) << bs < nt; ++wd) {
             uint32_t b = bad[wd];
@@ -833,7 +860,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         }
         if (ok) {
             const int splits = spot.splits, mine_rows = min(32, row_hi - row_lo - w * 32);
-            const float l = s_sum[ti], inv = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+            const float l = s_sum[ti] + s_sum[kMmaRows + ti], inv = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
             for (int i = 0; i < HD; i += 4)
                 *reinterpret_cast<float4*>(staged_at(ti, 4 * i)) =
@@ -865,10 +892,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 }
             }
         }
-    } else if (warp < 16) {
+    } else if (warp < kMmaWarp) {
         // ------------------------------------------------- splitting K and V
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        const int w = warp - 8;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::REG_K));
+        const bool isv = warp >= kSplitWarp + 4;
+        const int w = warp & 3;
+        uint64_t *full = isv ? v_full : k_full, *empty = isv ? v_empty : k_empty, *land = isv ? v_land : k_land;
+        const int ring = isv ? NB : 2 * NB;
         auto hand_over = [&](uint64_t* bar) {
             fence_proxy_async_smem();  // these stores, before the products read them
             __syncwarp();
@@ -878,86 +908,95 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             if (lane == 0) atomicOr(&bad[(t >> bs) >> 5], 1u << ((t >> bs) & 31));
         };
         bool ok = true;
+        int st = 0, ph = 0, fu = 0, sc_at = 0;  // ring of NB tiles and its phase, of `full`, of the scales
+        auto next = [&]() {
+            if (++st == NB) st = 0, ph ^= 1;
+            if (++fu == ring) fu = 0;
+            if (++sc_at == 2 * NB) sc_at = 0;
+        };
         if (SH::F32) {
-            // Halves of a tile in the order K0 K1 V0 K2 V1 K3 ..., so that no K waits for the products of a V before it.
-            const int sub = lane / SH::LPR, col = lane % SH::LPR, halves = 2 * nt;
-            const uint8_t* raw = sm + SH::RAW + w * SH::RPW * HD * 4 + lane * 16;
+            // Half a tile's rows at a time, RPW of them this warp's: out of the raw place into registers, which frees it,
+            // then split and stored.
+            const int sub = lane / SH::LPR, col = lane % SH::LPR;
+            const uint8_t* raw = sm + SH::RAW + (isv ? 2 * SH::RAWB : 0) + w * SH::RPW * HD * 4 + lane * 16;
+            uint64_t* freed = raw_free + (isv ? 2 : 0);
             const int in_half = (4 * col) % 64 * 2;  // byte of the lane's 4 values in a 128-byte row
-            uint8_t* home = tiles + (4 * col) / 64 * SH::COLS + w * SH::RPW * 128 + (in_half & 8);
-            uint64_t* due = nullptr;                 // a half that is stored and not yet handed over
+            uint8_t* home = tiles + (isv ? SH::HALF : 0) + (4 * col) / 64 * SH::COLS + w * SH::RPW * 128 + (in_half & 8);
+            uint64_t* due = nullptr;                 // a tile that is stored and not yet handed over
 #pragma unroll 1
-            for (int h = 0; ok && h < halves; ++h) {
-                const bool isv = nt == 1 ? h == 1 : h == halves - 1 || (h > 0 && !(h & 1));
-                const int t = isv ? (h == halves - 1 ? nt - 1 : h / 2 - 1) : (h + 1) / 2, st = t % NB;
-                ok = wait_warp(&k_land[h % SH::RAWS], h / SH::RAWS);
-                if (!ok) break;
-                const uint8_t* src = raw + (h % SH::RAWS) * SH::RAWB;
-                float4 x[8];
-                float big[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; ok && t < nt; ++t) {
+#pragma unroll 1
+                for (int s = 0; s < 2; ++s) {
+                    ok = wait_warp(&land[s], t);
+                    if (!ok) break;
+                    const uint8_t* src = raw + s * SH::RAWB;
+                    float4 x[8];
+                    float big[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const float4*>(src + i * 512);
-                const int left = end - (t0 + t) * T - w * SH::RPW - sub;  // rows in front of the end
-                if (left < SH::RPW) {                                     // the last tile: what lies behind is nothing
+                    for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const float4*>(src + i * 512);
+                    const int left = end - (t0 + t) * T - (s * 4 + w) * SH::RPW - sub;  // rows in front of the end
+                    if (left < SH::RPW) {                                               // the last tile: what lies behind is nothing
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (i * SH::RPC >= left) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        for (int i = 0; i < 8; ++i)
+                            if (i * SH::RPC >= left) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        big[(2 * i) & 3] = max3_abs_nan(big[(2 * i) & 3], x[i].x, x[i].y);
+                        big[(2 * i + 1) & 3] = max3_abs_nan(big[(2 * i + 1) & 3], x[i].z, x[i].w);
+                    }
+                    uint32_t mx = __reduce_max_sync(
+                        0xffffffffu, __float_as_uint(max3_abs_nan(max3_abs_nan(big[0], big[1], big[2]), big[3], 0.f)));
+                    if (lane == 0) mbar_arrive(&freed[s]);  // all lanes hold theirs
+                    if (s == 0) {
+                        if (due) hand_over(due);            // the tile before: its stores are through by now
+                        if (t == SH::QTILE) ok = wait_warp(q_full, 0);  // the staged queries' place is written over
+                        if (ok && t >= NB) ok = wait_warp(&empty[st], ph ^ 1);
+                        if (!ok) break;
+                    }
+                    if (isv && mx >= 0x7f800000u) {  // rare: take what is not finite out, and remember the tile
+                        float4 y[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) y[i] = x[i];
+                        mx = clean(y);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[i] = y[i];
+                        note_bad(t);
+                    }
+                    const int a = scale_of(mx, isv ? 60 : 100);
+                    const float f = pow2(a);
+                    const f32x2 f2 = pair(f, f);
+                    uint8_t* dst = home + st * 2 * SH::HALF + s * 4 * SH::RPW * 128;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        uint2 hi, lo;
+                        split2(mul2(pair(x[i].x, x[i].y), f2), hi.x, lo.x);
+                        split2(mul2(pair(x[i].z, x[i].w), f2), hi.y, lo.y);
+                        const int rr = i * SH::RPC + sub;
+                        uint8_t* d = dst + rr * 128 + (((in_half >> 4) ^ (rr & 7)) << 4);
+                        *reinterpret_cast<uint2*>(d) = hi;
+                        *reinterpret_cast<uint2*>(d + SH::TILE) = lo;
+                    }
+                    if (lane == 0) {
+                        float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + s * 4 + w;
+                        sc[0] = isv ? (float)-a : pow2(-a);
+                        if (isv) sc[SH::GROUPS] = f;
+                    }
                 }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    big[(2 * i) & 3] = max3_abs_nan(big[(2 * i) & 3], x[i].x, x[i].y);
-                    big[(2 * i + 1) & 3] = max3_abs_nan(big[(2 * i + 1) & 3], x[i].z, x[i].w);
-                }
-                uint32_t mx = __reduce_max_sync(
-                    0xffffffffu, __float_as_uint(max3_abs_nan(max3_abs_nan(big[0], big[1], big[2]), big[3], 0.f)));
-                if (lane == 0) mbar_arrive(&raw_free[h % SH::RAWS]);  // all lanes hold theirs
-                if (due) hand_over(due);                             // the half before: its stores are through by now
-                due = nullptr;
-                if (t == SH::QTILE) ok = wait_warp(q_full, 0);  // the staged queries' place is written over
-                if (ok && t >= NB) ok = wait_warp(isv ? &v_empty[st] : &k_empty[st], t / NB - 1);
-                if (!ok) break;
-                if (isv && mx >= 0x7f800000u) {  // rare: take what is not finite out, and remember the tile
-                    float4 y[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) y[i] = x[i];
-                    mx = clean(y);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = y[i];
-                    note_bad(t);
-                }
-                const int a = scale_of(mx, isv ? 60 : 100);
-                const float f = pow2(a);
-                const f32x2 f2 = pair(f, f);
-                uint8_t* dst = home + (st * 2 + (isv ? 1 : 0)) * SH::HALF;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    uint2 hi, lo;
-                    split2(mul2(pair(x[i].x, x[i].y), f2), hi.x, lo.x);
-                    split2(mul2(pair(x[i].z, x[i].w), f2), hi.y, lo.y);
-                    const int rr = i * SH::RPC + sub;
-                    uint8_t* d = dst + rr * 128 + (((in_half >> 4) ^ (rr & 7)) << 4);
-                    *reinterpret_cast<uint2*>(d) = hi;
-                    *reinterpret_cast<uint2*>(d + SH::TILE) = lo;
-                }
-                if (lane == 0) {
-                    float* sc = scales + ((t % (2 * NB)) * 3 + (isv ? 1 : 0)) * SH::GROUPS + w;
-                    sc[0] = isv ? (float)-a : pow2(-a);
-                    if (isv) sc[SH::GROUPS] = f;
-                }
-                due = isv ? &v_full[st] : &k_full[t % (2 * NB)];
+                due = &full[fu];
+                next();
             }
-            if (due) hand_over(due);
-        } else {
+            if (ok && due) hand_over(due);
+        } else if (TYPE == AF_KV_BF16 || isv) {
             // 512 bytes of the warp's rows: 4 rows of 64 values; in place
-            const int NC = 4;
-            auto place = [&](int t, int isv, int i) -> uint8_t* {
-                constexpr int PER = SH::RPW / 4;  // accesses of 64 values of the warp's rows
-                return tiles + ((t % NB) * 2 + isv) * SH::HALF + (i / PER) * SH::COLS + (w * SH::RPW + (i % PER) * 4) * 128 + lane * 16;
-            };
-            auto fix = [&](int t, int isv) {
+            constexpr int NC = 4, PER = SH::RPW / 4;  // accesses of a group; of its rows' 64 values
+            auto fix = [&](int t, int s) {
+                uint8_t* at = tiles + (st * 2 + (isv ? 1 : 0)) * SH::HALF + (s * 4 + w) * SH::RPW * 128 + lane * 16;
+                auto place = [&](int i) { return at + (i / PER) * SH::COLS + (i % PER) * 512; };
                 uint4 x[NC];
                 uint32_t* e = &x[0].x;
 #pragma unroll
-                for (int i = 0; i < NC; ++i) x[i] = *reinterpret_cast<const uint4*>(place(t, isv, i));
+                for (int i = 0; i < NC; ++i) x[i] = *reinterpret_cast<const uint4*>(place(i));
                 if (TYPE == AF_KV_F16) {
                     __half2 z = __float2half2_rn(0.f);  // x·0 is 0 for what is finite, NaN otherwise
 #pragma unroll
@@ -971,15 +1010,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                             if ((e[i] & 0x7c000000u) == 0x7c000000u) e[i] &= 0x0000ffffu;
                         }
 #pragma unroll
-                        for (int i = 0; i < NC; ++i) *reinterpret_cast<uint4*>(place(t, isv, i)) = x[i];
+                        for (int i = 0; i < NC; ++i) *reinterpret_cast<uint4*>(place(i)) = x[i];
                         note_bad(t);
                     }
                 } else {
-                    const int left = end - (t0 + t) * T - w * SH::RPW - lane / 8;  // rows in front of the end
-                    if (left < SH::RPW) {                                          // the last tile: what lies behind is nothing
+                    const int left = end - (t0 + t) * T - (s * 4 + w) * SH::RPW - lane / 8;  // rows in front of the end
+                    if (left < SH::RPW) {                                                    // the last tile: what lies behind is nothing
 #pragma unroll
                         for (int i = 0; i < NC; ++i)
-                            if (i % (SH::RPW / 4) * 4 >= left) x[i] = make_uint4(0u, 0u, 0u, 0u);
+                            if (i % PER * 4 >= left) x[i] = make_uint4(0u, 0u, 0u, 0u);
                     }
                     uint32_t b = 0;
 #pragma unroll
@@ -1006,33 +1045,32 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                         e[i] = pack2(lo, hi);
                     }
 #pragma unroll
-                    for (int i = 0; i < NC; ++i) *reinterpret_cast<uint4*>(place(t, isv, i)) = x[i];
+                    for (int i = 0; i < NC; ++i) *reinterpret_cast<uint4*>(place(i)) = x[i];
                     if (lane == 0) {
-                        float* sc = scales + ((t % (2 * NB)) * 3 + isv) * SH::GROUPS + w;
+                        float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + s * 4 + w;
                         sc[0] = isv ? (float)-a : pow2(-a);
                         if (isv) sc[SH::GROUPS] = f;
                     }
                 }
             };
 #pragma unroll 1
-            for (int t = 0; ok && t < nt; ++t) {
-                if (TYPE != AF_KV_F16) {
-                    ok = wait_warp(&k_land[t % NB], t / NB);
-                    if (!ok) break;
-                    fix(t, 0);
-                    hand_over(&k_full[t % (2 * NB)]);
-                }
-                ok = wait_warp(&v_land[t % NB], t / NB);
+            for (int t = 0; t < nt; ++t) {
+                ok = wait_warp(&land[st], ph);
                 if (!ok) break;
+                fix(t, 0);
                 fix(t, 1);
-                hand_over(&v_full[t % NB]);
+                hand_over(&full[fu]);
+                next();
             }
         }
         if (!ok) *flag = 1;
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp == 17 && nt > 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::REG_M));
+        if ((warp == kCopyWarp || warp == kCopyWarp + 1) && nt > 0) {
             // --------------------------------------------------- copies
+            const bool isv = warp != kCopyWarp;
+            const CUtensorMap* map = isv ? &mp.v_map : &mp.k_map;
+            const uint32_t leader = elect_one();
             const int R = mp.box_rows;  // a box never crosses a page
             const int* table = p.b.table ? p.b.table + (long long)seq * p.b.max_blocks : nullptr;
             const int page0 = (int)min((long long)seq * p.b.max_blocks, (long long)p.kv.n_pages);  // no table: pages in order
@@ -1042,70 +1080,58 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 const int blk = pos >> p.kv.ps_shift;
                 return table ? __ldg(table + blk) : page0 + blk;
             };
-            bool ok = true;
-            // the boxes of K or V of tile t (column halves for 16 bits): a lane a box
-            auto send = [&](int t, bool isv, uint8_t* dst, uint64_t* bar, int page_a) {
-                constexpr int HALVES = SH::F32 ? 1 : HD / 64;
-                const int p0 = (t0 + t) * T, live = (min(T, end - p0) + R - 1) / R;
-                // bytes first: a box of a page that is none does not come
-                int count = 0;
-                for (int b0 = 0; b0 < live; b0 += 32) {
-                    const int page = b0 ? fetch(t, b0 + lane) : page_a;
-                    count += __popc(__ballot_sync(0xffffffffu, b0 + lane < live && (unsigned)page < (unsigned)p.kv.n_pages));
+            // pool row of this lane's box of tile t; a page that is none: the error word, and row 0
+            auto row_of = [&](int t, int box, int page) -> int {
+                if ((unsigned)page >= (unsigned)p.kv.n_pages) {
+                    set_err_at(p.b.err, kErrBadArgs);
+                    page = 0;
                 }
-                if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(count * R * HD * SH::SIZE));
-                __syncwarp();
-                for (int b0 = 0; b0 < live; b0 += 32) {
-                    const int box = b0 + lane, page = b0 ? fetch(t, box) : page_a;
-                    if (box < live) {
-                        if ((unsigned)page < (unsigned)p.kv.n_pages) {
-                            const int z = (page << p.kv.ps_shift) + ((p0 + box * R) & in_page);
-#pragma unroll
-                            for (int c = 0; c < HALVES; ++c)
-                                tma_rows(smem_u32(dst) + c * SH::COLS + box * R * (SH::F32 ? HD * 4 : 128),
-                                         isv ? &mp.v_map : &mp.k_map, 64 * c, kvh, z, bar);
-                        } else {
-                            set_err_at(p.b.err, kErrBadArgs);
-                        }
-                    }
-                }
-                __syncwarp();
+                return (page << p.kv.ps_shift) + (((t0 + t) * T + box * R) & in_page);
             };
+            // boxes [first, first + n) of tile t, as far as they are in front of the end, to dst
+            auto send = [&](int t, int first, int n_boxes, uint8_t* dst, uint64_t* bar, int row) {
+                constexpr int HALVES = SH::F32 ? 1 : HD / 64, ROWB = SH::F32 ? HD * 4 : 128;
+                const int live = max(0, min(n_boxes, (end - (t0 + t) * T + R - 1) / R - first));
+                const uint32_t b = smem_u32(bar), d = smem_u32(dst);
+                if (leader) mbar_arrive_expect_tx(bar, (uint32_t)(live * R * HD * SH::SIZE));
+                __syncwarp();
+                for (int i = 0; i < live; ++i) {
+                    const int box = first + i;
+                    if (box && !(box & 31)) row = row_of(t, box + lane, fetch(t, box + lane));  // pages of one or two rows
+                    const int z = __shfl_sync(0xffffffffu, row, box & 31);
+#pragma unroll
+                    for (int c = 0; c < HALVES; ++c)
+                        tma_rows(leader, d + c * SH::COLS + i * R * ROWB, map, 64 * c, kvh, z, b);
+                }
+                return row;
+            };
+            bool ok = true;
             int page = fetch(0, lane);
-            if (SH::F32) {
-                int page_v = page, page_n = fetch(1, lane);  // of the next V's tile; of the next K's
-                const int halves = 2 * nt;
-                for (int h = 0; ok && h < halves; ++h) {
-                    const bool isv = nt == 1 ? h == 1 : h == halves - 1 || (h > 0 && !(h & 1));
-                    const int t = isv ? (h == halves - 1 ? nt - 1 : h / 2 - 1) : (h + 1) / 2;
-                    if (h >= SH::RAWS) ok = wait_warp(&raw_free[h % SH::RAWS], h / SH::RAWS - 1);
-                    if (!ok) break;
-                    send(t, isv, sm + SH::RAW + (h % SH::RAWS) * SH::RAWB, &k_land[h % SH::RAWS], isv ? page_v : page);
-                    if (isv) {
-                        page_v = page;
-                        page = page_n;
-                        page_n = fetch(t + 3, lane);
-                    } else if (t == 0) {
-                        page = page_n;
-                        page_n = fetch(2, lane);
+            int st = 0, ph = 0, kt = 0;
+            for (int t = 0; t < nt; ++t) {
+                int row = row_of(t, lane, page);
+                page = fetch(t + 1, lane);
+                if (SH::F32) {
+                    const int half = T / 2 / R;
+#pragma unroll 1
+                    for (int s = 0; ok && s < 2; ++s) {
+                        if (t) ok = wait_warp(&raw_free[(isv ? 2 : 0) + s], t - 1);
+                        if (ok)
+                            row = send(t, s * half, half, sm + SH::RAW + ((isv ? 2 : 0) + s) * SH::RAWB, (isv ? v_land : k_land) + s, row);
                     }
-                }
-            } else {
-                for (int t = 0; ok && t < nt; ++t) {
-                    const int next = fetch(t + 1, lane);
+                } else {
                     if (t == SH::QTILE) ok = wait_warp(q_full, 0);  // the staged queries' place is written over
-                    uint8_t* dst = tiles + (t % NB) * 2 * SH::HALF;
-                    if (ok && t >= NB) ok = wait_warp(&k_empty[t % NB], t / NB - 1);
-                    if (!ok) break;
-                    send(t, false, dst, TYPE == AF_KV_F16 ? &k_full[t % (2 * NB)] : &k_land[t % NB], page);
-                    if (t >= NB) ok = wait_warp(&v_empty[t % NB], t / NB - 1);
-                    if (!ok) break;
-                    send(t, true, dst + SH::HALF, &v_land[t % NB], page);
-                    page = next;
+                    if (ok && t >= NB) ok = wait_warp(isv ? &v_empty[st] : &k_empty[st], ph ^ 1);
+                    if (ok)
+                        send(t, 0, T / R, tiles + (st * 2 + (isv ? 1 : 0)) * SH::HALF,
+                             isv ? &v_land[st] : TYPE == AF_KV_F16 ? &k_full[kt] : &k_land[st], row);
                 }
+                if (!ok) break;
+                if (++st == NB) st = 0, ph ^= 1;
+                if (++kt == 2 * NB) kt = 0;
             }
             if (!ok) *flag = 1;
-        } else if (warp == 16 && nt > 0) {
+        } else if (warp == kMmaWarp && nt > 0) {
             // --------------------------------------------------- products
             constexpr uint32_t base = (1u << 4) | ((uint32_t)(kMmaRows >> 4) << 24);  // f32 accumulators, f16 operands
             constexpr uint32_t ids = base | ((uint32_t)(T >> 3) << 17);
@@ -1151,18 +1177,25 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 tc_fence_after();
                 scores(0, 0);
             }
+            int st = 0, ph = 0, sl = 0, sl_ph = 0;          // tile t
+            int st1 = 1 % NB, kt1 = 1, kt1_ph = 0, sl1 = 1;  // tile t + 1
             for (int t = 0; ok && t < n_tiles; ++t) {
                 if (t + 1 < n_tiles) {  // the next tile's scores, over the weights of t - 2
                     // (whose P·V is over: that of t - 1 waited until it was taken)
-                    ok = wait_warp(&k_full[(t + 1) % (2 * NB)], (t + 1) / (2 * NB));
+                    ok = wait_warp(&k_full[kt1], kt1_ph);
                     if (!ok) break;
                     tc_fence_after();
-                    scores((t + 1) % NB, (t + 1) % NS);
+                    scores(st1, sl1);
                 }
-                ok = wait_warp(&p_full[t % NS], t / NS) && wait_warp(&v_full[t % NB], t / NB) && (t < 1 || wait_warp(o_free, t - 1));
+                ok = wait_warp(&p_full[sl], sl_ph) && wait_warp(&v_full[st], ph) && (t < 1 || wait_warp(o_free, t - 1));
                 if (!ok) break;
                 tc_fence_after();
-                values(t % NB, t % NS);
+                values(st, sl);
+                if (++st == NB) st = 0, ph ^= 1;
+                if (++sl == NS) sl = 0, sl_ph ^= 1;
+                if (++st1 == NB) st1 = 0;
+                if (++sl1 == NS) sl1 = 0;
+                if (++kt1 == 2 * NB) kt1 = 0, kt1_ph ^= 1;
             }
             if (!ok) *flag = 1;
             // whatever was issued ends before tensor memory is given back
@@ -1175,7 +1208,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 16) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
 }
@@ -1309,7 +1342,7 @@ cudaError_t tree_launch(const TreeParams& p, const TreePlan& pl, int max_nodes, 
         mp.blocks = pl.blocks;
         mp.slots = pl.slots;
         mp.part = static_cast<float*>(ws);
-        mp.box_rows = std::min(1 << p.kv.ps_shift, p.kv.hd == 128 ? 64 : 128);
+        mp.box_rows = std::min(1 << p.kv.ps_shift, (p.kv.hd == 128 ? 64 : 128) / (TYPE == AF_KV_F32 ? 2 : 1));
         if (!tree_map(&mp.k_map, p, TYPE, p.kv.k, mp.box_rows) || !tree_map(&mp.v_map, p, TYPE, p.kv.v, mp.box_rows)) {
             set_last_error("af_attention_tree_f32: the cache cannot be described to the copy engine");
             return cudaErrorInvalidValue;
@@ -1329,6 +1362,8 @@ std::string tree_wrong(const af_attention_tree_args& a) {
     if (a.n_rows < 0 || a.n_heads <= 0 || a.n_heads > 65535 || a.n_heads % a.kv.n_kv_heads)
         return "need n_rows >= 0 and n_heads a multiple of n_kv_heads";
     if (a.max_len < 0) return "max_len must not be negative";
+    const long long G = a.n_heads / a.kv.n_kv_heads;
+    if (a.batch.max_nodes * G > (1ll << 31) / G) return "max_nodes times the square of n_heads / n_kv_heads must be at most 2^31";
     if (a.mask && (a.mask_words <= 0 || (long long)a.mask_words * 64 < a.batch.max_nodes))
         return "mask_words must cover max_nodes";
     const long long qd = (long long)a.n_heads * a.kv.head_dim;
@@ -1369,6 +1404,7 @@ extern "C" cudaError_t af_attention_tree_f32(const af_attention_tree_args* a, cu
     p.n_rows = a->n_rows;
     p.H = a->n_heads;
     p.G = a->n_heads / a->kv.n_kv_heads;
+    p.G_inv = (uint32_t)(((1ull << 32) + p.G - 1) / p.G);
     p.q = a->q;
     p.out = a->out;
     p.qs = a->q_stride ? a->q_stride : qd;
