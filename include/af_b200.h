@@ -234,7 +234,7 @@ cudaError_t af_rope_f32(float* d_q, int n_heads, int head_dim, int pos, float th
  * whose body is a stub, src/engine.cpp:334-347.)  A pool holds
  * [n_layers][n_pages][page_size][n_kv_heads][head_dim] values of `type` for K
  * and as many for V; an engine's own cache is such a pool too (type
- * AF_KV_F32, pages of consecutive positions, layer_stride = n_ctx rows).
+ * AF_KV_F32, pages of consecutive positions).
  * page_size is a power of two, head_dim a multiple of 8 up to 256, k and v are
  * 16-byte aligned, layer_stride (values from one layer to the next; 0 = the
  * dense n_pages*page_size*n_kv_heads*head_dim) is a multiple of 8. */
@@ -467,6 +467,34 @@ cudaError_t af_engine_prefill(af_engine* e, const int32_t* h_tokens, int n, int3
  * Tensor-parallel engines fall back to af_engine_prefill. */
 cudaError_t af_engine_prefill_batched(af_engine* e, const int32_t* h_tokens, int n, int32_t pos0,
                                       float* h_logits, int32_t* h_next);
+/* One pass over a drafted tree of n <= 256 tokens behind the cached positions
+ * 0..pos0-1: node i descends from node h_parents[i] < i, or from position
+ * pos0-1 where that is -1, and is rotated as the token pos0 + its depth.  K and V
+ * of node i are kept at position pos0 + i (af_engine_accept_path moves an
+ * accepted path together); h_next[i] is the greedy id behind node i and
+ * h_logits (optional) [n][vocab] the nodes' logits.  The reference decodes one
+ * token at a time; a chain (h_parents[i] = i-1) gives what
+ * af_engine_prefill gives for each of its tokens, up to the batched linear
+ * layers' rounding (~1e-5 for n <= 32, ~2e-4 above).  One GPU. */
+cudaError_t af_engine_step_tree(af_engine* e, const int32_t* h_tokens, const int32_t* h_parents, int n, int32_t pos0,
+                                float* h_logits, int32_t* h_next);
+/* Keep the nodes h_path[0..n_path) (rising) of the tree that was stepped at
+ * pos0: their K and V rows move to positions pos0 .. pos0+n_path-1 of every
+ * layer, and decoding goes on at pos0 + n_path. */
+cudaError_t af_engine_accept_path(af_engine* e, const int32_t* h_path, int n_path, int32_t pos0);
+/* Beam search with n_beams <= 32 beams: BOS prepended unless present, then per
+ * step the 2*n_beams best continuations (af_beam_select_f32); one that ends in
+ * EOS among the first n_beams is a finished hypothesis, the others go on until
+ * n_beams do.  Hypotheses are rated by their log-probability over
+ * length^length_penalty (length counts EOS); the search ends at max_new tokens,
+ * at the context cap, or when n_beams are finished and the best live beam is
+ * rated no better than the last of them.  h_out / n_out: the best
+ * hypothesis without EOS, h_score (optional) its rating.  The beams share the
+ * prompt's pages of the engine's cache; cudaErrorMemoryAllocation when the
+ * context has no room for their own.  The cache holds no single sequence
+ * afterwards.  One GPU. */
+cudaError_t af_engine_generate_beam(af_engine* e, const int32_t* h_prompt, int n_prompt, int max_new, int n_beams,
+                                    float length_penalty, int32_t* h_out, int* n_out, float* h_score);
 /* Device-fed greedy decode: n_steps graph launches, each feeding its argmax to
  * the next; ids written to h_out (may be NULL).  No host round trip per step. */
 cudaError_t af_engine_decode_greedy(af_engine* e, int32_t first_token, int32_t pos0, int n_steps,

@@ -152,6 +152,9 @@ def load() -> C.CDLL:
         "af_engine_step": (i, [vp, C.c_int32, C.c_int32, fp, ip]),
         "af_engine_prefill": (i, [vp, ip, i, C.c_int32, fp, ip]),
         "af_engine_prefill_batched": (i, [vp, ip, i, C.c_int32, fp, ip]),
+        "af_engine_step_tree": (i, [vp, ip, ip, i, C.c_int32, fp, ip]),
+        "af_engine_accept_path": (i, [vp, ip, i, C.c_int32]),
+        "af_engine_generate_beam": (i, [vp, ip, i, i, i, f, ip, C.POINTER(C.c_int), fp]),
         "af_engine_decode_greedy": (i, [vp, C.c_int32, C.c_int32, i, ip]),
         "af_engine_generate": (i, [vp, ip, i, i, ip, C.POINTER(C.c_int)]),
         "af_sample_f32": (i, [vp, i, vp, i, C.POINTER(Sampling), f, vp, vp]),

@@ -22,6 +22,7 @@
 // The argmax is one all-reduce (max) of a packed (value, ~index) key.
 #include <nccl.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdlib>
 #include <thread>
@@ -58,6 +59,12 @@ struct LayerW {
     DevMat wq, wk, wv, wo, wg, wu, wd;
 };
 
+// The engine's cache as pages of consecutive positions (af_kv_cache): a drafted
+// tree sees one sequence in large pages, a beam search shares smaller ones.
+constexpr int kKvPage = 64;
+constexpr int kBeamPage = 16;
+constexpr int kMaxNodes = 256;  // of a drafted tree
+
 // [lo, hi) of `n` super-blocks for rank r of t, remainder to the low ranks
 // (ffn_down K = 11008 = 43 blocks splits 22/21, 11/11/11/10, 6,6,6,5,5,5,5,5).
 void block_split(int n, int r, int t, int& lo, int& hi) {
@@ -78,6 +85,7 @@ struct af_engine {
     bool pdl = true;  // programmatic dependent launch between the step's kernels (AF_PDL=0 disables)
 
     // local shard geometry
+    int kv_rows = 0;  // cache rows of a layer: n_ctx, rounded up to whole pages of kKvPage
     int hd = 0, Hl = 0, KVl = 0, F0 = 0, F1 = 0, Fl = 0, V0 = 0, V1 = 0, Vl = 0, Vmax = 0;
 
     // weights
@@ -103,7 +111,7 @@ struct af_engine {
     int* h_tokpos = nullptr;  // pinned host mirror
     int* h_pin = nullptr;     // pinned prompt staging of af_engine_prefill (grown on demand)
     size_t h_pin_n = 0;
-    void* pf_ws = nullptr;    // device rows of af_engine_prefill_batched (grown on demand)
+    void* pf_ws = nullptr;    // device rows of the batched passes (grown on demand)
     size_t pf_ws_bytes = 0;
     int nsplit = 1;
 
@@ -309,7 +317,7 @@ cudaError_t enqueue_step(af_engine* e, Prof* prof = nullptr) {
             a.q = e->q;
             a.k = e->k;
             a.v = e->v;
-            const size_t lsz = (size_t)c.n_ctx * e->KVl * e->hd;
+            const size_t lsz = (size_t)e->kv_rows * e->KVl * e->hd;
             a.kc = e->kcache + (size_t)l * lsz;
             a.vc = e->vcache + (size_t)l * lsz;
             a.out = e->attn;
@@ -568,7 +576,7 @@ cudaError_t build_step(af_engine* e) {
         a.q = e->q;
         a.k = e->k;
         a.v = e->v;
-        const size_t lsz = (size_t)c.n_ctx * e->KVl * e->hd;
+        const size_t lsz = (size_t)e->kv_rows * e->KVl * e->hd;
         a.kc = e->kcache + (size_t)l * lsz;
         a.vc = e->vcache + (size_t)l * lsz;
         a.out = e->attn;
@@ -720,6 +728,147 @@ cudaError_t gather_logits(af_engine* e, float* h_logits) {
         off += hi - lo;
     }
     return cudaSuccess;
+}
+
+}  // namespace
+
+namespace {
+
+size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+// Rows of a batched pass (one GPU): the workspace that the engine keeps and
+// grows on demand, with `extra` bytes behind the activations.
+struct RowBufs {
+    float *x, *xn, *tmp, *q, *k, *v, *att, *g, *u;
+    void* extra;
+};
+
+cudaError_t row_bufs(af_engine* e, int T, size_t extra, RowBufs& b) {
+    const int E = e->cfg.n_embd, QD = e->Hl * e->hd, KD = e->KVl * e->hd, F = e->Fl;
+    const size_t need = 3 * align256((size_t)T * E * 4) + 2 * align256((size_t)T * QD * 4) +
+                        2 * align256((size_t)T * KD * 4) + 2 * align256((size_t)T * F * 4) + align256(extra);
+    if (e->pf_ws_bytes < need) {
+        ENG_TRY(cudaStreamSynchronize(e->stream));
+        if (e->pf_ws) cudaFree(e->pf_ws);
+        e->pf_ws = nullptr;
+        e->pf_ws_bytes = 0;
+        if (cudaMalloc(&e->pf_ws, need) != cudaSuccess)
+            return fail("out of device memory for the rows of a batched pass", cudaErrorMemoryAllocation);
+        e->pf_ws_bytes = need;
+    }
+    size_t off = 0;
+    auto take = [&](size_t bytes) {
+        void* p = static_cast<uint8_t*>(e->pf_ws) + off;
+        off += align256(bytes);
+        return p;
+    };
+    auto rows = [&](int n) { return static_cast<float*>(take((size_t)T * n * 4)); };
+    b.x = rows(E), b.xn = rows(E), b.tmp = rows(E);
+    b.q = rows(QD), b.k = rows(KD), b.v = rows(KD), b.att = rows(QD);
+    b.g = rows(F), b.u = rows(F);
+    b.extra = take(extra);
+    return cudaSuccess;
+}
+
+// Embedding and all layers of T rows; attend(l) turns b.q, b.k, b.v of layer
+// l into b.att and keeps K and V.  The rows' residual stream is left in b.x.
+template <typename Attend>
+cudaError_t row_layers(af_engine* e, const RowBufs& b, const int* d_tokens, int T, const Attend& attend) {
+    const auto& c = e->cfg;
+    const int E = c.n_embd, QD = e->Hl * e->hd, KD = e->KVl * e->hd, F = e->Fl;
+    ENG_TRY(prompt_embed_launch(b.x, e->tok_embd.w, e->tok_embd.type, E, e->tok_embd.stride, d_tokens, T, e->stream));
+    for (int l = 0; l < c.n_layer; ++l) {
+        const LayerW& L = e->layers[l];
+        ENG_TRY(rows_rmsnorm_launch(b.xn, b.x, L.attn_norm, E, T, c.eps, e->stream));
+        ENG_TRY(prefill_gemm_launch(b.q, L.wq.w, L.wq.type, b.xn, QD, E, T, e->stream));
+        ENG_TRY(prefill_gemm_launch(b.k, L.wk.w, L.wk.type, b.xn, KD, E, T, e->stream));
+        ENG_TRY(prefill_gemm_launch(b.v, L.wv.w, L.wv.type, b.xn, KD, E, T, e->stream));
+        if (L.bq) ENG_TRY(rows_bias_launch(b.q, L.bq, QD, T, e->stream));
+        if (L.bk) ENG_TRY(rows_bias_launch(b.k, L.bk, KD, T, e->stream));
+        if (L.bv) ENG_TRY(rows_bias_launch(b.v, L.bv, KD, T, e->stream));
+        ENG_CALL(attend(l));
+        ENG_TRY(prefill_gemm_launch(b.tmp, L.wo.w, L.wo.type, b.att, E, QD, T, e->stream));
+        ENG_TRY(rows_add_launch(b.x, b.tmp, (long long)T * E, e->stream));
+        ENG_TRY(rows_rmsnorm_launch(b.xn, b.x, L.ffn_norm, E, T, c.eps, e->stream));
+        ENG_TRY(prefill_gemm_launch(b.g, L.wg.w, L.wg.type, b.xn, F, E, T, e->stream));
+        ENG_TRY(prefill_gemm_launch(b.u, L.wu.w, L.wu.type, b.xn, F, E, T, e->stream));
+        ENG_TRY(rows_swiglu_launch(b.g, b.u, (long long)T * F, e->stream));
+        ENG_TRY(prefill_gemm_launch(b.tmp, L.wd.w, L.wd.type, b.g, E, F, T, e->stream));
+        ENG_TRY(rows_add_launch(b.x, b.tmp, (long long)T * E, e->stream));
+    }
+    return cudaSuccess;
+}
+
+// Final norm and LM head of T rows: d_logits [T][vocab].
+cudaError_t row_logits(af_engine* e, const RowBufs& b, int T, float* d_logits) {
+    ENG_TRY(rows_rmsnorm_launch(b.xn, b.x, e->out_norm, e->cfg.n_embd, T, e->cfg.eps, e->stream));
+    ENG_TRY(prefill_gemm_launch(d_logits, e->output.w, e->output.type, b.xn, e->cfg.vocab, e->cfg.n_embd, T, e->stream));
+    return cudaSuccess;
+}
+
+// The engine's cache in pages of `page` positions.
+af_kv_cache engine_cache(const af_engine* e, int page) {
+    af_kv_cache c = {};
+    c.k = e->kcache;
+    c.v = e->vcache;
+    c.type = AF_KV_F32;
+    c.n_layers = e->cfg.n_layer;
+    c.n_pages = e->kv_rows / page;
+    c.page_size = page;
+    c.n_kv_heads = e->KVl;
+    c.head_dim = e->hd;
+    return c;
+}
+
+// RoPE, K/V rows and attention of layer l for rows whose sequences `batch` describes.
+struct RowAttention {
+    af_kv_cache kv;
+    af_kv_batch batch;
+    const int32_t* depth;
+    const uint64_t* mask;
+    int mask_words, n_rows, max_len;
+    void* ws;
+    size_t ws_bytes;
+};
+af_attention_tree_args tree_args(const af_engine* e, const RowAttention& r, const RowBufs& b, int l) {
+    af_attention_tree_args a = {};
+    a.kv = r.kv;
+    a.batch = r.batch;
+    a.layer = l;
+    a.n_rows = r.n_rows;
+    a.n_heads = e->Hl;
+    a.q = b.q;
+    a.out = b.att;
+    a.mask = r.mask;
+    a.mask_words = r.mask_words;
+    a.max_len = r.max_len;
+    a.ws = r.ws;
+    a.ws_bytes = r.ws_bytes;
+    return a;
+}
+cudaError_t row_attend(const af_engine* e, const RowAttention& r, const RowBufs& b, int l) {
+    const LayerW& L = e->layers[l];
+    af_kv_store_args st = {};
+    st.kv = r.kv;
+    st.batch = r.batch;
+    st.layer = l;
+    st.n_rows = r.n_rows;
+    st.q = b.q;
+    st.k = b.k;
+    st.v = b.v;
+    st.q_out = b.q;
+    st.depth = r.depth;
+    st.cos = e->cos_t;
+    st.sin = e->sin_t;
+    st.n_ctx = e->cfg.n_ctx;
+    st.n_heads = e->Hl;
+    st.qk_norm_order = L.q_norm || L.k_norm ? e->cfg.qk_norm_order : 0;
+    st.q_norm = L.q_norm;
+    st.k_norm = L.k_norm;
+    st.eps = e->cfg.eps;
+    ENG_CALL(af_kv_store_f32(&st, e->stream));
+    const af_attention_tree_args a = tree_args(e, r, b, l);
+    return af_attention_tree_f32(&a, e->stream);
 }
 
 }  // namespace
@@ -987,7 +1136,8 @@ cudaError_t af_engine_finalize(af_engine* e) {
         e->ypart = static_cast<float*>(e->dalloc((size_t)E * 4));
         e->logits = static_cast<float*>(e->dalloc((size_t)e->Vmax * 4));
         if (e->tp > 1) e->logits_all = static_cast<float*>(e->dalloc((size_t)e->Vmax * e->tp * 4));
-        const size_t kvn = (size_t)c.n_layer * c.n_ctx * e->KVl * hd;
+        e->kv_rows = (c.n_ctx + kKvPage - 1) / kKvPage * kKvPage;
+        const size_t kvn = (size_t)c.n_layer * e->kv_rows * e->KVl * hd;
         e->kcache = static_cast<float*>(e->dalloc(kvn * 4));
         e->vcache = static_cast<float*>(e->dalloc(kvn * 4));
         ENG_TRY(cudaMemset(e->kcache, 0, kvn * 4));
@@ -1125,102 +1275,322 @@ cudaError_t af_engine_prefill_batched(af_engine* e, const int32_t* h_tokens, int
     const auto& c = e->cfg;
     const int T = n - 1;
     if (T == 0 || e->tp != 1) return af_engine_prefill(e, h_tokens, n, pos0, h_logits, h_next);
-    const int E = c.n_embd, QD = e->Hl * e->hd, KD = e->KVl * e->hd, F = e->Fl;
-    // one workspace for the prompt rows, kept by the engine and grown on demand
-    auto al = [](size_t b) { return (b + 255) & ~(size_t)255; };
-    const size_t need = 3 * al((size_t)T * E * 4) + 2 * al((size_t)T * QD * 4) + 2 * al((size_t)T * KD * 4) +
-                        2 * al((size_t)T * F * 4) + al((size_t)2 * T * 4);
-    if (e->pf_ws_bytes < need) {
-        ENG_TRY(cudaStreamSynchronize(e->stream));
-        if (e->pf_ws) cudaFree(e->pf_ws);
-        e->pf_ws = nullptr;
-        e->pf_ws_bytes = 0;
-        if (cudaMalloc(&e->pf_ws, need) != cudaSuccess)
-            return fail("af_engine_prefill_batched: out of device memory for the prompt rows",
-                        cudaErrorMemoryAllocation);
-        e->pf_ws_bytes = need;
+    const int QD = e->Hl * e->hd, KD = e->KVl * e->hd;
+    RowBufs b;
+    AF_CUDA_TRY(row_bufs(e, T, align256((size_t)2 * T * 4), b));
+    int* d_tp = static_cast<int*>(b.extra);  // tokens, then positions
+    std::vector<int32_t> tp((size_t)2 * T);
+    for (int t = 0; t < T; ++t) {
+        tp[t] = h_tokens[t];
+        tp[T + t] = pos0 + t;
     }
-    size_t ws_off = 0;
-    auto take = [&](size_t bytes) {
-        void* p = static_cast<uint8_t*>(e->pf_ws) + ws_off;
-        ws_off += al(bytes);
-        return p;
-    };
-    float* x = static_cast<float*>(take((size_t)T * E * 4));
-    float* xn = static_cast<float*>(take((size_t)T * E * 4));
-    float* tmp = static_cast<float*>(take((size_t)T * E * 4));
-    float* q = static_cast<float*>(take((size_t)T * QD * 4));
-    float* k = static_cast<float*>(take((size_t)T * KD * 4));
-    float* v = static_cast<float*>(take((size_t)T * KD * 4));
-    float* att = static_cast<float*>(take((size_t)T * QD * 4));
-    float* g = static_cast<float*>(take((size_t)T * F * 4));
-    float* u = static_cast<float*>(take((size_t)T * F * 4));
-    int* d_tp = static_cast<int*>(take((size_t)2 * T * 4));  // tokens, then positions
-    cudaError_t err = cudaSuccess;
-    auto run = [&]() -> cudaError_t {
-        std::vector<int32_t> tp((size_t)2 * T);
-        for (int t = 0; t < T; ++t) {
-            tp[t] = h_tokens[t];
-            tp[T + t] = pos0 + t;
+    ENG_TRY(cudaMemcpyAsync(d_tp, tp.data(), tp.size() * 4, cudaMemcpyHostToDevice, e->stream));
+    auto attend = [&](int l) -> cudaError_t {
+        const LayerW& L = e->layers[l];
+        float *q = b.q, *k = b.k, *v = b.v, *att = b.att;
+        const size_t lsz = (size_t)e->kv_rows * KD;
+        if (prompt_attention_supported(e->hd)) {
+            // all T tokens at once: RoPE / Q-K norms, the KV rows, causal attention
+            ENG_TRY(prompt_attention_launch(q, k, v, e->kcache + (size_t)l * lsz, e->vcache + (size_t)l * lsz, att,
+                                            e->cos_t, e->sin_t, L.q_norm, L.k_norm, T, pos0, e->Hl, e->KVl, e->hd,
+                                            c.qk_norm_order, c.eps, e->stream));
         }
-        ENG_TRY(cudaMemcpyAsync(d_tp, tp.data(), tp.size() * 4, cudaMemcpyHostToDevice, e->stream));
-        ENG_TRY(prompt_embed_launch(x, e->tok_embd.w, e->tok_embd.type, E, e->tok_embd.stride, d_tp, T, e->stream));
-        for (int l = 0; l < c.n_layer; ++l) {
-            const LayerW& L = e->layers[l];
-            ENG_TRY(rows_rmsnorm_launch(xn, x, L.attn_norm, E, T, c.eps, e->stream));
-            ENG_TRY(prefill_gemm_launch(q, L.wq.w, L.wq.type, xn, QD, E, T, e->stream));
-            ENG_TRY(prefill_gemm_launch(k, L.wk.w, L.wk.type, xn, KD, E, T, e->stream));
-            ENG_TRY(prefill_gemm_launch(v, L.wv.w, L.wv.type, xn, KD, E, T, e->stream));
-            if (L.bq) ENG_TRY(rows_bias_launch(q, L.bq, QD, T, e->stream));
-            if (L.bk) ENG_TRY(rows_bias_launch(k, L.bk, KD, T, e->stream));
-            if (L.bv) ENG_TRY(rows_bias_launch(v, L.bv, KD, T, e->stream));
-            const size_t lsz = (size_t)c.n_ctx * KD;
-            if (prompt_attention_supported(e->hd)) {
-                // all T tokens at once: RoPE / Q-K norms, the KV rows, causal attention
-                ENG_TRY(prompt_attention_launch(q, k, v, e->kcache + (size_t)l * lsz, e->vcache + (size_t)l * lsz, att,
-                                                e->cos_t, e->sin_t, L.q_norm, L.k_norm, T, pos0, e->Hl, e->KVl, e->hd,
-                                                c.qk_norm_order, c.eps, e->stream));
-            }
-            for (int t = 0; t < T && !prompt_attention_supported(e->hd); ++t) {
-                AttnParams a = {};
-                a.q = q + (size_t)t * QD;
-                a.k = k + (size_t)t * KD;
-                a.v = v + (size_t)t * KD;
-                a.kc = e->kcache + (size_t)l * lsz;
-                a.vc = e->vcache + (size_t)l * lsz;
-                a.out = att + (size_t)t * QD;
-                a.cos_t = e->cos_t;
-                a.sin_t = e->sin_t;
-                a.q_norm = L.q_norm;
-                a.k_norm = L.k_norm;
-                a.part = e->apart;
-                a.counter = e->acount;
-                a.pos = d_tp + T + t;
-                a.n_heads = e->Hl;
-                a.n_kv_heads = e->KVl;
-                a.head_dim = e->hd;
-                a.n_ctx = c.n_ctx;
-                a.nsplit = e->nsplit;
-                a.qk_norm_order = c.qk_norm_order;
-                a.eps = c.eps;
-                a.scale = 1.f / std::sqrt((float)e->hd);
-                ENG_TRY(attention_launch(a, e->stream, false));
-            }
-            ENG_TRY(prefill_gemm_launch(tmp, L.wo.w, L.wo.type, att, E, QD, T, e->stream));
-            ENG_TRY(rows_add_launch(x, tmp, (long long)T * E, e->stream));
-            ENG_TRY(rows_rmsnorm_launch(xn, x, L.ffn_norm, E, T, c.eps, e->stream));
-            ENG_TRY(prefill_gemm_launch(g, L.wg.w, L.wg.type, xn, F, E, T, e->stream));
-            ENG_TRY(prefill_gemm_launch(u, L.wu.w, L.wu.type, xn, F, E, T, e->stream));
-            ENG_TRY(rows_swiglu_launch(g, u, (long long)T * F, e->stream));
-            ENG_TRY(prefill_gemm_launch(tmp, L.wd.w, L.wd.type, g, E, F, T, e->stream));
-            ENG_TRY(rows_add_launch(x, tmp, (long long)T * E, e->stream));
+        for (int t = 0; t < T && !prompt_attention_supported(e->hd); ++t) {
+            AttnParams a = {};
+            a.q = q + (size_t)t * QD;
+            a.k = k + (size_t)t * KD;
+            a.v = v + (size_t)t * KD;
+            a.kc = e->kcache + (size_t)l * lsz;
+            a.vc = e->vcache + (size_t)l * lsz;
+            a.out = att + (size_t)t * QD;
+            a.cos_t = e->cos_t;
+            a.sin_t = e->sin_t;
+            a.q_norm = L.q_norm;
+            a.k_norm = L.k_norm;
+            a.part = e->apart;
+            a.counter = e->acount;
+            a.pos = d_tp + T + t;
+            a.n_heads = e->Hl;
+            a.n_kv_heads = e->KVl;
+            a.head_dim = e->hd;
+            a.n_ctx = c.n_ctx;
+            a.nsplit = e->nsplit;
+            a.qk_norm_order = c.qk_norm_order;
+            a.eps = c.eps;
+            a.scale = 1.f / std::sqrt((float)e->hd);
+            ENG_TRY(attention_launch(a, e->stream, false));
         }
-        ENG_TRY(cudaStreamSynchronize(e->stream));
         return cudaSuccess;
     };
-    err = run();
-    if (err != cudaSuccess) return err;
+    AF_CUDA_TRY(row_layers(e, b, d_tp, T, attend));
+    ENG_TRY(cudaStreamSynchronize(e->stream));
     return af_engine_prefill(e, h_tokens + T, 1, pos0 + T, h_logits, h_next);
+}
+
+// A drafted tree in one pass (one GPU): node t is a row, kept at position
+// pos0 + t, rotated by its depth, seeing the cached positions and its
+// ancestors; linear layers as in the batched prompt pass (up to 32 rows stream
+// the weights once).
+cudaError_t af_engine_step_tree(af_engine* e, const int32_t* h_tokens, const int32_t* h_parents, int n, int32_t pos0,
+                                float* h_logits, int32_t* h_next) {
+    AF_CUDA_TRY(check_ready(e));
+    if (e->tp != 1) return fail("af_engine_step_tree: one GPU only", cudaErrorNotSupported);
+    if (n <= 0 || n > kMaxNodes) return fail("af_engine_step_tree: a tree has 1.." + std::to_string(kMaxNodes) + " nodes");
+    if (!h_tokens || !h_parents || !h_next) return fail("af_engine_step_tree: null argument");
+    if (pos0 < 0 || pos0 > e->cfg.n_ctx - n) return fail("af_engine_step_tree: positions outside the context");
+    const int V = e->cfg.vocab, words = (n + 63) / 64;
+    // tokens, depths, length, row range; masks
+    std::vector<int32_t> ints((size_t)2 * n + 3);
+    std::vector<uint64_t> mask((size_t)n * words);
+    for (int i = 0; i < n; ++i) {
+        const int par = h_parents[i];
+        if (h_tokens[i] < 0 || h_tokens[i] >= V) return fail("af_engine_step_tree: token id outside the vocabulary");
+        if (par < -1 || par >= i) return fail("af_engine_step_tree: a node's parent is a node before it, or -1");
+        ints[i] = h_tokens[i];
+        ints[n + i] = par < 0 ? 0 : ints[n + par] + 1;
+        if (par >= 0) std::copy_n(&mask[(size_t)par * words], words, &mask[(size_t)i * words]);
+        mask[(size_t)i * words + i / 64] |= 1ull << (i % 64);
+    }
+    ints[2 * n] = pos0;
+    ints[2 * n + 1] = 0;
+    ints[2 * n + 2] = n;
+    RowAttention r = {};
+    r.kv = engine_cache(e, kKvPage);
+    r.batch = {nullptr, nullptr, nullptr, 1, r.kv.n_pages, n};
+    r.n_rows = n;
+    r.mask_words = words;
+    r.max_len = pos0 + n;
+    RowBufs b = {};
+    const af_attention_tree_args probe = [&] {
+        RowAttention p = r;
+        int32_t one = 0;
+        p.batch.len = &one;  // sizes only
+        return tree_args(e, p, b, 0);
+    }();
+    r.ws_bytes = af_attention_tree_f32_workspace(&probe);
+    const size_t ib = align256(ints.size() * 4), mb = align256(mask.size() * 8), lb = align256((size_t)n * V * 4),
+                 nb = align256((size_t)n * 4);
+    AF_CUDA_TRY(row_bufs(e, n, ib + mb + lb + nb + align256(r.ws_bytes), b));
+    uint8_t* at = static_cast<uint8_t*>(b.extra);
+    int32_t* d_ints = reinterpret_cast<int32_t*>(at);
+    uint64_t* d_mask = reinterpret_cast<uint64_t*>(at + ib);
+    float* d_logits = reinterpret_cast<float*>(at + ib + mb);
+    int32_t* d_next = reinterpret_cast<int32_t*>(at + ib + mb + lb);
+    r.ws = at + ib + mb + lb + nb;
+    ENG_TRY(cudaMemcpyAsync(d_ints, ints.data(), ints.size() * 4, cudaMemcpyHostToDevice, e->stream));
+    ENG_TRY(cudaMemcpyAsync(d_mask, mask.data(), mask.size() * 8, cudaMemcpyHostToDevice, e->stream));
+    if (r.ws_bytes) ENG_TRY(cudaMemsetAsync(r.ws, 0, r.ws_bytes, e->stream));
+    r.batch.len = d_ints + 2 * n;
+    r.batch.first = d_ints + 2 * n + 1;
+    r.depth = d_ints + n;
+    r.mask = d_mask;
+    AF_CUDA_TRY(row_layers(e, b, d_ints, n, [&](int l) { return row_attend(e, r, b, l); }));
+    AF_CUDA_TRY(row_logits(e, b, n, d_logits));
+    ENG_TRY(rows_argmax_launch(d_next, d_logits, V, n, e->stream));
+    ENG_TRY(cudaMemcpyAsync(h_next, d_next, (size_t)n * 4, cudaMemcpyDeviceToHost, e->stream));
+    if (h_logits) ENG_TRY(cudaMemcpyAsync(h_logits, d_logits, (size_t)n * V * 4, cudaMemcpyDeviceToHost, e->stream));
+    ENG_TRY(cudaStreamSynchronize(e->stream));
+    return cudaSuccess;
+}
+
+cudaError_t af_engine_accept_path(af_engine* e, const int32_t* h_path, int n_path, int32_t pos0) {
+    AF_CUDA_TRY(check_ready(e));
+    if (e->tp != 1) return fail("af_engine_accept_path: one GPU only", cudaErrorNotSupported);
+    if (n_path < 0 || n_path > kMaxNodes || (n_path > 0 && !h_path)) return fail("af_engine_accept_path: bad arguments");
+    for (int i = 0; i < n_path; ++i)
+        if (h_path[i] < 0 || h_path[i] >= kMaxNodes || (i && h_path[i] <= h_path[i - 1]))
+            return fail("af_engine_accept_path: a path is nodes of the tree in rising order");
+    if (pos0 < 0 || (n_path > 0 && pos0 > e->cfg.n_ctx - 1 - h_path[n_path - 1]))
+        return fail("af_engine_accept_path: positions outside the context");
+    if (n_path == 0) return cudaSuccess;
+    RowBufs b = {};
+    AF_CUDA_TRY(row_bufs(e, 1, ((size_t)n_path + 3) * 4, b));
+    std::vector<int32_t> ints(h_path, h_path + n_path);
+    ints.push_back(n_path);
+    ints.push_back(pos0);
+    int32_t* d = static_cast<int32_t*>(b.extra);
+    ENG_TRY(cudaMemcpyAsync(d, ints.data(), ints.size() * 4, cudaMemcpyHostToDevice, e->stream));
+    af_kv_compact_args a = {};
+    a.kv = engine_cache(e, kKvPage);
+    a.batch = {nullptr, d + n_path + 1, nullptr, 1, a.kv.n_pages, 0};
+    a.path = d;
+    a.n_path = d + n_path;
+    a.max_path = n_path;
+    a.len_out = d + n_path + 2;
+    ENG_CALL(af_kv_compact(&a, e->stream));
+    ENG_TRY(cudaStreamSynchronize(e->stream));
+    return cudaSuccess;
+}
+
+// Beams are sequences over the engine's cache in pages of kBeamPage positions:
+// the prompt's rows are the first pages, af_kv_fork shares them and moves the
+// beams on, and the beams' tokens go through the layers as rows.
+cudaError_t af_engine_generate_beam(af_engine* e, const int32_t* h_prompt, int n_prompt, int max_new, int n_beams,
+                                    float length_penalty, int32_t* h_out, int* n_out, float* h_score) {
+    AF_CUDA_TRY(check_ready(e));
+    if (e->tp != 1) return fail("af_engine_generate_beam: one GPU only", cudaErrorNotSupported);
+    if (!n_out || (max_new > 0 && !h_out) || (n_prompt > 0 && !h_prompt)) return fail("af_engine_generate_beam: null argument");
+    if (n_prompt <= 0) return fail("af_engine_generate_beam: empty prompt");
+    if (n_beams < 1 || n_beams > 32) return fail("af_engine_generate_beam: n_beams must be in 1..32");
+    *n_out = 0;
+    if (h_score) *h_score = 0.f;
+    std::vector<int32_t> ids(h_prompt, h_prompt + n_prompt);
+    if (ids[0] != e->cfg.bos_id) ids.insert(ids.begin(), e->cfg.bos_id);
+    const int np = (int)ids.size(), V = e->cfg.vocab, B = n_beams;
+    if (np > e->cfg.n_ctx) return fail("af_engine_generate_beam: prompt longer than the context");
+    const int budget = std::min(max_new, e->cfg.n_ctx - np);
+    if (budget <= 0) return cudaSuccess;
+    AF_CUDA_TRY(af_engine_prefill(e, ids.data(), np, 0, nullptr, nullptr));
+
+    RowAttention r = {};
+    r.kv = engine_cache(e, kBeamPage);
+    const int pages = r.kv.n_pages, blocks = std::min(pages, (np + budget + kBeamPage - 1) / kBeamPage), K = (int)std::min<long long>(2 * B, V);
+    r.batch = {nullptr, nullptr, nullptr, B, blocks, 1};
+    r.n_rows = B;
+    RowBufs b = {};
+    af_kv_fork_args fk = {};
+    fk.kv = r.kv;
+    fk.n_in = 1;
+    fk.n_out = B;
+    fk.max_blocks = blocks;
+    af_beam_select_args sel = {};
+    sel.n_seq = 1;
+    sel.n_beams = B;
+    sel.vocab = V;
+    sel.n_out = K;
+    {
+        int32_t one = 0;
+        RowAttention p = r;
+        p.batch.len = p.batch.block_table = &one;  // sizes only
+        const af_attention_tree_args a = tree_args(e, p, b, 0);
+        r.ws_bytes = af_attention_tree_f32_workspace(&a);
+    }
+    fk.ws_bytes = af_kv_fork_workspace(&fk);
+    const size_t sel_bytes = af_beam_select_f32_workspace(&sel);
+    size_t total = 0;
+    auto part = [&](size_t bytes) {
+        const size_t o = total;
+        total += align256(bytes);
+        return o;
+    };
+    const size_t o_tab = part((size_t)2 * B * blocks * 4), o_len = part((size_t)2 * B * 4), o_ref = part((size_t)pages * 4),
+                 o_in = part((size_t)4 * B * 4), o_out = part((size_t)3 * K * 4 + 4), o_log = part((size_t)B * V * 4),
+                 o_aws = part(r.ws_bytes), o_fws = part(fk.ws_bytes), o_sws = part(sel_bytes);
+    AF_CUDA_TRY(row_bufs(e, B, total, b));
+    uint8_t* at = static_cast<uint8_t*>(b.extra);
+    int32_t* d_tab[2] = {reinterpret_cast<int32_t*>(at + o_tab), reinterpret_cast<int32_t*>(at + o_tab) + (size_t)B * blocks};
+    int32_t* d_len[2] = {reinterpret_cast<int32_t*>(at + o_len), reinterpret_cast<int32_t*>(at + o_len) + B};
+    int32_t *d_ref = reinterpret_cast<int32_t*>(at + o_ref), *d_in = reinterpret_cast<int32_t*>(at + o_in);
+    int32_t* d_res = reinterpret_cast<int32_t*>(at + o_out);  // scores, rows, tokens; pages short
+    float* d_logits = reinterpret_cast<float*>(at + o_log);
+    ENG_TRY(cudaMemsetAsync(at + o_aws, 0, total - o_aws, e->stream));
+    r.ws = at + o_aws;
+    fk.ws = at + o_fws;
+    sel.ws = at + o_sws;
+    sel.ws_bytes = sel_bytes;
+    {  // the prompt: one sequence, its pages in order
+        const int held = (np + kBeamPage - 1) / kBeamPage;
+        std::vector<int32_t> tab(blocks, -1), ref(pages, 0);
+        for (int i = 0; i < held; ++i) tab[i] = i, ref[i] = 1;
+        ENG_TRY(cudaMemcpyAsync(d_tab[0], tab.data(), tab.size() * 4, cudaMemcpyHostToDevice, e->stream));
+        ENG_TRY(cudaMemcpyAsync(d_ref, ref.data(), ref.size() * 4, cudaMemcpyHostToDevice, e->stream));
+        ENG_TRY(cudaMemcpyAsync(d_len[0], &np, 4, cudaMemcpyHostToDevice, e->stream));
+        ENG_TRY(cudaStreamSynchronize(e->stream));
+    }
+
+    struct Hyp {
+        std::vector<int32_t> ids;
+        double score;
+    };
+    std::vector<Hyp> live(1), best;
+    live[0].score = 0.;
+    auto rated = [&](double score, int len) { return score / std::pow((double)std::max(len, 1), (double)length_penalty); };
+    auto finish = [&](std::vector<int32_t> h, double score, int len) {  // the n_beams best, best first
+        Hyp f = {std::move(h), rated(score, len)};
+        auto pos = std::find_if(best.begin(), best.end(), [&](const Hyp& o) { return o.score < f.score; });
+        best.insert(pos, std::move(f));
+        if ((int)best.size() > B) best.pop_back();
+    };
+    std::vector<int32_t> res((size_t)3 * K + 1), in((size_t)4 * B);
+    int cur = 0, n_in = 1, len = np;
+    for (int step = 1;; ++step) {
+        // the best continuations of the live beams
+        sel.logits = step == 1 ? e->logits : d_logits;
+        sel.n_beams = n_in;
+        sel.n_out = (int)std::min<long long>(K, (long long)n_in * V);
+        std::vector<float> sc(n_in);
+        for (int i = 0; i < n_in; ++i) sc[i] = (float)live[i].score;
+        ENG_TRY(cudaMemcpyAsync(d_in, sc.data(), (size_t)n_in * 4, cudaMemcpyHostToDevice, e->stream));
+        sel.scores = reinterpret_cast<float*>(d_in);
+        sel.out_score = reinterpret_cast<float*>(d_res);
+        sel.out_beam = d_res + K;
+        sel.out_token = d_res + 2 * K;
+        ENG_CALL(af_beam_select_f32(&sel, e->stream));
+        ENG_TRY(cudaMemcpyAsync(res.data(), d_res, (size_t)3 * K * 4, cudaMemcpyDeviceToHost, e->stream));
+        ENG_TRY(cudaStreamSynchronize(e->stream));
+        std::vector<Hyp> next;
+        std::vector<int32_t> parent;
+        for (int i = 0; i < sel.n_out && (int)next.size() < B; ++i) {
+            float s;
+            std::memcpy(&s, &res[i], 4);
+            const int row = res[K + i], tok = res[2 * K + i];
+            if (!(s > -INFINITY) || row < 0 || row >= n_in) continue;
+            if (tok == e->cfg.eos_id) {  // only one that would have been kept ends a hypothesis
+                if (i < B) finish(live[row].ids, s, step);
+                continue;
+            }
+            next.push_back({live[row].ids, s});
+            next.back().ids.push_back(tok);
+            parent.push_back(row);
+        }
+        if (next.empty()) break;
+        live = std::move(next);
+        const int n = (int)live.size();
+        if (step >= budget || ((int)best.size() >= B && best.back().score >= rated(live[0].score, step))) {
+            for (Hyp& h : live) finish(std::move(h.ids), h.score, step);
+            break;
+        }
+        // the beams move on to their parents' pages, with room for the token
+        std::fill(in.begin(), in.end(), 0);
+        for (int i = 0; i < n; ++i) {
+            in[i] = parent[i];
+            in[B + i] = 1;
+            in[2 * B + i] = live[i].ids.back();
+        }
+        ENG_TRY(cudaMemcpyAsync(d_in, in.data(), in.size() * 4, cudaMemcpyHostToDevice, e->stream));
+        fk.table_in = d_tab[cur];
+        fk.len_in = d_len[cur];
+        fk.ref_in = fk.ref_out = d_ref;
+        fk.table_out = d_tab[cur ^ 1];
+        fk.len_out = d_len[cur ^ 1];
+        fk.parent = d_in;
+        fk.n_new = d_in + B;
+        fk.n_short = d_res + 3 * K;
+        fk.n_in = n_in;
+        fk.n_out = n;
+        ENG_CALL(af_kv_fork(&fk, e->stream));
+        ENG_TRY(cudaMemcpyAsync(&res[3 * K], d_res + 3 * K, 4, cudaMemcpyDeviceToHost, e->stream));
+        ENG_TRY(cudaStreamSynchronize(e->stream));
+        if (res[3 * K]) return fail("af_engine_generate_beam: the context has no room for the beams", cudaErrorMemoryAllocation);
+        cur ^= 1;
+        r.batch.block_table = d_tab[cur];
+        r.batch.len = d_len[cur];
+        r.batch.n_seq = r.n_rows = n;
+        r.max_len = len + 1;
+        AF_CUDA_TRY(row_layers(e, b, d_in + 2 * B, n, [&](int l) { return row_attend(e, r, b, l); }));
+        AF_CUDA_TRY(row_logits(e, b, n, d_logits));
+        ++len;
+        std::vector<int32_t> lens(n, len);
+        ENG_TRY(cudaMemcpyAsync(d_len[cur], lens.data(), (size_t)n * 4, cudaMemcpyHostToDevice, e->stream));
+        ENG_TRY(cudaStreamSynchronize(e->stream));
+        n_in = n;
+    }
+    if (best.empty()) return cudaSuccess;
+    const Hyp& w = best.front();
+    std::copy(w.ids.begin(), w.ids.end(), h_out);
+    *n_out = (int)w.ids.size();
+    if (h_score) *h_score = (float)w.score;
+    return cudaSuccess;
 }
 
 cudaError_t af_engine_decode_greedy(af_engine* e, int32_t first_token, int32_t pos0, int n_steps, int32_t* h_out) {
@@ -1358,7 +1728,7 @@ cudaError_t af_engine_kv(af_engine* e, int layer, int which_v, int n_pos, float*
     AF_CUDA_TRY(check_ready(e));
     if (layer < 0 || layer >= e->cfg.n_layer || n_pos < 0 || n_pos > e->cfg.n_ctx) return fail("af_engine_kv: range");
     const size_t row = (size_t)e->KVl * e->hd;
-    const float* base = (which_v ? e->vcache : e->kcache) + (size_t)layer * e->cfg.n_ctx * row;
+    const float* base = (which_v ? e->vcache : e->kcache) + (size_t)layer * e->kv_rows * row;
     ENG_TRY(cudaMemcpyAsync(h_out, base, (size_t)n_pos * row * 4, cudaMemcpyDeviceToHost, e->stream));
     ENG_TRY(cudaStreamSynchronize(e->stream));
     return cudaSuccess;

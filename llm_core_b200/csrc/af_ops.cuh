@@ -84,6 +84,7 @@ cudaError_t rows_rmsnorm_launch(float* y, const float* x, const float* w, int n,
 cudaError_t rows_bias_launch(float* y, const float* b, int n, int T, cudaStream_t st);
 cudaError_t rows_swiglu_launch(float* g, const float* u, long long count, cudaStream_t st);
 cudaError_t rows_add_launch(float* x, const float* y, long long count, cudaStream_t st);
+cudaError_t rows_argmax_launch(int* ids, const float* logits, int n, int T, cudaStream_t st);
 
 // Decode attention (af_attention.cu).
 struct AttnParams {

@@ -460,6 +460,22 @@ __global__ void rows_add_kernel(float* __restrict__ x, const float* __restrict__
     if (i < count) x[i] += y[i];
 }
 
+// ids[t] = the first largest of logits[t][0..n) (argmax_key's rule); one block per row.
+__global__ void rows_argmax_kernel(int* __restrict__ ids, const float* __restrict__ logits, int n) {
+    __shared__ unsigned long long red[32];
+    const float* x = logits + (size_t)blockIdx.x * n;
+    unsigned long long best = 0;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) best = max(best, argmax_key(x[i], (uint32_t)i));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < (int)(blockDim.x >> 5); ++w) best = max(best, red[w]);
+        ids[blockIdx.x] = (int)(0xFFFFFFFFu - (uint32_t)best);
+    }
+}
+
 // ---- causal attention of the batched prompt pass
 
 // Per (token, head row): the Q/K head norm (qwen3 before RoPE, hunyuan after
@@ -734,6 +750,11 @@ cudaError_t rows_bias_launch(float* y, const float* b, int n, int T, cudaStream_
 
 cudaError_t rows_swiglu_launch(float* g, const float* u, long long count, cudaStream_t st) {
     rows_swiglu_kernel<<<(unsigned)((count + 255) / 256), 256, 0, st>>>(g, u, count);
+    return cudaGetLastError();
+}
+
+cudaError_t rows_argmax_launch(int* ids, const float* logits, int n, int T, cudaStream_t st) {
+    rows_argmax_kernel<<<T, 512, 0, st>>>(ids, logits, n);
     return cudaGetLastError();
 }
 

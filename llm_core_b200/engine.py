@@ -155,6 +155,37 @@ class LlamaCudaModel:
                  C.byref(nxt)), "af_engine_prefill")
         return nxt.value, lg
 
+    def step_tree(self, tokens, parents, pos0: int, want_logits: bool = False):
+        """One pass over a drafted tree behind positions 0..pos0-1 (af_engine_step_tree):
+        the greedy id behind every node, and the nodes' logits if wanted."""
+        t, p = (np.ascontiguousarray(x, dtype=np.int32) for x in (tokens, parents))
+        if t.size != p.size:
+            raise ValueError("step_tree: a parent per token")
+        lg = np.zeros((t.size, self.cfg.vocab), np.float32) if want_logits else None
+        nxt = np.zeros(max(t.size, 1), np.int32)
+        ip = C.POINTER(C.c_int32)
+        check(self.lib.af_engine_step_tree(self.h, t.ctypes.data_as(ip), p.ctypes.data_as(ip), t.size, pos0,
+                                           lg.ctypes.data_as(C.POINTER(C.c_float)) if want_logits else None,
+                                           nxt.ctypes.data_as(ip)), "af_engine_step_tree")
+        return nxt[:t.size], lg
+
+    def accept_path(self, path, pos0: int):
+        """Keep these nodes of the tree stepped at pos0 (af_engine_accept_path)."""
+        p = np.ascontiguousarray(path, dtype=np.int32)
+        check(self.lib.af_engine_accept_path(self.h, p.ctypes.data_as(C.POINTER(C.c_int32)), p.size, pos0),
+              "af_engine_accept_path")
+
+    def generate_beam(self, prompt_ids, n_beams: int, max_new_tokens: int, length_penalty: float = 1.0):
+        """Beam search (af_engine_generate_beam): the best hypothesis and its rating."""
+        p = np.ascontiguousarray(prompt_ids, dtype=np.int32)
+        out = np.zeros(max(max_new_tokens, 1), np.int32)
+        n, score = C.c_int(), C.c_float()
+        ip = C.POINTER(C.c_int32)
+        check(self.lib.af_engine_generate_beam(self.h, p.ctypes.data_as(ip), p.size, max_new_tokens, n_beams,
+                                               float(length_penalty), out.ctypes.data_as(ip), C.byref(n),
+                                               C.byref(score)), "af_engine_generate_beam")
+        return out[:n.value].tolist(), float(score.value)
+
     def decode_greedy(self, first_token: int, pos0: int, n_steps: int) -> np.ndarray:
         out = np.zeros(max(n_steps, 1), np.int32)
         check(self.lib.af_engine_decode_greedy(self.h, first_token, pos0, n_steps,

@@ -162,3 +162,14 @@ def test_workspace_sizes():
     assert lib.af_beam_select_f32_workspace(C.byref(beam())) > 0
     assert lib.af_beam_select_f32_workspace(C.byref(beam(n_out=0))) == 0
     assert lib.af_kv_fork_workspace(C.byref(fork())) >= 2 * 16 + 8 * 4
+
+
+def test_tree_and_beam_engine_entries_reject_a_null_engine():
+    lib = _lib.load()
+    i1 = (C.c_int32 * 1)()
+    n = C.c_int(0)
+    for call in (lambda: lib.af_engine_step_tree(None, i1, i1, 1, 0, None, i1),
+                 lambda: lib.af_engine_accept_path(None, i1, 1, 0),
+                 lambda: lib.af_engine_generate_beam(None, i1, 1, 1, 1, 1.0, i1, C.byref(n), None)):
+        assert call() != 0
+        assert b"not finalized" in lib.af_last_error()
