@@ -291,19 +291,22 @@ __device__ __forceinline__ float pow2(int a) { return __int_as_float((a + 127) <
 constexpr int kMmaThreads = 768;
 constexpr int kOutWarp = 8, kSplitWarp = 12, kMmaWarp = 20, kCopyWarp = 21;  // softmax 0-7, splitting K 12-15, V 16-19, copies 21, 22
 constexpr int kMmaRows = 128;
+constexpr int kTreeTile = 64;
 constexpr int kMmaBadWords = 512;  // tiles of a split whose V holds something non-finite, a bit each
 
 template <int TYPE, int HD>
 struct MmaShape {
     static constexpr bool F32 = TYPE == AF_KV_F32;
     static constexpr int SIZE = F32 ? 4 : 2;
-    static constexpr int T = HD == 128 ? 64 : 128;      // positions of a tile
+    static constexpr int T = kTreeTile;                 // positions of a tile
     static constexpr int TERMS = F32 ? 2 : 1;           // hi, lo of K and V
     static constexpr int COLS = T * 128;                // 64 values of every row
-    static constexpr int TILE = HD / 64 * COLS;         // 16,384
+    static constexpr int TILE = HD / 64 * COLS;
     static constexpr int HALF = TERMS * TILE;           // K or V of a tile: hi, lo
-    static constexpr int NB = F32 ? 2 : 6;              // tiles in shared memory: K V K V ...
-    static constexpr int RAWB = T / 2 * HD * 4;         // f32: half the rows of K or V as they are, 16,384
+    static constexpr int NB = F32 ? 256 / HD : 6;       // tiles in shared memory: K V K V ...
+    static constexpr int LA = F32 ? 1 : 2;              // tiles whose scores are issued ahead of the products of one
+    static constexpr int RING = NB + LA + 2;            // barriers and scales of K (see k_full)
+    static constexpr int RAWB = T / 2 * HD * 4;         // f32: half the rows of K or V as they are
     static constexpr int RPW = T / 8;                   // rows that share a power of two: a splitting warp's, of half a tile
     static constexpr int LPR = HD * SIZE / 16;          // lanes of a row (f32)
     static constexpr int RPC = 32 / LPR;                // rows of a warp's 512 bytes (f32)
@@ -312,18 +315,18 @@ struct MmaShape {
     static constexpr int QTILE = NB - (kMmaRows * QROW + 2 * HALF - 1) / (2 * HALF);
     static_assert(QTILE >= 1, "the first tile does not wait for the queries");
     // registers
-    static constexpr int REG_S = HD == 128 ? 72 : 88, REG_O = HD == 128 ? 168 : 128, REG_K = 64, REG_M = 40;
+    static constexpr int REG_S = 72, REG_O = HD == 128 ? 168 : 128, REG_K = 64, REG_M = 40;
     static_assert(2 * REG_S + REG_O + 2 * REG_K + REG_M <= 6 * 80, "what the launch gives: 768 threads of 80");
     // tensor memory columns
-    static constexpr int NS = 3;                          // score tiles (each becomes its weights)
+    static constexpr int NS = 4;                          // score tiles (each becomes its weights)
     static constexpr int QH = 0, QL = HD / 2, S0 = HD, O0 = HD + NS * T;
     static_assert(O0 + HD <= 512, "tensor memory");
     // shared memory, behind 768 bytes of mbarriers
     static constexpr int BAD = 768;                       // kMmaBadWords words
     static constexpr int ROWS = BAD + kMmaBadWords * 4;   // [128] query scales, [NS][128] corrections, [2][2][128] exchange, [128] tops, [2][128] sums
     static constexpr int GROUPS = 8;                      // of RPW rows
-    static constexpr int SCALE = ROWS + (8 + NS) * kMmaRows * 4;  // [2 NB][3][GROUPS] floats
-    static constexpr int TILES = (SCALE + 2 * NB * 3 * GROUPS * 4 + 1023) / 1024 * 1024;
+    static constexpr int SCALE = ROWS + (8 + NS) * kMmaRows * 4;  // [RING][3][GROUPS] floats
+    static constexpr int TILES = (SCALE + RING * 3 * GROUPS * 4 + 1023) / 1024 * 1024;
     static constexpr int RAW = TILES + NB * 2 * HALF;
     static constexpr int BYTES = RAW + (F32 ? 4 * RAWB : 0);  // K, K, V, V
     static_assert(BYTES <= 227 * 1024 - 128, "shared memory");
@@ -341,9 +344,10 @@ __device__ __forceinline__ void tma_rows(uint32_t leader, uint32_t dst, const CU
 }
 
 // Zeros for what is not finite; the largest of the rest, over the warp.
-__device__ __noinline__ uint32_t clean(float4 (&x)[8]) {
+template <int N>
+__device__ __noinline__ uint32_t clean(float4 (&x)[N]) {
     uint32_t b = 0;
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < N; ++i) {
         float* e = &x[i].x;
         for (int j = 0; j < 4; ++j) {
             if (!(fabsf(e[j]) < INFINITY)) e[j] = 0.f;
@@ -501,13 +505,14 @@ template <int TYPE, int HD>
 __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_constant__ MmaParams mp) {
     using SH = MmaShape<TYPE, HD>;
     using E = KvElem<TYPE>;
-    constexpr int T = SH::T, NB = SH::NB, NS = SH::NS;
+    constexpr int T = SH::T, NB = SH::NB, NS = SH::NS, RING = SH::RING;
     extern __shared__ __align__(1024) uint8_t sm[];
     const TreeParams& p = mp.t;
-    // A waiter never falls a whole ring behind: K of t + NB may be there before the softmax looks for K of t, so
-    // its barriers (and the scales) are 2 NB; every other one's next phase needs what the waiter of this one does.
-    uint64_t* k_full = reinterpret_cast<uint64_t*>(sm);  // [2 NB] K of a tile is ready: 4 splitting warps (f16: the copy)
-    uint64_t* v_full = k_full + 2 * NB;                  // [NB] V, 4 splitting warps
+    // A waiter never falls a whole ring behind.  K of t + RING is written when the scores of t + RING - NB =
+    // t + LA + 2 are done; those are issued behind the products of t + 1, so the softmax is through with K of t.
+    // Every other barrier's next phase needs what the waiter of this one does.
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(sm);  // [RING] K of a tile is ready: 4 splitting warps (f16: the copy)
+    uint64_t* v_full = k_full + RING;                    // [NB] V, 4 splitting warps
     uint64_t* k_empty = v_full + NB;                     // [NB] scores done
     uint64_t* v_empty = k_empty + NB;                    // [NB] P·V done
     uint64_t* k_land = v_empty + NB;                     // [NB] copies of K landed (f32: [2] halves of its rows)
@@ -522,7 +527,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     uint64_t* fin = q_full + 1;                          // softmax warps: tops and sums written
     uint64_t* done = fin + 1;                            // every product done
     uint64_t* x_full = done + 1;                         // [4] the two softmax warps of 32 rows: largest scores written
-    static_assert((7 * NB + 3 * NS + 13) * 8 + 16 <= SH::BAD, "barriers");
+    static_assert((RING + 5 * NB + 3 * NS + 13) * 8 + 16 <= SH::BAD, "barriers");
     uint32_t* tslot = reinterpret_cast<uint32_t*>(x_full + 4);
     volatile int* flag = reinterpret_cast<volatile int*>(tslot + 1);
     uint32_t* bad = reinterpret_cast<uint32_t*>(sm + SH::BAD);
@@ -558,14 +563,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         }
     } else if (warp == 1 && lane == 0) {
         for (int i = 0; i < NB; ++i) {
-            mbar_init(&k_full[i], TYPE == AF_KV_F16 ? 1 : 4);
-            mbar_init(&k_full[NB + i], TYPE == AF_KV_F16 ? 1 : 4);
             mbar_init(&v_full[i], 4);
             mbar_init(&k_empty[i], 1);
             mbar_init(&v_empty[i], 1);
             mbar_init(&k_land[i], 1);
             mbar_init(&v_land[i], 1);
         }
+        for (int i = 0; i < RING; ++i) mbar_init(&k_full[i], TYPE == AF_KV_F16 ? 1 : 4);
         for (int i = 0; i < 4; ++i) mbar_init(&raw_free[i], 4);
         for (int i = 0; i < NS; ++i) mbar_init(&s_full[i], 1);
         mbar_init(o_full, 1);
@@ -694,7 +698,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             if (lane == 0) mbar_arrive(&p_full[sl]);
         };
         const int tiles_mine = w4 < live_warps ? nt : 0;
-        int sl = 0, sl_ph = 0, st = 0, st_ph = 0, kt = 0, kt_ph = 0;  // rings of NS, NB, 2 NB and their phases
+        int sl = 0, sl_ph = 0, st = 0, st_ph = 0, kt = 0, kt_ph = 0;  // rings of NS, NB, RING and their phases
         for (int t = 0; t < tiles_mine; ++t) {
             ok = (TYPE == AF_KV_F16 || wait_warp(&k_full[kt], kt_ph)) && wait_warp(&s_full[sl], sl_ph);
             if (!ok) break;
@@ -748,7 +752,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             const float corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
             m = mn;
             if (half == 0) {
-                // its place is free: these scores were issued behind P·V of t - 2, which waited until t - NS was taken
+                // its place is free: these scores were issued behind the products of t - LA - 1, which waited until those
+                // of t - LA - 2 (or t - NS) were taken
                 s_corr[sl * kMmaRows + ti] = corr;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c_full[sl]);
@@ -789,7 +794,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             }
             if (++sl == NS) sl = 0, sl_ph ^= 1;
             if (++st == NB) st = 0, st_ph ^= 1;
-            if (++kt == 2 * NB) kt = 0, kt_ph ^= 1;
+            if (++kt == RING) kt = 0, kt_ph ^= 1;
         }
         if (ok && tiles_mine) publish(sl ? sl - 1 : NS - 1);
         if (!ok) *flag = 1;
@@ -898,7 +903,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         const bool isv = warp >= kSplitWarp + 4;
         const int w = warp & 3;
         uint64_t *full = isv ? v_full : k_full, *empty = isv ? v_empty : k_empty, *land = isv ? v_land : k_land;
-        const int ring = isv ? NB : 2 * NB;
+        const int ring = isv ? NB : RING;
         auto hand_over = [&](uint64_t* bar) {
             fence_proxy_async_smem();  // these stores, before the products read them
             __syncwarp();
@@ -912,11 +917,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         auto next = [&]() {
             if (++st == NB) st = 0, ph ^= 1;
             if (++fu == ring) fu = 0;
-            if (++sc_at == 2 * NB) sc_at = 0;
+            if (++sc_at == RING) sc_at = 0;
         };
         if (SH::F32) {
             // Half a tile's rows at a time, RPW of them this warp's: out of the raw place into registers, which frees it,
             // then split and stored.
+            constexpr int NX = SH::RPW * HD * 4 / 512;  // a warp's loads of its rows
             const int sub = lane / SH::LPR, col = lane % SH::LPR;
             const uint8_t* raw = sm + SH::RAW + (isv ? 2 * SH::RAWB : 0) + w * SH::RPW * HD * 4 + lane * 16;
             uint64_t* freed = raw_free + (isv ? 2 : 0);
@@ -930,18 +936,18 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                     ok = wait_warp(&land[s], t);
                     if (!ok) break;
                     const uint8_t* src = raw + s * SH::RAWB;
-                    float4 x[8];
+                    float4 x[NX];
                     float big[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const float4*>(src + i * 512);
+                    for (int i = 0; i < NX; ++i) x[i] = *reinterpret_cast<const float4*>(src + i * 512);
                     const int left = end - (t0 + t) * T - (s * 4 + w) * SH::RPW - sub;  // rows in front of the end
                     if (left < SH::RPW) {                                               // the last tile: what lies behind is nothing
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
+                        for (int i = 0; i < NX; ++i)
                             if (i * SH::RPC >= left) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                    for (int i = 0; i < NX; ++i) {
                         big[(2 * i) & 3] = max3_abs_nan(big[(2 * i) & 3], x[i].x, x[i].y);
                         big[(2 * i + 1) & 3] = max3_abs_nan(big[(2 * i + 1) & 3], x[i].z, x[i].w);
                     }
@@ -955,12 +961,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                         if (!ok) break;
                     }
                     if (isv && mx >= 0x7f800000u) {  // rare: take what is not finite out, and remember the tile
-                        float4 y[8];
+                        float4 y[NX];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) y[i] = x[i];
+                        for (int i = 0; i < NX; ++i) y[i] = x[i];
                         mx = clean(y);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] = y[i];
+                        for (int i = 0; i < NX; ++i) x[i] = y[i];
                         note_bad(t);
                     }
                     const int a = scale_of(mx, isv ? 60 : 100);
@@ -968,7 +974,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                     const f32x2 f2 = pair(f, f);
                     uint8_t* dst = home + st * 2 * SH::HALF + s * 4 * SH::RPW * 128;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                    for (int i = 0; i < NX; ++i) {
                         uint2 hi, lo;
                         split2(mul2(pair(x[i].x, x[i].y), f2), hi.x, lo.x);
                         split2(mul2(pair(x[i].z, x[i].w), f2), hi.y, lo.y);
@@ -989,7 +995,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             if (ok && due) hand_over(due);
         } else if (TYPE == AF_KV_BF16 || isv) {
             // 512 bytes of the warp's rows: 4 rows of 64 values; in place
-            constexpr int NC = 4, PER = SH::RPW / 4;  // accesses of a group; of its rows' 64 values
+            constexpr int NC = SH::RPW * HD * 2 / 512, PER = SH::RPW / 4;  // accesses of a group; of its rows' 64 values
             auto fix = [&](int t, int s) {
                 uint8_t* at = tiles + (st * 2 + (isv ? 1 : 0)) * SH::HALF + (s * 4 + w) * SH::RPW * 128 + lane * 16;
                 auto place = [&](int i) { return at + (i / PER) * SH::COLS + (i % PER) * 512; };
@@ -1128,7 +1134,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 }
                 if (!ok) break;
                 if (++st == NB) st = 0, ph ^= 1;
-                if (++kt == 2 * NB) kt = 0;
+                if (++kt == RING) kt = 0;
             }
             if (!ok) *flag = 1;
         } else if (warp == kMmaWarp && nt > 0) {
@@ -1172,30 +1178,30 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 tc_commit(leader, o_full);
                 tc_commit(leader, &v_empty[st]);
             };
-            bool ok = wait_warp(q_full, 0) && wait_warp(&k_full[0], 0);
-            if (ok) {
+            int st = 0, ph = 0, sl = 0, sl_ph = 0;       // tile t
+            int st1 = 0, kt1 = 0, kt1_ph = 0, sl1 = 0;  // the tile whose scores are next
+            auto next_scores = [&]() -> bool {
+                if (!wait_warp(&k_full[kt1], kt1_ph)) return false;
                 tc_fence_after();
-                scores(0, 0);
-            }
-            int st = 0, ph = 0, sl = 0, sl_ph = 0;          // tile t
-            int st1 = 1 % NB, kt1 = 1, kt1_ph = 0, sl1 = 1;  // tile t + 1
+                scores(st1, sl1);
+                if (++st1 == NB) st1 = 0;
+                if (++sl1 == NS) sl1 = 0;
+                if (++kt1 == RING) kt1 = 0, kt1_ph ^= 1;
+                return true;
+            };
+            bool ok = wait_warp(q_full, 0);
+            for (int t = 0; ok && t < min(SH::LA, n_tiles); ++t) ok = next_scores();
             for (int t = 0; ok && t < n_tiles; ++t) {
-                if (t + 1 < n_tiles) {  // the next tile's scores, over the weights of t - 2
-                    // (whose P·V is over: that of t - 1 waited until it was taken)
-                    ok = wait_warp(&k_full[kt1], kt1_ph);
-                    if (!ok) break;
-                    tc_fence_after();
-                    scores(st1, sl1);
-                }
+                // scores of t + LA, over the weights of t + LA - NS (whose products are over: those of the tile behind
+                // them were issued when they had been taken)
+                if (t + SH::LA < n_tiles) ok = next_scores();
+                if (!ok) break;
                 ok = wait_warp(&p_full[sl], sl_ph) && wait_warp(&v_full[st], ph) && (t < 1 || wait_warp(o_free, t - 1));
                 if (!ok) break;
                 tc_fence_after();
                 values(st, sl);
                 if (++st == NB) st = 0, ph ^= 1;
                 if (++sl == NS) sl = 0, sl_ph ^= 1;
-                if (++st1 == NB) st1 = 0;
-                if (++sl1 == NS) sl1 = 0;
-                if (++kt1 == 2 * NB) kt1 = 0, kt1_ph ^= 1;
             }
             if (!ok) *flag = 1;
             // whatever was issued ends before tensor memory is given back
@@ -1276,8 +1282,7 @@ TreePlan tree_plan(const af_attention_tree_args& a) {
     if (!pl.mma) return pl;
     const long long cap = (long long)a.batch.max_blocks * a.kv.page_size;
     const long long max_len = a.max_len > 0 ? std::min((long long)a.max_len, cap) : cap;
-    const int T = hd == 128 ? 64 : 128;
-    const long long tiles = (max_len + T - 1) / T, most = (tiles + kTreeMinTiles - 1) / kTreeMinTiles;
+    const long long tiles = (max_len + kTreeTile - 1) / kTreeTile, most = (tiles + kTreeMinTiles - 1) / kTreeMinTiles;
     const long long items = ((long long)a.batch.max_nodes * G + kMmaRows - 1) / kMmaRows * a.kv.n_kv_heads * a.batch.n_seq;
     const long long split = items <= kTreeItems ? (items + kTreeSms - 1) / kTreeSms * kTreeSms : items + 2 * kTreeItems;
     pl.blocks = (int)std::min({split, items * std::max(1ll, most), (long long)INT_MAX});
@@ -1342,7 +1347,7 @@ cudaError_t tree_launch(const TreeParams& p, const TreePlan& pl, int max_nodes, 
         mp.blocks = pl.blocks;
         mp.slots = pl.slots;
         mp.part = static_cast<float*>(ws);
-        mp.box_rows = std::min(1 << p.kv.ps_shift, (p.kv.hd == 128 ? 64 : 128) / (TYPE == AF_KV_F32 ? 2 : 1));
+        mp.box_rows = std::min(1 << p.kv.ps_shift, kTreeTile / (TYPE == AF_KV_F32 ? 2 : 1));
         if (!tree_map(&mp.k_map, p, TYPE, p.kv.k, mp.box_rows) || !tree_map(&mp.v_map, p, TYPE, p.kv.v, mp.box_rows)) {
             set_last_error("af_attention_tree_f32: the cache cannot be described to the copy engine");
             return cudaErrorInvalidValue;
