@@ -288,8 +288,8 @@ __device__ __forceinline__ int scale_of(uint32_t max_bits, int top) {
 }
 __device__ __forceinline__ float pow2(int a) { return __int_as_float((a + 127) << 23); }
 
-constexpr int kMmaThreads = 768;
-constexpr int kOutWarp = 8, kSplitWarp = 12, kMmaWarp = 20, kCopyWarp = 21;  // softmax 0-7, splitting K 12-15, V 16-19, copies 21, 22
+constexpr int kMmaThreads = 1024;
+constexpr int kMmaWarp = 28, kCopyWarp = 29;  // copies of K, of V
 constexpr int kMmaRows = 128;
 constexpr int kTreeTile = 64;
 constexpr int kMmaBadWords = 512;  // tiles of a split whose V holds something non-finite, a bit each
@@ -300,6 +300,10 @@ struct MmaShape {
     static constexpr int SIZE = F32 ? 4 : 2;
     static constexpr int T = kTreeTile;                 // positions of a tile
     static constexpr int TERMS = F32 ? 2 : 1;           // hi, lo of K and V
+    static constexpr int SETS = F32 ? 1 : 2;            // of 8 softmax warps, which take the tiles in turn
+    static constexpr int SW = F32 ? 8 : 4;              // splitting warps of K, of V
+    static constexpr int OUT = 8 * SETS, SPLIT_K = OUT + 4, SPLIT_V = SPLIT_K + SW;  // first warps
+    static_assert(SPLIT_V + SW == kMmaWarp, "warps");
     static constexpr int COLS = T * 128;                // 64 values of every row
     static constexpr int TILE = HD / 64 * COLS;
     static constexpr int HALF = TERMS * TILE;           // K or V of a tile: hi, lo
@@ -307,7 +311,7 @@ struct MmaShape {
     static constexpr int LA = F32 ? 1 : 2;              // tiles whose scores are issued ahead of the products of one
     static constexpr int RING = NB + LA + 2;            // barriers and scales of K (see k_full)
     static constexpr int RAWB = T / 2 * HD * 4;         // f32: half the rows of K or V as they are
-    static constexpr int RPW = T / 8;                   // rows that share a power of two: a splitting warp's, of half a tile
+    static constexpr int RPW = T / 2 / SW;              // rows that share a power of two: a splitting warp's, of half a tile
     static constexpr int LPR = HD * SIZE / 16;          // lanes of a row (f32)
     static constexpr int RPC = 32 / LPR;                // rows of a warp's 512 bytes (f32)
     // queries in, rows out: 128 rows over the last tiles' place, 16-byte columns swizzled by the row
@@ -315,17 +319,17 @@ struct MmaShape {
     static constexpr int QTILE = NB - (kMmaRows * QROW + 2 * HALF - 1) / (2 * HALF);
     static_assert(QTILE >= 1, "the first tile does not wait for the queries");
     // registers
-    static constexpr int REG_S = 72, REG_O = HD == 128 ? 168 : 128, REG_K = 64, REG_M = 40;
-    static_assert(2 * REG_S + REG_O + 2 * REG_K + REG_M <= 6 * 80, "what the launch gives: 768 threads of 80");
+    static constexpr int REG_S = F32 ? 72 : HD == 128 ? 56 : 64, REG_O = HD == 128 ? 168 : 104, REG_K = !F32 && HD == 64 ? 56 : 40, REG_M = 40;
+    static_assert(2 * SETS * REG_S + REG_O + SW / 2 * REG_K + REG_M <= 8 * 64, "what the launch gives: 1,024 threads of 64");
     // tensor memory columns
     static constexpr int NS = 4;                          // score tiles (each becomes its weights)
     static constexpr int QH = 0, QL = HD / 2, S0 = HD, O0 = HD + NS * T;
     static_assert(O0 + HD <= 512, "tensor memory");
     // shared memory, behind 768 bytes of mbarriers
     static constexpr int BAD = 768;                       // kMmaBadWords words
-    static constexpr int ROWS = BAD + kMmaBadWords * 4;   // [128] query scales, [NS][128] corrections, [2][2][128] exchange, [128] tops, [2][128] sums
-    static constexpr int GROUPS = 8;                      // of RPW rows
-    static constexpr int SCALE = ROWS + (8 + NS) * kMmaRows * 4;  // [RING][3][GROUPS] floats
+    static constexpr int ROWS = BAD + kMmaBadWords * 4;   // [128] query scales, [NS][128] tops of tiles; a set's [2][2][128] exchange, [128] tops, [2][128] sums
+    static constexpr int GROUPS = T / RPW;
+    static constexpr int SCALE = ROWS + (1 + NS + 7 * SETS) * kMmaRows * 4;  // [RING][3][GROUPS] floats
     static constexpr int TILES = (SCALE + RING * 3 * GROUPS * 4 + 1023) / 1024 * 1024;
     static constexpr int RAW = TILES + NB * 2 * HALF;
     static constexpr int BYTES = RAW + (F32 ? 4 * RAWB : 0);  // K, K, V, V
@@ -505,37 +509,38 @@ template <int TYPE, int HD>
 __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_constant__ MmaParams mp) {
     using SH = MmaShape<TYPE, HD>;
     using E = KvElem<TYPE>;
-    constexpr int T = SH::T, NB = SH::NB, NS = SH::NS, RING = SH::RING;
+    constexpr int T = SH::T, NB = SH::NB, NS = SH::NS, RING = SH::RING, SETS = SH::SETS, SW = SH::SW;
+    constexpr int kOutWarp = SH::OUT, kSplitWarp = SH::SPLIT_K;
     extern __shared__ __align__(1024) uint8_t sm[];
     const TreeParams& p = mp.t;
     // A waiter never falls a whole ring behind.  K of t + RING is written when the scores of t + RING - NB =
     // t + LA + 2 are done; those are issued behind the products of t + 1, so the softmax is through with K of t.
     // Every other barrier's next phase needs what the waiter of this one does.
-    uint64_t* k_full = reinterpret_cast<uint64_t*>(sm);  // [RING] K of a tile is ready: 4 splitting warps (f16: the copy)
-    uint64_t* v_full = k_full + RING;                    // [NB] V, 4 splitting warps
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(sm);  // [RING] K of a tile is ready: its splitting warps (f16: the copy)
+    uint64_t* v_full = k_full + RING;                    // [NB] V, its splitting warps
     uint64_t* k_empty = v_full + NB;                     // [NB] scores done
     uint64_t* v_empty = k_empty + NB;                    // [NB] P·V done
     uint64_t* k_land = v_empty + NB;                     // [NB] copies of K landed (f32: [2] halves of its rows)
     uint64_t* v_land = k_land + NB;                      // [NB] copies of V
-    uint64_t* raw_free = v_land + NB;                    // [2][2] f32: 4 splitting warps have half of K's, V's rows in registers
+    uint64_t* raw_free = v_land + NB;                    // [2][2] f32: the splitting warps have half of K's, V's rows in registers
     uint64_t* s_full = raw_free + 4;              // [NS] scores done
     uint64_t* p_full = s_full + NS;                      // [NS] softmax warps: weights written
-    uint64_t* c_full = p_full + NS;                      // [NS] softmax warps: correction written
+    uint64_t* c_full = p_full + NS;                      // [NS] softmax warps: largest score written
     uint64_t* o_full = c_full + NS;                      // P·V done
     uint64_t* o_free = o_full + 1;                       // output warps: P·V and correction taken
     uint64_t* q_full = o_free + 1;                       // softmax and output warps: queries written
     uint64_t* fin = q_full + 1;                          // softmax warps: tops and sums written
     uint64_t* done = fin + 1;                            // every product done
-    uint64_t* x_full = done + 1;                         // [4] the two softmax warps of 32 rows: largest scores written
-    static_assert((RING + 5 * NB + 3 * NS + 13) * 8 + 16 <= SH::BAD, "barriers");
-    uint32_t* tslot = reinterpret_cast<uint32_t*>(x_full + 4);
+    uint64_t* x_full = done + 1;                         // [SETS][4] the two softmax warps of 32 rows: largest scores written
+    static_assert((RING + 5 * NB + 3 * NS + 9 + 4 * SETS) * 8 + 16 <= SH::BAD, "barriers");
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(x_full + 4 * SETS);
     volatile int* flag = reinterpret_cast<volatile int*>(tslot + 1);
     uint32_t* bad = reinterpret_cast<uint32_t*>(sm + SH::BAD);
     float* s_rs = reinterpret_cast<float*>(sm + SH::ROWS);
-    float* s_corr = s_rs + kMmaRows;
-    float* s_other = s_corr + NS * kMmaRows;
-    float* s_top = s_other + 4 * kMmaRows;
-    float* s_sum = s_top + kMmaRows;
+    float* s_tile = s_rs + kMmaRows;
+    float* s_other = s_tile + NS * kMmaRows;
+    float* s_top = s_other + SETS * 4 * kMmaRows;
+    float* s_sum = s_top + SETS * kMmaRows;
     float* scales = reinterpret_cast<float*>(sm + SH::SCALE);
     uint8_t* tiles = sm + SH::TILES;
     uint8_t* staged = tiles + SH::QTILE * 2 * SH::HALF;
@@ -563,19 +568,19 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         }
     } else if (warp == 1 && lane == 0) {
         for (int i = 0; i < NB; ++i) {
-            mbar_init(&v_full[i], 4);
+            mbar_init(&v_full[i], SW);
             mbar_init(&k_empty[i], 1);
             mbar_init(&v_empty[i], 1);
             mbar_init(&k_land[i], 1);
             mbar_init(&v_land[i], 1);
         }
-        for (int i = 0; i < RING; ++i) mbar_init(&k_full[i], TYPE == AF_KV_F16 ? 1 : 4);
-        for (int i = 0; i < 4; ++i) mbar_init(&raw_free[i], 4);
+        for (int i = 0; i < RING; ++i) mbar_init(&k_full[i], TYPE == AF_KV_F16 ? 1 : SW);
+        for (int i = 0; i < 4; ++i) mbar_init(&raw_free[i], SW);
         for (int i = 0; i < NS; ++i) mbar_init(&s_full[i], 1);
         mbar_init(o_full, 1);
-        mbar_init(q_full, 12);
+        mbar_init(q_full, kOutWarp + 4);
         mbar_init(done, 1);
-        for (int i = 0; i < 4; ++i) mbar_init(&x_full[i], 2);
+        for (int i = 0; i < 4 * SETS; ++i) mbar_init(&x_full[i], 2);
         *flag = 0;
     } else if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(512u)
@@ -597,7 +602,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             mbar_init(&c_full[i], live_warps);
         }
         mbar_init(o_free, live_warps);
-        mbar_init(fin, 2 * live_warps);
+        mbar_init(fin, SETS * 2 * live_warps);
     }
     if (tid < 64) fence_mbar_init();
     tc_fence_before();
@@ -620,22 +625,22 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     // place, from there a row a thread (hi by softmax warps 0-3, lo by 4-7) into tensor memory.  Rows that are
     // none keep what is there: what comes of them stays in their own row.
     auto queries = [&]() {
-        constexpr int Q4 = HD / 4, QR = 32 / Q4, QN = (128 / QR + 11) / 12;  // lanes of a row at 16 bytes, rows and number of a warp's loads
+        constexpr int QW = kOutWarp + 4, Q4 = HD / 4, QR = 32 / Q4, QN = (128 / QR + QW - 1) / QW;  // lanes of a row at 16 bytes, rows and number of a warp's loads
         const int sub = lane / Q4, col = lane % Q4, rows = row_hi - row_lo;
         const bool wide = ((reinterpret_cast<uintptr_t>(p.q) & 15) | (p.qs & 3)) == 0;
         float4 f[QN];  // all in flight
 #pragma unroll
         for (int j = 0; j < QN; ++j) {
-            if ((warp + 12 * j) * QR >= rows) break;
-            const int x = row_lo + min((warp + 12 * j) * QR + sub, rows - 1), node = node_of(p, x);
+            if ((warp + QW * j) * QR >= rows) break;
+            const int x = row_lo + min((warp + QW * j) * QR + sub, rows - 1), node = node_of(p, x);
             const float* q = p.q + (long long)(r0 + node) * p.qs + (kvh * p.G + x - node * p.G) * HD + 4 * col;
             if (wide) f[j] = __ldg(reinterpret_cast<const float4*>(q));
             else f[j] = make_float4(q[0], q[1], q[2], q[3]);
         }
 #pragma unroll
         for (int j = 0; j < QN; ++j) {
-            if ((warp + 12 * j) * QR >= rows) break;
-            const int i = (warp + 12 * j) * QR + sub;
+            if ((warp + QW * j) * QR >= rows) break;
+            const int i = (warp + QW * j) * QR + sub;
             uint32_t mx = __float_as_uint(max3_abs_nan(max3_abs_nan(0.f, f[j].x, f[j].y), f[j].z, f[j].w));
             if (QR == 1) {
                 mx = __reduce_max_sync(0xffffffffu, mx);
@@ -654,7 +659,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 if (col == 0) s_rs[i] = p.scale * pow2(-a);
             }
         }
-        asm volatile("bar.sync 1, 384;" ::: "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(QW * 32) : "memory");
         const int mine = tid & 127;
         if (warp < 8 && (mine & ~31) < rows) {
             const int from = warp < 4 ? 0 : 2 * HD;
@@ -676,12 +681,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
 
     if (warp < kOutWarp) {
         // ------------------------------------------------------- softmax
-        // Warps 0-3 have the first half of a tile's columns, 4-7 the second, of the same rows; a row's two threads
-        // tell each other their largest value and keep sums of their own.
-        if constexpr (SH::REG_S > 80) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH::REG_S));
-        else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::REG_S));
+        // A set of 8 warps takes every SETS-th tile: its warps 0-3 have the first half of a tile's columns, 4-7 the
+        // second, of the same rows.  A row's two threads tell each other their largest value and keep sums of their
+        // own; the sets know nothing of each other, the output warps bring their tiles to one largest value.
+        if constexpr (SH::REG_S > 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH::REG_S));
+        else if constexpr (SH::REG_S < 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::REG_S));
         constexpr int C = T / 2;
-        const int half = warp >> 2, ti = tid & 127, w4 = warp & 3;
+        const int set = warp >> 3, half = (warp >> 2) & 1, ti = tid & 127, w4 = warp & 3;
+        uint64_t* x_mine = x_full + 4 * set + w4;
+        float* other = s_other + (set * 4 + half) * kMmaRows + ti;  // [in turn][half][row]
         const uint32_t lanes = (uint32_t)(w4 * 32) << 16;
         const int r = row_lo + ti;
         const bool live = r < row_hi;
@@ -698,8 +706,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             if (lane == 0) mbar_arrive(&p_full[sl]);
         };
         const int tiles_mine = w4 < live_warps ? nt : 0;
-        int sl = 0, sl_ph = 0, st = 0, st_ph = 0, kt = 0, kt_ph = 0;  // rings of NS, NB, RING and their phases
-        for (int t = 0; t < tiles_mine; ++t) {
+        int sl = set, sl_ph = 0, st = set, st_ph = 0, kt = set, kt_ph = 0;  // rings of NS, NB, RING and their phases
+        static_assert(NS % SETS == 0 && NB % SETS == 0 && RING % SETS == 0, "rings");
+        int turn = 0;
+        for (int t = set; t < tiles_mine; t += SETS, ++turn) {
             ok = (TYPE == AF_KV_F16 || wait_warp(&k_full[kt], kt_ph)) && wait_warp(&s_full[sl], sl_ph);
             if (!ok) break;
             tc_fence_after();
@@ -707,27 +717,30 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             float v[C];
 #pragma unroll
             for (int c = 0; c < C / 32; ++c) tc_ld32(sb + 32 * c, v + 32 * c);
-            if (t) publish(sl ? sl - 1 : NS - 1);
+            if (SETS == 1 && t) publish(sl ? sl - 1 : NS - 1);
             tc_wait_ld();
 #pragma unroll
             for (int i = 0; i < C; ++i) asm volatile("" : "+f"(v[i]));  // no use may move above the wait
-            const float4* kc = reinterpret_cast<const float4*>(scales + kt * 3 * SH::GROUPS) + half;  // 2^-a of K
+            const float4* kc = reinterpret_cast<const float4*>(scales + kt * 3 * SH::GROUPS) + half * (SH::GROUPS / 8);  // 2^-a of K
             const float4* vf = kc + SH::GROUPS / 4;                                                   // -a of V
             const float4* vg = vf + SH::GROUPS / 4;                                                   // 2^a of V
             if (TYPE != AF_KV_F16) ok = wait_warp(&v_full[st], st_ph);
             if (!ok) break;
             {
-                float c[4] = {rs, rs, rs, rs}, f[4] = {0.f, 0.f, 0.f, 0.f};
-                if (TYPE != AF_KV_F16) {
-                    const float4 x = *kc, z = *vf;
-                    c[0] *= x.x, c[1] *= x.y, c[2] *= x.z, c[3] *= x.w;
-                    f[0] = z.x, f[1] = z.y, f[2] = z.z, f[3] = z.w;
-                }
 #pragma unroll
-                for (int e = 0; e < C; e += 2) {
-                    const int g = e / SH::RPW;
-                    const f32x2 x = pair(v[e], v[e + 1]), cc = pair(c[g], c[g]);
-                    unpair(TYPE == AF_KV_F16 ? mul2(x, cc) : fma2(x, cc, pair(f[g], f[g])), v[e], v[e + 1]);
+                for (int e = 0; e < C; e += 4 * SH::RPW) {
+                    float c[4] = {rs, rs, rs, rs}, f[4] = {0.f, 0.f, 0.f, 0.f};
+                    if (TYPE != AF_KV_F16) {
+                        const float4 x = kc[e / (4 * SH::RPW)], z = vf[e / (4 * SH::RPW)];
+                        c[0] *= x.x, c[1] *= x.y, c[2] *= x.z, c[3] *= x.w;
+                        f[0] = z.x, f[1] = z.y, f[2] = z.z, f[3] = z.w;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4 * SH::RPW; i += 2) {
+                        const int g = i / SH::RPW;
+                        const f32x2 x = pair(v[e + i], v[e + i + 1]), cc = pair(c[g], c[g]);
+                        unpair(TYPE == AF_KV_F16 ? mul2(x, cc) : fma2(x, cc, pair(f[g], f[g])), v[e + i], v[e + i + 1]);
+                    }
                 }
             }
             const int p0 = (t0 + t) * T + half * C;
@@ -742,33 +755,33 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             for (int i = 4; i + 1 < C; i += 2) top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], v[i], v[i + 1]);
             float mn = max3(m, fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
             // the row's other half, in two places in turn: this one is written again when both have read it
-            s_other[((t & 1) * 2 + half) * kMmaRows + ti] = mn;
+            other[(turn & 1) * 2 * kMmaRows] = mn;
             __syncwarp();
-            if (lane == 0) mbar_arrive(&x_full[w4]);
-            ok = wait_warp(&x_full[w4], t);
+            if (lane == 0) mbar_arrive(x_mine);
+            ok = wait_warp(x_mine, turn);
             if (!ok) break;
-            mn = fmaxf(mn, s_other[((t & 1) * 2 + (half ^ 1)) * kMmaRows + ti]);
+            mn = fmaxf(mn, other[((turn & 1) * 2 + (half ? -1 : 1)) * kMmaRows]);
             const float ms = mn == -INFINITY ? 0.f : mn - 14.f;  // weights times 2^14
             const float corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
             m = mn;
             if (half == 0) {
                 // its place is free: these scores were issued behind the products of t - LA - 1, which waited until those
                 // of t - LA - 2 (or t - NS) were taken
-                s_corr[sl * kMmaRows + ti] = corr;
+                s_tile[sl * kMmaRows + ti] = mn;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c_full[sl]);
             }
             f32x2 sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
             const f32x2 ms2 = pair(-ms, -ms);
-            float g4[4];
-            if (TYPE != AF_KV_F16) {
-                const float4 x = *vg;
-                g4[0] = x.x, g4[1] = x.y, g4[2] = x.z, g4[3] = x.w;
-            }
 #pragma unroll
             for (int c = 0; c < C / 16; ++c) {
                 uint32_t hi[8], lo[8];
                 float w[16];
+                float g4[4];
+                if (TYPE != AF_KV_F16) {
+                    const float4 x = vg[16 * c / (4 * SH::RPW)];
+                    g4[0] = x.x, g4[1] = x.y, g4[2] = x.z, g4[3] = x.w;
+                }
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) unpair(add2(pair(v[16 * c + i], v[16 * c + i + 1]), ms2), w[i], w[i + 1]);
 #pragma unroll
@@ -779,7 +792,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                     if (TYPE == AF_KV_F16) {
                         sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], x);
                     } else {
-                        const float g = g4[(16 * c + i) / SH::RPW];
+                        const float g = g4[(16 * c + i) / SH::RPW % 4];
                         sum[(i >> 1) & 1] = fma2(x, pair(g, g), sum[(i >> 1) & 1]);
                     }
                     split2(x, hi[i / 2], lo[i / 2]);
@@ -792,14 +805,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 unpair(add2(sum[0], sum[1]), a, b);
                 l = fmaf(l, corr, a + b);
             }
-            if (++sl == NS) sl = 0, sl_ph ^= 1;
-            if (++st == NB) st = 0, st_ph ^= 1;
-            if (++kt == RING) kt = 0, kt_ph ^= 1;
+            if (SETS > 1) publish(sl);
+            if ((sl += SETS) >= NS) sl -= NS, sl_ph ^= 1;
+            if ((st += SETS) >= NB) st -= NB, st_ph ^= 1;
+            if ((kt += SETS) >= RING) kt -= RING, kt_ph ^= 1;
         }
-        if (ok && tiles_mine) publish(sl ? sl - 1 : NS - 1);
+        if (SETS == 1 && ok && tiles_mine) publish(sl ? sl - 1 : NS - 1);
         if (!ok) *flag = 1;
-        if (half == 0) s_top[ti] = m;
-        s_sum[half * kMmaRows + ti] = l;
+        if (half == 0) s_top[set * kMmaRows + ti] = m;
+        s_sum[(2 * set + half) * kMmaRows + ti] = l;
         __syncwarp();
         if (lane == 0 && w4 < live_warps) mbar_arrive(fin);
     } else if (warp < kSplitWarp) {
@@ -815,11 +829,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         for (int i = 0; i < HD; ++i) acc[i] = 0.f;
         bool ok = w < live_warps;
         int sl = 0, sl_ph = 0;
-        for (int t = 0; ok && t < nt; ++t) {  // acc = acc·corr + (P·V)(t)
+        float top = -INFINITY;  // what acc is relative to
+        for (int t = 0; ok && t < nt; ++t) {  // acc = acc·2^(old top - top) + (P·V)(t)·2^(its top - top)
             ok = wait_warp(&c_full[sl], sl_ph) && wait_warp(o_full, t);
             if (!ok) break;
             tc_fence_after();
-            const float corr = s_corr[sl * kMmaRows + ti];
+            const float mine = s_tile[sl * kMmaRows + ti], to = fmaxf(top, mine), at = to == -INFINITY ? 0.f : to;
+            const float corr = ex2(top - at), f = SETS > 1 ? ex2(mine - at) : 1.f;
+            top = to;
             if (++sl == NS) sl = 0, sl_ph ^= 1;
 #pragma unroll
             for (int c = 0; c < HD / 16; ++c) {
@@ -832,7 +849,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 for (int i = 0; i < 16; i += 2) {
                     float& x = acc[16 * c + i];
                     float& y = acc[16 * c + i + 1];
-                    unpair(fma2(pair(x, y), pair(corr, corr), pair(o[i], o[i + 1])), x, y);
+                    f32x2 add = pair(o[i], o[i + 1]);
+                    if (SETS > 1) add = mul2(add, pair(f, f));
+                    unpair(fma2(pair(x, y), pair(corr, corr), add), x, y);
                 }
             }
             tc_fence_before();
@@ -865,7 +884,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         }
         if (ok) {
             const int splits = spot.splits, mine_rows = min(32, row_hi - row_lo - w * 32);
-            const float l = s_sum[ti] + s_sum[kMmaRows + ti], inv = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+            float l = s_sum[ti] + s_sum[kMmaRows + ti];
+            if (SETS > 1) {  // top is the larger of the two sets'
+                const float at = top == -INFINITY ? 0.f : top;
+                l *= ex2(s_top[ti] - at);
+                l = fmaf(s_sum[2 * kMmaRows + ti] + s_sum[3 * kMmaRows + ti], ex2(s_top[kMmaRows + ti] - at), l);
+            }
+            const float inv = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
             for (int i = 0; i < HD; i += 4)
                 *reinterpret_cast<float4*>(staged_at(ti, 4 * i)) =
@@ -881,7 +906,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                         *reinterpret_cast<float4*>(o + i * HD) = from(i);
                 if (lane < mine_rows)
                     *reinterpret_cast<float2*>(mp.part + (long long)mp.slots * kMmaRows * HD + (at + lane) * 2) =
-                        make_float2(s_top[ti], l);
+                        make_float2(top, l);
             } else {
                 float* orow = live ? p.out + (long long)row * p.os + (long long)head * HD : nullptr;
                 const bool wide_out = ((reinterpret_cast<uintptr_t>(p.out) & 15) | (p.os & 3)) == 0;
@@ -900,8 +925,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     } else if (warp < kMmaWarp) {
         // ------------------------------------------------- splitting K and V
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::REG_K));
-        const bool isv = warp >= kSplitWarp + 4;
-        const int w = warp & 3;
+        const bool isv = warp >= kSplitWarp + SW;
+        const int w = (warp - kSplitWarp) % SW;
         uint64_t *full = isv ? v_full : k_full, *empty = isv ? v_empty : k_empty, *land = isv ? v_land : k_land;
         const int ring = isv ? NB : RING;
         auto hand_over = [&](uint64_t* bar) {
@@ -940,7 +965,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                     float big[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int i = 0; i < NX; ++i) x[i] = *reinterpret_cast<const float4*>(src + i * 512);
-                    const int left = end - (t0 + t) * T - (s * 4 + w) * SH::RPW - sub;  // rows in front of the end
+                    const int left = end - (t0 + t) * T - (s * SW + w) * SH::RPW - sub;  // rows in front of the end
                     if (left < SH::RPW) {                                               // the last tile: what lies behind is nothing
 #pragma unroll
                         for (int i = 0; i < NX; ++i)
@@ -972,19 +997,19 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                     const int a = scale_of(mx, isv ? 60 : 100);
                     const float f = pow2(a);
                     const f32x2 f2 = pair(f, f);
-                    uint8_t* dst = home + st * 2 * SH::HALF + s * 4 * SH::RPW * 128;
+                    uint8_t* dst = home + st * 2 * SH::HALF + s * SW * SH::RPW * 128;
 #pragma unroll
                     for (int i = 0; i < NX; ++i) {
                         uint2 hi, lo;
                         split2(mul2(pair(x[i].x, x[i].y), f2), hi.x, lo.x);
                         split2(mul2(pair(x[i].z, x[i].w), f2), hi.y, lo.y);
                         const int rr = i * SH::RPC + sub;
-                        uint8_t* d = dst + rr * 128 + (((in_half >> 4) ^ (rr & 7)) << 4);
+                        uint8_t* d = dst + rr * 128 + (((in_half >> 4) ^ ((w * SH::RPW + rr) & 7)) << 4);
                         *reinterpret_cast<uint2*>(d) = hi;
                         *reinterpret_cast<uint2*>(d + SH::TILE) = lo;
                     }
                     if (lane == 0) {
-                        float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + s * 4 + w;
+                        float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + s * SW + w;
                         sc[0] = isv ? (float)-a : pow2(-a);
                         if (isv) sc[SH::GROUPS] = f;
                     }
@@ -997,7 +1022,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             // 512 bytes of the warp's rows: 4 rows of 64 values; in place
             constexpr int NC = SH::RPW * HD * 2 / 512, PER = SH::RPW / 4;  // accesses of a group; of its rows' 64 values
             auto fix = [&](int t, int s) {
-                uint8_t* at = tiles + (st * 2 + (isv ? 1 : 0)) * SH::HALF + (s * 4 + w) * SH::RPW * 128 + lane * 16;
+                uint8_t* at = tiles + (st * 2 + (isv ? 1 : 0)) * SH::HALF + (s * SW + w) * SH::RPW * 128 + lane * 16;
                 auto place = [&](int i) { return at + (i / PER) * SH::COLS + (i % PER) * 512; };
                 uint4 x[NC];
                 uint32_t* e = &x[0].x;
@@ -1020,7 +1045,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                         note_bad(t);
                     }
                 } else {
-                    const int left = end - (t0 + t) * T - (s * 4 + w) * SH::RPW - lane / 8;  // rows in front of the end
+                    const int left = end - (t0 + t) * T - (s * SW + w) * SH::RPW - lane / 8;  // rows in front of the end
                     if (left < SH::RPW) {                                                    // the last tile: what lies behind is nothing
 #pragma unroll
                         for (int i = 0; i < NC; ++i)
@@ -1053,7 +1078,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
 #pragma unroll
                     for (int i = 0; i < NC; ++i) *reinterpret_cast<uint4*>(place(i)) = x[i];
                     if (lane == 0) {
-                        float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + s * 4 + w;
+                        float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + s * SW + w;
                         sc[0] = isv ? (float)-a : pow2(-a);
                         if (isv) sc[SH::GROUPS] = f;
                     }
