@@ -5,6 +5,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -291,27 +292,29 @@ __device__ __forceinline__ float pow2(int a) { return __int_as_float((a + 127) <
 constexpr int kMmaThreads = 1024;
 constexpr int kMmaWarp = 28, kCopyWarp = 29;  // copies of K, of V
 constexpr int kMmaRows = 128;
-constexpr int kTreeTile = 64;
+constexpr int tree_tile(int type) { return type == AF_KV_F32 ? 64 : 128; }  // positions of a tile
 constexpr int kMmaBadWords = 512;  // tiles of a split whose V holds something non-finite, a bit each
 
 template <int TYPE, int HD>
 struct MmaShape {
     static constexpr bool F32 = TYPE == AF_KV_F32;
     static constexpr int SIZE = F32 ? 4 : 2;
-    static constexpr int T = kTreeTile;                 // positions of a tile
+    static constexpr int T = tree_tile(TYPE);
     static constexpr int TERMS = F32 ? 2 : 1;           // hi, lo of K and V
-    static constexpr int SETS = F32 ? 1 : 2;            // of 8 softmax warps, which take the tiles in turn
+    static constexpr int PARTS = T / 32;                // of a row's scores: 32 a softmax thread
     static constexpr int SW = F32 ? 8 : 4;              // splitting warps of K, of V
-    static constexpr int OUT = 8 * SETS, SPLIT_K = OUT + 4, SPLIT_V = SPLIT_K + SW;  // first warps
+    static constexpr int OUT = 4 * PARTS, SPLIT_K = OUT + 4, SPLIT_V = SPLIT_K + SW;  // first warps
     static_assert(SPLIT_V + SW == kMmaWarp, "warps");
     static constexpr int COLS = T * 128;                // 64 values of every row
     static constexpr int TILE = HD / 64 * COLS;
     static constexpr int HALF = TERMS * TILE;           // K or V of a tile: hi, lo
-    static constexpr int NB = F32 ? 256 / HD : 6;       // tiles in shared memory: K V K V ...
-    static constexpr int LA = F32 ? 1 : 2;              // tiles whose scores are issued ahead of the products of one
+    static constexpr int NB = F32 ? 256 / HD : 3;       // tiles in shared memory: K V K V ...
+    static constexpr int NS = F32 ? 4 : HD == 128 ? 2 : 3;  // score tiles in tensor memory (each becomes its weights)
+    static constexpr int LA = F32 ? 1 : NS - 1;         // tiles whose scores are issued ahead of the products of one
+    static constexpr int NC = LA + 2;                   // corrections
     static constexpr int RING = NB + LA + 2;            // barriers and scales of K (see k_full)
     static constexpr int RAWB = T / 2 * HD * 4;         // f32: half the rows of K or V as they are
-    static constexpr int RPW = T / 2 / SW;              // rows that share a power of two: a splitting warp's, of half a tile
+    static constexpr int RPW = 8;                       // rows that share a power of two: a splitting warp takes them together
     static constexpr int LPR = HD * SIZE / 16;          // lanes of a row (f32)
     static constexpr int RPC = 32 / LPR;                // rows of a warp's 512 bytes (f32)
     // queries in, rows out: 128 rows over the last tiles' place, 16-byte columns swizzled by the row
@@ -319,17 +322,17 @@ struct MmaShape {
     static constexpr int QTILE = NB - (kMmaRows * QROW + 2 * HALF - 1) / (2 * HALF);
     static_assert(QTILE >= 1, "the first tile does not wait for the queries");
     // registers
-    static constexpr int REG_S = F32 ? 72 : HD == 128 ? 56 : 64, REG_O = HD == 128 ? 168 : 104, REG_K = !F32 && HD == 64 ? 56 : 40, REG_M = 40;
-    static_assert(2 * SETS * REG_S + REG_O + SW / 2 * REG_K + REG_M <= 8 * 64, "what the launch gives: 1,024 threads of 64");
+    static constexpr int REG_S = F32 || HD == 64 ? 64 : 56, REG_O = HD == 64 ? 104 : F32 ? 160 : 168,
+                         REG_K = F32 ? 48 : HD == 64 ? 56 : 40, REG_M = F32 && HD == 128 ? 32 : 40;
+    static_assert(PARTS * REG_S + REG_O + SW / 2 * REG_K + REG_M <= 8 * 64, "what the launch gives: 1,024 threads of 64");
     // tensor memory columns
-    static constexpr int NS = 4;                          // score tiles (each becomes its weights)
     static constexpr int QH = 0, QL = HD / 2, S0 = HD, O0 = HD + NS * T;
     static_assert(O0 + HD <= 512, "tensor memory");
     // shared memory, behind 768 bytes of mbarriers
     static constexpr int BAD = 768;                       // kMmaBadWords words
-    static constexpr int ROWS = BAD + kMmaBadWords * 4;   // [128] query scales, [NS][128] tops of tiles; a set's [2][2][128] exchange, [128] tops, [2][128] sums
+    static constexpr int ROWS = BAD + kMmaBadWords * 4;   // [128] query scales, [NC][128] corrections, [2][PARTS][128] exchange, [128] tops, [PARTS][128] sums
     static constexpr int GROUPS = T / RPW;
-    static constexpr int SCALE = ROWS + (1 + NS + 7 * SETS) * kMmaRows * 4;  // [RING][3][GROUPS] floats
+    static constexpr int SCALE = ROWS + (2 + NC + 3 * PARTS) * kMmaRows * 4;  // [RING][3][GROUPS] floats
     static constexpr int TILES = (SCALE + RING * 3 * GROUPS * 4 + 1023) / 1024 * 1024;
     static constexpr int RAW = TILES + NB * 2 * HALF;
     static constexpr int BYTES = RAW + (F32 ? 4 * RAWB : 0);  // K, K, V, V
@@ -509,7 +512,7 @@ template <int TYPE, int HD>
 __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_constant__ MmaParams mp) {
     using SH = MmaShape<TYPE, HD>;
     using E = KvElem<TYPE>;
-    constexpr int T = SH::T, NB = SH::NB, NS = SH::NS, RING = SH::RING, SETS = SH::SETS, SW = SH::SW;
+    constexpr int T = SH::T, NB = SH::NB, NS = SH::NS, NC = SH::NC, RING = SH::RING, SW = SH::SW, PARTS = SH::PARTS;
     constexpr int kOutWarp = SH::OUT, kSplitWarp = SH::SPLIT_K;
     extern __shared__ __align__(1024) uint8_t sm[];
     const TreeParams& p = mp.t;
@@ -525,22 +528,21 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     uint64_t* raw_free = v_land + NB;                    // [2][2] f32: the splitting warps have half of K's, V's rows in registers
     uint64_t* s_full = raw_free + 4;              // [NS] scores done
     uint64_t* p_full = s_full + NS;                      // [NS] softmax warps: weights written
-    uint64_t* c_full = p_full + NS;                      // [NS] softmax warps: largest score written
-    uint64_t* o_full = c_full + NS;                      // P·V done
+    uint64_t* c_full = p_full + NS;                      // [NC] softmax warps: correction written
+    uint64_t* o_full = c_full + NC;                      // P·V done
     uint64_t* o_free = o_full + 1;                       // output warps: P·V and correction taken
     uint64_t* q_full = o_free + 1;                       // softmax and output warps: queries written
     uint64_t* fin = q_full + 1;                          // softmax warps: tops and sums written
     uint64_t* done = fin + 1;                            // every product done
-    uint64_t* x_full = done + 1;                         // [SETS][4] the two softmax warps of 32 rows: largest scores written
-    static_assert((RING + 5 * NB + 3 * NS + 9 + 4 * SETS) * 8 + 16 <= SH::BAD, "barriers");
-    uint32_t* tslot = reinterpret_cast<uint32_t*>(x_full + 4 * SETS);
+    static_assert((RING + 5 * NB + 2 * NS + NC + 9) * 8 + 16 <= SH::BAD, "barriers");
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(done + 1);
     volatile int* flag = reinterpret_cast<volatile int*>(tslot + 1);
     uint32_t* bad = reinterpret_cast<uint32_t*>(sm + SH::BAD);
     float* s_rs = reinterpret_cast<float*>(sm + SH::ROWS);
-    float* s_tile = s_rs + kMmaRows;
-    float* s_other = s_tile + NS * kMmaRows;
-    float* s_top = s_other + SETS * 4 * kMmaRows;
-    float* s_sum = s_top + SETS * kMmaRows;
+    float* s_corr = s_rs + kMmaRows;
+    float* s_other = s_corr + NC * kMmaRows;
+    float* s_top = s_other + 2 * PARTS * kMmaRows;
+    float* s_sum = s_top + kMmaRows;
     float* scales = reinterpret_cast<float*>(sm + SH::SCALE);
     uint8_t* tiles = sm + SH::TILES;
     uint8_t* staged = tiles + SH::QTILE * 2 * SH::HALF;
@@ -575,12 +577,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             mbar_init(&v_land[i], 1);
         }
         for (int i = 0; i < RING; ++i) mbar_init(&k_full[i], TYPE == AF_KV_F16 ? 1 : SW);
-        for (int i = 0; i < 4; ++i) mbar_init(&raw_free[i], SW);
+        for (int i = 0; i < 4; ++i) mbar_init(&raw_free[i], SW / 2);
         for (int i = 0; i < NS; ++i) mbar_init(&s_full[i], 1);
         mbar_init(o_full, 1);
         mbar_init(q_full, kOutWarp + 4);
         mbar_init(done, 1);
-        for (int i = 0; i < 4 * SETS; ++i) mbar_init(&x_full[i], 2);
         *flag = 0;
     } else if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(512u)
@@ -598,11 +599,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     const int live_warps = (row_hi - row_lo + 31) / 32;  // of every 4 that work on rows; the others have none
     if (tid == 0 && seq >= 0) {
         for (int i = 0; i < NS; ++i) {
-            mbar_init(&p_full[i], 2 * live_warps);
-            mbar_init(&c_full[i], live_warps);
+            mbar_init(&p_full[i], PARTS * live_warps);
         }
+        for (int i = 0; i < NC; ++i) mbar_init(&c_full[i], live_warps);
         mbar_init(o_free, live_warps);
-        mbar_init(fin, SETS * 2 * live_warps);
+        mbar_init(fin, PARTS * live_warps);
     }
     if (tid < 64) fence_mbar_init();
     tc_fence_before();
@@ -649,14 +650,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 for (int o = 1; o < Q4; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
             }
             const int a = scale_of(mx, 100);
-            const f32x2 s = pair(pow2(a), pow2(a));
+            const float sg = copysignf(pow2(a), p.scale);  // a negative scale turns the query around
+            const f32x2 s = pair(sg, sg);
             uint2 hi, lo;
             split2(mul2(pair(f[j].x, f[j].y), s), hi.x, lo.x);
             split2(mul2(pair(f[j].z, f[j].w), s), hi.y, lo.y);
             if (i < rows) {
                 *reinterpret_cast<uint2*>(staged_at(i, 8 * col)) = hi;
                 *reinterpret_cast<uint2*>(staged_at(i, 2 * HD + 8 * col)) = lo;
-                if (col == 0) s_rs[i] = p.scale * pow2(-a);
+                if (col == 0) s_rs[i] = fmaxf(fabsf(p.scale) * pow2(-a), FLT_MIN);
             }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(QW * 32) : "memory");
@@ -681,15 +683,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
 
     if (warp < kOutWarp) {
         // ------------------------------------------------------- softmax
-        // A set of 8 warps takes every SETS-th tile: its warps 0-3 have the first half of a tile's columns, 4-7 the
-        // second, of the same rows.  A row's two threads tell each other their largest value and keep sums of their
-        // own; the sets know nothing of each other, the output warps bring their tiles to one largest value.
+        // Four warps have 32 of a tile's columns, the next four the next 32, of the same rows.  A row's threads tell
+        // one another their largest value and keep sums of their own.
         if constexpr (SH::REG_S > 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH::REG_S));
         else if constexpr (SH::REG_S < 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::REG_S));
-        constexpr int C = T / 2;
-        const int set = warp >> 3, half = (warp >> 2) & 1, ti = tid & 127, w4 = warp & 3;
-        uint64_t* x_mine = x_full + 4 * set + w4;
-        float* other = s_other + (set * 4 + half) * kMmaRows + ti;  // [in turn][half][row]
+        constexpr int C = 32;
+        const int part = warp >> 2, ti = tid & 127, w4 = warp & 3;
         const uint32_t lanes = (uint32_t)(w4 * 32) << 16;
         const int r = row_lo + ti;
         const bool live = r < row_hi;
@@ -698,7 +697,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         const float rs = s_rs[ti];  // what a raw score is times, but for K's power of two
-        // weights written: said a little late, when the next scores are on their way
         auto publish = [&](int sl) {
             tc_wait_st();
             tc_fence_before();
@@ -706,44 +704,35 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             if (lane == 0) mbar_arrive(&p_full[sl]);
         };
         const int tiles_mine = w4 < live_warps ? nt : 0;
-        int sl = set, sl_ph = 0, st = set, st_ph = 0, kt = set, kt_ph = 0;  // rings of NS, NB, RING and their phases
-        static_assert(NS % SETS == 0 && NB % SETS == 0 && RING % SETS == 0, "rings");
-        int turn = 0;
-        for (int t = set; t < tiles_mine; t += SETS, ++turn) {
+        int sl = 0, sl_ph = 0, st = 0, st_ph = 0, kt = 0, kt_ph = 0, co = 0;  // rings of NS, NB, RING, NC and their phases
+        int met = 0;  // the tiles at which the row's warps have met
+        for (int t = 0; t < tiles_mine; ++t) {
             ok = (TYPE == AF_KV_F16 || wait_warp(&k_full[kt], kt_ph)) && wait_warp(&s_full[sl], sl_ph);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t sb = tmem + lanes + SH::S0 + sl * T + half * C;
+            const uint32_t sb = tmem + lanes + SH::S0 + sl * T + part * C;
             float v[C];
 #pragma unroll
             for (int c = 0; c < C / 32; ++c) tc_ld32(sb + 32 * c, v + 32 * c);
-            if (SETS == 1 && t) publish(sl ? sl - 1 : NS - 1);
             tc_wait_ld();
 #pragma unroll
             for (int i = 0; i < C; ++i) asm volatile("" : "+f"(v[i]));  // no use may move above the wait
-            const float4* kc = reinterpret_cast<const float4*>(scales + kt * 3 * SH::GROUPS) + half * (SH::GROUPS / 8);  // 2^-a of K
+            static_assert(C == 4 * SH::RPW, "a thread's powers of two are four");
+            const float4* kc = reinterpret_cast<const float4*>(scales + kt * 3 * SH::GROUPS) + part;  // 2^-a of K
             const float4* vf = kc + SH::GROUPS / 4;                                                   // -a of V
             const float4* vg = vf + SH::GROUPS / 4;                                                   // 2^a of V
             if (TYPE != AF_KV_F16) ok = wait_warp(&v_full[st], st_ph);
             if (!ok) break;
-            {
+            if (TYPE != AF_KV_F16) {
+                const float4 x = *kc, z = *vf;
+                const float c[4] = {rs * x.x, rs * x.y, rs * x.z, rs * x.w}, f[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
-                for (int e = 0; e < C; e += 4 * SH::RPW) {
-                    float c[4] = {rs, rs, rs, rs}, f[4] = {0.f, 0.f, 0.f, 0.f};
-                    if (TYPE != AF_KV_F16) {
-                        const float4 x = kc[e / (4 * SH::RPW)], z = vf[e / (4 * SH::RPW)];
-                        c[0] *= x.x, c[1] *= x.y, c[2] *= x.z, c[3] *= x.w;
-                        f[0] = z.x, f[1] = z.y, f[2] = z.z, f[3] = z.w;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4 * SH::RPW; i += 2) {
-                        const int g = i / SH::RPW;
-                        const f32x2 x = pair(v[e + i], v[e + i + 1]), cc = pair(c[g], c[g]);
-                        unpair(TYPE == AF_KV_F16 ? mul2(x, cc) : fma2(x, cc, pair(f[g], f[g])), v[e + i], v[e + i + 1]);
-                    }
+                for (int e = 0; e < C; e += 2) {
+                    const int g = e / SH::RPW;
+                    unpair(fma2(pair(v[e], v[e + 1]), pair(c[g], c[g]), pair(f[g], f[g])), v[e], v[e + 1]);
                 }
             }
-            const int p0 = (t0 + t) * T + half * C;
+            const int p0 = (t0 + t) * T + part * C;
             if (p0 + C > len) {
                 unsigned long long see = live ? tree_window(p, row, node, n, len, p0) : 0ull;
 #pragma unroll
@@ -753,37 +742,43 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
             for (int i = 4; i + 1 < C; i += 2) top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], v[i], v[i + 1]);
-            float mn = max3(m, fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            // the row's other half, in two places in turn: this one is written again when both have read it
-            other[(turn & 1) * 2 * kMmaRows] = mn;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(x_mine);
-            ok = wait_warp(x_mine, turn);
-            if (!ok) break;
-            mn = fmaxf(mn, other[((turn & 1) * 2 + (half ? -1 : 1)) * kMmaRows]);
+            float mn = max3(top[0], top[1], fmaxf(top[2], top[3]));
+            if (TYPE == AF_KV_F16 && mn != -INFINITY) mn *= rs;  // rs > 0: raw scores have the same largest one
+            mn = fmaxf(m, mn);
+            // the row's other parts, in two places in turn: this one is written again when all have read it
+            float* others = s_other + (t & 1) * PARTS * kMmaRows + ti;
+            others[part * kMmaRows] = mn;
+            asm volatile("bar.sync %0, %1;" ::"r"(2 + w4), "n"(PARTS * 32) : "memory");
+            ++met;
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) mn = fmaxf(mn, others[i * kMmaRows]);
             const float ms = mn == -INFINITY ? 0.f : mn - 14.f;  // weights times 2^14
             const float corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
             m = mn;
-            if (half == 0) {
+            if (part == 0) {
                 // its place is free: these scores were issued behind the products of t - LA - 1, which waited until those
-                // of t - LA - 2 (or t - NS) were taken
-                s_tile[sl * kMmaRows + ti] = mn;
+                // of t - NC were taken
+                s_corr[co * kMmaRows + ti] = corr;
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&c_full[sl]);
+                if (lane == 0) mbar_arrive(&c_full[co]);
             }
+            if (++co == NC) co = 0;
             f32x2 sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-            const f32x2 ms2 = pair(-ms, -ms);
+            const f32x2 ms2 = pair(-ms, -ms), rs2 = pair(rs, rs);
+            float g4[4];
+            if (TYPE != AF_KV_F16) {
+                const float4 x = *vg;
+                g4[0] = x.x, g4[1] = x.y, g4[2] = x.z, g4[3] = x.w;
+            }
 #pragma unroll
             for (int c = 0; c < C / 16; ++c) {
                 uint32_t hi[8], lo[8];
                 float w[16];
-                float g4[4];
-                if (TYPE != AF_KV_F16) {
-                    const float4 x = vg[16 * c / (4 * SH::RPW)];
-                    g4[0] = x.x, g4[1] = x.y, g4[2] = x.z, g4[3] = x.w;
-                }
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) unpair(add2(pair(v[16 * c + i], v[16 * c + i + 1]), ms2), w[i], w[i + 1]);
+                for (int i = 0; i < 16; i += 2) {
+                    const f32x2 x = pair(v[16 * c + i], v[16 * c + i + 1]);
+                    unpair(TYPE == AF_KV_F16 ? fma2(x, rs2, ms2) : add2(x, ms2), w[i], w[i + 1]);
+                }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) w[i] = ex2(w[i]);
 #pragma unroll
@@ -792,7 +787,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                     if (TYPE == AF_KV_F16) {
                         sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], x);
                     } else {
-                        const float g = g4[(16 * c + i) / SH::RPW % 4];
+                        const float g = g4[(16 * c + i) / SH::RPW];
                         sum[(i >> 1) & 1] = fma2(x, pair(g, g), sum[(i >> 1) & 1]);
                     }
                     split2(x, hi[i / 2], lo[i / 2]);
@@ -805,15 +800,16 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 unpair(add2(sum[0], sum[1]), a, b);
                 l = fmaf(l, corr, a + b);
             }
-            if (SETS > 1) publish(sl);
-            if ((sl += SETS) >= NS) sl -= NS, sl_ph ^= 1;
-            if ((st += SETS) >= NB) st -= NB, st_ph ^= 1;
-            if ((kt += SETS) >= RING) kt -= RING, kt_ph ^= 1;
+            publish(sl);
+            if (++sl == NS) sl = 0, sl_ph ^= 1;
+            if (++st == NB) st = 0, st_ph ^= 1;
+            if (++kt == RING) kt = 0, kt_ph ^= 1;
         }
-        if (SETS == 1 && ok && tiles_mine) publish(sl ? sl - 1 : NS - 1);
+        // one that leaves early is counted at the others' remaining meetings: nobody is left waiting
+        for (; met < tiles_mine; ++met) asm volatile("bar.arrive %0, %1;" ::"r"(2 + w4), "n"(PARTS * 32) : "memory");
         if (!ok) *flag = 1;
-        if (half == 0) s_top[set * kMmaRows + ti] = m;
-        s_sum[(2 * set + half) * kMmaRows + ti] = l;
+        if (part == 0) s_top[ti] = m;
+        s_sum[part * kMmaRows + ti] = l;
         __syncwarp();
         if (lane == 0 && w4 < live_warps) mbar_arrive(fin);
     } else if (warp < kSplitWarp) {
@@ -828,16 +824,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
 #pragma unroll
         for (int i = 0; i < HD; ++i) acc[i] = 0.f;
         bool ok = w < live_warps;
-        int sl = 0, sl_ph = 0;
-        float top = -INFINITY;  // what acc is relative to
-        for (int t = 0; ok && t < nt; ++t) {  // acc = acc·2^(old top - top) + (P·V)(t)·2^(its top - top)
-            ok = wait_warp(&c_full[sl], sl_ph) && wait_warp(o_full, t);
+        int co = 0, co_ph = 0;
+        for (int t = 0; ok && t < nt; ++t) {  // acc = acc·corr + (P·V)(t)
+            ok = wait_warp(&c_full[co], co_ph) && wait_warp(o_full, t);
             if (!ok) break;
             tc_fence_after();
-            const float mine = s_tile[sl * kMmaRows + ti], to = fmaxf(top, mine), at = to == -INFINITY ? 0.f : to;
-            const float corr = ex2(top - at), f = SETS > 1 ? ex2(mine - at) : 1.f;
-            top = to;
-            if (++sl == NS) sl = 0, sl_ph ^= 1;
+            const float corr = s_corr[co * kMmaRows + ti];
+            if (++co == NC) co = 0, co_ph ^= 1;
 #pragma unroll
             for (int c = 0; c < HD / 16; ++c) {
                 float o[16];
@@ -849,9 +842,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 for (int i = 0; i < 16; i += 2) {
                     float& x = acc[16 * c + i];
                     float& y = acc[16 * c + i + 1];
-                    f32x2 add = pair(o[i], o[i + 1]);
-                    if (SETS > 1) add = mul2(add, pair(f, f));
-                    unpair(fma2(pair(x, y), pair(corr, corr), add), x, y);
+                    unpair(fma2(pair(x, y), pair(corr, corr), pair(o[i], o[i + 1])), x, y);
                 }
             }
             tc_fence_before();
@@ -884,12 +875,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         }
         if (ok) {
             const int splits = spot.splits, mine_rows = min(32, row_hi - row_lo - w * 32);
-            float l = s_sum[ti] + s_sum[kMmaRows + ti];
-            if (SETS > 1) {  // top is the larger of the two sets'
-                const float at = top == -INFINITY ? 0.f : top;
-                l *= ex2(s_top[ti] - at);
-                l = fmaf(s_sum[2 * kMmaRows + ti] + s_sum[3 * kMmaRows + ti], ex2(s_top[kMmaRows + ti] - at), l);
-            }
+            float l = 0.f;
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) l += s_sum[i * kMmaRows + ti];
             const float inv = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
             for (int i = 0; i < HD; i += 4)
@@ -906,7 +894,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                         *reinterpret_cast<float4*>(o + i * HD) = from(i);
                 if (lane < mine_rows)
                     *reinterpret_cast<float2*>(mp.part + (long long)mp.slots * kMmaRows * HD + (at + lane) * 2) =
-                        make_float2(top, l);
+                        make_float2(s_top[ti], l);
             } else {
                 float* orow = live ? p.out + (long long)row * p.os + (long long)head * HD : nullptr;
                 const bool wide_out = ((reinterpret_cast<uintptr_t>(p.out) & 15) | (p.os & 3)) == 0;
@@ -945,8 +933,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             if (++sc_at == RING) sc_at = 0;
         };
         if (SH::F32) {
-            // Half a tile's rows at a time, RPW of them this warp's: out of the raw place into registers, which frees it,
-            // then split and stored.
+            // RPW rows of the tile, half a tile being in flight: out of the raw place into registers, which frees it, then
+            // split and stored.
             constexpr int NX = SH::RPW * HD * 4 / 512;  // a warp's loads of its rows
             const int sub = lane / SH::LPR, col = lane % SH::LPR;
             const uint8_t* raw = sm + SH::RAW + (isv ? 2 * SH::RAWB : 0) + w * SH::RPW * HD * 4 + lane * 16;
@@ -956,63 +944,57 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             uint64_t* due = nullptr;                 // a tile that is stored and not yet handed over
 #pragma unroll 1
             for (int t = 0; ok && t < nt; ++t) {
-#pragma unroll 1
-                for (int s = 0; s < 2; ++s) {
-                    ok = wait_warp(&land[s], t);
-                    if (!ok) break;
-                    const uint8_t* src = raw + s * SH::RAWB;
-                    float4 x[NX];
-                    float big[4] = {0.f, 0.f, 0.f, 0.f};
+                ok = wait_warp(&land[w / (SW / 2)], t);
+                if (!ok) break;
+                float4 x[NX];
+                float big[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int i = 0; i < NX; ++i) x[i] = *reinterpret_cast<const float4*>(src + i * 512);
-                    const int left = end - (t0 + t) * T - (s * SW + w) * SH::RPW - sub;  // rows in front of the end
-                    if (left < SH::RPW) {                                               // the last tile: what lies behind is nothing
+                for (int i = 0; i < NX; ++i) x[i] = *reinterpret_cast<const float4*>(raw + i * 512);
+                const int left = end - (t0 + t) * T - w * SH::RPW - sub;  // rows in front of the end
+                if (left < SH::RPW) {                                               // the last tile: what lies behind is nothing
 #pragma unroll
-                        for (int i = 0; i < NX; ++i)
-                            if (i * SH::RPC >= left) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    }
+                    for (int i = 0; i < NX; ++i)
+                        if (i * SH::RPC >= left) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
 #pragma unroll
-                    for (int i = 0; i < NX; ++i) {
-                        big[(2 * i) & 3] = max3_abs_nan(big[(2 * i) & 3], x[i].x, x[i].y);
-                        big[(2 * i + 1) & 3] = max3_abs_nan(big[(2 * i + 1) & 3], x[i].z, x[i].w);
-                    }
-                    uint32_t mx = __reduce_max_sync(
-                        0xffffffffu, __float_as_uint(max3_abs_nan(max3_abs_nan(big[0], big[1], big[2]), big[3], 0.f)));
-                    if (lane == 0) mbar_arrive(&freed[s]);  // all lanes hold theirs
-                    if (s == 0) {
-                        if (due) hand_over(due);            // the tile before: its stores are through by now
-                        if (t == SH::QTILE) ok = wait_warp(q_full, 0);  // the staged queries' place is written over
-                        if (ok && t >= NB) ok = wait_warp(&empty[st], ph ^ 1);
-                        if (!ok) break;
-                    }
-                    if (isv && mx >= 0x7f800000u) {  // rare: take what is not finite out, and remember the tile
-                        float4 y[NX];
+                for (int i = 0; i < NX; ++i) {
+                    big[(2 * i) & 3] = max3_abs_nan(big[(2 * i) & 3], x[i].x, x[i].y);
+                    big[(2 * i + 1) & 3] = max3_abs_nan(big[(2 * i + 1) & 3], x[i].z, x[i].w);
+                }
+                uint32_t mx = __reduce_max_sync(
+                    0xffffffffu, __float_as_uint(max3_abs_nan(max3_abs_nan(big[0], big[1], big[2]), big[3], 0.f)));
+                if (lane == 0) mbar_arrive(&freed[w / (SW / 2)]);  // all lanes hold theirs
+                if (due) hand_over(due);                        // the tile before: its stores are through by now
+                if (t == SH::QTILE) ok = wait_warp(q_full, 0);  // the staged queries' place is written over
+                if (ok && t >= NB) ok = wait_warp(&empty[st], ph ^ 1);
+                if (!ok) break;
+                if (isv && mx >= 0x7f800000u) {  // rare: take what is not finite out, and remember the tile
+                    float4 y[NX];
 #pragma unroll
-                        for (int i = 0; i < NX; ++i) y[i] = x[i];
-                        mx = clean(y);
+                    for (int i = 0; i < NX; ++i) y[i] = x[i];
+                    mx = clean(y);
 #pragma unroll
-                        for (int i = 0; i < NX; ++i) x[i] = y[i];
-                        note_bad(t);
-                    }
-                    const int a = scale_of(mx, isv ? 60 : 100);
-                    const float f = pow2(a);
-                    const f32x2 f2 = pair(f, f);
-                    uint8_t* dst = home + st * 2 * SH::HALF + s * SW * SH::RPW * 128;
+                    for (int i = 0; i < NX; ++i) x[i] = y[i];
+                    note_bad(t);
+                }
+                const int a = scale_of(mx, isv ? 60 : 100);
+                const float f = pow2(a);
+                const f32x2 f2 = pair(f, f);
+                uint8_t* dst = home + st * 2 * SH::HALF;
 #pragma unroll
-                    for (int i = 0; i < NX; ++i) {
-                        uint2 hi, lo;
-                        split2(mul2(pair(x[i].x, x[i].y), f2), hi.x, lo.x);
-                        split2(mul2(pair(x[i].z, x[i].w), f2), hi.y, lo.y);
-                        const int rr = i * SH::RPC + sub;
-                        uint8_t* d = dst + rr * 128 + (((in_half >> 4) ^ ((w * SH::RPW + rr) & 7)) << 4);
-                        *reinterpret_cast<uint2*>(d) = hi;
-                        *reinterpret_cast<uint2*>(d + SH::TILE) = lo;
-                    }
-                    if (lane == 0) {
-                        float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + s * SW + w;
-                        sc[0] = isv ? (float)-a : pow2(-a);
-                        if (isv) sc[SH::GROUPS] = f;
-                    }
+                for (int i = 0; i < NX; ++i) {
+                    uint2 hi, lo;
+                    split2(mul2(pair(x[i].x, x[i].y), f2), hi.x, lo.x);
+                    split2(mul2(pair(x[i].z, x[i].w), f2), hi.y, lo.y);
+                    const int rr = i * SH::RPC + sub;
+                    uint8_t* d = dst + rr * 128 + (((in_half >> 4) ^ ((w * SH::RPW + rr) & 7)) << 4);
+                    *reinterpret_cast<uint2*>(d) = hi;
+                    *reinterpret_cast<uint2*>(d + SH::TILE) = lo;
+                }
+                if (lane == 0) {
+                    float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + w;
+                    sc[0] = isv ? (float)-a : pow2(-a);
+                    if (isv) sc[SH::GROUPS] = f;
                 }
                 due = &full[fu];
                 next();
@@ -1051,10 +1033,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                         for (int i = 0; i < NC; ++i)
                             if (i % PER * 4 >= left) x[i] = make_uint4(0u, 0u, 0u, 0u);
                     }
-                    uint32_t b = 0;
+                    uint32_t b = 0;  // two at once: bf16's magnitudes are ordered as 16-bit numbers
 #pragma unroll
-                    for (int i = 0; i < 4 * NC; ++i) b = max(b, max((e[i] << 16) & 0x7fff0000u, e[i] & 0x7fff0000u));
-                    uint32_t mx = __reduce_max_sync(0xffffffffu, b);
+                    for (int i = 0; i < 4 * NC; ++i) b = __vmaxu2(b, e[i] & 0x7fff7fffu);
+                    uint32_t mx = __reduce_max_sync(0xffffffffu, max(b << 16, b & 0xffff0000u));
                     if (isv && mx >= 0x7f800000u) {
                         b = 0;
 #pragma unroll
@@ -1088,8 +1070,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             for (int t = 0; t < nt; ++t) {
                 ok = wait_warp(&land[st], ph);
                 if (!ok) break;
-                fix(t, 0);
-                fix(t, 1);
+#pragma unroll
+                for (int s = 0; s < T / (SW * SH::RPW); ++s) fix(t, s);
                 hand_over(&full[fu]);
                 next();
             }
@@ -1217,9 +1199,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             bool ok = wait_warp(q_full, 0);
             for (int t = 0; ok && t < min(SH::LA, n_tiles); ++t) ok = next_scores();
             for (int t = 0; ok && t < n_tiles; ++t) {
-                // scores of t + LA, over the weights of t + LA - NS (whose products are over: those of the tile behind
-                // them were issued when they had been taken)
-                if (t + SH::LA < n_tiles) ok = next_scores();
+                if (t + SH::LA < n_tiles) {
+                    // over the weights of t + LA - NS, whose products are over: either those of the tile behind them
+                    // were issued when they had been taken, or they are waited for
+                    if (NS == SH::LA + 1 && t) ok = wait_warp(&v_empty[st ? st - 1 : NB - 1], st ? ph : ph ^ 1);
+                    ok = ok && next_scores();
+                }
                 if (!ok) break;
                 ok = wait_warp(&p_full[sl], sl_ph) && wait_warp(&v_full[st], ph) && (t < 1 || wait_warp(o_free, t - 1));
                 if (!ok) break;
@@ -1307,7 +1292,8 @@ TreePlan tree_plan(const af_attention_tree_args& a) {
     if (!pl.mma) return pl;
     const long long cap = (long long)a.batch.max_blocks * a.kv.page_size;
     const long long max_len = a.max_len > 0 ? std::min((long long)a.max_len, cap) : cap;
-    const long long tiles = (max_len + kTreeTile - 1) / kTreeTile, most = (tiles + kTreeMinTiles - 1) / kTreeMinTiles;
+    const int T = tree_tile(a.kv.type);
+    const long long tiles = (max_len + T - 1) / T, most = (tiles + kTreeMinTiles - 1) / kTreeMinTiles;
     const long long items = ((long long)a.batch.max_nodes * G + kMmaRows - 1) / kMmaRows * a.kv.n_kv_heads * a.batch.n_seq;
     const long long split = items <= kTreeItems ? (items + kTreeSms - 1) / kTreeSms * kTreeSms : items + 2 * kTreeItems;
     pl.blocks = (int)std::min({split, items * std::max(1ll, most), (long long)INT_MAX});
@@ -1372,7 +1358,7 @@ cudaError_t tree_launch(const TreeParams& p, const TreePlan& pl, int max_nodes, 
         mp.blocks = pl.blocks;
         mp.slots = pl.slots;
         mp.part = static_cast<float*>(ws);
-        mp.box_rows = std::min(1 << p.kv.ps_shift, kTreeTile / (TYPE == AF_KV_F32 ? 2 : 1));
+        mp.box_rows = std::min(1 << p.kv.ps_shift, tree_tile(TYPE) / (TYPE == AF_KV_F32 ? 2 : 1));
         if (!tree_map(&mp.k_map, p, TYPE, p.kv.k, mp.box_rows) || !tree_map(&mp.v_map, p, TYPE, p.kv.v, mp.box_rows)) {
             set_last_error("af_attention_tree_f32: the cache cannot be described to the copy engine");
             return cudaErrorInvalidValue;
