@@ -290,7 +290,7 @@ __device__ __forceinline__ int scale_of(uint32_t max_bits, int top) {
 __device__ __forceinline__ float pow2(int a) { return __int_as_float((a + 127) << 23); }
 
 constexpr int kMmaThreads = 1024;
-constexpr int kMmaWarp = 28, kCopyWarp = 29;  // copies of K, of V
+constexpr int kMmaWarp = 28, kCopyWarp = 29, kScoreWarp = 31;  // copies of K, of V: 29, 30
 constexpr int kMmaRows = 128;
 constexpr int tree_tile(int type) { return type == AF_KV_F32 ? 64 : 128; }  // positions of a tile
 constexpr int kMmaBadWords = 512;  // tiles of a split whose V holds something non-finite, a bit each
@@ -310,9 +310,8 @@ struct MmaShape {
     static constexpr int HALF = TERMS * TILE;           // K or V of a tile: hi, lo
     static constexpr int NB = F32 ? 256 / HD : 3;       // tiles in shared memory: K V K V ...
     static constexpr int NS = F32 ? 4 : HD == 128 ? 2 : 3;  // score tiles in tensor memory (each becomes its weights)
-    static constexpr int LA = F32 ? 1 : NS - 1;         // tiles whose scores are issued ahead of the products of one
-    static constexpr int NC = LA + 2;                   // corrections
-    static constexpr int RING = NB + LA + 2;            // barriers and scales of K (see k_full)
+    static constexpr int NC = NS + 1;                   // corrections (see c_full)
+    static constexpr int RING = NB + NS;                // barriers and scales of K (see k_full)
     static constexpr int RAWB = T / 2 * HD * 4;         // f32: half the rows of K or V as they are
     static constexpr int RPW = 8;                       // rows that share a power of two: a splitting warp takes them together
     static constexpr int LPR = HD * SIZE / 16;          // lanes of a row (f32)
@@ -516,9 +515,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     constexpr int kOutWarp = SH::OUT, kSplitWarp = SH::SPLIT_K;
     extern __shared__ __align__(1024) uint8_t sm[];
     const TreeParams& p = mp.t;
-    // A waiter never falls a whole ring behind.  K of t + RING is written when the scores of t + RING - NB =
-    // t + LA + 2 are done; those are issued behind the products of t + 1, so the softmax is through with K of t.
-    // Every other barrier's next phase needs what the waiter of this one does.
+    // A waiter never falls a whole ring behind.  Scores of tile u are issued when the products of u - NS are done, and
+    // those are issued when the weights of u - NS are there and the products before them were taken.  So K of t + RING,
+    // written when the scores of t + NS are done, finds the softmax through with tile t, and the correction of t + NC
+    // finds that of t taken.  Every other barrier's next phase needs what the waiter of this one does.
     uint64_t* k_full = reinterpret_cast<uint64_t*>(sm);  // [RING] K of a tile is ready: its splitting warps (f16: the copy)
     uint64_t* v_full = k_full + RING;                    // [NB] V, its splitting warps
     uint64_t* k_empty = v_full + NB;                     // [NB] scores done
@@ -533,9 +533,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     uint64_t* o_free = o_full + 1;                       // output warps: P·V and correction taken
     uint64_t* q_full = o_free + 1;                       // softmax and output warps: queries written
     uint64_t* fin = q_full + 1;                          // softmax warps: tops and sums written
-    uint64_t* done = fin + 1;                            // every product done
-    static_assert((RING + 5 * NB + 2 * NS + NC + 9) * 8 + 16 <= SH::BAD, "barriers");
-    uint32_t* tslot = reinterpret_cast<uint32_t*>(done + 1);
+    uint64_t* done = fin + 1;                            // everything issued is done: scores, products
+    uint64_t* w_empty = done + 1;                        // [NS] P·V done: the weights' place is free
+    static_assert((RING + 5 * NB + 3 * NS + NC + 9) * 8 + 16 <= SH::BAD, "barriers");
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(w_empty + NS);
     volatile int* flag = reinterpret_cast<volatile int*>(tslot + 1);
     uint32_t* bad = reinterpret_cast<uint32_t*>(sm + SH::BAD);
     float* s_rs = reinterpret_cast<float*>(sm + SH::ROWS);
@@ -559,6 +560,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         set_err_at(p.b.err, kErrMbarTimeout);
         return false;
     };
+    // Several at once: the looks overlap where all have come already.
+    auto wait_both = [&](uint64_t* a, int pa, uint64_t* b, int pb) -> bool {
+        const bool x = mbar_try_wait(a, (uint32_t)pa & 1u), y = mbar_try_wait(b, (uint32_t)pb & 1u);
+        return __all_sync(0xffffffffu, x && y) || (wait_warp(a, pa) && wait_warp(b, pb));
+    };
+    auto wait_three = [&](uint64_t* a, int pa, uint64_t* b, int pb, uint64_t* c, int pc) -> bool {
+        const bool x = mbar_try_wait(a, (uint32_t)pa & 1u), y = mbar_try_wait(b, (uint32_t)pb & 1u), z = mbar_try_wait(c, (uint32_t)pc & 1u);
+        return __all_sync(0xffffffffu, x && y && z) || (wait_warp(a, pa) && wait_warp(b, pb) && wait_warp(c, pc));
+    };
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     __shared__ TreeSpot spot;
     pdl_launch_dependents();
@@ -578,10 +588,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         }
         for (int i = 0; i < RING; ++i) mbar_init(&k_full[i], TYPE == AF_KV_F16 ? 1 : SW);
         for (int i = 0; i < 4; ++i) mbar_init(&raw_free[i], SW / 2);
-        for (int i = 0; i < NS; ++i) mbar_init(&s_full[i], 1);
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&w_empty[i], 1);
+        }
         mbar_init(o_full, 1);
         mbar_init(q_full, kOutWarp + 4);
-        mbar_init(done, 1);
+        mbar_init(done, 2);
         *flag = 0;
     } else if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(512u)
@@ -707,7 +720,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         int sl = 0, sl_ph = 0, st = 0, st_ph = 0, kt = 0, kt_ph = 0, co = 0;  // rings of NS, NB, RING, NC and their phases
         int met = 0;  // the tiles at which the row's warps have met
         for (int t = 0; t < tiles_mine; ++t) {
-            ok = (TYPE == AF_KV_F16 || wait_warp(&k_full[kt], kt_ph)) && wait_warp(&s_full[sl], sl_ph);
+            ok = TYPE == AF_KV_F16 ? wait_warp(&s_full[sl], sl_ph)
+                                   : wait_three(&k_full[kt], kt_ph, &s_full[sl], sl_ph, &v_full[st], st_ph);
             if (!ok) break;
             tc_fence_after();
             const uint32_t sb = tmem + lanes + SH::S0 + sl * T + part * C;
@@ -721,8 +735,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             const float4* kc = reinterpret_cast<const float4*>(scales + kt * 3 * SH::GROUPS) + part;  // 2^-a of K
             const float4* vf = kc + SH::GROUPS / 4;                                                   // -a of V
             const float4* vg = vf + SH::GROUPS / 4;                                                   // 2^a of V
-            if (TYPE != AF_KV_F16) ok = wait_warp(&v_full[st], st_ph);
-            if (!ok) break;
             if (TYPE != AF_KV_F16) {
                 const float4 x = *kc, z = *vf;
                 const float c[4] = {rs * x.x, rs * x.y, rs * x.z, rs * x.w}, f[4] = {z.x, z.y, z.z, z.w};
@@ -756,8 +768,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             const float corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
             m = mn;
             if (part == 0) {
-                // its place is free: these scores were issued behind the products of t - LA - 1, which waited until those
-                // of t - NC were taken
                 s_corr[co * kMmaRows + ti] = corr;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c_full[co]);
@@ -826,7 +836,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         bool ok = w < live_warps;
         int co = 0, co_ph = 0;
         for (int t = 0; ok && t < nt; ++t) {  // acc = acc·corr + (P·V)(t)
-            ok = wait_warp(&c_full[co], co_ph) && wait_warp(o_full, t);
+            ok = wait_both(&c_full[co], co_ph, o_full, t);
             if (!ok) break;
             tc_fence_after();
             const float corr = s_corr[co * kMmaRows + ti];
@@ -1144,7 +1154,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 if (++kt == RING) kt = 0;
             }
             if (!ok) *flag = 1;
-        } else if (warp == kMmaWarp && nt > 0) {
+        } else if ((warp == kMmaWarp || warp == kScoreWarp) && nt > 0) {
             // --------------------------------------------------- products
             constexpr uint32_t base = (1u << 4) | ((uint32_t)(kMmaRows >> 4) << 24);  // f32 accumulators, f16 operands
             constexpr uint32_t ids = base | ((uint32_t)(T >> 3) << 17);
@@ -1152,72 +1162,65 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             const uint32_t leader = elect_one();
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             const int n_tiles = __shfl_sync(0xffffffffu, nt, 0);
-            // K: 8-row groups 1,024 bytes apart, 16 values 32 bytes on; V: 64 values COLS bytes apart, 16 positions 2,048 on
-            const uint64_t kd = tile_desc(smem_u32(tiles), 16, 1024), vd = tile_desc(smem_u32(tiles) + SH::HALF, SH::COLS, 1024);
-            auto k_step = [](int ks) { return (uint32_t)((ks >> 2) * SH::COLS + (ks & 3) * 32) >> 4; };
-            auto scores = [&](int st, int sl) {
-                const uint64_t k = kd + (uint32_t)(st * (2 * SH::HALF >> 4));
-                const uint32_t d = tm + SH::S0 + sl * T;
+            bool ok = true;
+            int st = 0, ph = 0, sl = 0, sl_ph = 0;
+            if (warp == kScoreWarp) {
+                // K: 8-row groups 1,024 bytes apart, 16 values 32 bytes on
+                const uint64_t kd = tile_desc(smem_u32(tiles), 16, 1024);
+                auto k_step = [](int ks) { return (uint32_t)((ks >> 2) * SH::COLS + (ks & 3) * 32) >> 4; };
+                int kt = 0, kt_ph = 0;
+                ok = wait_warp(q_full, 0);
+                for (int t = 0; ok && t < n_tiles; ++t) {
+                    ok = t < NS ? wait_warp(&k_full[kt], kt_ph) : wait_both(&k_full[kt], kt_ph, &w_empty[sl], sl_ph ^ 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t k = kd + (uint32_t)(st * (2 * SH::HALF >> 4));
+                    const uint32_t d = tm + SH::S0 + sl * T;
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks) tc_mma_ts(leader, d, tm + SH::QL + 8 * ks, k + k_step(ks), ids, ks > 0);
-                if (SH::TERMS == 2) {
+                    for (int ks = 0; ks < HD / 16; ++ks) tc_mma_ts(leader, d, tm + SH::QL + 8 * ks, k + k_step(ks), ids, ks > 0);
+                    if (SH::TERMS == 2) {
 #pragma unroll
-                    for (int ks = 0; ks < HD / 16; ++ks)
-                        tc_mma_ts(leader, d, tm + SH::QH + 8 * ks, k + (SH::TILE >> 4) + k_step(ks), ids, true);
+                        for (int ks = 0; ks < HD / 16; ++ks)
+                            tc_mma_ts(leader, d, tm + SH::QH + 8 * ks, k + (SH::TILE >> 4) + k_step(ks), ids, true);
+                    }
+#pragma unroll
+                    for (int ks = 0; ks < HD / 16; ++ks) tc_mma_ts(leader, d, tm + SH::QH + 8 * ks, k + k_step(ks), ids, true);
+                    tc_commit(leader, &s_full[sl]);
+                    tc_commit(leader, &k_empty[st]);
+                    if (++st == NB) st = 0;
+                    if (++sl == NS) sl = 0, sl_ph ^= 1;
+                    if (++kt == RING) kt = 0, kt_ph ^= 1;
                 }
+            } else {
+                // V: 64 values COLS bytes apart, 16 positions 2,048 on
+                const uint64_t vd = tile_desc(smem_u32(tiles) + SH::HALF, SH::COLS, 1024);
+                for (int t = 0; ok && t < n_tiles; ++t) {
+                    ok = t ? wait_three(&p_full[sl], sl_ph, &v_full[st], ph, o_free, t - 1) : wait_both(&p_full[sl], sl_ph, &v_full[st], ph);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t v = vd + (uint32_t)(st * (2 * SH::HALF >> 4));
+                    const uint32_t w = tm + SH::S0 + sl * T, d = tm + SH::O0;
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks) tc_mma_ts(leader, d, tm + SH::QH + 8 * ks, k + k_step(ks), ids, true);
-                tc_commit(leader, &s_full[sl]);
-                tc_commit(leader, &k_empty[st]);
-            };
-            auto values = [&](int st, int sl) {
-                const uint64_t v = vd + (uint32_t)(st * (2 * SH::HALF >> 4));
-                const uint32_t w = tm + SH::S0 + sl * T, d = tm + SH::O0;
+                    for (int ks = 0; ks < T / 16; ++ks) tc_mma_ts(leader, d, w + 8 + 16 * ks, v + (2048 * ks >> 4), ido, ks > 0);
+                    if (SH::TERMS == 2) {
 #pragma unroll
-                for (int ks = 0; ks < T / 16; ++ks) tc_mma_ts(leader, d, w + 8 + 16 * ks, v + (2048 * ks >> 4), ido, ks > 0);
-                if (SH::TERMS == 2) {
+                        for (int ks = 0; ks < T / 16; ++ks)
+                            tc_mma_ts(leader, d, w + 16 * ks, v + ((SH::TILE + 2048 * ks) >> 4), ido, true);
+                    }
 #pragma unroll
-                    for (int ks = 0; ks < T / 16; ++ks)
-                        tc_mma_ts(leader, d, w + 16 * ks, v + ((SH::TILE + 2048 * ks) >> 4), ido, true);
+                    for (int ks = 0; ks < T / 16; ++ks) tc_mma_ts(leader, d, w + 16 * ks, v + (2048 * ks >> 4), ido, true);
+                    tc_commit(leader, o_full);
+                    tc_commit(leader, &v_empty[st]);
+                    tc_commit(leader, &w_empty[sl]);
+                    if (++st == NB) st = 0, ph ^= 1;
+                    if (++sl == NS) sl = 0, sl_ph ^= 1;
                 }
-#pragma unroll
-                for (int ks = 0; ks < T / 16; ++ks) tc_mma_ts(leader, d, w + 16 * ks, v + (2048 * ks >> 4), ido, true);
-                tc_commit(leader, o_full);
-                tc_commit(leader, &v_empty[st]);
-            };
-            int st = 0, ph = 0, sl = 0, sl_ph = 0;       // tile t
-            int st1 = 0, kt1 = 0, kt1_ph = 0, sl1 = 0;  // the tile whose scores are next
-            auto next_scores = [&]() -> bool {
-                if (!wait_warp(&k_full[kt1], kt1_ph)) return false;
-                tc_fence_after();
-                scores(st1, sl1);
-                if (++st1 == NB) st1 = 0;
-                if (++sl1 == NS) sl1 = 0;
-                if (++kt1 == RING) kt1 = 0, kt1_ph ^= 1;
-                return true;
-            };
-            bool ok = wait_warp(q_full, 0);
-            for (int t = 0; ok && t < min(SH::LA, n_tiles); ++t) ok = next_scores();
-            for (int t = 0; ok && t < n_tiles; ++t) {
-                if (t + SH::LA < n_tiles) {
-                    // over the weights of t + LA - NS, whose products are over: either those of the tile behind them
-                    // were issued when they had been taken, or they are waited for
-                    if (NS == SH::LA + 1 && t) ok = wait_warp(&v_empty[st ? st - 1 : NB - 1], st ? ph : ph ^ 1);
-                    ok = ok && next_scores();
-                }
-                if (!ok) break;
-                ok = wait_warp(&p_full[sl], sl_ph) && wait_warp(&v_full[st], ph) && (t < 1 || wait_warp(o_free, t - 1));
-                if (!ok) break;
-                tc_fence_after();
-                values(st, sl);
-                if (++st == NB) st = 0, ph ^= 1;
-                if (++sl == NS) sl = 0, sl_ph ^= 1;
             }
             if (!ok) *flag = 1;
             // whatever was issued ends before tensor memory is given back
             tc_commit(leader, done);
             __syncwarp();
-            mbar_wait_at(done, 0u, p.b.err, nullptr);
+            if (warp == kMmaWarp) mbar_wait_at(done, 0u, p.b.err, nullptr);
         }
         __syncwarp();
     }
