@@ -313,7 +313,7 @@ struct MmaShape {
     static constexpr int NC = NS + 1;                   // corrections (see c_full)
     static constexpr int RING = NB + NS;                // barriers and scales of K (see k_full)
     static constexpr int RAWB = T / 2 * HD * 4;         // f32: half the rows of K or V as they are
-    static constexpr int RPW = 8;                       // rows that share a power of two: a splitting warp takes them together
+    static constexpr int RPW = T / SW;                  // rows that share a power of two: a splitting warp's
     static constexpr int LPR = HD * SIZE / 16;          // lanes of a row (f32)
     static constexpr int RPC = 32 / LPR;                // rows of a warp's 512 bytes (f32)
     // queries in, rows out: 128 rows over the last tiles' place, 16-byte columns swizzled by the row
@@ -731,18 +731,16 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             tc_wait_ld();
 #pragma unroll
             for (int i = 0; i < C; ++i) asm volatile("" : "+f"(v[i]));  // no use may move above the wait
-            static_assert(C == 4 * SH::RPW, "a thread's powers of two are four");
-            const float4* kc = reinterpret_cast<const float4*>(scales + kt * 3 * SH::GROUPS) + part;  // 2^-a of K
-            const float4* vf = kc + SH::GROUPS / 4;                                                   // -a of V
-            const float4* vg = vf + SH::GROUPS / 4;                                                   // 2^a of V
-            if (TYPE != AF_KV_F16) {
-                const float4 x = *kc, z = *vf;
+            // f32: a power of two per 8 columns; bf16: one for the thread's 32, taken care of in the exponent
+            const float* sc = scales + kt * 3 * SH::GROUPS + part * (C / SH::RPW);  // 2^-a of K, -a of V, 2^a of V
+            float scale = rs, shift = 0.f, share = 1.f;
+            if (TYPE == AF_KV_BF16) scale = fmaxf(rs * sc[0], FLT_MIN), shift = sc[SH::GROUPS], share = sc[2 * SH::GROUPS];
+            if (SH::F32) {
+                const float4 x = *reinterpret_cast<const float4*>(sc), z = *reinterpret_cast<const float4*>(sc + SH::GROUPS);
                 const float c[4] = {rs * x.x, rs * x.y, rs * x.z, rs * x.w}, f[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
-                for (int e = 0; e < C; e += 2) {
-                    const int g = e / SH::RPW;
-                    unpair(fma2(pair(v[e], v[e + 1]), pair(c[g], c[g]), pair(f[g], f[g])), v[e], v[e + 1]);
-                }
+                for (int e = 0; e < C; e += 2)
+                    unpair(fma2(pair(v[e], v[e + 1]), pair(c[e / 8], c[e / 8]), pair(f[e / 8], f[e / 8])), v[e], v[e + 1]);
             }
             const int p0 = (t0 + t) * T + part * C;
             if (p0 + C > len) {
@@ -755,7 +753,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
 #pragma unroll
             for (int i = 4; i + 1 < C; i += 2) top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], v[i], v[i + 1]);
             float mn = max3(top[0], top[1], fmaxf(top[2], top[3]));
-            if (TYPE == AF_KV_F16 && mn != -INFINITY) mn *= rs;  // rs > 0: raw scores have the same largest one
+            if (!SH::F32 && mn != -INFINITY) mn = fmaf(mn, scale, shift);  // scale > 0: raw scores have the same largest one
             mn = fmaxf(m, mn);
             // the row's other parts, in two places in turn: this one is written again when all have read it
             float* others = s_other + (t & 1) * PARTS * kMmaRows + ti;
@@ -774,10 +772,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             }
             if (++co == NC) co = 0;
             f32x2 sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-            const f32x2 ms2 = pair(-ms, -ms), rs2 = pair(rs, rs);
+            const f32x2 ms2 = pair(shift - ms, shift - ms), rs2 = pair(scale, scale);
             float g4[4];
-            if (TYPE != AF_KV_F16) {
-                const float4 x = *vg;
+            if (SH::F32) {
+                const float4 x = *reinterpret_cast<const float4*>(sc + 2 * SH::GROUPS);
                 g4[0] = x.x, g4[1] = x.y, g4[2] = x.z, g4[3] = x.w;
             }
 #pragma unroll
@@ -787,18 +785,18 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
                     const f32x2 x = pair(v[16 * c + i], v[16 * c + i + 1]);
-                    unpair(TYPE == AF_KV_F16 ? fma2(x, rs2, ms2) : add2(x, ms2), w[i], w[i + 1]);
+                    unpair(SH::F32 ? add2(x, ms2) : fma2(x, rs2, ms2), w[i], w[i + 1]);
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) w[i] = ex2(w[i]);
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
                     const f32x2 x = pair(w[i], w[i + 1]);
-                    if (TYPE == AF_KV_F16) {
-                        sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], x);
-                    } else {
-                        const float g = g4[(16 * c + i) / SH::RPW];
+                    if (SH::F32) {
+                        const float g = g4[(16 * c + i) / 8];
                         sum[(i >> 1) & 1] = fma2(x, pair(g, g), sum[(i >> 1) & 1]);
+                    } else {
+                        sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], x);
                     }
                     split2(x, hi[i / 2], lo[i / 2]);
                 }
@@ -808,7 +806,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             {
                 float a, b;
                 unpair(add2(sum[0], sum[1]), a, b);
-                l = fmaf(l, corr, a + b);
+                l = fmaf(l, corr, share * (a + b));
             }
             publish(sl);
             if (++sl == NS) sl = 0, sl_ph ^= 1;
@@ -1011,56 +1009,73 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             }
             if (ok && due) hand_over(due);
         } else if (TYPE == AF_KV_BF16 || isv) {
-            // 512 bytes of the warp's rows: 4 rows of 64 values; in place
-            constexpr int NC = SH::RPW * HD * 2 / 512, PER = SH::RPW / 4;  // accesses of a group; of its rows' 64 values
-            auto fix = [&](int t, int s) {
-                uint8_t* at = tiles + (st * 2 + (isv ? 1 : 0)) * SH::HALF + (s * SW + w) * SH::RPW * 128 + lane * 16;
-                auto place = [&](int i) { return at + (i / PER) * SH::COLS + (i % PER) * 512; };
+            // in place; an access takes 512 bytes: 4 rows of 64 values
+            constexpr int ALL = SH::RPW * HD * 2 / 512, NC = 4, PER = SH::RPW / 4;  // accesses; at a time; of the rows' 64 values
+            auto fix = [&](int t) {
+                uint8_t* at = tiles + (st * 2 + (isv ? 1 : 0)) * SH::HALF + w * SH::RPW * 128 + lane * 16;
+                auto place = [&](int i) { return reinterpret_cast<uint4*>(at + (i / PER) * SH::COLS + (i % PER) * 512); };
                 uint4 x[NC];
                 uint32_t* e = &x[0].x;
+                const int left = end - (t0 + t) * T - w * SH::RPW - lane / 8;  // rows in front of the end
+                auto load = [&](int i0) {
 #pragma unroll
-                for (int i = 0; i < NC; ++i) x[i] = *reinterpret_cast<const uint4*>(place(i));
-                if (TYPE == AF_KV_F16) {
-                    __half2 z = __float2half2_rn(0.f);  // x·0 is 0 for what is finite, NaN otherwise
-#pragma unroll
-                    for (int i = 0; i < 4 * NC; ++i)
-                        z = __hfma2(*reinterpret_cast<const __half2*>(&e[i]), __float2half2_rn(0.f), z);
-                    const uint32_t zz = *reinterpret_cast<const uint32_t*>(&z) & 0x7fff7fffu;
-                    if (__any_sync(0xffffffffu, zz != 0)) {
-#pragma unroll
-                        for (int i = 0; i < 4 * NC; ++i) {
-                            if ((e[i] & 0x7c00u) == 0x7c00u) e[i] &= 0xffff0000u;
-                            if ((e[i] & 0x7c000000u) == 0x7c000000u) e[i] &= 0x0000ffffu;
-                        }
-#pragma unroll
-                        for (int i = 0; i < NC; ++i) *reinterpret_cast<uint4*>(place(i)) = x[i];
-                        note_bad(t);
-                    }
-                } else {
-                    const int left = end - (t0 + t) * T - (s * SW + w) * SH::RPW - lane / 8;  // rows in front of the end
-                    if (left < SH::RPW) {                                                    // the last tile: what lies behind is nothing
+                    for (int i = 0; i < NC; ++i) x[i] = *place(i0 + i);
+                    if (TYPE == AF_KV_BF16 && left < SH::RPW) {  // the last tile: what lies behind is nothing
 #pragma unroll
                         for (int i = 0; i < NC; ++i)
-                            if (i % PER * 4 >= left) x[i] = make_uint4(0u, 0u, 0u, 0u);
+                            if ((i0 + i) % PER * 4 >= left) x[i] = make_uint4(0u, 0u, 0u, 0u);
                     }
-                    uint32_t b = 0;  // two at once: bf16's magnitudes are ordered as 16-bit numbers
+                };
+                auto without = [&]() {  // zeros for what is not finite
+                    constexpr uint32_t top = TYPE == AF_KV_F16 ? 0x7c00u : 0x7f80u;
 #pragma unroll
-                    for (int i = 0; i < 4 * NC; ++i) b = __vmaxu2(b, e[i] & 0x7fff7fffu);
-                    uint32_t mx = __reduce_max_sync(0xffffffffu, max(b << 16, b & 0xffff0000u));
-                    if (isv && mx >= 0x7f800000u) {
-                        b = 0;
+                    for (int i = 0; i < 4 * NC; ++i) {
+                        if ((e[i] & top) == top) e[i] &= 0xffff0000u;
+                        if ((e[i] & top << 16) == top << 16) e[i] &= 0x0000ffffu;
+                    }
+                };
+                if (TYPE == AF_KV_F16) {
+#pragma unroll 1
+                    for (int i0 = 0; i0 < ALL; i0 += NC) {
+                        load(i0);
+                        __half2 z = __float2half2_rn(0.f);  // x·0 is 0 for what is finite, NaN otherwise
 #pragma unroll
-                        for (int i = 0; i < 4 * NC; ++i) {
-                            if (((e[i] << 16) & 0x7fff0000u) >= 0x7f800000u) e[i] &= 0xffff0000u;
-                            if ((e[i] & 0x7fff0000u) >= 0x7f800000u) e[i] &= 0x0000ffffu;
-                            b = max(b, max((e[i] << 16) & 0x7fff0000u, e[i] & 0x7fff0000u));
+                        for (int i = 0; i < 4 * NC; ++i)
+                            z = __hfma2(*reinterpret_cast<const __half2*>(&e[i]), __float2half2_rn(0.f), z);
+                        const uint32_t zz = *reinterpret_cast<const uint32_t*>(&z) & 0x7fff7fffu;
+                        if (__any_sync(0xffffffffu, zz != 0)) {
+                            without();
+#pragma unroll
+                            for (int i = 0; i < NC; ++i) *place(i0 + i) = x[i];
+                            note_bad(t);
                         }
-                        mx = __reduce_max_sync(0xffffffffu, b);
-                        note_bad(t);
                     }
-                    const int a = scale_of(mx, isv ? 60 : 100);
-                    const float f = pow2(a);
-                    const f32x2 f2 = pair(f, f);
+                    return;
+                }
+                auto largest = [&](bool finite) {
+                    uint32_t b = 0;  // two at once: bf16's magnitudes are ordered as 16-bit numbers
+#pragma unroll 1
+                    for (int i0 = 0; i0 < ALL; i0 += NC) {
+                        load(i0);
+                        if (finite) without();
+#pragma unroll
+                        for (int i = 0; i < 4 * NC; ++i) b = __vmaxu2(b, e[i] & 0x7fff7fffu);
+                    }
+                    return __reduce_max_sync(0xffffffffu, max(b << 16, b & 0xffff0000u));
+                };
+                uint32_t mx = largest(false);
+                const bool odd = isv && mx >= 0x7f800000u;
+                if (odd) {
+                    mx = largest(true);
+                    note_bad(t);
+                }
+                const int a = scale_of(mx, isv ? 60 : 100);
+                const float f = pow2(a);
+                const f32x2 f2 = pair(f, f);
+#pragma unroll 1
+                for (int i0 = 0; i0 < ALL; i0 += NC) {
+                    load(i0);
+                    if (odd) without();
 #pragma unroll
                     for (int i = 0; i < 4 * NC; ++i) {
                         float lo, hi;
@@ -1068,20 +1083,19 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                         e[i] = pack2(lo, hi);
                     }
 #pragma unroll
-                    for (int i = 0; i < NC; ++i) *reinterpret_cast<uint4*>(place(i)) = x[i];
-                    if (lane == 0) {
-                        float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + s * SW + w;
-                        sc[0] = isv ? (float)-a : pow2(-a);
-                        if (isv) sc[SH::GROUPS] = f;
-                    }
+                    for (int i = 0; i < NC; ++i) *place(i0 + i) = x[i];
+                }
+                if (lane == 0) {
+                    float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + w;
+                    sc[0] = isv ? (float)-a : pow2(-a);
+                    if (isv) sc[SH::GROUPS] = f;
                 }
             };
 #pragma unroll 1
             for (int t = 0; t < nt; ++t) {
                 ok = wait_warp(&land[st], ph);
                 if (!ok) break;
-#pragma unroll
-                for (int s = 0; s < T / (SW * SH::RPW); ++s) fix(t, s);
+                fix(t);
                 hand_over(&full[fu]);
                 next();
             }
