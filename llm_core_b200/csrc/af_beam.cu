@@ -80,6 +80,16 @@ __device__ __forceinline__ T warp_sort_desc(T v, int lane) {
     return v;
 }
 
+// The warp's n-th largest value, equal ones counted one by one, n <= 32 (values > 0).
+__device__ __forceinline__ uint32_t warp_nth(uint32_t v, int n) {
+    for (;;) {
+        const uint32_t m = __reduce_max_sync(0xffffffffu, v);
+        n -= __popc(__ballot_sync(0xffffffffu, v == m));
+        if (n <= 0 || m == 0) return m;
+        if (v == m) v = 0;
+    }
+}
+
 __device__ __forceinline__ float beam_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -99,6 +109,17 @@ struct BeamShared {
 // The buffer's K best keys, in order, to its front (fewer where it has fewer).
 __device__ void beam_cut(BeamShared& sh, int K) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = sh.count;
+    if (n <= kBeamThreads) {  // a key a thread: its rank among all
+        const u64 k = tid < n ? sh.key[tid] : 0;
+        int rank = 0;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) rank += sh.key[i] > k;
+        __syncthreads();
+        if (tid < n && rank < K) sh.key[rank] = k;
+        if (tid == 0) sh.count = min(n, K);
+        __syncthreads();
+        return;
+    }
     u64 best = 0;
     for (int i = tid; i < n; i += kBeamThreads) best = max(best, sh.key[i]);
     best = warp_sort_desc(best, lane);
@@ -108,8 +129,7 @@ __device__ void beam_cut(BeamShared& sh, int K) {
     u64 thr = sh.wkey[0];
 #pragma unroll
     for (int w = 1; w < kBeamThreads / 32; ++w) thr = min(thr, sh.wkey[w]);
-    // their order among what passes (where that is more than sel holds, as equal keys' neighbours never are but
-    // rising ones may be, among all)
+    // their order among what passes, or, where that is more than sel holds (rising logits), among all
     for (int i = tid; i < n; i += kBeamThreads) {
         const u64 k = sh.key[i];
         if (k >= thr) {
@@ -143,7 +163,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParam
     BeamShared& sh = *reinterpret_cast<BeamShared*>(sm);
     pdl_launch_dependents();  // the merge kernel may start launching
     const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (dead_score(p.scores[row])) return;
+    const float score = p.scores[row];
     const int lo = blockIdx.x * p.seg, hi = min(lo + p.seg, p.vocab), K = p.K;
     const float* x = p.logits + (long long)row * p.stride;
     auto token = [&](int t0, int j) { return t0 + (j >> 2) * (4 * kBeamThreads) + 4 * tid + (j & 3); };
@@ -169,7 +189,8 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParam
         }
     };
     float next[kBeamPer];
-    load(lo, next);
+    load(lo, next);  // beside the beam's score, not behind it
+    if (dead_score(score)) return;
     if (tid == 0) sh.count = 0;
     __syncthreads();
     float top = -INFINITY, thr = 0.f;
@@ -206,8 +227,8 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParam
         const int step = (t0 - lo) / kBeamStep + 1;
         const bool raise = (step & (step - 1)) == 0;
         if (raise) {
-            const float s = warp_sort_desc(top, lane);
-            if (lane == (K + 7) / 8 - 1) sh.wval[warp] = s;
+            const uint32_t s = warp_nth(float_to_ordered(top), (K + 7) / 8);
+            if (lane == 0) sh.wval[warp] = ordered_to_float(s);
         }
         if (begin) {
             __syncthreads();
@@ -278,19 +299,27 @@ struct Cand {
 };
 __device__ __forceinline__ bool better(u64 s, unsigned f, u64 s2, unsigned f2) { return s > s2 || (s == s2 && f < f2); }
 
-constexpr int kMergeSmem = kBeamLists * 12 + kBeamMaxK * kBeamMaxK * 12 + 64 * 8 + (2 + kBeamMaxK) * 4;
+constexpr int kMergeKeys = 4096;  // keys of a sequence that are brought to shared memory, when they are no more
+constexpr int kMergeSmem = kBeamLists * 12 + kBeamMaxK * kBeamMaxK * 12 + 64 * 8 + kMergeKeys * 8 + (2 + kBeamMaxK) * 4;
 
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamParams p) {
     extern __shared__ __align__(16) uint8_t sm[];
     u64* hs = reinterpret_cast<u64*>(sm);                        // [lists] heads
     u64* cs = hs + kBeamLists;                                   // [K*K] candidates
     double* base = reinterpret_cast<double*>(cs + kBeamMaxK * kBeamMaxK);  // [beams]
-    unsigned* hf = reinterpret_cast<unsigned*>(base + 64);
+    u64* near = reinterpret_cast<u64*>(base + 64);               // [lists][K], if they fit
+    unsigned* hf = reinterpret_cast<unsigned*>(near + kMergeKeys);
     unsigned* cf = hf + kBeamLists;
     int* ctl = reinterpret_cast<int*>(cf + kBeamMaxK * kBeamMaxK);  // candidates, lists, the lists with the best heads
     const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row0 = seq * p.beams, K = p.K;
+    const int lists = p.beams * p.chunks;
+    const bool here = lists * K <= kMergeKeys;
+    const u64* keys = p.keys + (long long)row0 * p.chunks * K;
     pdl_wait();
+    if (here)
+        for (int i = tid; i < lists * K; i += kMergeThreads) near[i] = keys[i];
+    if (here) keys = near;
     // a beam's base: scores[b] - log Σ exp, -inf for a dead one
     for (int b = warp; b < p.beams; b += kMergeThreads / 32) {
         const float s = p.scores[row0 + b];
@@ -324,14 +353,13 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamParams p)
             f = (unsigned)b * p.vocab + c;
             return true;
         }
-        const u64 k = p.keys[((long long)(row0 + b) * p.chunks + chunk) * K + c];
+        const u64 k = keys[list * K + c];
         if (!k) return false;
         const double x = (double)ordered_to_float((uint32_t)(k >> 32));
         s = double_ordered(base[b] + x);
         f = (unsigned)b * p.vocab + (0xFFFFFFFFu - (uint32_t)k);
         return true;
     };
-    const int lists = p.beams * p.chunks;
     for (int l = tid; l < lists; l += kMergeThreads) {
         u64 ms = 0;
         unsigned mf = UINT_MAX;  // no entry at all
@@ -370,23 +398,25 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamParams p)
             best = max(best, s);
         }
     }
-    // a score that at least K reach: the smallest of the warps' ceil(K/8)-th best
-    best = warp_sort_desc(best, lane);
-    if (lane == (K + 7) / 8 - 1) hs[warp] = best;
-    if (tid == 0) ctl[1] = 0;
-    __syncthreads();
-    u64 thr = hs[0];
-    for (int w = 1; w < kMergeThreads / 32; ++w) thr = min(thr, hs[w]);
+    unsigned* sel = hf;  // the candidates to rank, up to kBeamLists
     __syncthreads();
     const int cnt = ctl[0];
-    unsigned* sel = hf;  // the candidates that reach it, up to kBeamLists
-    for (int c = tid; c < cnt; c += kMergeThreads)
-        if (cs[c] >= thr) {
-            const int at = atomicAdd(&ctl[1], 1);
-            if (at < kBeamLists) sel[at] = c;
-        }
-    __syncthreads();
-    const bool few = ctl[1] <= kBeamLists;
+    if (cnt > kMergeThreads) {
+        // a score that at least K reach: the smallest of the warps' ceil(K/8)-th best
+        best = warp_sort_desc(best, lane);
+        if (lane == (K + 7) / 8 - 1) hs[warp] = best;
+        if (tid == 0) ctl[1] = 0;
+        __syncthreads();
+        u64 thr = hs[0];
+        for (int w = 1; w < kMergeThreads / 32; ++w) thr = min(thr, hs[w]);
+        for (int c = tid; c < cnt; c += kMergeThreads)
+            if (cs[c] >= thr) {
+                const int at = atomicAdd(&ctl[1], 1);
+                if (at < kBeamLists) sel[at] = c;
+            }
+        __syncthreads();
+    }
+    const bool few = cnt > kMergeThreads && ctl[1] <= kBeamLists;
     const int m = few ? ctl[1] : cnt;
     for (int i = tid; i < m; i += kMergeThreads) {
         const int c = few ? sel[i] : i;
