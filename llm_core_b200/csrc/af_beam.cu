@@ -34,6 +34,7 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kBeamThreads = 256;
+constexpr int kBeamBlocks = 3;                          // on an SM
 constexpr int kBeamPer = 16;                            // logits of a thread in a step
 constexpr int kBeamStep = kBeamThreads * kBeamPer;      // 4096
 constexpr int kBeamFull = 2048;                         // keys kept: cut back when more are there
@@ -109,26 +110,17 @@ struct BeamShared {
 // The buffer's K best keys, in order, to its front (fewer where it has fewer).
 __device__ void beam_cut(BeamShared& sh, int K) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = sh.count;
-    if (n <= kBeamThreads) {  // a key a thread: its rank among all
-        const u64 k = tid < n ? sh.key[tid] : 0;
-        int rank = 0;
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) rank += sh.key[i] > k;
-        __syncthreads();
-        if (tid < n && rank < K) sh.key[rank] = k;
-        if (tid == 0) sh.count = min(n, K);
-        __syncthreads();
-        return;
-    }
     u64 best = 0;
-    for (int i = tid; i < n; i += kBeamThreads) best = max(best, sh.key[i]);
-    best = warp_sort_desc(best, lane);
-    if (lane == (K + 7) / 8 - 1) sh.wkey[warp] = best;  // 0 where the warp has fewer: everything passes
+    // every warp has its share of them: key i is warp i % W's; a warp's n-th is of its threads' best values
+    constexpr int W = kBeamThreads / 32;
+    for (int i = lane * W + warp; i < n; i += kBeamThreads) best = max(best, sh.key[i]);
+    const uint32_t nth = warp_nth((uint32_t)(best >> 32), (K + W - 1) / W);  // 0 where the warp has fewer: everything passes
+    if (lane == 0) sh.wkey[warp] = (u64)nth << 32;
     if (tid == 0) sh.kept = 0;
     __syncthreads();
     u64 thr = sh.wkey[0];
 #pragma unroll
-    for (int w = 1; w < kBeamThreads / 32; ++w) thr = min(thr, sh.wkey[w]);
+    for (int w = 1; w < W; ++w) thr = min(thr, sh.wkey[w]);
     // their order among what passes, or, where that is more than sel holds (rising logits), among all
     for (int i = tid; i < n; i += kBeamThreads) {
         const u64 k = sh.key[i];
@@ -157,7 +149,7 @@ __device__ void beam_cut(BeamShared& sh, int K) {
     __syncthreads();
 }
 
-__global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParams p) {
+__global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_segment_kernel(BeamParams p) {
     constexpr int W = kBeamThreads / 32;
     extern __shared__ __align__(16) uint8_t sm[];
     BeamShared& sh = *reinterpret_cast<BeamShared*>(sm);
@@ -188,9 +180,10 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParam
             }
         }
     };
-    float next[kBeamPer];
-    load(lo, next);  // beside the beam's score, not behind it
+    float even[kBeamPer], odd[kBeamPer];  // a step's logits, and the next one's, on their way
+    load(lo, even);                       // beside the beam's score, not behind it
     if (dead_score(score)) return;
+    if (lo + kBeamStep < hi) load(lo + kBeamStep, odd);
     if (tid == 0) sh.count = 0;
     __syncthreads();
     float top = -INFINITY, thr = 0.f;
@@ -202,11 +195,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParam
         for (int w = 1; w < W; ++w) m = fminf(m, sh.wval[w]);
         return m;
     };
-    for (int t0 = lo; t0 < hi; t0 += kBeamStep) {
-        float v[kBeamPer];
-#pragma unroll
-        for (int j = 0; j < kBeamPer; ++j) v[j] = next[j];
-        if (t0 + kBeamStep < hi) load(t0 + kBeamStep, next);
+    auto step = [&](int t0, float (&v)[kBeamPer]) {
         float m[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) m[j] = fmaxf(fmaxf(v[4 * j], v[4 * j + 1]), fmaxf(v[4 * j + 2], v[4 * j + 3]));
@@ -217,15 +206,22 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParam
         }
         // a step's terms in 32 bits, the rest in 64; NaN stays NaN, and where all is -inf, nothing is added
         const float off = top > -INFINITY ? top : 0.f;
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        f32x2 part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+        const f32x2 less = pair(-off, -off), log2e = pair(kLog2e, kLog2e);
 #pragma unroll
-        for (int j = 0; j < kBeamPer; ++j) part[j & 3] += beam_exp2((v[j] - off) * kLog2e);
-        sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
+        for (int j = 0; j < kBeamPer; j += 2) {
+            float a, b;
+            unpair(mul2(add2(pair(v[j], v[j + 1]), less), log2e), a, b);
+            part[(j >> 1) & 1] = add2(part[(j >> 1) & 1], pair(beam_exp2(a), beam_exp2(b)));
+        }
+        float pa, pb;
+        unpair(add2(part[0], part[1]), pa, pb);
+        sum += (double)(pa + pb);
         const bool begin = t0 == lo;
         // The threshold, of the first step before anything is kept; of all steps so far behind steps 1, 2, 4, 8, ...,
         // which halves how many pass each time (top is the thread's largest so far).
-        const int step = (t0 - lo) / kBeamStep + 1;
-        const bool raise = (step & (step - 1)) == 0;
+        const int nr = (t0 - lo) / kBeamStep + 1;
+        const bool raise = (nr & (nr - 1)) == 0;
         if (raise) {
             const uint32_t s = warp_nth(float_to_ordered(top), (K + 7) / 8);
             if (lane == 0) sh.wval[warp] = ordered_to_float(s);
@@ -250,6 +246,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParam
                     if (v[i] > thr) keep(i);
             }
         }
+        if (t0 + 2 * kBeamStep < hi) load(t0 + 2 * kBeamStep, v);
         // at most a step's keys came on top of at most kBeamFull
         if (__syncthreads_or(tid == 0 && sh.count > kBeamFull)) {
             beam_cut(sh, K);
@@ -260,6 +257,10 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(BeamParam
             thr = fmaxf(thr, lowest());
             __syncthreads();
         }
+    };
+    for (int t0 = lo; t0 < hi; t0 += 2 * kBeamStep) {
+        step(t0, even);
+        if (t0 + kBeamStep < hi) step(t0 + kBeamStep, odd);
     }
     beam_cut(sh, K);
     const long long list = (long long)row * p.chunks + blockIdx.x;
@@ -453,11 +454,11 @@ std::string beam_wrong(const af_beam_select_args& a) {
     return "";
 }
 
-// Segments of a row: enough blocks to fill the SMs four times, none below kBeamChunk logits.
+// Segments of a row: as many blocks as the SMs hold at once, none below kBeamChunk logits.
 int beam_segments(const af_beam_select_args& a) {
     const int most = (a.vocab + kBeamChunk - 1) / kBeamChunk;
     const long long rows = std::max(1ll, (long long)a.n_seq * a.n_beams);
-    return (int)std::min((long long)most, std::max(1ll, 4 * 148 / rows));
+    return (int)std::min((long long)most, std::max(1ll, kBeamBlocks * 148 / rows));
 }
 
 size_t beam_ws(const af_beam_select_args& a) {
