@@ -992,10 +992,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 uint4 x[NC];
                 uint32_t* e = &x[0].x;
                 const int left = end - (t0 + t) * T - w * SH::RPW - lane / 8;  // rows in front of the end
+                const bool last = left + lane / 8 < SH::RPW;                   // the same in the whole warp
                 auto load = [&](int i0) {
 #pragma unroll
                     for (int i = 0; i < NC; ++i) x[i] = *place(i0 + i);
-                    if (TYPE == AF_KV_BF16 && left < SH::RPW) {  // the last tile: what lies behind is nothing
+                    if (last) {  // what lies behind the end is nothing: whatever was in that place before
 #pragma unroll
                         for (int i = 0; i < NC; ++i)
                             if ((i0 + i) % PER * 4 >= left) x[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -1018,11 +1019,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                         for (int i = 0; i < 4 * NC; ++i)
                             z = __hfma2(*reinterpret_cast<const __half2*>(&e[i]), __float2half2_rn(0.f), z);
                         const uint32_t zz = *reinterpret_cast<const uint32_t*>(&z) & 0x7fff7fffu;
-                        if (__any_sync(0xffffffffu, zz != 0)) {
+                        const bool odd = __any_sync(0xffffffffu, zz != 0);
+                        if (odd) {
                             without();
+                            note_bad(t);
+                        }
+                        if (odd || last) {
 #pragma unroll
                             for (int i = 0; i < NC; ++i) *place(i0 + i) = x[i];
-                            note_bad(t);
                         }
                     }
                     return;
