@@ -1273,13 +1273,247 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
     for (int d = 0; d < PER; ++d) out[d] = acc[d] * inv;
 }
 
+// ------------------------------------------------------------ small calls
+//
+// Few rows over few positions, where the kernel above spends its time on
+// setting up: a cluster of blocks per (16 query rows, kv head, sequence) takes
+// tiles of 32 positions in turn, K and V in shared memory as f32 with the next
+// tile's on their way, products on the f32 units.  A warp has two rows: their
+// scores, a position a lane, and their softmax; in P·V a thread has a dimension
+// and some rows.  In the end the blocks read one another's sums.  What bounds
+// it is the latency of its steps: lengths, pages, K and V, three passes over
+// shared memory.
+
+constexpr int kSmallThreads = 256;
+constexpr int kSmallRows = 16;
+constexpr int kSmallTile = 32;
+
+template <int HD>
+struct SmallShape {
+    static constexpr int T = kSmallTile;
+    static constexpr int KS = HD + 4, PS = kSmallRows + 4;  // floats from row to row: K's, the weights' of a position
+    static constexpr int DR = kSmallRows * HD / kSmallThreads;  // rows of a thread in P·V
+    static constexpr int BYTES = (T * (KS + HD + PS) + 2 * kSmallRows * HD + 3 * kSmallRows) * 4;
+};
+
+// 16 bytes of the cache as f32.
+template <int TYPE>
+__device__ __forceinline__ void widen(const uint4& x, float* f) {
+    const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (TYPE == AF_KV_F32) {
+            f[i] = __uint_as_float(e[i]);
+        } else if (TYPE == AF_KV_F16) {
+            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&e[i]));
+            f[2 * i] = y.x, f[2 * i + 1] = y.y;
+        } else {
+            f[2 * i] = __uint_as_float(e[i] << 16), f[2 * i + 1] = __uint_as_float(e[i] & 0xffff0000u);
+        }
+    }
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float cluster_ld(const float* mine, int rank) {
+    uint32_t a;
+    float f;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
+    return f;
+}
+
+template <int TYPE, int HD>
+__global__ void __launch_bounds__(kSmallThreads, 2) tree_small_kernel(TreeParams p, int blocks) {  // of a cluster
+    using SH = SmallShape<HD>;
+    using E = KvElem<TYPE>;
+    constexpr int T = SH::T, KS = SH::KS, PS = SH::PS, DR = SH::DR;
+    extern __shared__ __align__(1024) uint8_t sm[];  // declared alike everywhere: the strictest alignment is tree_mma_kernel's
+    float* sk = reinterpret_cast<float*>(sm);        // [T][KS]
+    float* sv = sk + T * KS;                         // [T][HD]
+    float* sw = sv + T * HD;                         // [T][PS] weights
+    float* sq = sw + T * PS;                         // [16][HD] queries, times the scale
+    float* so = sq + kSmallRows * HD;                // [16][HD] this block's sums of weighted V
+    float* s_m = so + kSmallRows * HD;               // [16] its largest score
+    float* s_l = s_m + kSmallRows;                   // [16] its sum of weights
+    float* s_c = s_l + kSmallRows;                   // [16] the tile's correction
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, seq = blockIdx.y;
+    const int rank = blocks > 1 ? blockIdx.x % blocks : 0, kvh = blocks > 1 ? blockIdx.x / blocks : blockIdx.x;
+    int r0, n;
+    kv_nodes(p.b, p.n_rows, seq, r0, n);
+    const int len = kv_len(p.kv, p.b, seq, n);
+    const int x0 = blockIdx.z * kSmallRows, rows = min(kSmallRows, n * p.G - x0);
+    if (len < 0 || rows <= 0) return;  // the whole cluster
+    const int end = p.mask ? len + n : len + node_of(p, x0 + rows - 1) + 1;
+    // K and V of a tile, 16 bytes a load
+    constexpr int VPL = 16 / (int)sizeof(typename E::T), LPR = HD / VPL, N = T * LPR / kSmallThreads;
+    uint4 k[N], v[N];
+    auto fetch = [&](int t0) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int i = tid + j * kSmallThreads, pos = t0 + i / LPR;
+            k[j] = v[j] = make_uint4(0u, 0u, 0u, 0u);
+            if (pos >= end) continue;
+            const long long at = kv_row(p.kv, p.b, seq, pos);
+            if (at < 0) {
+                set_err_at(p.b.err, kErrBadArgs);
+                continue;
+            }
+            const long long from = p.layer * p.kv.layer_bytes + at + (kvh * HD + i % LPR * VPL) * (int)sizeof(typename E::T);
+            k[j] = __ldg(reinterpret_cast<const uint4*>(p.kv.k + from));
+            v[j] = __ldg(reinterpret_cast<const uint4*>(p.kv.v + from));
+        }
+    };
+    fetch(rank * T);
+    for (int i = tid; i < kSmallRows * HD; i += kSmallThreads) {
+        float q = 0.f;
+        if (i / HD < rows) {
+            const int x = x0 + i / HD, node = node_of(p, x);
+            q = p.q[(long long)(r0 + node) * p.qs + (kvh * p.G + x - node * p.G) * HD + i % HD] * p.scale;
+        }
+        sq[i] = q;
+    }
+    const int r2 = 2 * warp;  // the warp's rows
+    int row[2], node[2];
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        node[i] = r2 + i < rows ? node_of(p, x0 + r2 + i) : -1;
+        row[i] = r0 + node[i];
+    }
+    const int d = tid % HD, dr = tid / HD * DR;  // of P·V: a dimension, the first row
+    float acc[DR];
+#pragma unroll
+    for (int i = 0; i < DR; ++i) acc[i] = 0.f;
+    for (int t0 = rank * T; t0 < end; t0 += blocks * T) {
+        bool odd = false;  // V with something that is not finite
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int i = tid + j * kSmallThreads, at = i / LPR, col = i % LPR * VPL;
+            float f[VPL], g[VPL];
+            widen<TYPE>(k[j], f);
+            widen<TYPE>(v[j], g);
+#pragma unroll
+            for (int c = 0; c < VPL; c += 4) {
+                *reinterpret_cast<float4*>(sk + at * KS + col + c) = make_float4(f[c], f[c + 1], f[c + 2], f[c + 3]);
+                *reinterpret_cast<float4*>(sv + at * HD + col + c) = make_float4(g[c], g[c + 1], g[c + 2], g[c + 3]);
+                const float z = fmaf(g[c], 0.f, fmaf(g[c + 1], 0.f, fmaf(g[c + 2], 0.f, g[c + 3] * 0.f)));
+                odd = odd || z != 0.f;  // NaN
+            }
+        }
+        odd = __syncthreads_or(odd);
+        if (t0 + blocks * T < end) fetch(t0 + blocks * T);
+        if (r2 < rows) {
+            float s[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll 8
+            for (int c = 0; c < HD; c += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(sk + lane * KS + c);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float4 q = *reinterpret_cast<const float4*>(sq + (r2 + i) * HD + c);
+                    s[i][0] = fmaf(q.y, x.y, fmaf(q.x, x.x, s[i][0]));
+                    s[i][1] = fmaf(q.w, x.w, fmaf(q.z, x.z, s[i][1]));
+                }
+            }
+            float w[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int j = t0 + lane - len;
+                const bool sees = node[i] >= 0 && t0 + lane < end && (j < 0 || tree_sees(p, row[i], node[i], j));
+                const float x = sees ? s[i][0] + s[i][1] : -INFINITY;
+                const float mn = fmaxf(m[i], warp_max(x)), ms = mn == -INFINITY ? 0.f : mn;
+                // what the row sees keeps a weight: an infinite value of V counts however small that is; NaN stays
+                w[i] = !sees ? 0.f : isnan(x) ? x : fmaxf(ex2(x - ms), __int_as_float(1));
+                const float corr = ex2(m[i] - ms);
+                l[i] = fmaf(l[i], corr, warp_sum(w[i]));
+                m[i] = mn;
+                if (lane == 0) s_c[r2 + i] = corr;
+            }
+            *reinterpret_cast<float2*>(sw + lane * PS + r2) = make_float2(w[0], w[1]);
+        }
+        __syncthreads();
+        if (dr < rows) {
+#pragma unroll
+            for (int i = 0; i < DR; ++i) acc[i] *= dr + i < rows ? s_c[dr + i] : 0.f;
+            const int last = min(T, end - t0);
+            auto add = [&](bool guard) {
+#pragma unroll 8
+                for (int j = 0; j < last; ++j) {
+                    const float y = sv[j * HD + d];
+#pragma unroll
+                    for (int i = 0; i < DR; i += 4) {
+                        const float4 w = *reinterpret_cast<const float4*>(sw + j * PS + dr + i);
+                        if (!guard || w.x != 0.f) acc[i] = fmaf(w.x, y, acc[i]);
+                        if (!guard || w.y != 0.f) acc[i + 1] = fmaf(w.y, y, acc[i + 1]);
+                        if (!guard || w.z != 0.f) acc[i + 2] = fmaf(w.z, y, acc[i + 2]);
+                        if (!guard || w.w != 0.f) acc[i + 3] = fmaf(w.w, y, acc[i + 3]);
+                    }
+                }
+            };
+            if (odd) add(true);
+            else add(false);
+        }
+        __syncthreads();
+    }
+    if (lane < 2 && r2 + lane < rows) {
+        s_m[r2 + lane] = lane ? m[1] : m[0];
+        s_l[r2 + lane] = lane ? l[1] : l[0];
+    }
+#pragma unroll
+    for (int i = 0; i < DR; ++i) so[(dr + i) * HD + d] = acc[i];
+    if (blocks > 1) cluster_sync();
+    else __syncthreads();
+    for (int i = rank * kSmallThreads + tid; i < rows * HD; i += blocks * kSmallThreads) {
+        const int r = i / HD, c = i % HD, x = x0 + r, nd = node_of(p, x);
+        float top = s_m[r], sum = s_l[r], o = so[i];
+        if (blocks > 1) {  // Σ 2^(m_b - m)·O_b / Σ 2^(m_b - m)·l_b, in the blocks' order
+            top = -INFINITY;
+            for (int b = 0; b < blocks; ++b) top = fmaxf(top, cluster_ld(s_m + r, b));
+            sum = o = 0.f;
+            for (int b = 0; b < blocks; ++b) {
+                const float lb = cluster_ld(s_l + r, b), mb = cluster_ld(s_m + r, b);
+                if (mb == -INFINITY && lb == 0.f) continue;  // a block that the row sees nothing of
+                const float f = ex2(mb - top);
+                sum = fmaf(f, lb, sum);
+                o = fmaf(f, cluster_ld(so + i, b), o);
+            }
+        }
+        p.out[(long long)(r0 + nd) * p.os + (kvh * p.G + x - nd * p.G) * HD + c] = sum == 0.f ? 0.f : o / sum;
+    }
+    if (blocks > 1) cluster_sync();  // a block's sums stay until all have read them
+}
+
 // ------------------------------------------------------------------ launch
 
 struct TreePlan {
-    bool mma;
+    bool mma, small;
+    long long max_len;
     int blocks, slots;  // slots 0: nothing is split, no second launch
     size_t ws;
 };
+
+constexpr int kSmallFill = 2 * kTreeSms;  // blocks up to which a small call's items are split over clusters
+
+// Which kernel: the smaller of two estimates in µs, from the sizes alone.  A
+// small call's tile costs its block about 1.2 µs (head_dim 64) or 2.2 µs (128;
+// 1.2 where three blocks share an SM), and up to 8 blocks share an item; the
+// tensor-core kernel costs 10 to 12 µs a wave of 148 items and its tiles.
+// Measured, small / tensor-core kernel, f32, 32/4 heads of 64: one row of 137
+// and 1,000 positions 5.9 / 11.9 and 11.6 / 14.7 µs; 16 sequences of 250 8.1 /
+// 15.3, of 1,000 20.4 / 19.8; 16 rows each of 250 40 / 18.  16 sequences with 32
+// kv heads of 128, a row each of 137: 19.7 / 45.5, of 1,000 95 / 98.
+bool small_call(const af_attention_tree_args& a, long long max_len) {
+    const bool f32 = a.kv.type == AF_KV_F32, narrow = a.kv.head_dim == 64;
+    const long long rows = (long long)a.batch.max_nodes * (a.n_heads / a.kv.n_kv_heads), heads = (long long)a.batch.n_seq * a.kv.n_kv_heads;
+    const long long items = (rows + kSmallRows - 1) / kSmallRows * heads, tiles = (max_len + kSmallTile - 1) / kSmallTile;
+    const double each = narrow || items >= kSmallFill ? 1.2 : 2.2;
+    const double small = 5. + std::max(each * (double)items * (double)tiles / kTreeSms, (narrow ? 1.6 : 2.4) * (double)((tiles + 7) / 8));
+    const double work = (double)((rows + kMmaRows - 1) / kMmaRows * heads) / kTreeSms;
+    const double mma = (f32 ? 12. : 10.) * std::max(1., work) + work * (double)((max_len + 63) / 64) * (narrow ? .5 : 1.) * (f32 ? 1. : .5);
+    return rows <= 65535ll * kSmallRows && a.batch.n_seq <= 65535 && small < mma;
+}
 
 TreePlan tree_plan(const af_attention_tree_args& a) {
     TreePlan pl = {};
@@ -1288,6 +1522,9 @@ TreePlan tree_plan(const af_attention_tree_args& a) {
     if (!pl.mma) return pl;
     const long long cap = (long long)a.batch.max_blocks * a.kv.page_size;
     const long long max_len = a.max_len > 0 ? std::min((long long)a.max_len, cap) : cap;
+    pl.max_len = max_len;
+    pl.small = small_call(a, max_len);
+    if (pl.small) return pl;
     const int T = tree_tile(a.kv.type);
     const long long tiles = (max_len + T - 1) / T, most = (tiles + kTreeMinTiles - 1) / kTreeMinTiles;
     const long long items = ((long long)a.batch.max_nodes * G + kMmaRows - 1) / kMmaRows * a.kv.n_kv_heads * a.batch.n_seq;
@@ -1346,8 +1583,31 @@ cudaError_t mma_launch(const MmaParams& mp, int n_seq, int max_nodes, cudaStream
     return cudaLaunchKernelEx(&cfg, tree_merge_kernel<HD>, mp);
 }
 
+template <int TYPE, int HD>
+cudaError_t small_launch(const TreeParams& p, int max_nodes, long long max_len, cudaStream_t st) {
+    constexpr int smem = SmallShape<HD>::BYTES;
+    AF_CUDA_TRY(cudaFuncSetAttribute(tree_small_kernel<TYPE, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    // as many blocks a cluster (a power of two up to 8) as keep the SMs at most twice filled
+    const long long tiles = (max_nodes * p.G + kSmallRows - 1) / kSmallRows, items = tiles * p.b.n_seq * p.kv.kv_heads;
+    int blocks = 1;
+    while (blocks < 8 && 2 * blocks * items <= kSmallFill && blocks * kSmallTile < max_len) blocks *= 2;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)blocks, 1, 1};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.kv.kv_heads * blocks, p.b.n_seq, (unsigned)tiles);
+    cfg.blockDim = dim3(kSmallThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, tree_small_kernel<TYPE, HD>, p, blocks);
+}
+
 template <int TYPE>
 cudaError_t tree_launch(const TreeParams& p, const TreePlan& pl, int max_nodes, void* ws, cudaStream_t st) {
+    if (pl.small) return p.kv.hd == 64 ? small_launch<TYPE, 64>(p, max_nodes, pl.max_len, st)
+                                           : small_launch<TYPE, 128>(p, max_nodes, pl.max_len, st);
     if (pl.mma) {
         MmaParams mp = {};
         mp.t = p;

@@ -161,8 +161,13 @@ def plain_beams(ref, cfg, prompt, n_beams, max_new, penalty, stepped):
 @pytest.mark.parametrize("with_eos", [False, True])
 def test_beam_search_matches_plain_search(gpu, preset, seed, n_beams, max_new, penalty, with_eos):
     """The same hypothesis and rating as a search over sequences stepped from
-    their start.  The linear layers of beams and steps agree to ~1e-5 of a
-    logit's size of a few units, so ratings agree to far below 2e-3."""
+    their start.  Beams go through the linear layers as rows, whose rounding is
+    not that of single steps, and a layer behind another amplifies it: on the
+    random qwen2 preset 2e-5 in the first layer's values is 2e-3 in the logits,
+    with either attention kernel.  So the rating's tolerance follows from the
+    logits: two rows of logits that differ by at most d give log-probabilities
+    that differ by at most 2 d, d being what step_tree's rows of the winning
+    hypothesis differ by from its steps, and the beams' rows by as much again."""
     path = model_path(preset, seed)
     cfg = read_config(path)
     rng = np.random.default_rng(seed)
@@ -175,8 +180,17 @@ def test_beam_search_matches_plain_search(gpu, preset, seed, n_beams, max_new, p
         score, ids = plain_beams(ref, cfg, prompt, n_beams, max_new, penalty, stepped)
     m = LlamaCudaModel(path, config=cfg)
     got, rating = m.generate_beam(prompt, n_beams, max_new, penalty)
-    assert abs(rating - score) < 2e-3
     assert got == ids
+    start = prompt if prompt[0] == cfg.bos_id else [cfg.bos_id] + prompt
+    ended = len(ids) < min(max_new, cfg.n_ctx - len(start))  # one log-probability more, of the end
+    length = len(ids) + ended
+    row, fed = ref.prefill(start, 0)[1], ids[:length - 1]
+    rows = [row]
+    if fed:
+        rows += list(ref.step_tree(fed, list(range(-1, len(fed) - 1)), len(start), want_logits=True)[1])
+    steps = [row] + [ref.step(t, len(start) + i)[1] for i, t in enumerate(fed)]
+    apart = sum(float(np.abs(r - s).max()) for r, s in zip(rows, steps))
+    assert abs(rating - score) <= (2 * 2 * apart + 1e-5 * abs(score)) / length ** penalty + 1e-5
     # and the engine generates as before afterwards
     again = m.generate(prompt, LlamaConfig(max_new_tokens=6, temperature=0))
     fresh = LlamaCudaModel(path, config=cfg)
