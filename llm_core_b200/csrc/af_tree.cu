@@ -1,6 +1,11 @@
 // af_tree.cu — attention of drafted tokens over a paged cache
 // (af_attention_tree_f32): the nodes of every sequence see its cached
-// positions and, by a bit mask, one another.
+// positions and, by a bit mask, one another,
+//     out = Σ_j 2^(s_j - m)·v_j / Σ_j 2^(s_j - m),  s_j = q·k_j·scale·log2(e),  m = max s_j
+// over the positions j that the row sees, in one pass with a running m.
+// Three kernels: tree_mma_kernel for head_dim 64 and 128, tree_small_kernel for
+// the same where the call is small (small_call), tree_row_kernel for every other
+// head_dim.
 #define AF_WHOLE_PROGRAM  // the register split below (setmaxnreg) holds only without separate compilation
 #include <cuda.h>
 
@@ -39,7 +44,8 @@ constexpr int kTreeThreads = 128;
 
 // One block per row and head: its warps take the positions in turn, a lane
 // the dimensions lane, lane + 32, ...; each warp keeps a running maximum, sum
-// and output, merged at the end.
+// and output, merged at the end.  Every row reads K and V again and a warp has
+// one position at a time: bound by the latency of its loads.
 template <int TYPE>
 __global__ void __launch_bounds__(kTreeThreads) tree_row_kernel(TreeParams p) {
     using E = KvElem<TYPE>;
@@ -138,16 +144,30 @@ __global__ void __launch_bounds__(kTreeThreads) tree_row_kernel(TreeParams p) {
 // The tensor cores truncate when they add to an accumulator (measured: sums
 // of 400 and 4000 positive products came out 3.9e-5 and 4.0e-4 low, 1e-7 an
 // instruction), so no accumulator lives longer than a tile: small products
-// first, then the hi·hi ones, and the softmax warps add each tile's P·V to
-// sums in registers, which round to nearest.
+// first, then the hi·hi ones, and the output warps add each tile's P·V to sums
+// in registers, which round to nearest.
 //
-// Warps (24): 0-7 turn scores into weights, half a query row a thread; 8-11
-// add up the tiles' P·V and write the rows out; 12-15 put K and 16-19 V into
-// the form that the products take (split, scaled; a cache in f16 only has its V
-// looked through); 20 issues the products; 21 and 22 the copies of K and V, a
-// box of rows per page by the TMA engine (single rows by bulk copies run at 2.3 TB/s).  Registers a
-// thread (setmaxnreg): 72 / 168 / 64 / 40 for head_dim 128, 88 / 128 / 64 / 40
-// for 64, whose tiles have 128 positions, out of the launch's 768·80.
+// Warps (32): first the softmax warps, 32 of a tile's columns of 32 rows each
+// (f32: 8 warps for 64 positions; others: 16 for 128); four add up the tiles'
+// P·V and write the rows out; 8 for K and 8 for V (f32) or 4 and 4 put the
+// tiles into the form that the products take (split, scaled; a cache in f16
+// only has its V looked through); 28 issues P·V and 31 the scores, each behind
+// its own barriers (one warp for both: 52 us where two take 47); 29 and 30 copy
+// K and V, a box of rows per page by the TMA engine (single rows by bulk copies
+// run at 2.3 TB/s).  Registers (setmaxnreg): MmaShape's REG_*, out of the
+// launch's 1,024·64.
+//
+// Measured with inputs out of L2, device time: 26 nodes over 4,000 positions, 32
+// heads of 128, f32, 46.5 us (2.8 TB/s of the 132 MB; bound by the splitting
+// warps: each waits, reads, splits and stores its rows in turn, ~3,700 cycles a
+// tile); 16 sequences of 0 to 8,190 positions with 31 nodes, 16/2 heads of 128,
+// f16, 48 us (1.6 TB/s; ~2,900 cycles a tile of 128, the softmax's chain, of
+// which the exponentials fill 1,024 on the special function units, and ~16,000
+// cycles of plan, queries, and sums at both ends); chunks of 509 over up to 16,001
+// positions, 32/4 heads of 64, bf16, 218 us (315 TFLOP/s; the same chain, ~3,100
+// cycles a tile).  Steps that got there: K and V by single bulk copies -> boxes;
+// 4 -> 8 -> 16 softmax warps (chunk 402 -> 333 -> 266 us); tiles of 64 -> 128
+// positions with a power of two per 32 bf16 rows (241 -> 218 us).
 //
 // Tiles in shared memory: rows of 64 values (128 bytes) in the 128-byte
 // swizzle, K-major for K, the same tile MN-major for V; for f32 the TMA engine
@@ -343,11 +363,11 @@ __device__ __noinline__ uint32_t clean(float4 (&x)[N]) {
 // device alone (lengths, counts), so every block finds its place itself: the
 // smallest t for which the blocks fit the waves that the items need anyway.  A
 // ragged batch then costs its average and not its longest: 16 sequences of
-// 8190 to 0 positions, 120 -> 75 us.
+// 8190 to 0 positions, 120 -> 82 us when it came in.
 constexpr int kTreeSms = 148;
 constexpr int kTreeWaves = 4;                                // beyond so many the items balance one another
 constexpr int kTreeItems = kTreeSms * kTreeWaves;
-constexpr int kTreeMinTiles = 3;                             // a shorter split costs more than it saves
+constexpr int kTreeMinTiles = 3;                             // a shorter split costs more than it saves: a block's set-up is 10,000 cycles, a tile ~3,000
 
 struct MmaParams {
     CUtensorMap k_map, v_map;  // [rows of the layer's pool][kv heads][HD], boxes of box_rows rows
