@@ -237,7 +237,10 @@ cudaError_t af_rope_f32(float* d_q, int n_heads, int head_dim, int pos, float th
  * AF_KV_F32, pages of consecutive positions).
  * page_size is a power of two, head_dim a multiple of 8 up to 256, k and v are
  * 16-byte aligned, layer_stride (values from one layer to the next; 0 = the
- * dense n_pages*page_size*n_kv_heads*head_dim) is a multiple of 8. */
+ * dense n_pages*page_size*n_kv_heads*head_dim) is a multiple of 8.
+ * n_pages*page_size stays below 2^31, n_kv_heads at most 65535.  Pointers
+ * belong to the current device; the first call of each of these entries on a
+ * device comes before any stream capture. */
 #define AF_KV_F32 0
 #define AF_KV_F16 1
 #define AF_KV_BF16 2
@@ -303,12 +306,16 @@ cudaError_t af_kv_store_f32(const af_kv_store_args* args, cudaStream_t stream);
  * a prompt.  K and V of the nodes are in the cache already (af_kv_store_f32).
  * out[row][h] = softmax over what the row sees of q·k·scale, times v; scale 0
  * = 1/sqrt(head_dim); a row that sees nothing gives zeros; what no row may see
- * may hold anything, infinities and NaN too.  q, out [n_rows][n_heads]
+ * may hold anything, infinities and NaN too; an infinite or NaN value of V
+ * reaches the rows that see it, a key that is not finite leaves the rows that
+ * see it undefined, and magnitudes stay below 2^100.  q, out [n_rows][n_heads]
  * [head_dim] f32 (strides as above), fp32 accuracy for every cache type.
  * max_len: no sequence has more positions, cached and new (it sizes the
  * launch; 0 = max_blocks*page_size).  ws: af_attention_tree_f32_workspace
- * bytes, zeroed before its first use and left ready for the next; calls that
- * may overlap on the GPU need workspaces of their own. */
+ * bytes (0 for small calls, which a call's sizes decide), zeroed before its
+ * first use and left ready for the next; calls that may overlap on the GPU need
+ * workspaces of their own.  max_nodes times the square of n_heads/n_kv_heads is
+ * at most 2^31. */
 typedef struct {
     af_kv_cache kv;
     af_kv_batch batch;
@@ -334,8 +341,8 @@ cudaError_t af_attention_tree_f32(const af_attention_tree_args* args, cudaStream
  * out_beam is the logits row, so that it serves as af_kv_fork's parent.  A
  * beam whose score is -inf or NaN, or whose logits hold NaN or +inf or nothing
  * above -inf, scores -inf throughout.  n_out <= 64 and <= n_beams*vocab,
- * n_beams <= 64.  ws: af_beam_select_f32_workspace bytes, zeroed before its
- * first use; calls that may overlap need workspaces of their own. */
+ * n_beams <= 64, n_beams * ceil(vocab / 8192) <= 1024.  ws:
+ * af_beam_select_f32_workspace bytes, zeroed before its first use; calls that may overlap need workspaces of their own. */
 typedef struct {
     const float* logits;
     int64_t logits_stride;
