@@ -312,9 +312,9 @@ cudaError_t af_kv_store_f32(const af_kv_store_args* args, cudaStream_t stream);
  * [head_dim] f32 (strides as above), fp32 accuracy for every cache type.
  * max_len: no sequence has more positions, cached and new (it sizes the
  * launch; 0 = max_blocks*page_size).  ws: af_attention_tree_f32_workspace
- * bytes (0 for small calls, which a call's sizes decide), zeroed before its
- * first use and left ready for the next; calls that may overlap on the GPU need
- * workspaces of their own.  max_nodes times the square of n_heads/n_kv_heads is
+ * bytes, enough for every call with no more sequences, nodes and positions,
+ * zeroed before its first use and left ready for the next; calls that may
+ * overlap on the GPU need workspaces of their own.  max_nodes times the square of n_heads/n_kv_heads is
  * at most 2^31. */
 typedef struct {
     af_kv_cache kv;

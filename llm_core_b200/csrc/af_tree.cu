@@ -1544,7 +1544,8 @@ TreePlan tree_plan(const af_attention_tree_args& a) {
     const long long max_len = a.max_len > 0 ? std::min((long long)a.max_len, cap) : cap;
     pl.max_len = max_len;
     pl.small = small_call(a, max_len);
-    if (pl.small) return pl;
+    // the workspace does not ask which kernel: it grows with every size, so one for the largest call serves smaller
+    // ones, which may go to the other kernel
     const int T = tree_tile(a.kv.type);
     const long long tiles = (max_len + T - 1) / T, most = (tiles + kTreeMinTiles - 1) / kTreeMinTiles;
     const long long items = ((long long)a.batch.max_nodes * G + kMmaRows - 1) / kMmaRows * a.kv.n_kv_heads * a.batch.n_seq;
@@ -1684,7 +1685,7 @@ extern "C" cudaError_t af_attention_tree_f32(const af_attention_tree_args* a, cu
     if (a->n_rows == 0 || a->batch.n_seq == 0) return cudaSuccess;
     if (!a->q || !a->out) return refuse("null q or out");
     const TreePlan pl = tree_plan(*a);
-    if (pl.ws && (!a->ws || a->ws_bytes < pl.ws || (reinterpret_cast<uintptr_t>(a->ws) & 15)))
+    if (!pl.small && pl.ws && (!a->ws || a->ws_bytes < pl.ws || (reinterpret_cast<uintptr_t>(a->ws) & 15)))
         return refuse("ws must hold af_attention_tree_f32_workspace bytes, 16-byte aligned");
     const long long qd = (long long)a->n_heads * a->kv.head_dim;
     TreeParams p = {};

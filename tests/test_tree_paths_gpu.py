@@ -7,7 +7,7 @@ import kv_helpers as kh
 import test_tree_attention_gpu as ta
 
 pytestmark = pytest.mark.gpu
-MMA_WS = 1 << 20  # its sums of split items; the kernel for small calls needs no workspace
+MMA_WS = 1 << 20  # sums of split items (148 blocks of 128 rows and more): what a call for long sequences asks for
 
 
 @pytest.fixture
@@ -96,3 +96,30 @@ def test_small_calls(gpu, kv, hd, lengths, counts):
     """Clusters of one block to eight, tiles that end inside, empty sequences."""
     for H, KV in ((8, 8), (12, 4)):
         ta.run_case(gpu, kv, H, KV, hd, lengths, counts, page=8)
+
+
+def test_a_workspace_for_the_largest_call_serves_smaller_ones(gpu):
+    """Sizes on both sides of the choice between the kernels."""
+    def bytes_for(n_seq, max_len, hd, H=8, KV=8):
+        c = kh.Cache("f32", KV, hd, [1] * n_seq, page=16, extra_blocks=1024)
+        q = kh.torch.zeros((n_seq, H, hd), device="cuda")
+        a = kh.attention_args(c, q, q, kh.ints([0] * n_seq), kh.ints(range(n_seq + 1)), 1, max_len=max_len)
+        return gpu.af_attention_tree_f32_workspace(a)
+
+    for hd in (64, 128):
+        most = bytes_for(40, 4000, hd)
+        for n_seq in (1, 36, 37, 38, 40):
+            for max_len in (1, 100, 256, 1000, 4000):
+                assert bytes_for(n_seq, max_len, hd) <= most
+
+
+@pytest.mark.parametrize("kv,hd", [("f16", 64), ("f32", 128)])
+def test_more_items_than_blocks_at_once(gpu, room, kv, hd):
+    """640 items and more, some of them long: beyond the blocks of four waves."""
+    ta.run_case(gpu, kv, 16, 16, hd, [7 * i for i in range(39)] + [3000], [1 + i % 2 for i in range(40)], seed=3)
+
+
+@pytest.mark.parametrize("page", [1, 2, 4])
+def test_pages_of_few_positions(gpu, room, page):
+    for kv in ("f32", "bf16"):
+        ta.run_case(gpu, kv, 8, 4, 64, [77, 300], [9, 20], page=page)
