@@ -65,7 +65,7 @@ __device__ __forceinline__ void store_row(const StoreParams& p, int row, StorePl
     if (tid == 0) out->seq = -1;
     __syncthreads();
     if (p.b.first) {
-        for (int s = tid; s < p.b.n_seq; s += kStoreThreads) {
+        for (int s = tid; s < p.b.n_seq; s += blockDim.x) {
             const int f = p.b.first[s], e = p.b.first[s + 1], len = p.b.len[s];
             if (f <= row && row < e) *out = {s, row - f, len};
         }
@@ -75,11 +75,38 @@ __device__ __forceinline__ void store_row(const StoreParams& p, int row, StorePl
     __syncthreads();
 }
 
+// The same by one warp.
+__device__ __forceinline__ StorePlace store_row_warp(const StoreParams& p, int row) {
+    const int lane = threadIdx.x & 31;
+    StorePlace w = {-1, 0, 0};
+    if (!p.b.first) {
+        const int s = row / p.b.max_nodes;
+        if (s < p.b.n_seq) w = {s, row % p.b.max_nodes, p.b.len[s]};
+        return w;
+    }
+    for (int s0 = 0; s0 < p.b.n_seq; s0 += 32) {
+        const int s = s0 + lane;
+        StorePlace mine = {-1, 0, 0};
+        if (s < p.b.n_seq) {
+            const int f = p.b.first[s], e = p.b.first[s + 1], len = p.b.len[s];
+            if (f <= row && row < e) mine = {s, row - f, len};
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, mine.seq >= 0);
+        if (hit) {
+            const int src = 31 - __clz(hit);  // first[] that does not rise: the last one, as a block takes it or another
+            w.seq = __shfl_sync(0xffffffffu, mine.seq, src);
+            w.node = __shfl_sync(0xffffffffu, mine.node, src);
+            w.len = __shfl_sync(0xffffffffu, mine.len, src);
+        }
+    }
+    return w;
+}
+
 // Where the row's rotation and cache position are; false (and the error word) where it has none.
 __device__ __forceinline__ bool store_place(const StoreParams& p, const StorePlace& w, int depth, long long& at, long long& slot) {
     at = (long long)w.len + (p.depth ? depth : w.node);
     if (w.len < 0 || at < 0 || at >= p.n_ctx || w.node < 0 || w.node >= p.b.max_nodes) {
-        if (threadIdx.x == 0) set_err_at(p.b.err, kErrBadArgs);
+        set_err_at(p.b.err, kErrBadArgs);
         return false;
     }
     const long long pos = (long long)w.len + w.node;
@@ -87,21 +114,23 @@ __device__ __forceinline__ bool store_place(const StoreParams& p, const StorePla
     return true;
 }
 
-// A block per row, its heads (queries, keys, values) over the warps.  HD 64
-// and 128 with 16-byte rows: a lane holds 4 values, HD/4 lanes a head, the
-// partner of a rotation sits HD/8 lanes away; a warp's first heads (up to 3)
-// are loaded before the row's place is known.  Bound by memory, q, k, v once
-// in, once out, and by a row's chain of loads (counts, then table and
-// rotation), waited for by every block: 8 sequences of up to 509 rows, 16/2
-// heads of 128, bf16, 20.5 us (3.3 TB/s); one row 2.8 us, a launch.  Measured and
-// not taken: 2 to 8 rows a block with the next row's loads ahead, 27 us (64
-// registers, fewer blocks an SM).
-template <int TYPE, int HD>
-__global__ void __launch_bounds__(kStoreThreads, 5) kv_store_vec_kernel(StoreParams p) {
-    constexpr int LH = HD / 4, HPW = 32 / LH, W = kStoreThreads / 32, U = 3;
+// A block per row, its heads (queries, keys, values) over the warps, or, where
+// rows are many, a warp per row.  HD 64 and 128 with 16-byte rows: a lane holds 4
+// values, HD/4 lanes a head, the partner of a rotation sits HD/8 lanes away; a
+// warp's first heads (U) are loaded before the row's place is known.  Bound by
+// memory, q, k, v once in, once out, and by a row's chain of loads (counts, then
+// table and rotation), hidden behind other rows': 8 sequences of up to 509 rows,
+// 16/2 heads of 128, bf16, 16.7 us a warp a row (4.1 TB/s), 20.5 a block of 8 warps,
+// 18.3 of 4; one row 2.7 us, a launch.  Measured and not taken: 2 to 8 rows a block with the next row's loads
+// ahead, 27 us (64 registers, fewer blocks an SM).
+template <int TYPE, int HD, bool WARP>
+__global__ void __launch_bounds__(kStoreThreads, WARP ? 4 : 5) kv_store_vec_kernel(StoreParams p) {
+    constexpr int LH = HD / 4, HPW = 32 / LH, W = WARP ? 1 : kStoreThreads / 32, U = WARP ? 5 : 3;
     using E = KvElem<TYPE>;
-    __shared__ StorePlace where;
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ StorePlace shared;
+    const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int row = WARP ? blockIdx.x * (kStoreThreads / 32) + (threadIdx.x >> 5) : blockIdx.x;
+    if (WARP && row >= p.n_rows) return;
     const int sub = lane / LH, col = lane % LH, KV = p.kv.kv_heads, heads = p.H + 2 * KV;
     const float* q = p.q + (long long)row * p.qs + 4 * col;
     const float* k = p.k + (long long)row * p.ks + 4 * col - p.H * HD;         // by the head's number
@@ -116,7 +145,13 @@ __global__ void __launch_bounds__(kStoreThreads, 5) kv_store_vec_kernel(StorePar
         if (h < heads) x[u] = load(h);
     }
     const int depth = p.depth ? p.depth[row] : 0;
-    store_row(p, row, &where);
+    StorePlace where;
+    if (WARP) {
+        where = store_row_warp(p, row);
+    } else {
+        store_row(p, row, &shared);
+        where = shared;
+    }
     if (where.seq < 0) return;
     long long at, slot;
     if (!store_place(p, where, depth, at, slot)) return;
@@ -631,8 +666,15 @@ extern "C" cudaError_t af_kv_store_f32(const af_kv_store_args* a, cudaStream_t s
                       vec(p.sin_t) && vec(p.q_norm) && vec(p.k_norm) && !((p.qs | p.ks | p.vs | p.os) & 3);
     auto go = [&](auto type) {
         constexpr int TYPE = decltype(type)::value;
-        if (wide && hd == 64) kv_store_vec_kernel<TYPE, 64><<<p.n_rows, kStoreThreads, 0, stream>>>(p);
-        else if (wide) kv_store_vec_kernel<TYPE, 128><<<p.n_rows, kStoreThreads, 0, stream>>>(p);
+        // A warp a row where rows are so many that a row's chain hides behind others'.  Bf16, 16/2 heads of 128, block
+        // a row / warp a row: 667 rows 5.0 / 9.7 us, 1,667 10.5 / 11.6, 3,333 20.8 / 17.2; 32/32 heads 13.6 / 40.7, 33.8 /
+        // 47.1, 57.3 / 57.6.
+        const bool many = p.n_rows > 15 * 148;
+        const int packed = (p.n_rows + kStoreThreads / 32 - 1) / (kStoreThreads / 32);
+        if (wide && hd == 64 && many) kv_store_vec_kernel<TYPE, 64, true><<<packed, kStoreThreads, 0, stream>>>(p);
+        else if (wide && many) kv_store_vec_kernel<TYPE, 128, true><<<packed, kStoreThreads, 0, stream>>>(p);
+        else if (wide && hd == 64) kv_store_vec_kernel<TYPE, 64, false><<<p.n_rows, kStoreThreads, 0, stream>>>(p);
+        else if (wide) kv_store_vec_kernel<TYPE, 128, false><<<p.n_rows, kStoreThreads, 0, stream>>>(p);
         else kv_store_kernel<TYPE><<<p.n_rows, kStoreThreads, 0, stream>>>(p);
     };
     switch (a->kv.type) {
