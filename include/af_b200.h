@@ -238,9 +238,10 @@ cudaError_t af_rope_f32(float* d_q, int n_heads, int head_dim, int pos, float th
  * page_size is a power of two, head_dim a multiple of 8 up to 256, k and v are
  * 16-byte aligned, layer_stride (values from one layer to the next; 0 = the
  * dense n_pages*page_size*n_kv_heads*head_dim) is a multiple of 8.
- * n_pages*page_size stays below 2^31, n_kv_heads at most 65535.  Pointers
- * belong to the current device; the first call of each of these entries on a
- * device comes before any stream capture. */
+ * n_pages*page_size stays below 2^31, n_kv_heads at most 65535, n_layers at
+ * most 32767, max_blocks*page_size (below) at most 2^30.  Pointers belong to the
+ * current device; the first call of each of these entries on a device comes
+ * before any stream capture. */
 #define AF_KV_F32 0
 #define AF_KV_F16 1
 #define AF_KV_BF16 2

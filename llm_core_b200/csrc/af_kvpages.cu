@@ -16,7 +16,7 @@ std::string kv_cache_wrong(const af_kv_cache& c) {
     if (c.page_size <= 0 || c.page_size > (1 << 20) || (c.page_size & (c.page_size - 1)))
         return "page_size must be a power of two up to 2^20";
     if (c.head_dim <= 0 || c.head_dim > 256 || c.head_dim % 8) return "head_dim must be a multiple of 8 up to 256";
-    if (c.n_kv_heads > 65535) return "n_kv_heads must be at most 65535";
+    if (c.n_kv_heads > 65535 || c.n_layers > 32767) return "n_kv_heads must be at most 65535, n_layers at most 32767";
     if ((long long)c.n_pages * c.page_size > INT_MAX) return "n_pages * page_size must be below 2^31";
     const long long dense = (long long)c.n_pages * c.page_size * c.n_kv_heads * c.head_dim;
     if (c.layer_stride < 0 || c.layer_stride % 8 || (c.layer_stride && c.n_layers > 1 && c.layer_stride < dense))
@@ -738,7 +738,6 @@ extern "C" cudaError_t af_kv_compact(const af_kv_compact_args* a, cudaStream_t s
     if (a->max_path < 0) return refuse(me, "max_path must not be negative");
     if (a->batch.n_seq == 0) return cudaSuccess;
     if (!a->len_out || !a->n_path || (a->max_path > 0 && !a->path)) return refuse(me, "null path, n_path or len_out");
-    if (a->kv.n_layers > 32767) return refuse(me, "n_layers must be at most 32767");
     const KvView kv = kv_view(a->kv);
     int* err = nullptr;
     AF_CUDA_TRY(device_error_word(&err));

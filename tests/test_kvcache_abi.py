@@ -164,6 +164,14 @@ def test_workspace_sizes():
     assert lib.af_kv_fork_workspace(C.byref(fork())) >= 2 * 16 + 8 * 4
 
 
+def test_a_cache_of_too_many_layers_is_refused_before_anything_is_launched():
+    lib = _lib.load()
+    many = cache(n_layers=32768)
+    for name, a in (("af_kv_fork", fork(kv=many)), ("af_kv_compact", compact(kv=many))):
+        assert getattr(lib, name)(C.byref(a), None) != 0
+        assert b"n_layers" in lib.af_last_error()
+
+
 def test_tree_and_beam_engine_entries_reject_a_null_engine():
     lib = _lib.load()
     i1 = (C.c_int32 * 1)()
