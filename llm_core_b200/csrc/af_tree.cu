@@ -306,7 +306,7 @@ struct MmaShape {
     static constexpr int NB = F32 ? 256 / HD : 3;       // tiles in shared memory: K V K V ...
     static constexpr int NS = F32 ? 4 : HD == 128 ? 2 : 3;  // score tiles in tensor memory (each becomes its weights)
     static constexpr int NC = NS + 1;                   // corrections (see c_full)
-    static constexpr int RING = NB + NS;                // barriers and scales of K (see k_full)
+    static constexpr int RING = NB + NS + 1;            // barriers and powers of two (see k_full)
     static constexpr int RAWB = T / 2 * HD * 4;         // f32: half the rows of K or V as they are
     static constexpr int RPW = T / SW;                  // rows that share a power of two: a splitting warp's
     static constexpr int LPR = HD * SIZE / 16;          // lanes of a row (f32)
@@ -511,9 +511,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     extern __shared__ __align__(1024) uint8_t sm[];
     const TreeParams& p = mp.t;
     // A waiter never falls a whole ring behind.  Scores of tile u are issued when the products of u - NS are done, and
-    // those are issued when the weights of u - NS are there and the products before them were taken.  So K of t + RING,
-    // written when the scores of t + NS are done, finds the softmax through with tile t, and the correction of t + NC
-    // finds that of t taken.  Every other barrier's next phase needs what the waiter of this one does.
+    // those are issued when the weights of u - NS are there and the products before them were taken.  K's powers of
+    // two of t + RING are written behind the tile before, whose place is free when the scores of t + RING - 1 - NB =
+    // t + NS are done, so the softmax is through with tile t, and the correction of t + NC finds that of t taken;
+    // V's are written when the products of t + RING - 1 - NB are done.  Every other barrier's next phase needs what
+    // the waiter of this one does.
     uint64_t* k_full = reinterpret_cast<uint64_t*>(sm);  // [RING] K of a tile is ready: its splitting warps (f16: the copy)
     uint64_t* v_full = k_full + RING;                    // [NB] V, its splitting warps
     uint64_t* k_empty = v_full + NB;                     // [NB] scores done
@@ -530,8 +532,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     uint64_t* fin = q_full + 1;                          // softmax warps: tops and sums written
     uint64_t* done = fin + 1;                            // everything issued is done: scores, products
     uint64_t* w_empty = done + 1;                        // [NS] P·V done: the weights' place is free
-    static_assert((RING + 5 * NB + 3 * NS + NC + 9) * 8 + 16 <= SH::BAD, "barriers");
-    uint32_t* tslot = reinterpret_cast<uint32_t*>(w_empty + NS);
+    uint64_t* v_scale = w_empty + NS;                    // [RING] V's powers of two are written: its splitting warps
+    static_assert((2 * RING + 5 * NB + 3 * NS + NC + 9) * 8 + 16 <= SH::BAD, "barriers");
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(v_scale + RING);
     volatile int* flag = reinterpret_cast<volatile int*>(tslot + 1);
     uint32_t* bad = reinterpret_cast<uint32_t*>(sm + SH::BAD);
     float* s_rs = reinterpret_cast<float*>(sm + SH::ROWS);
@@ -581,7 +584,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             mbar_init(&k_land[i], 1);
             mbar_init(&v_land[i], 1);
         }
-        for (int i = 0; i < RING; ++i) mbar_init(&k_full[i], TYPE == AF_KV_F16 ? 1 : SW);
+        for (int i = 0; i < RING; ++i) {
+            mbar_init(&k_full[i], TYPE == AF_KV_F16 ? 1 : SW);
+            mbar_init(&v_scale[i], SW);
+        }
         for (int i = 0; i < 4; ++i) mbar_init(&raw_free[i], SW / 2);
         for (int i = 0; i < NS; ++i) {
             mbar_init(&s_full[i], 1);
@@ -712,11 +718,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             if (lane == 0) mbar_arrive(&p_full[sl]);
         };
         const int tiles_mine = w4 < live_warps ? nt : 0;
-        int sl = 0, sl_ph = 0, st = 0, st_ph = 0, kt = 0, kt_ph = 0, co = 0;  // rings of NS, NB, RING, NC and their phases
+        int sl = 0, sl_ph = 0, kt = 0, kt_ph = 0, co = 0;  // rings of NS, RING, NC and their phases
         int met = 0;  // the tiles at which the row's warps have met
         for (int t = 0; t < tiles_mine; ++t) {
             ok = TYPE == AF_KV_F16 ? wait_warp(&s_full[sl], sl_ph)
-                                   : wait_three(&k_full[kt], kt_ph, &s_full[sl], sl_ph, &v_full[st], st_ph);
+                                   : wait_three(&k_full[kt], kt_ph, &s_full[sl], sl_ph, &v_scale[kt], kt_ph);
             if (!ok) break;
             tc_fence_after();
             const uint32_t sb = tmem + lanes + SH::S0 + sl * T + part * C;
@@ -805,7 +811,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             }
             publish(sl);
             if (++sl == NS) sl = 0, sl_ph ^= 1;
-            if (++st == NB) st = 0, st_ph ^= 1;
             if (++kt == RING) kt = 0, kt_ph ^= 1;
         }
         // one that leaves early is counted at the others' remaining meetings: nobody is left waiting
@@ -967,10 +972,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 uint32_t mx = __reduce_max_sync(
                     0xffffffffu, __float_as_uint(max3_abs_nan(max3_abs_nan(big[0], big[1], big[2]), big[3], 0.f)));
                 if (lane == 0) mbar_arrive(&freed[w / (SW / 2)]);  // all lanes hold theirs
-                if (due) hand_over(due);                        // the tile before: its stores are through by now
-                if (t == SH::QTILE) ok = wait_warp(q_full, 0);  // the staged queries' place is written over
-                if (ok && t >= NB) ok = wait_warp(&empty[st], ph ^ 1);
-                if (!ok) break;
                 if (isv && mx >= 0x7f800000u) {  // rare: take what is not finite out, and remember the tile
                     float4 y[NX];
 #pragma unroll
@@ -983,6 +984,18 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 const int a = scale_of(mx, isv ? 60 : 100);
                 const float f = pow2(a);
                 const f32x2 f2 = pair(f, f);
+                if (lane == 0) {
+                    float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + w;
+                    sc[0] = isv ? (float)-a : pow2(-a);
+                    if (isv) {
+                        sc[SH::GROUPS] = f;
+                        mbar_arrive(&v_scale[sc_at]);  // the softmax need not wait for the tile itself
+                    }
+                }
+                if (due) hand_over(due);                        // the tile before: its stores are through by now
+                if (t == SH::QTILE) ok = wait_warp(q_full, 0);  // the staged queries' place is written over
+                if (ok && t >= NB) ok = wait_warp(&empty[st], ph ^ 1);
+                if (!ok) break;
                 uint8_t* dst = home + st * 2 * SH::HALF;
 #pragma unroll
                 for (int i = 0; i < NX; ++i) {
@@ -993,11 +1006,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                     uint8_t* d = dst + rr * 128 + (((in_half >> 4) ^ ((w * SH::RPW + rr) & 7)) << 4);
                     *reinterpret_cast<uint2*>(d) = hi;
                     *reinterpret_cast<uint2*>(d + SH::TILE) = lo;
-                }
-                if (lane == 0) {
-                    float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + w;
-                    sc[0] = isv ? (float)-a : pow2(-a);
-                    if (isv) sc[SH::GROUPS] = f;
                 }
                 due = &full[fu];
                 next();
@@ -1071,6 +1079,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 const int a = scale_of(mx, isv ? 60 : 100);
                 const float f = pow2(a);
                 const f32x2 f2 = pair(f, f);
+                if (lane == 0) {
+                    float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + w;
+                    sc[0] = isv ? (float)-a : pow2(-a);
+                    if (isv) {
+                        sc[SH::GROUPS] = f;
+                        mbar_arrive(&v_scale[sc_at]);
+                    }
+                }
 #pragma unroll 1
                 for (int i0 = 0; i0 < ALL; i0 += NC) {
                     load(i0);
@@ -1083,11 +1099,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                     }
 #pragma unroll
                     for (int i = 0; i < NC; ++i) *place(i0 + i) = x[i];
-                }
-                if (lane == 0) {
-                    float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + w;
-                    sc[0] = isv ? (float)-a : pow2(-a);
-                    if (isv) sc[SH::GROUPS] = f;
                 }
             };
 #pragma unroll 1
