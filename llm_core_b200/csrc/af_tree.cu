@@ -158,16 +158,19 @@ __global__ void __launch_bounds__(kTreeThreads) tree_row_kernel(TreeParams p) {
 // launch's 1,024·64.
 //
 // Measured with inputs out of L2, device time: 26 nodes over 4,000 positions, 32
-// heads of 128, f32, 46.5 us (2.8 TB/s of the 132 MB; bound by the splitting
-// warps: each waits, reads, splits and stores its rows in turn, ~3,700 cycles a
-// tile); 16 sequences of 0 to 8,190 positions with 31 nodes, 16/2 heads of 128,
+// heads of 128, f32, 45.2 us (2.9 TB/s of the 132 MB; bound by the splitting
+// warps: each reads, splits and stores its rows in turn, ~2,900 cycles a tile, of
+// which the stores' part 1,850; and ~15,000 cycles before the first tile's
+// products); 16 sequences of 0 to 8,190 positions with 31 nodes, 16/2 heads of 128,
 // f16, 48 us (1.6 TB/s; ~2,900 cycles a tile of 128, the softmax's chain, of
 // which the exponentials fill 1,024 on the special function units, and ~16,000
 // cycles of plan, queries, and sums at both ends); chunks of 509 over up to 16,001
 // positions, 32/4 heads of 64, bf16, 218 us (315 TFLOP/s; the same chain, ~3,100
 // cycles a tile).  Steps that got there: K and V by single bulk copies -> boxes;
 // 4 -> 8 -> 16 softmax warps (chunk 402 -> 333 -> 266 us); tiles of 64 -> 128
-// positions with a power of two per 32 bf16 rows (241 -> 218 us).
+// positions with a power of two per 32 bf16 rows (241 -> 218 us); V's powers of
+// two said before its tile (46.4 -> 45.2 us).  Not taken: two sets of softmax warps
+// that take the tiles in turn (220 us: 66 % of the issue slots are busy already).
 //
 // Tiles in shared memory: rows of 64 values (128 bytes) in the 128-byte
 // swizzle, K-major for K, the same tile MN-major for V; for f32 the TMA engine
