@@ -61,7 +61,8 @@ struct BeamParams {
     float* tops;    // [rows][chunks]
 };
 
-__device__ __forceinline__ u64 logit_key(float v, int token) { return argmax_key(v, (uint32_t)token); }
+// -0 and 0 are one value: v + 0 is never -0.
+__device__ __forceinline__ u64 logit_key(float v, int token) { return argmax_key(v + 0.f, (uint32_t)token); }
 
 __device__ __forceinline__ double warp_sum_d(double v) {
 #pragma unroll
