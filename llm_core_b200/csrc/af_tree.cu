@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_row_kernel(TreeParams p) {
 // a tile of K or V rows — in shared memory.
 //
 // fp32 accuracy out of f16 operands: x·2^a (a power of two that puts the
-// largest of a row, or of the rows of one 512-byte load, in [2^14, 2^15)) is
+// largest of a query, or of 8 rows of f32, 32 of bf16, in [2^14, 2^15)) is
 // split as hi + lo, both f16: 22 bits, and what is lost below is 2^-39 of that
 // largest value.  x·y = hi·hi + hi·lo + lo·hi to 2^-22.  A cache in f16 needs
 // no scale and no lo, one in bf16 a scale and no lo (8 bits in 11).  The
@@ -162,10 +162,10 @@ __global__ void __launch_bounds__(kTreeThreads) tree_row_kernel(TreeParams p) {
 // warps: each reads, splits and stores its rows in turn, ~2,900 cycles a tile, of
 // which the stores' part 1,850; and ~15,000 cycles before the first tile's
 // products); 16 sequences of 0 to 8,190 positions with 31 nodes, 16/2 heads of 128,
-// f16, 48 us (1.6 TB/s; ~2,900 cycles a tile of 128, the softmax's chain, of
+// f16, 47.4 us (1.6 TB/s; ~2,900 cycles a tile of 128, the softmax's chain, of
 // which the exponentials fill 1,024 on the special function units, and ~16,000
 // cycles of plan, queries, and sums at both ends); chunks of 509 over up to 16,001
-// positions, 32/4 heads of 64, bf16, 218 us (315 TFLOP/s; the same chain, ~3,100
+// positions, 32/4 heads of 64, bf16, 220 us (310 TFLOP/s; the same chain, ~3,100
 // cycles a tile).  Steps that got there: K and V by single bulk copies -> boxes;
 // 4 -> 8 -> 16 softmax warps (chunk 402 -> 333 -> 266 us); tiles of 64 -> 128
 // positions with a power of two per 32 bf16 rows (241 -> 218 us); V's powers of
@@ -303,6 +303,7 @@ struct MmaShape {
     static constexpr int SW = F32 ? 8 : 4;              // splitting warps of K, of V
     static constexpr int OUT = 4 * PARTS, SPLIT_K = OUT + 4, SPLIT_V = SPLIT_K + SW;  // first warps
     static_assert(SPLIT_V + SW == kMmaWarp, "warps");
+    static constexpr int QW = TYPE == AF_KV_F16 ? kMmaWarp : OUT + 4;  // warps that bring the queries in: f16 has nothing to split yet
     static constexpr int COLS = T * 128;                // 64 values of every row
     static constexpr int TILE = HD / 64 * COLS;
     static constexpr int HALF = TERMS * TILE;           // K or V of a tile: hi, lo
@@ -531,7 +532,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     uint64_t* c_full = p_full + NS;                      // [NC] softmax warps: correction written
     uint64_t* o_full = c_full + NC;                      // P·V done
     uint64_t* o_free = o_full + 1;                       // output warps: P·V and correction taken
-    uint64_t* q_full = o_free + 1;                       // softmax and output warps: queries written
+    uint64_t* q_full = o_free + 1;                       // QW warps: queries written
     uint64_t* fin = q_full + 1;                          // softmax warps: tops and sums written
     uint64_t* done = fin + 1;                            // everything issued is done: scores, products
     uint64_t* w_empty = done + 1;                        // [NS] P·V done: the weights' place is free
@@ -597,7 +598,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             mbar_init(&w_empty[i], 1);
         }
         mbar_init(o_full, 1);
-        mbar_init(q_full, kOutWarp + 4);
+        mbar_init(q_full, SH::QW);
         mbar_init(done, 2);
         *flag = 0;
     } else if (warp == kMmaWarp) {
@@ -639,11 +640,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     int bs = 0;  // tiles of a bit of bad[]: 1 << bs
     while (nt > (kMmaBadWords * 32) << bs) ++bs;
 
-    // Queries, by the softmax and output warps: a row a warp in turn — its largest value, hi and lo — into the staging
+    // Queries, by QW warps: a row a warp in turn — its largest value, hi and lo — into the staging
     // place, from there a row a thread (hi by softmax warps 0-3, lo by 4-7) into tensor memory.  Rows that are
     // none keep what is there: what comes of them stays in their own row.
     auto queries = [&]() {
-        constexpr int QW = kOutWarp + 4, Q4 = HD / 4, QR = 32 / Q4, QN = (128 / QR + QW - 1) / QW;  // lanes of a row at 16 bytes, rows and number of a warp's loads
+        constexpr int QW = SH::QW, Q4 = HD / 4, QR = 32 / Q4, QN = (128 / QR + QW - 1) / QW;  // lanes of a row at 16 bytes, rows and number of a warp's loads
         const int sub = lane / Q4, col = lane % Q4, rows = row_hi - row_lo;
         const bool wide = ((reinterpret_cast<uintptr_t>(p.q) & 15) | (p.qs & 3)) == 0;
         float4 f[QN];  // all in flight
@@ -924,6 +925,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     } else if (warp < kMmaWarp) {
         // ------------------------------------------------- splitting K and V
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::REG_K));
+        if (TYPE == AF_KV_F16) queries();
         const bool isv = warp >= kSplitWarp + SW;
         const int w = (warp - kSplitWarp) % SW;
         uint64_t *full = isv ? v_full : k_full, *empty = isv ? v_empty : k_empty, *land = isv ? v_land : k_land;
