@@ -165,12 +165,13 @@ __global__ void __launch_bounds__(kTreeThreads) tree_row_kernel(TreeParams p) {
 // f16, 47.4 us (1.6 TB/s; ~2,900 cycles a tile of 128, the softmax's chain, of
 // which the exponentials fill 1,024 on the special function units, and ~16,000
 // cycles of plan, queries, and sums at both ends); chunks of 509 over up to 16,001
-// positions, 32/4 heads of 64, bf16, 220 us (310 TFLOP/s; the same chain, ~3,100
+// positions, 32/4 heads of 64, bf16, 209 us (326 TFLOP/s; the same chain, ~3,100
 // cycles a tile).  Steps that got there: K and V by single bulk copies -> boxes;
 // 4 -> 8 -> 16 softmax warps (chunk 402 -> 333 -> 266 us); tiles of 64 -> 128
 // positions with a power of two per 32 bf16 rows (241 -> 218 us); V's powers of
 // two said before its tile (46.4 -> 45.2 us).  Not taken: two sets of softmax warps
-// that take the tiles in turn (220 us: 66 % of the issue slots are busy already).
+// that take the tiles in turn (220 us where one set took 218: 66 % of the issue slots
+// are busy already).
 //
 // Tiles in shared memory: rows of 64 values (128 bytes) in the 128-byte
 // swizzle, K-major for K, the same tile MN-major for V; for f32 the TMA engine
@@ -319,9 +320,10 @@ struct MmaShape {
     static constexpr int QROW = HD * 4;
     static constexpr int QTILE = NB - (kMmaRows * QROW + 2 * HALF - 1) / (2 * HALF);
     static_assert(QTILE >= 1, "the first tile does not wait for the queries");
-    // registers
-    static constexpr int REG_S = F32 || HD == 64 ? 64 : 56, REG_O = HD == 64 ? 104 : F32 ? 160 : 168,
-                         REG_K = F32 ? 48 : HD == 64 ? 56 : 40, REG_M = F32 && HD == 128 ? 32 : 40;
+    // registers: what does not fit is spilled, where it costs least (16 bits, head_dim 64: 64 for the softmax 220 us of
+    // chunks, 72 taken from the others 209; head_dim 128: 32 for the splitting warps 52 us of the batch, 40 47)
+    static constexpr int REG_S = F32 ? 64 : HD == 64 ? 72 : 56, REG_O = HD == 64 ? F32 ? 104 : 96 : F32 ? 160 : 168,
+                         REG_K = F32 ? 48 : 40, REG_M = F32 && HD == 128 ? 32 : 40;
     static_assert(PARTS * REG_S + REG_O + SW / 2 * REG_K + REG_M <= 8 * 64, "what the launch gives: 1,024 threads of 64");
     // tensor memory columns
     static constexpr int QH = 0, QL = HD / 2, S0 = HD, O0 = HD + NS * T;
