@@ -236,7 +236,12 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_segment_kernel
             __syncthreads();
             thr = lowest();
         }
-        auto keep = [&](int j) { sh.key[atomicAdd(&sh.count, 1)] = logit_key(v[j], token(t0, j)); };
+        bool full = false;  // this thread's last key came behind kBeamFull others
+        auto keep = [&](int j) {
+            const int at = atomicAdd(&sh.count, 1);
+            sh.key[at] = logit_key(v[j], token(t0, j));
+            full = at >= kBeamFull;
+        };
         if (begin) {
             if (big >= thr) {
 #pragma unroll
@@ -253,8 +258,9 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamBlocks) beam_segment_kernel
             }
         }
         if (t0 + 2 * kBeamStep < hi) load(t0 + 2 * kBeamStep, v);
-        // at most a step's keys came on top of at most kBeamFull
-        if (__syncthreads_or(tid == 0 && sh.count > kBeamFull)) {
+        // Whoever added the last key knows that it was one too many; the count itself may still grow when another looks.
+        // So at most a step's keys come on top of at most kBeamFull.
+        if (__syncthreads_or(full)) {
             beam_cut(sh, K);
             thr = fmaxf(thr, ordered_to_float((uint32_t)(sh.key[K - 1] >> 32)));
             __syncthreads();
