@@ -1528,6 +1528,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2) tree_small_kernel(TreeParams
 struct TreePlan {
     bool mma, small;
     long long max_len;
+    int nodes;          // of a sequence, at most: max_nodes may be far above the call's rows
     int blocks, slots;  // slots 0: nothing is split, no second launch
     size_t ws;
 };
@@ -1542,9 +1543,9 @@ constexpr int kSmallFill = 2 * kTreeSms;  // blocks up to which a small call's i
 // and 1,000 positions 5.9 / 11.9 and 11.6 / 14.7 µs; 16 sequences of 250 8.1 /
 // 15.3, of 1,000 20.4 / 19.8; 16 rows each of 250 40 / 18.  16 sequences with 32
 // kv heads of 128, a row each of 137: 19.7 / 45.5, of 1,000 95 / 98.
-bool small_call(const af_attention_tree_args& a, long long max_len) {
+bool small_call(const af_attention_tree_args& a, int nodes, long long max_len) {
     const bool f32 = a.kv.type == AF_KV_F32, narrow = a.kv.head_dim == 64;
-    const long long rows = (long long)a.batch.max_nodes * (a.n_heads / a.kv.n_kv_heads), heads = (long long)a.batch.n_seq * a.kv.n_kv_heads;
+    const long long rows = (long long)nodes * (a.n_heads / a.kv.n_kv_heads), heads = (long long)a.batch.n_seq * a.kv.n_kv_heads;
     const long long items = (rows + kSmallRows - 1) / kSmallRows * heads, tiles = (max_len + kSmallTile - 1) / kSmallTile;
     const double each = narrow || items >= kSmallFill ? 1.2 : 2.2;
     const double small = 5. + std::max(each * (double)items * (double)tiles / kTreeSms, (narrow ? 1.6 : 2.4) * (double)((tiles + 7) / 8));
@@ -1561,15 +1562,21 @@ TreePlan tree_plan(const af_attention_tree_args& a) {
     const long long cap = (long long)a.batch.max_blocks * a.kv.page_size;
     const long long max_len = a.max_len > 0 ? std::min((long long)a.max_len, cap) : cap;
     pl.max_len = max_len;
-    pl.small = small_call(a, max_len);
+    pl.nodes = std::max(1, std::min(a.batch.max_nodes, a.n_rows));
+    pl.small = small_call(a, pl.nodes, max_len);
     // the workspace does not ask which kernel: it grows with every size, so one for the largest call serves smaller
     // ones, which may go to the other kernel
     const int T = tree_tile(a.kv.type);
     const long long tiles = (max_len + T - 1) / T, most = (tiles + kTreeMinTiles - 1) / kTreeMinTiles;
-    const long long items = ((long long)a.batch.max_nodes * G + kMmaRows - 1) / kMmaRows * a.kv.n_kv_heads * a.batch.n_seq;
-    const long long split = items <= kTreeItems ? (items + kTreeSms - 1) / kTreeSms * kTreeSms : items + 2 * kTreeItems;
-    pl.blocks = (int)std::min({split, items * std::max(1ll, most), (long long)INT_MAX});
-    if (most > 1) pl.slots = (int)std::min((long long)pl.blocks, 2ll * kTreeItems);
+    auto blocks = [&](long long items) {
+        const long long split = items <= kTreeItems ? (items + kTreeSms - 1) / kTreeSms * kTreeSms : items + 2 * kTreeItems;
+        return std::min({split, items * std::max(1ll, most), (long long)INT_MAX});
+    };
+    const long long n_seq = a.batch.n_seq, kv = a.kv.n_kv_heads;
+    auto items = [&](long long nodes) { return (nodes * G + kMmaRows - 1) / kMmaRows * n_seq; };  // of a kv head
+    // the launch also knows the call's rows, of which a sequence leaves one item partly filled
+    pl.blocks = (int)blocks(std::min(items(pl.nodes), (long long)a.n_rows * G / kMmaRows + n_seq) * kv);
+    if (most > 1) pl.slots = (int)std::min(blocks(items(a.batch.max_nodes) * kv), 2ll * kTreeItems);
     if (pl.slots) pl.ws = (size_t)pl.slots * kMmaRows * (hd + 2) * sizeof(float) + (size_t)a.batch.n_seq * sizeof(int2);
     return pl;
 }
@@ -1604,7 +1611,7 @@ bool tree_map(CUtensorMap* map, const TreeParams& p, int type, uint8_t* pool, in
 }
 
 template <int TYPE, int HD>
-cudaError_t mma_launch(const MmaParams& mp, int n_seq, int max_nodes, cudaStream_t st) {
+cudaError_t mma_launch(const MmaParams& mp, int n_seq, int nodes, cudaStream_t st) {
     constexpr int smem = MmaShape<TYPE, HD>::BYTES;
     AF_CUDA_TRY(cudaFuncSetAttribute(tree_mma_kernel<TYPE, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     tree_mma_kernel<TYPE, HD><<<mp.blocks, kMmaThreads, smem, st>>>(mp);
@@ -1614,7 +1621,7 @@ cudaError_t mma_launch(const MmaParams& mp, int n_seq, int max_nodes, cudaStream
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(((long long)max_nodes * mp.t.H + 7) / 8), n_seq);
+    cfg.gridDim = dim3((unsigned)(((long long)nodes * mp.t.H + 7) / 8), n_seq);
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cfg.attrs = attr;
@@ -1623,11 +1630,11 @@ cudaError_t mma_launch(const MmaParams& mp, int n_seq, int max_nodes, cudaStream
 }
 
 template <int TYPE, int HD>
-cudaError_t small_launch(const TreeParams& p, int max_nodes, long long max_len, cudaStream_t st) {
+cudaError_t small_launch(const TreeParams& p, int nodes, long long max_len, cudaStream_t st) {
     constexpr int smem = SmallShape<HD>::BYTES;
     AF_CUDA_TRY(cudaFuncSetAttribute(tree_small_kernel<TYPE, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     // as many blocks a cluster (a power of two up to 8) as keep the SMs at most twice filled
-    const long long tiles = (max_nodes * p.G + kSmallRows - 1) / kSmallRows, items = tiles * p.b.n_seq * p.kv.kv_heads;
+    const long long tiles = (nodes * p.G + kSmallRows - 1) / kSmallRows, items = tiles * p.b.n_seq * p.kv.kv_heads;
     int blocks = 1;
     while (blocks < 8 && 2 * blocks * items <= kSmallFill && blocks * kSmallTile < max_len) blocks *= 2;
     cudaLaunchAttribute attr[1];
@@ -1644,9 +1651,9 @@ cudaError_t small_launch(const TreeParams& p, int max_nodes, long long max_len, 
 }
 
 template <int TYPE>
-cudaError_t tree_launch(const TreeParams& p, const TreePlan& pl, int max_nodes, void* ws, cudaStream_t st) {
-    if (pl.small) return p.kv.hd == 64 ? small_launch<TYPE, 64>(p, max_nodes, pl.max_len, st)
-                                           : small_launch<TYPE, 128>(p, max_nodes, pl.max_len, st);
+cudaError_t tree_launch(const TreeParams& p, const TreePlan& pl, void* ws, cudaStream_t st) {
+    if (pl.small) return p.kv.hd == 64 ? small_launch<TYPE, 64>(p, pl.nodes, pl.max_len, st)
+                                       : small_launch<TYPE, 128>(p, pl.nodes, pl.max_len, st);
     if (pl.mma) {
         MmaParams mp = {};
         mp.t = p;
@@ -1659,7 +1666,7 @@ cudaError_t tree_launch(const TreeParams& p, const TreePlan& pl, int max_nodes, 
             return cudaErrorInvalidValue;
         }
         if (pl.slots) mp.plan = reinterpret_cast<int2*>(mp.part + (size_t)pl.slots * kMmaRows * (p.kv.hd + 2));
-        return p.kv.hd == 64 ? mma_launch<TYPE, 64>(mp, p.b.n_seq, max_nodes, st) : mma_launch<TYPE, 128>(mp, p.b.n_seq, max_nodes, st);
+        return p.kv.hd == 64 ? mma_launch<TYPE, 64>(mp, p.b.n_seq, pl.nodes, st) : mma_launch<TYPE, 128>(mp, p.b.n_seq, pl.nodes, st);
     }
     tree_row_kernel<TYPE><<<dim3(p.n_rows, p.H), kTreeThreads, 0, st>>>(p);
     return cudaGetLastError();
@@ -1675,6 +1682,9 @@ std::string tree_wrong(const af_attention_tree_args& a) {
     if (a.max_len < 0) return "max_len must not be negative";
     const long long G = a.n_heads / a.kv.n_kv_heads;
     if (a.batch.max_nodes * G > (1ll << 31) / G) return "max_nodes times the square of n_heads / n_kv_heads must be at most 2^31";
+    const bool mma = a.kv.head_dim == 64 || a.kv.head_dim == 128;  // its merge numbers rows and heads with 32 bits
+    if (mma && (long long)std::min(a.batch.max_nodes, a.n_rows) * a.n_heads > INT_MAX - 8)
+        return "n_rows times n_heads must be below 2^31";
     if (a.mask && (a.mask_words <= 0 || (long long)a.mask_words * 64 < a.batch.max_nodes))
         return "mask_words must cover max_nodes";
     const long long qd = (long long)a.n_heads * a.kv.head_dim;
@@ -1724,8 +1734,8 @@ extern "C" cudaError_t af_attention_tree_f32(const af_attention_tree_args* a, cu
     p.mask_words = a->mask_words;
     p.scale = (a->scale != 0.f ? a->scale : 1.f / std::sqrt((float)a->kv.head_dim)) * 1.4426950408889634f;
     switch (a->kv.type) {
-        case AF_KV_F32: return tree_launch<AF_KV_F32>(p, pl, a->batch.max_nodes, a->ws, stream);
-        case AF_KV_F16: return tree_launch<AF_KV_F16>(p, pl, a->batch.max_nodes, a->ws, stream);
-        default: return tree_launch<AF_KV_BF16>(p, pl, a->batch.max_nodes, a->ws, stream);
+        case AF_KV_F32: return tree_launch<AF_KV_F32>(p, pl, a->ws, stream);
+        case AF_KV_F16: return tree_launch<AF_KV_F16>(p, pl, a->ws, stream);
+        default: return tree_launch<AF_KV_BF16>(p, pl, a->ws, stream);
     }
 }

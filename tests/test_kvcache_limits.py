@@ -1,0 +1,27 @@
+"""Limits of the cache and tree-attention entries that need no device."""
+import ctypes as C
+
+from llm_core_b200 import _lib
+from test_kvcache_abi import attention, batch, cache
+
+
+def test_rows_that_the_merge_cannot_number_are_refused():
+    lib = _lib.load()
+    big = batch(max_nodes=1 << 30)
+    a = attention(kv=cache(n_kv_heads=4), batch=big, n_heads=4, n_rows=1 << 30)
+    assert lib.af_attention_tree_f32(C.byref(a), None) != 0
+    assert b"2^31" in lib.af_last_error()
+    # a limit alone is none: the call has 2 rows, and fails for its workspace only
+    a = attention(kv=cache(n_kv_heads=4, n_pages=4096), batch=batch(max_nodes=1 << 30, max_blocks=4096), n_heads=4, n_rows=2)
+    size = lib.af_attention_tree_f32_workspace(C.byref(a))
+    assert 0 < size < 1 << 28
+    assert lib.af_attention_tree_f32(C.byref(a), None) != 0
+    assert b"ws must hold" in lib.af_last_error()
+
+
+def test_the_workspace_does_not_follow_the_rows():
+    """One workspace serves calls of fewer rows and of more, up to the limits it was asked for with."""
+    lib = _lib.load()
+    sizes = {lib.af_attention_tree_f32_workspace(C.byref(attention(
+        kv=cache(n_pages=4096), batch=batch(max_nodes=500, max_blocks=4096), n_rows=n))) for n in (0, 1, 7, 500)}
+    assert len(sizes) == 1 and sizes.pop() > 0
