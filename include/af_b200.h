@@ -376,9 +376,10 @@ cudaError_t af_beam_select_f32(const af_beam_select_args* args, cudaStream_t str
  * count too and stay.  table_out and len_out may not overlap the inputs.
  * Where pages run out, or max_blocks would be passed, entries stay -1,
  * len_out[i] falls to the last whole page if its partly filled page is
- * missing, and *n_short (device) is the number of pages missing, else 0.
- * n_in, n_out <= 4096.  ws: af_kv_fork_workspace bytes, zeroed before its
- * first use; calls that may overlap need workspaces of their own. */
+ * missing, and *n_short (device) is the number of pages missing (at most
+ * 2^31-1), else 0.  n_in, n_out <= 4096, n_out * max_blocks < 2^31.  ws:
+ * af_kv_fork_workspace bytes, zeroed before its first use; calls that may
+ * overlap need workspaces of their own. */
 typedef struct {
     af_kv_cache kv;
     const int32_t* table_in;

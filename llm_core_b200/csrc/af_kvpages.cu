@@ -337,7 +337,8 @@ __global__ void __launch_bounds__(kForkThreads) kv_fork_kernel(ForkParams p) {
     ForkNeed* needs = reinterpret_cast<ForkNeed*>(sm);        // [n_out]
     int* eldest = reinterpret_cast<int*>(needs + kForkMax);  // [n_in]
     __shared__ int wsum[32];
-    __shared__ int s_total, s_missing;
+    __shared__ int s_total;
+    __shared__ unsigned long long s_missing;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_pages = p.kv.n_pages, nb = p.in.max_blocks;
     const bool in_place = p.ref_out == p.ref_in;
     const int* ref = in_place ? p.before : p.ref_in;  // the counts as they came
@@ -361,7 +362,7 @@ __global__ void __launch_bounds__(kForkThreads) kv_fork_kernel(ForkParams p) {
         if (n.parent >= 0) atomicMin(&eldest[j], i);
         const long long blocks = ((long long)n.len + more + (1 << p.kv.ps_shift) - 1) >> p.kv.ps_shift;
         n.need = (int)min(blocks, (long long)nb);
-        if (blocks > n.need) atomicAdd(&s_missing, (int)min(blocks - n.need, (long long)INT_MAX));
+        if (blocks > n.need) atomicAdd(&s_missing, (unsigned long long)(blocks - n.need));
         needs[i] = n;
     }
     // the counts, where they go
@@ -481,9 +482,9 @@ __global__ void __launch_bounds__(kForkThreads) kv_fork_kernel(ForkParams p) {
         }
     }
     missing = __reduce_add_sync(0xffffffffu, missing);
-    if (lane == 0 && missing) atomicAdd(&s_missing, missing);
+    if (lane == 0 && missing) atomicAdd(&s_missing, (unsigned long long)missing);
     __syncthreads();
-    if (tid == 0) *p.n_short = s_missing;
+    if (tid == 0) *p.n_short = (int)min(s_missing, (unsigned long long)INT_MAX);
 }
 
 constexpr int kCopyThreads = 256;
@@ -599,6 +600,7 @@ std::string fork_wrong(const af_kv_fork_args& a) {
     if (a.n_in < 0 || a.n_in > kForkMax || a.n_out < 0 || a.n_out > kForkMax) return "n_in and n_out must be in 0..4096";
     if (a.max_blocks <= 0 || (long long)a.max_blocks * a.kv.page_size > (1ll << 30))
         return "max_blocks must be positive and max_blocks * page_size at most 2^30";
+    if ((long long)a.n_out * a.max_blocks > INT_MAX) return "n_out * max_blocks must be below 2^31";
     if (!a.ref_in || !a.ref_out || !a.n_short) return "null ref_in, ref_out or n_short";
     if (a.n_in > 0 && (!a.table_in || !a.len_in)) return "null table_in or len_in";
     if (a.n_out > 0 && (!a.table_out || !a.len_out || !a.parent)) return "null table_out, len_out or parent";

@@ -2,7 +2,7 @@
 import ctypes as C
 
 from llm_core_b200 import _lib
-from test_kvcache_abi import attention, batch, cache
+from test_kvcache_abi import attention, batch, cache, fork
 
 
 def test_rows_that_the_merge_cannot_number_are_refused():
@@ -25,3 +25,10 @@ def test_the_workspace_does_not_follow_the_rows():
     sizes = {lib.af_attention_tree_f32_workspace(C.byref(attention(
         kv=cache(n_pages=4096), batch=batch(max_nodes=500, max_blocks=4096), n_rows=n))) for n in (0, 1, 7, 500)}
     assert len(sizes) == 1 and sizes.pop() > 0
+
+
+def test_fork_tables_of_more_entries_than_32_bits_number_are_refused():
+    lib = _lib.load()
+    a = fork(n_out=4096, max_blocks=1 << 20)
+    assert lib.af_kv_fork(C.byref(a), None) != 0
+    assert b"n_out * max_blocks" in lib.af_last_error()
