@@ -374,6 +374,10 @@ cudaError_t af_beam_select_f32(const af_beam_select_args* args, cudaStream_t str
  * ref_in / ref_out [n_pages] count the table entries that hold a page (0 =
  * free); ref_out may be ref_in.  Entries of other tables that share the pool
  * count too and stay.  table_out and len_out may not overlap the inputs.
+ * An entry of table_in that is neither -1 nor a page of the pool, and a
+ * position below its length that a parent holds no page for, set the device
+ * error word: such an entry counts as -1, and len_out[i] falls to the whole
+ * pages in front of the first such position.
  * Where pages run out, or max_blocks would be passed, entries stay -1,
  * len_out[i] falls to the last whole page if its partly filled page is
  * missing, and *n_short (device) is the number of pages missing (at most

@@ -447,8 +447,9 @@ __global__ void __launch_bounds__(kForkThreads) kv_fork_kernel(ForkParams p) {
     const int avail = min(found, total);
     // one off for every entry of the inputs
     for (long long e = tid; e < (long long)p.in.n_seq * nb; e += kForkThreads) {
-        const int page = kv_page(p.in, n_pages, (int)(e / nb), (int)(e % nb));
-        if (page >= 0) atomicSub(&p.ref_out[page], 1);
+        const int page = p.in.table[e];
+        if (page >= 0 && page < n_pages) atomicSub(&p.ref_out[page], 1);
+        else if (page != -1) set_err_at(p.in.err, kErrBadArgs);  // nobody's page
     }
     int missing = 0;
     for (int i = warp; i < p.n_out; i += kForkThreads / 32) {
@@ -474,7 +475,13 @@ __global__ void __launch_bounds__(kForkThreads) kv_fork_kernel(ForkParams p) {
             if (page >= 0) atomicAdd(&p.ref_out[page], 1);
             // the partly filled page
             if (b == full && b < nb) p.copies[i] = make_int4(old, page, take && page >= 0 && old >= 0 ? rows : 0, 0);
-            if (__any_sync(0xffffffffu, b == full && rows > 0 && page < 0)) len = full << p.kv.ps_shift;
+            if (__any_sync(0xffffffffu, b == full && rows > 0 && page < 0)) len = min(len, full << p.kv.ps_shift);
+            // a position below the length that the parent holds no page for: the child ends in front of it
+            const unsigned hole = __ballot_sync(0xffffffffu, b < full + (rows > 0) && old < 0);
+            if (hole) {
+                len = min(len, (b0 + __ffs(hole) - 1) << p.kv.ps_shift);
+                set_err_at(p.in.err, kErrBadArgs);
+            }
         }
         if (lane == 0) {
             if (full >= nb) p.copies[i] = make_int4(-1, -1, 0, 0);
