@@ -344,8 +344,10 @@ cudaError_t af_attention_tree_f32(const af_attention_tree_args* args, cudaStream
  * out_beam is the logits row, so that it serves as af_kv_fork's parent.  A
  * beam whose score is -inf or NaN, or whose logits hold NaN or +inf or nothing
  * above -inf, scores -inf throughout.  n_out <= 64 and <= n_beams*vocab,
- * n_beams <= 64, n_beams * ceil(vocab / 8192) <= 1024.  ws:
- * af_beam_select_f32_workspace bytes, zeroed before its first use; calls that may overlap need workspaces of their own. */
+ * n_beams <= 64, n_seq*n_beams <= 65535, n_beams * ceil(vocab / 8192) <= 1024.
+ * ws: af_beam_select_f32_workspace bytes, enough for every call with no more
+ * rows (n_seq*n_beams), vocab and n_out, zeroed before its first use; calls
+ * that may overlap need workspaces of their own. */
 typedef struct {
     const float* logits;
     int64_t logits_stride;

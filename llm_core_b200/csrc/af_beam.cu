@@ -466,15 +466,20 @@ std::string beam_wrong(const af_beam_select_args& a) {
     return "";
 }
 
+constexpr int kBeamFill = kBeamBlocks * 148;  // blocks that the SMs hold at once
+
+int beam_most(int vocab) { return (int)(((long long)vocab + kBeamChunk - 1) / kBeamChunk); }
+
 // Segments of a row: as many blocks as the SMs hold at once, none below kBeamChunk logits.
 int beam_segments(const af_beam_select_args& a) {
-    const int most = (a.vocab + kBeamChunk - 1) / kBeamChunk;
     const long long rows = std::max(1ll, (long long)a.n_seq * a.n_beams);
-    return (int)std::min((long long)most, std::max(1ll, kBeamBlocks * 148 / rows));
+    return (int)std::min((long long)beam_most(a.vocab), std::max(1ll, kBeamFill / rows));
 }
 
+// Fewer rows have more segments each: room for the most lists that any number of rows up to this one makes.
 size_t beam_ws(const af_beam_select_args& a) {
-    const size_t lists = (size_t)a.n_seq * a.n_beams * beam_segments(a);
+    const size_t rows = (size_t)a.n_seq * a.n_beams;
+    const size_t lists = std::min(rows * beam_most(a.vocab), std::max(rows, (size_t)kBeamFill));
     return lists * ((size_t)a.n_out * 8 + 16);
 }
 

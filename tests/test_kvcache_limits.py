@@ -2,7 +2,7 @@
 import ctypes as C
 
 from llm_core_b200 import _lib
-from test_kvcache_abi import attention, batch, cache, fork
+from test_kvcache_abi import attention, batch, beam, cache, fork
 
 
 def test_rows_that_the_merge_cannot_number_are_refused():
@@ -32,3 +32,21 @@ def test_fork_tables_of_more_entries_than_32_bits_number_are_refused():
     a = fork(n_out=4096, max_blocks=1 << 20)
     assert lib.af_kv_fork(C.byref(a), None) != 0
     assert b"n_out * max_blocks" in lib.af_last_error()
+
+
+def test_a_beam_workspace_serves_every_smaller_call():
+    """Also one of fewer rows, which have more segments each: a search whose beams die."""
+    lib = _lib.load()
+
+    def size(n_seq, n_beams, vocab, n_out):
+        return lib.af_beam_select_f32_workspace(C.byref(beam(n_seq=n_seq, n_beams=n_beams, vocab=vocab, n_out=n_out)))
+
+    for n_seq, n_beams, vocab in ((1, 32, 151936), (1, 64, 100000), (16, 8, 151936), (5, 7, 40000), (500, 2, 30000)):
+        most = size(n_seq, n_beams, vocab, 64)
+        for s in {1, (n_seq + 1) // 2, n_seq}:
+            for b in range(1, n_beams + 1):
+                for v in (64, 8192, 8193, vocab // 2, vocab):
+                    # as many lists of n_out keys, a sum and a maximum as the rows have segments
+                    rows, k = s * b, 64
+                    segments = min(-(-v // 8192), max(1, 444 // rows))
+                    assert rows * segments * (8 * k + 16) <= size(s, b, v, k) <= most
