@@ -315,7 +315,8 @@ cudaError_t af_kv_store_f32(const af_kv_store_args* args, cudaStream_t stream);
  * launch; 0 = max_blocks*page_size).  ws: af_attention_tree_f32_workspace
  * bytes, enough for every call with no more sequences, nodes and positions,
  * zeroed before its first use and left ready for the next; calls that may
- * overlap on the GPU need workspaces of their own.  n_heads is at most 65535,
+ * overlap on the GPU need workspaces of their own.  n_heads is at most 65535, a
+ * sequence has at most 1,048,448 nodes where head_dim is 64 or 128, and
  * max_nodes times the square of n_heads/n_kv_heads at most 2^31, n_rows (or
  * max_nodes, if that is less) times n_heads below 2^31 where head_dim is 64 or
  * 128. */

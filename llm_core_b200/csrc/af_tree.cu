@@ -14,6 +14,7 @@
 #include <climits>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "af_kvpages.cuh"
 #include "af_ops.cuh"
@@ -281,9 +282,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // The power of two for values whose largest has these bits: max·2^a in
-// [2^14, 2^15), a within [-113, top]; 0 for an infinity or NaN.
+// [2^14, 2^15), a within [-113, top]; -113 beside an infinity or NaN, which no other value then joins.
 __device__ __forceinline__ int scale_of(uint32_t max_bits, int top) {
-    if (max_bits >= 0x7f800000u) return 0;
+    if (max_bits >= 0x7f800000u) return -113;
     return min(top, 14 - ((int)(max_bits >> 23) - 127));
 }
 __device__ __forceinline__ float pow2(int a) { return __int_as_float((a + 127) << 23); }
@@ -293,6 +294,7 @@ constexpr int kMmaWarp = 28, kCopyWarp = 29, kScoreWarp = 31;  // copies of K, o
 constexpr int kMmaRows = 128;
 constexpr int tree_tile(int type) { return type == AF_KV_F32 ? 64 : 128; }  // positions of a tile
 constexpr int kMmaBadWords = 512;  // tiles of a split whose V holds something non-finite, a bit each
+constexpr int kMmaMaxNodes = (1 << 20) - 128;  // of a sequence, so that every group of them has a bit (APART)
 
 template <int TYPE, int HD>
 struct MmaShape {
@@ -330,10 +332,13 @@ struct MmaShape {
     static_assert(O0 + HD <= 512, "tensor memory");
     // shared memory, behind 768 bytes of mbarriers
     static constexpr int BAD = 768;                       // kMmaBadWords words
-    static constexpr int ROWS = BAD + kMmaBadWords * 4;   // [128] query scales, [NC][128] corrections, [2][PARTS][128] exchange, [128] tops, [PARTS][128] sums
     static constexpr int GROUPS = T / RPW;
-    static constexpr int SCALE = ROWS + (2 + NC + 3 * PARTS) * kMmaRows * 4;  // [RING][3][GROUPS] floats
-    static constexpr int TILES = (SCALE + RING * 3 * GROUPS * 4 + 1023) / 1024 * 1024;
+    static constexpr int APART_WORDS = TYPE == AF_KV_F16 ? 0 : (1 << 20) / RPW / 32;
+    static constexpr int APART = BAD + kMmaBadWords * 4;  // groups with nodes that are left to the output warps, a bit each
+    static constexpr int ROWS = APART + APART_WORDS * 4;  // [128] query scales, [NC][128] corrections, [2][PARTS][128] exchange, [128] tops, [PARTS][128] sums
+    static_assert(APART % 16 == 0 && ROWS % 16 == 0, "read 16 bytes at a time");
+    static constexpr int SCALE = ROWS + (2 + NC + 3 * PARTS) * kMmaRows * 4;  // [RING][4][GROUPS] floats: 2^-a of K; -a, 2^a of V; 0 of K
+    static constexpr int TILES = (SCALE + RING * 4 * GROUPS * 4 + 1023) / 1024 * 1024;
     static constexpr int RAW = TILES + NB * 2 * HALF;
     static constexpr int BYTES = RAW + (F32 ? 4 * RAWB : 0);  // K, K, V, V
     static_assert(BYTES <= 227 * 1024 - 128, "shared memory");
@@ -362,6 +367,18 @@ __device__ __noinline__ uint32_t clean(float4 (&x)[N]) {
         }
     }
     return __reduce_max_sync(0xffffffffu, b);
+}
+
+// Nodes are not seen by every row, so what one holds must not cost its neighbours their bits.  Whether the rows of a
+// group with nodes may differ too much to share a power of two: `mx` is the group's largest value, `low` the smallest
+// largest value of any 16 bytes that hold something (bits, less 1: zeros are all ones).  2^-39 of mx is lost, 2^-27 of
+// values 2^12 below.  Such a group is left out of the products (its -a of V, or what stands beside K's power of two, is
+// -inf, so that no row gives it a weight) and added position by position in the end.  Looking costs 4 to 10 % where all
+// tiles have nodes (500 tokens, bf16: 32/4 heads of 64 19.8 -> 20.8 us, 16/2 of 128 25.9 -> 28.0) and 1 % of a tree over
+// 3,989 positions.  Not taken: a power of two per row, which the softmax then has to take apart (chunk 209 -> 222 us).
+__device__ __forceinline__ bool rows_differ(uint32_t mx, uint32_t low) {
+    low = __reduce_min_sync(0xffffffffu, low);
+    return mx >= 0x7f800000u || (low != 0xffffffffu && (mx >> 23) > ((low + 1u) >> 23) + 12);
 }
 
 // Work: an item is 128 rows of a sequence with one kv head, its tiles split
@@ -508,6 +525,60 @@ __device__ __forceinline__ unsigned long long tree_window(const TreeParams& p, i
     return (w & ones(len + n - p0)) | ones(len - p0);
 }
 
+// Groups whose nodes differ too much (rows_differ), position by position on the f32 units, as the softmax would have had
+// them: `mine` holds the row's sums (columns as staged_at has them, by turn), m and *l their maximum and sum of weights.
+// Ends with what the row's place is to hold.
+template <int TYPE, int HD>
+__device__ __noinline__ float add_apart(const MmaParams& mp, const TreeSpot& spot, const uint32_t* apart, int end, int row, int head,
+                                        float4* mine, int turn, float m, float* l) {
+    using SH = MmaShape<TYPE, HD>;
+    using E = KvElem<TYPE>;
+    const TreeParams& p = mp.t;
+    const int tiles = (end + SH::T - 1) / SH::T, n = spot.n, len = spot.len, node = row - spot.r0;
+    const int t0 = (int)((long long)tiles * spot.split / spot.splits), t1 = (int)((long long)tiles * (spot.split + 1) / spot.splits);
+    const int first = max(t0, len / SH::T);  // tile with nodes
+    const float* q = p.q + (long long)row * p.qs + (long long)head * HD;
+    float sum = *l;
+    for (int g = 0; g < (t1 - first) * SH::GROUPS; ++g) {
+        if (!((apart[g >> 5] >> (g & 31)) & 1)) continue;
+        const int p0 = first * SH::T + g * SH::RPW;
+        for (int pos = p0; pos < min(p0 + SH::RPW, end); ++pos) {
+            if (!(tree_window(p, row, node, n, len, pos) & 1)) continue;
+            const long long at = kv_row(p.kv, p.b, spot.seq, pos);
+            if (at < 0) continue;
+            const long long from = p.layer * p.kv.layer_bytes + at + (long long)spot.kvh * HD * SH::SIZE;
+            const auto* kr = reinterpret_cast<const typename E::T*>(p.kv.k + from);
+            const auto* vr = reinterpret_cast<const typename E::T*>(p.kv.v + from);
+            float s = 0.f;
+#pragma unroll 8
+            for (int d = 0; d < HD; ++d) s = fmaf(q[d], E::load(kr[d]), s);
+            s *= p.scale;
+            // (the sums may hold infinities already, which no factor may turn into NaN)
+            const float mn = fmaxf(m, s), c = fmaxf(ex2(m - mn), __int_as_float(1)), w = ex2(s - mn + 14.f);
+            m = mn;
+            sum = fmaf(sum, c, w);
+            auto v = [&](int d) {
+                const float x = E::load(vr[d]);
+                return fabsf(x) < INFINITY ? x : 0.f;
+            };
+#pragma unroll 2
+            for (int d = 0; d < HD; d += 4) {
+                float4 f = mine[(d >> 2) ^ turn];
+                f.x = fmaf(w, v(d), f.x * c), f.y = fmaf(w, v(d + 1), f.y * c);
+                f.z = fmaf(w, v(d + 2), f.z * c), f.w = fmaf(w, v(d + 3), f.w * c);
+                mine[(d >> 2) ^ turn] = f;
+            }
+        }
+    }
+    *l = sum;
+    const float inv = spot.splits > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+    for (int d = 0; d < HD / 4; ++d) {
+        const float4 f = mine[d];
+        mine[d] = make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
+    }
+    return m;
+}
+
 template <int TYPE, int HD>
 __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_constant__ MmaParams mp) {
     using SH = MmaShape<TYPE, HD>;
@@ -542,7 +613,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
     static_assert((2 * RING + 5 * NB + 3 * NS + NC + 9) * 8 + 16 <= SH::BAD, "barriers");
     uint32_t* tslot = reinterpret_cast<uint32_t*>(v_scale + RING);
     volatile int* flag = reinterpret_cast<volatile int*>(tslot + 1);
+    int* any_apart = reinterpret_cast<int*>(tslot + 2);  // whether apart[] has a bit set
     uint32_t* bad = reinterpret_cast<uint32_t*>(sm + SH::BAD);
+    uint32_t* apart = reinterpret_cast<uint32_t*>(sm + SH::APART);
     float* s_rs = reinterpret_cast<float*>(sm + SH::ROWS);
     float* s_corr = s_rs + kMmaRows;
     float* s_other = s_corr + NC * kMmaRows;
@@ -603,6 +676,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         mbar_init(q_full, SH::QW);
         mbar_init(done, 2);
         *flag = 0;
+        *any_apart = 0;
     } else if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(512u)
                      : "memory");
@@ -611,7 +685,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         asm volatile("prefetch.tensormap [%0];" ::"l"(&mp.k_map) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&mp.v_map) : "memory");
     }
-    for (int i = tid; i < kMmaBadWords; i += kMmaThreads) bad[i] = 0;
+    for (int i = tid; i < kMmaBadWords + SH::APART_WORDS; i += kMmaThreads) bad[i] = 0;  // and apart[], behind it
     __syncthreads();
     const int seq = spot.seq, kvh = spot.kvh, r0 = spot.r0, n = spot.n, len = spot.len;
     // the block's rows and tiles (the same in every thread)
@@ -739,12 +813,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
 #pragma unroll
             for (int i = 0; i < C; ++i) asm volatile("" : "+f"(v[i]));  // no use may move above the wait
             // f32: a power of two per 8 columns; bf16: one for the thread's 32, taken care of in the exponent
-            const float* sc = scales + kt * 3 * SH::GROUPS + part * (C / SH::RPW);  // 2^-a of K, -a of V, 2^a of V
+            const float* sc = scales + kt * 4 * SH::GROUPS + part * (C / SH::RPW);  // 2^-a of K, -a of V, 2^a of V, 0 of K
             float scale = rs, shift = 0.f, share = 1.f;
-            if (TYPE == AF_KV_BF16) scale = fmaxf(rs * sc[0], FLT_MIN), shift = sc[SH::GROUPS], share = sc[2 * SH::GROUPS];
+            if (TYPE == AF_KV_BF16) scale = fmaxf(rs * sc[0], FLT_MIN), shift = sc[SH::GROUPS] + sc[3 * SH::GROUPS], share = sc[2 * SH::GROUPS];
             if (SH::F32) {
-                const float4 x = *reinterpret_cast<const float4*>(sc), z = *reinterpret_cast<const float4*>(sc + SH::GROUPS);
-                const float c[4] = {rs * x.x, rs * x.y, rs * x.z, rs * x.w}, f[4] = {z.x, z.y, z.z, z.w};
+                const float4 x = *reinterpret_cast<const float4*>(sc), z = *reinterpret_cast<const float4*>(sc + SH::GROUPS),
+                             y = *reinterpret_cast<const float4*>(sc + 3 * SH::GROUPS);
+                const float c[4] = {rs * x.x, rs * x.y, rs * x.z, rs * x.w}, f[4] = {z.x + y.x, z.y + y.y, z.z + y.z, z.w + y.w};
 #pragma unroll
                 for (int e = 0; e < C; e += 2)
                     unpair(fma2(pair(v[e], v[e + 1]), pair(c[e / 8], c[e / 8]), pair(f[e / 8], f[e / 8])), v[e], v[e + 1]);
@@ -892,11 +967,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
             float l = 0.f;
 #pragma unroll
             for (int i = 0; i < PARTS; ++i) l += s_sum[i * kMmaRows + ti];
-            const float inv = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+            const bool more = TYPE != AF_KV_F16 && *any_apart != 0;
+            const float inv = splits > 1 || more ? 1.f : l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
             for (int i = 0; i < HD; i += 4)
                 *reinterpret_cast<float4*>(staged_at(ti, 4 * i)) =
                     make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
+            if constexpr (TYPE != AF_KV_F16) {
+                if (more && live) s_top[ti] = add_apart<TYPE, HD>(mp, spot, apart, end, row, head, reinterpret_cast<float4*>(staged + ti * SH::QROW), ti & 7, s_top[ti], &l);
+            }
             __syncwarp();
             auto from = [&](int i) { return *reinterpret_cast<const float4*>(staged_at(w * 32 + i + sub, 16 * col)); };
             if (splits > 1) {  // the split's place in the workspace, rows of HD values side by side
@@ -942,6 +1021,25 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         };
         bool ok = true;
         int st = 0, ph = 0, fu = 0, sc_at = 0;  // ring of NB tiles and its phase, of `full`, of the scales
+        auto note_apart = [&](int t) {  // the group is left out of the products
+            const int i = (t - max(len / T - t0, 0)) * SH::GROUPS + w;  // of those of the tiles with nodes
+            if (lane == 0) {
+                atomicOr(&apart[i >> 5], 1u << (i & 31));
+                *any_apart = 1;
+            }
+        };
+        auto put_scale = [&](int a, float f, bool out) {  // the group's power of two
+            if (lane != 0) return;
+            float* sc = scales + sc_at * 4 * SH::GROUPS + w;
+            if (isv) {
+                sc[SH::GROUPS] = out ? -INFINITY : (float)-a;
+                sc[2 * SH::GROUPS] = f;
+                mbar_arrive(&v_scale[sc_at]);  // the softmax need not wait for the tile itself
+            } else {
+                sc[0] = out ? 0.f : pow2(-a);
+                sc[3 * SH::GROUPS] = out ? -INFINITY : 0.f;
+            }
+        };
         auto next = [&]() {
             if (++st == NB) st = 0, ph ^= 1;
             if (++fu == ring) fu = 0;
@@ -988,17 +1086,19 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                     for (int i = 0; i < NX; ++i) x[i] = y[i];
                     note_bad(t);
                 }
+                bool differ = false;
+                if ((t0 + t) * T + (w + 1) * SH::RPW > len) {  // the group has nodes
+                    uint32_t low = 0xffffffffu;
+#pragma unroll
+                    for (int i = 0; i < NX; ++i)
+                        low = min(low, __float_as_uint(max3_abs_nan(max3_abs_nan(0.f, x[i].x, x[i].y), x[i].z, x[i].w)) - 1u);
+                    differ = rows_differ(mx, low);
+                    if (differ) note_apart(t);
+                }
                 const int a = scale_of(mx, isv ? 60 : 100);
                 const float f = pow2(a);
                 const f32x2 f2 = pair(f, f);
-                if (lane == 0) {
-                    float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + w;
-                    sc[0] = isv ? (float)-a : pow2(-a);
-                    if (isv) {
-                        sc[SH::GROUPS] = f;
-                        mbar_arrive(&v_scale[sc_at]);  // the softmax need not wait for the tile itself
-                    }
-                }
+                put_scale(a, f, differ);
                 if (due) hand_over(due);                        // the tile before: its stores are through by now
                 if (t == SH::QTILE) ok = wait_warp(q_full, 0);  // the staged queries' place is written over
                 if (ok && t >= NB) ok = wait_warp(&empty[st], ph ^ 1);
@@ -1021,13 +1121,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
         } else if (TYPE == AF_KV_BF16 || isv) {
             // in place; an access takes 512 bytes: 4 rows of 64 values
             constexpr int ALL = SH::RPW * HD * 2 / 512, NC = 4, PER = SH::RPW / 4;  // accesses; at a time; of the rows' 64 values
-            auto fix = [&](int t) {
+            auto fix = [&](int t, auto with_nodes) {
+                constexpr bool NODES = decltype(with_nodes)::value;
                 uint8_t* at = tiles + (st * 2 + (isv ? 1 : 0)) * SH::HALF + w * SH::RPW * 128 + lane * 16;
                 auto place = [&](int i) { return reinterpret_cast<uint4*>(at + (i / PER) * SH::COLS + (i % PER) * 512); };
                 uint4 x[NC];
                 uint32_t* e = &x[0].x;
                 const int left = end - (t0 + t) * T - w * SH::RPW - lane / 8;  // rows in front of the end
-                const bool last = left + lane / 8 < SH::RPW;                   // the same in the whole warp
+                const bool last = NODES && left + lane / 8 < SH::RPW;          // the same in the whole warp
                 auto load = [&](int i0) {
 #pragma unroll
                     for (int i = 0; i < NC; ++i) x[i] = *place(i0 + i);
@@ -1066,7 +1167,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                     }
                     return;
                 }
-                auto largest = [&](bool finite) {
+                const bool nodes = NODES && (t0 + t) * T + (w + 1) * SH::RPW > len;
+                uint32_t low = 0xffffffffu;  // see rows_differ
+                auto largest = [&](bool finite, auto with_low) {
                     uint32_t b = 0;  // two at once: bf16's magnitudes are ordered as 16-bit numbers
 #pragma unroll 1
                     for (int i0 = 0; i0 < ALL; i0 += NC) {
@@ -1074,26 +1177,31 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                         if (finite) without();
 #pragma unroll
                         for (int i = 0; i < 4 * NC; ++i) b = __vmaxu2(b, e[i] & 0x7fff7fffu);
+                        if (decltype(with_low)::value) {
+#pragma unroll
+                            for (int i = 0; i < NC; ++i) {
+                                uint32_t z = e[4 * i] & 0x7fff7fffu;
+#pragma unroll
+                                for (int j = 1; j < 4; ++j) z = __vmaxu2(z, e[4 * i + j] & 0x7fff7fffu);
+                                low = min(low, max(z << 16, z & 0xffff0000u) - 1u);
+                            }
+                        }
                     }
                     return __reduce_max_sync(0xffffffffu, max(b << 16, b & 0xffff0000u));
                 };
-                uint32_t mx = largest(false);
+                uint32_t mx = nodes ? largest(false, std::true_type()) : largest(false, std::false_type());
                 const bool odd = isv && mx >= 0x7f800000u;
                 if (odd) {
-                    mx = largest(true);
+                    low = 0xffffffffu;
+                    mx = largest(true, std::integral_constant<bool, NODES>());
                     note_bad(t);
                 }
+                const bool differ = nodes && rows_differ(mx, low);
+                if (differ) note_apart(t);
                 const int a = scale_of(mx, isv ? 60 : 100);
                 const float f = pow2(a);
                 const f32x2 f2 = pair(f, f);
-                if (lane == 0) {
-                    float* sc = scales + (sc_at * 3 + (isv ? 1 : 0)) * SH::GROUPS + w;
-                    sc[0] = isv ? (float)-a : pow2(-a);
-                    if (isv) {
-                        sc[SH::GROUPS] = f;
-                        mbar_arrive(&v_scale[sc_at]);
-                    }
-                }
+                put_scale(a, f, differ);
 #pragma unroll 1
                 for (int i0 = 0; i0 < ALL; i0 += NC) {
                     load(i0);
@@ -1108,14 +1216,18 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                     for (int i = 0; i < NC; ++i) *place(i0 + i) = x[i];
                 }
             };
-#pragma unroll 1
-            for (int t = 0; t < nt; ++t) {
+            auto take = [&](int t, auto with_nodes) {
                 ok = wait_warp(&land[st], ph);
-                if (!ok) break;
-                fix(t);
+                if (!ok) return;
+                fix(t, with_nodes);
                 hand_over(&full[fu]);
                 next();
-            }
+            };
+            int t = 0;
+#pragma unroll 1
+            for (; TYPE != AF_KV_F16 && ok && t < nt && (t0 + t + 1) * T <= len; ++t) take(t, std::false_type());
+#pragma unroll 1
+            for (; ok && t < nt; ++t) take(t, std::true_type());
         }
         if (!ok) *flag = 1;
     } else {
@@ -1687,6 +1799,7 @@ std::string tree_wrong(const af_attention_tree_args& a) {
         return "n_rows times n_heads must be below 2^31";
     if (a.mask && (a.mask_words <= 0 || (long long)a.mask_words * 64 < a.batch.max_nodes))
         return "mask_words must cover max_nodes";
+    if (mma && std::min(a.batch.max_nodes, a.n_rows) > kMmaMaxNodes) return "a sequence has at most 1,048,448 nodes";
     const long long qd = (long long)a.n_heads * a.kv.head_dim;
     if ((a.q_stride && a.q_stride < qd) || (a.out_stride && a.out_stride < qd)) return "a row stride is shorter than a row";
     return "";

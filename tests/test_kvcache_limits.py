@@ -50,3 +50,14 @@ def test_a_beam_workspace_serves_every_smaller_call():
                     rows, k = s * b, 64
                     segments = min(-(-v // 8192), max(1, 444 // rows))
                     assert rows * segments * (8 * k + 16) <= size(s, b, v, k) <= most
+
+
+def test_more_nodes_than_are_kept_apart_are_refused():
+    lib = _lib.load()
+    for hd, refused in ((64, True), (128, True), (96, False)):
+        a = attention(kv=cache(head_dim=hd, n_kv_heads=4), batch=batch(max_nodes=1 << 21), n_heads=4, n_rows=1048449, q=None)
+        assert lib.af_attention_tree_f32(C.byref(a), None) != 0
+        assert (b"1,048,448 nodes" in lib.af_last_error()) == refused
+        a.n_rows = 1048448
+        assert lib.af_attention_tree_f32(C.byref(a), None) != 0
+        assert b"null q" in lib.af_last_error()
