@@ -309,7 +309,8 @@ cudaError_t af_kv_store_f32(const af_kv_store_args* args, cudaStream_t stream);
  * = 1/sqrt(head_dim); a row that sees nothing gives zeros; what no row may see
  * may hold anything, infinities and NaN too; an infinite or NaN value of V
  * reaches the rows that see it, a key that is not finite leaves the rows that
- * see it undefined, and magnitudes stay below 2^100.  q, out [n_rows][n_heads]
+ * see it undefined; magnitudes of q and K that a row sees stay below 2^100, of V
+ * below 2^56.  q, out [n_rows][n_heads]
  * [head_dim] f32 (strides as above), fp32 accuracy for every cache type.
  * max_len: no sequence has more positions, cached and new (it sizes the
  * launch; 0 = max_blocks*page_size).  ws: af_attention_tree_f32_workspace

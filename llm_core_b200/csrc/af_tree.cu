@@ -139,6 +139,9 @@ __global__ void __launch_bounds__(kTreeThreads) tree_row_kernel(TreeParams p) {
 // no scale and no lo, one in bf16 a scale and no lo (8 bits in 11).  The
 // powers of two are undone exactly: K's in the score, V's in the exponent of
 // the weight, 2^(s_j - a_j), whose sum Σ 2^(s_j - a_j)·2^a_j is the softmax's.
+// The running maximum is of s_j - a_j, a_j at most 60 (V of zeros), so that it rises by up to 46 + e + (s - s') when V
+// of magnitude 2^e follows zeros: below 126, where the factor 2^-126 of the sum so far would be 0, for e up to 55 and
+// scores 2^24 apart in weight.
 // Weights carry a factor 2^14, so that those as small as 2^-38 of the largest
 // keep f16's spacing.
 //
