@@ -263,7 +263,8 @@ typedef struct {
  * more than max_nodes nodes.  Lengths, tables and counts are read on the
  * device, so a captured graph follows them.  A page id or length outside its
  * range sets the device error word (af_device_error) and is neither read nor
- * written. */
+ * written; to attention a position without a page is a key and a value of
+ * zeros. */
 typedef struct {
     const int32_t* block_table;
     const int32_t* len;

@@ -82,17 +82,14 @@ __global__ void __launch_bounds__(kTreeThreads) tree_row_kernel(TreeParams p) {
     float m = -INFINITY, l = 0.f;
     for (int pos = warp; pos < len + s_n; pos += W) {
         if (pos >= len && !tree_sees(p, row, node, pos - len)) continue;
-        const long long at = kv_row(p.kv, p.b, seq, pos);
-        if (at < 0) {
-            set_err_at(p.b.err, kErrBadArgs);
-            continue;
-        }
+        const long long at = kv_row(p.kv, p.b, seq, pos);  // below 0: no page, a key and value of zeros
+        if (at < 0) set_err_at(p.b.err, kErrBadArgs);
         const auto* kr = reinterpret_cast<const typename E::T*>(p.kv.k + head + at);
         const auto* vr = reinterpret_cast<const typename E::T*>(p.kv.v + head + at);
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (lane + 32 * i < hd) s = fmaf(qv[i], E::load(kr[lane + 32 * i]), s);
+            if (at >= 0 && lane + 32 * i < hd) s = fmaf(qv[i], E::load(kr[lane + 32 * i]), s);
         s = warp_sum(s);
         const float mn = fmaxf(m, s), c = mn == -INFINITY ? 1.f : exp2f(m - mn);
         const float w = s == -INFINITY ? 0.f : exp2f(s - mn);
@@ -100,7 +97,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_row_kernel(TreeParams p) {
         l = l * c + w;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (lane + 32 * i < hd) o[i] = fmaf(w, E::load(vr[lane + 32 * i]), o[i] * c);
+            if (lane + 32 * i < hd) o[i] = fmaf(w, at >= 0 ? E::load(vr[lane + 32 * i]) : 0.f, o[i] * c);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) s_o[warp][lane + 32 * i] = o[i];
@@ -547,21 +544,20 @@ __device__ __noinline__ float add_apart(const MmaParams& mp, const TreeSpot& spo
         const int p0 = first * SH::T + g * SH::RPW;
         for (int pos = p0; pos < min(p0 + SH::RPW, end); ++pos) {
             if (!(tree_window(p, row, node, n, len, pos) & 1)) continue;
-            const long long at = kv_row(p.kv, p.b, spot.seq, pos);
-            if (at < 0) continue;
+            const long long at = kv_row(p.kv, p.b, spot.seq, pos);  // below 0: no page, a key and value of zeros
             const long long from = p.layer * p.kv.layer_bytes + at + (long long)spot.kvh * HD * SH::SIZE;
             const auto* kr = reinterpret_cast<const typename E::T*>(p.kv.k + from);
             const auto* vr = reinterpret_cast<const typename E::T*>(p.kv.v + from);
             float s = 0.f;
 #pragma unroll 8
-            for (int d = 0; d < HD; ++d) s = fmaf(q[d], E::load(kr[d]), s);
+            for (int d = 0; at >= 0 && d < HD; ++d) s = fmaf(q[d], E::load(kr[d]), s);
             s *= p.scale;
             // (the sums may hold infinities already, which no factor may turn into NaN)
             const float mn = fmaxf(m, s), c = fmaxf(ex2(m - mn), __int_as_float(1)), w = ex2(s - mn + 14.f);
             m = mn;
             sum = fmaf(sum, c, w);
             auto v = [&](int d) {
-                const float x = E::load(vr[d]);
+                const float x = at >= 0 ? E::load(vr[d]) : 0.f;
                 return fabsf(x) < INFINITY ? x : 0.f;
             };
 #pragma unroll 2
@@ -1249,11 +1245,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 const int blk = pos >> p.kv.ps_shift;
                 return table ? __ldg(table + blk) : page0 + blk;
             };
-            // pool row of this lane's box of tile t; a page that is none: the error word, and row 0
+            // pool row of this lane's box of tile t; a page that is none: the error word, and rows in front of the pool,
+            // which the copy fills with zeros
             auto row_of = [&](int t, int box, int page) -> int {
                 if ((unsigned)page >= (unsigned)p.kv.n_pages) {
                     set_err_at(p.b.err, kErrBadArgs);
-                    page = 0;
+                    return -R;
                 }
                 return (page << p.kv.ps_shift) + (((t0 + t) * T + box * R) & in_page);
             };
