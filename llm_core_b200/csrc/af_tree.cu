@@ -43,6 +43,10 @@ __device__ __forceinline__ bool tree_sees(const TreeParams& p, int row, int node
 
 constexpr int kTreeThreads = 128;
 
+// The least factor of something that a row sees: an infinite value of V counts however small its weight is, and is not
+// turned into NaN by a factor of 0.
+__device__ __forceinline__ float least() { return __int_as_float(1); }
+
 // One block per row and head: its warps take the positions in turn, a lane
 // the dimensions lane, lane + 32, ...; each warp keeps a running maximum, sum
 // and output, merged at the end.  Every row reads K and V again and a warp has
@@ -91,8 +95,8 @@ __global__ void __launch_bounds__(kTreeThreads) tree_row_kernel(TreeParams p) {
         for (int i = 0; i < 8; ++i)
             if (at >= 0 && lane + 32 * i < hd) s = fmaf(qv[i], E::load(kr[lane + 32 * i]), s);
         s = warp_sum(s);
-        const float mn = fmaxf(m, s), c = mn == -INFINITY ? 1.f : exp2f(m - mn);
-        const float w = s == -INFINITY ? 0.f : exp2f(s - mn);
+        const float mn = fmaxf(m, s), c = mn == -INFINITY ? 1.f : fmaxf(exp2f(m - mn), least());
+        const float w = s == -INFINITY ? 0.f : fmaxf(exp2f(s - mn), least());
         m = mn;
         l = l * c + w;
 #pragma unroll
@@ -110,7 +114,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_row_kernel(TreeParams p) {
     for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w]);
     float c[W];
     for (int w = 0; w < W; ++w) {
-        c[w] = s_m[w] == -INFINITY && s_l[w] == 0.f ? 0.f : exp2f(s_m[w] - top);
+        c[w] = s_m[w] == -INFINITY && s_l[w] == 0.f ? 0.f : fmaxf(exp2f(s_m[w] - top), least());
         sum += c[w] * s_l[w];
     }
     for (int d = tid; d < hd; d += kTreeThreads) {
@@ -552,8 +556,7 @@ __device__ __noinline__ float add_apart(const MmaParams& mp, const TreeSpot& spo
 #pragma unroll 8
             for (int d = 0; at >= 0 && d < HD; ++d) s = fmaf(q[d], E::load(kr[d]), s);
             s *= p.scale;
-            // (the sums may hold infinities already, which no factor may turn into NaN)
-            const float mn = fmaxf(m, s), c = fmaxf(ex2(m - mn), __int_as_float(1)), w = ex2(s - mn + 14.f);
+            const float mn = fmaxf(m, s), c = fmaxf(ex2(m - mn), least()), w = ex2(s - mn + 14.f);
             m = mn;
             sum = fmaf(sum, c, w);
             auto v = [&](int d) {
@@ -1404,7 +1407,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
     for (int s = 0; s < plan.y; ++s) {
         const float2 x = *reinterpret_cast<const float2*>(ml + s * (2 * kMmaRows));
         if (x.y == 0.f && x.x == -INFINITY) continue;  // a split that the row sees nothing of
-        const float c = ex2(x.x - top);
+        const float c = fmaxf(ex2(x.x - top), least());
         sum = fmaf(c, x.y, sum);
         float v[PER];
         if (PER == 4) {
@@ -1574,9 +1577,8 @@ __global__ void __launch_bounds__(kSmallThreads, 2) tree_small_kernel(TreeParams
                 const bool sees = node[i] >= 0 && t0 + lane < end && (j < 0 || tree_sees(p, row[i], node[i], j));
                 const float x = sees ? s[i][0] + s[i][1] : -INFINITY;
                 const float mn = fmaxf(m[i], warp_max(x)), ms = mn == -INFINITY ? 0.f : mn;
-                // what the row sees keeps a weight: an infinite value of V counts however small that is; NaN stays
-                w[i] = !sees ? 0.f : isnan(x) ? x : fmaxf(ex2(x - ms), __int_as_float(1));
-                const float corr = ex2(m[i] - ms);
+                w[i] = !sees ? 0.f : isnan(x) ? x : fmaxf(ex2(x - ms), least());  // NaN stays
+                const float corr = fmaxf(ex2(m[i] - ms), least());
                 l[i] = fmaf(l[i], corr, warp_sum(w[i]));
                 m[i] = mn;
                 if (lane == 0) s_c[r2 + i] = corr;
@@ -1625,7 +1627,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2) tree_small_kernel(TreeParams
             for (int b = 0; b < blocks; ++b) {
                 const float lb = cluster_ld(s_l + r, b), mb = cluster_ld(s_m + r, b);
                 if (mb == -INFINITY && lb == 0.f) continue;  // a block that the row sees nothing of
-                const float f = ex2(mb - top);
+                const float f = fmaxf(ex2(mb - top), least());
                 sum = fmaf(f, lb, sum);
                 o = fmaf(f, cluster_ld(so + i, b), o);
             }
