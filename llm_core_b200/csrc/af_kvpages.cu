@@ -675,10 +675,16 @@ extern "C" cudaError_t af_kv_store_f32(const af_kv_store_args* a, cudaStream_t s
                       vec(p.sin_t) && vec(p.q_norm) && vec(p.k_norm) && !((p.qs | p.ks | p.vs | p.os) & 3);
     auto go = [&](auto type) {
         constexpr int TYPE = decltype(type)::value;
-        // A warp a row where rows are so many that a row's chain hides behind others'.  Bf16, 16/2 heads of 128, block
-        // a row / warp a row: 667 rows 5.0 / 9.7 us, 1,667 10.5 / 11.6, 3,333 20.8 / 17.2; 32/32 heads 13.6 / 40.7, 33.8 /
-        // 47.1, 57.3 / 57.6.
-        const bool many = p.n_rows > 15 * 148;
+        // A warp a row where rows are so many that a row's chain hides behind others', and short enough: a warp has 5
+        // heads of 128 or 10 of 64 in flight and takes a row's heads in turn.  Block a row / warp a row, us:
+        //   heads         rows  bf16         f32
+        //   16/2 of 128   1,400  8.3 / 10.5   8.7 / 14.6     2,400 13.0 / 12.4  13.9 / 17.6     8,000 39.6 / 33.4  41.9 / 44.6
+        //   16/8 of 128   1,400 11.2 / 16.1  12.7 / 25.6     2,400 18.5 / 18.8  20.9 / 30.3     8,000 53.9 / 47.0  59.1 / 68.8
+        //   32/8 of 128   1,400 14.8 / 23.6  17.9 / 39.3     2,400 25.4 / 29.8  30.8 / 45.0     8,000 71.0 / 69.0  87.0 / 99.2
+        //   32/32 of 128  1,400 25.9 / 45.5  34.3 / 76.9     2,400 43.1 / 52.0  57.8 / 84.4     8,000  124 / 123    168 / 190
+        //   32/4 of 64    1,400  8.4 / 10.3   8.4 / 10.5     2,400 13.1 / 12.5  13.4 / 12.7     8,000 40.0 / 33.7  40.4 / 34.4
+        const int values = (p.H + 2 * p.kv.kv_heads) * hd;
+        const bool many = p.n_rows > 15 * 148 && values <= 4096 && (TYPE != AF_KV_F32 || hd == 64);
         const int packed = (p.n_rows + kStoreThreads / 32 - 1) / (kStoreThreads / 32);
         if (wide && hd == 64 && many) kv_store_vec_kernel<TYPE, 64, true><<<packed, kStoreThreads, 0, stream>>>(p);
         else if (wide && many) kv_store_vec_kernel<TYPE, 128, true><<<packed, kStoreThreads, 0, stream>>>(p);
