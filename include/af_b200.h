@@ -345,7 +345,7 @@ cudaError_t af_attention_tree_f32(const af_attention_tree_args* args, cudaStream
  * scores[row] + logit - log Σ exp logits, best first, ties to the lowest beam
  * and then the lowest token.  out_score / out_beam / out_token [n_seq][n_out];
  * out_beam is the logits row, so that it serves as af_kv_fork's parent.  A
- * beam whose score is -inf or NaN, or whose logits hold NaN or +inf or nothing
+ * beam whose score is not finite, or whose logits hold NaN or +inf or nothing
  * above -inf, scores -inf throughout.  n_out <= 64 and <= n_beams*vocab,
  * n_beams <= 64, n_seq*n_beams <= 65535, n_beams * ceil(vocab / 8192) <= 1024.
  * ws: af_beam_select_f32_workspace bytes, enough for every call with no more
@@ -504,7 +504,8 @@ cudaError_t af_engine_step_tree(af_engine* e, const int32_t* h_tokens, const int
  * layer, and decoding goes on at pos0 + n_path. */
 cudaError_t af_engine_accept_path(af_engine* e, const int32_t* h_path, int n_path, int32_t pos0);
 /* Beam search with n_beams <= 32 beams: BOS prepended unless present, then per
- * step the 2*n_beams best continuations (af_beam_select_f32); one that ends in
+ * step the 2*n_beams best continuations (af_beam_select_f32; no more than the
+ * vocabulary has tokens); one that ends in
  * EOS among the first n_beams is a finished hypothesis, the others go on until
  * n_beams do.  Hypotheses are rated by their log-probability over
  * length^length_penalty (length counts EOS); the search ends at max_new tokens,

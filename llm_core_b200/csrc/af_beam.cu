@@ -24,7 +24,7 @@
 //    compare as their definition does, and the K best of the segment lists: the
 //    K-th best list head is again a threshold, which at most K lists of K pass.
 //    Latency alone: 4 beams of 32,000 logits take 10 us, both kernels.
-//  * A beam that is dead before the call (score -inf or NaN) is not read.
+//  * A beam that is dead before the call (score not finite) is not read.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -70,7 +70,7 @@ __device__ __forceinline__ double warp_sum_d(double v) {
     return v;
 }
 
-__device__ __forceinline__ bool dead_score(float s) { return !(s > -INFINITY); }  // -inf and NaN
+__device__ __forceinline__ bool dead_score(float s) { return !(fabsf(s) < INFINITY); }  // infinities and NaN
 
 // This lane's value of the warp's 32 in descending order.
 template <typename T>
@@ -305,11 +305,7 @@ __device__ __forceinline__ double ordered_double(u64 k) {
     return __longlong_as_double((long long)((k >> 63) ? (k & ~(1ull << 63)) : ~k));
 }
 
-// A candidate: ordered score, then the lower (beam, token) first.
-struct Cand {
-    u64 score;
-    unsigned flat;
-};
+// Candidates: the higher score, then the lower (beam, token) first.
 __device__ __forceinline__ bool better(u64 s, unsigned f, u64 s2, unsigned f2) { return s > s2 || (s == s2 && f < f2); }
 
 constexpr int kMergeKeys = 4096;  // keys of a sequence that are brought to shared memory, when they are no more
