@@ -375,11 +375,12 @@ __device__ __noinline__ uint32_t clean(float4 (&x)[N]) {
 
 // Nodes are not seen by every row, so what one holds must not cost its neighbours their bits.  Whether the rows of a
 // group with nodes may differ too much to share a power of two: `mx` is the group's largest value, `low` the smallest
-// largest value of any 16 bytes that hold something (bits, less 1: zeros are all ones).  2^-39 of mx is lost, 2^-27 of
-// values 2^12 below.  Such a group is left out of the products (its -a of V, or what stands beside K's power of two, is
-// -inf, so that no row gives it a weight) and added position by position in the end.  Looking costs 4 to 10 % where all
-// tiles have nodes (500 tokens, bf16: 32/4 heads of 64 19.8 -> 20.8 us, 16/2 of 128 25.9 -> 28.0) and 1 % of a tree over
-// 3,989 positions.  Not taken: a power of two per row, which the softmax then has to take apart (chunk 209 -> 222 us).
+// largest value of any 16 bytes (bf16: of every other value there) that hold something (bits, less 1: zeros are all
+// ones).  2^-39 of mx is lost, 2^-27 of values 2^12 below.  Such a group is left out of the products (its -a of V, or what stands beside K's power of two, is
+// -inf, so that no row gives it a weight) and added position by position in the end.  Looking costs 3 to 10 % where all
+// tiles have nodes (500 tokens, bf16: 32/4 heads of 64 19.9 -> 20.6 us, 16/2 of 128 25.7 -> 27.4; 4 trees of 196, 32/32
+// heads of 128 34.7 -> 37.9) and 1 % of a tree over 3,989 positions.  Not taken: a power of two per row, which the softmax
+// then has to take apart (chunk 209 -> 222 us).
 __device__ __forceinline__ bool rows_differ(uint32_t mx, uint32_t low) {
     low = __reduce_min_sync(0xffffffffu, low);
     return mx >= 0x7f800000u || (low != 0xffffffffu && (mx >> 23) > ((low + 1u) >> 23) + 12);
@@ -1172,26 +1173,27 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                 const bool nodes = NODES && (t0 + t) * T + (w + 1) * SH::RPW > len;
                 uint32_t low = 0xffffffffu;  // see rows_differ
                 auto largest = [&](bool finite, auto with_low) {
-                    uint32_t b = 0;  // two at once: bf16's magnitudes are ordered as 16-bit numbers
+                    uint32_t b = 0, least = 0xffffffffu;  // two at once: bf16's magnitudes are ordered as 16-bit numbers
 #pragma unroll 1
                     for (int i0 = 0; i0 < ALL; i0 += NC) {
                         load(i0);
                         if (finite) without();
 #pragma unroll
-                        for (int i = 0; i < 4 * NC; ++i) b = __vmaxu2(b, e[i] & 0x7fff7fffu);
-                        if (decltype(with_low)::value) {
+                        for (int i = 0; i < NC; ++i) {
+                            uint32_t z = e[4 * i] & 0x7fff7fffu;
 #pragma unroll
-                            for (int i = 0; i < NC; ++i) {
-                                uint32_t z = e[4 * i] & 0x7fff7fffu;
-#pragma unroll
-                                for (int j = 1; j < 4; ++j) z = __vmaxu2(z, e[4 * i + j] & 0x7fff7fffu);
-                                low = min(low, max(z << 16, z & 0xffff0000u) - 1u);
-                            }
+                            for (int j = 1; j < 4; ++j) z = __vmaxu2(z, e[4 * i + j] & 0x7fff7fffu);
+                            b = __vmaxu2(b, z);
+                            if (decltype(with_low)::value) least = __vminu2(least, ((z | 0x80008000u) - 0x00010001u) ^ 0x80008000u);  // less 1, 0 the largest
                         }
+                    }
+                    if (decltype(with_low)::value) {
+                        least = min(least & 0xffffu, least >> 16);
+                        low = least == 0xffffu ? 0xffffffffu : (least << 16) + 0xffffu;
                     }
                     return __reduce_max_sync(0xffffffffu, max(b << 16, b & 0xffff0000u));
                 };
-                uint32_t mx = nodes ? largest(false, std::true_type()) : largest(false, std::false_type());
+                uint32_t mx = largest(false, std::integral_constant<bool, NODES>());
                 const bool odd = isv && mx >= 0x7f800000u;
                 if (odd) {
                     low = 0xffffffffu;
