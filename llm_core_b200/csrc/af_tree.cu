@@ -163,14 +163,14 @@ __global__ void __launch_bounds__(kTreeThreads) tree_row_kernel(TreeParams p) {
 // launch's 1,024·64.
 //
 // Measured with inputs out of L2, device time: 26 nodes over 4,000 positions, 32
-// heads of 128, f32, 45.2 us (2.9 TB/s of the 132 MB; bound by the splitting
+// heads of 128, f32, 45.7 us (2.9 TB/s of the 132 MB; bound by the splitting
 // warps: each reads, splits and stores its rows in turn, ~2,900 cycles a tile, of
 // which the stores' part 1,850; and ~15,000 cycles before the first tile's
 // products); 16 sequences of 0 to 8,190 positions with 31 nodes, 16/2 heads of 128,
-// f16, 47.4 us (1.6 TB/s; ~2,900 cycles a tile of 128, the softmax's chain, of
+// f16, 48.1 us (1.6 TB/s; ~2,900 cycles a tile of 128, the softmax's chain, of
 // which the exponentials fill 1,024 on the special function units, and ~16,000
 // cycles of plan, queries, and sums at both ends); chunks of 509 over up to 16,001
-// positions, 32/4 heads of 64, bf16, 209 us (326 TFLOP/s; the same chain, ~3,100
+// positions, 32/4 heads of 64, bf16, 212.7 us (321 TFLOP/s; the same chain, ~3,100
 // cycles a tile).  Steps that got there: K and V by single bulk copies -> boxes;
 // 4 -> 8 -> 16 softmax warps (chunk 402 -> 333 -> 266 us); tiles of 64 -> 128
 // positions with a power of two per 32 bf16 rows (241 -> 218 us); V's powers of
@@ -373,17 +373,43 @@ __device__ __noinline__ uint32_t clean(float4 (&x)[N]) {
     return __reduce_max_sync(0xffffffffu, b);
 }
 
-// Nodes are not seen by every row, so what one holds must not cost its neighbours their bits.  Whether the rows of a
-// group with nodes may differ too much to share a power of two: `mx` is the group's largest value, `low` the smallest
-// largest value of any 16 bytes (bf16: of every other value there) that hold something (bits, less 1: zeros are all
-// ones).  2^-39 of mx is lost, 2^-27 of values 2^12 below.  Such a group is left out of the products (its -a of V, or what stands beside K's power of two, is
-// -inf, so that no row gives it a weight) and added position by position in the end.  Looking costs 3 to 10 % where all
-// tiles have nodes (500 tokens, bf16: 32/4 heads of 64 19.9 -> 20.6 us, 16/2 of 128 25.7 -> 27.4; 4 trees of 196, 32/32
-// heads of 128 34.7 -> 37.9) and 1 % of a tree over 3,989 positions.  Not taken: a power of two per row, which the softmax
-// then has to take apart (chunk 209 -> 222 us).
-__device__ __forceinline__ bool rows_differ(uint32_t mx, uint32_t low) {
+// Nodes are not seen by every row, so what one holds must not cost its neighbours their bits: 2^-39 of a group's largest
+// value is lost.  A group with nodes that has a row whose largest is far below, or a key that is not finite, is left out
+// of the products (its -a of V, or what stands beside K's power of two, is -inf, so that no row gives it a weight) and
+// added position by position in the end, 4 to 9 us each.  Looked at is the smallest largest value of any 16 bytes (bf16:
+// of every other value there) that hold something; 2^14 below is far for f32, which leaves 2^-25 of such values; bf16
+// groups, of four times the rows, that have one 2^12 below are looked at row by row, so that channels that are large in
+// every row are none of it.  (f32 by rows too: 26 nodes over 3,989 positions 45.5 -> 46.8 us.)  Looking costs 3 to 10 %
+// where all tiles have nodes (500 tokens: bf16 32/4 heads of 64 19.9 -> 20.6 us, 16/2 of 128 25.7 -> 27.4, f32 28.4 ->
+// 29.9; 4 trees of 196, 32/32 heads of 128, bf16 34.7 -> 37.9) and 0 to 2 % over long caches.  Not taken: a power of two
+// per row, which the softmax then has to take apart (chunk 209 -> 222 us).
+// `mx`: the group's largest value, `low`: the smallest as above (bits, less 1: zeros are all ones).
+template <int TYPE>
+__device__ __forceinline__ bool far_apart(uint32_t mx, uint32_t low) {
     low = __reduce_min_sync(0xffffffffu, low);
-    return mx >= 0x7f800000u || (low != 0xffffffffu && (mx >> 23) > ((low + 1u) >> 23) + 12);
+    return mx >= 0x7f800000u || (low != 0xffffffffu && (mx >> 23) > ((low + 1u) >> 23) + (TYPE == AF_KV_F32 ? 14 : 12));
+}
+
+// The lane's part of `low` by whole rows, of a group of bf16 rows in shared memory: 4 rows of 64 values an access, HALVES
+// accesses of a row COLS bytes apart, `left` rows in front of the end; what is not finite is none.
+template <int RUNS, int HALVES, int COLS>
+__device__ __noinline__ uint32_t lowest_row(const uint8_t* at, int left) {
+    uint32_t low = 0xffffffffu;
+    for (int i = 0; i < RUNS; ++i) {
+        uint32_t r = 0;
+        for (int h = 0; h < HALVES; ++h) {
+            const uint4 x = *reinterpret_cast<const uint4*>(at + h * COLS + i * 512);
+            const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t a = e[j] << 16 & 0x7fff0000u, b = e[j] & 0x7fff0000u;
+                r = max(r, max(a < 0x7f800000u ? a : 0u, b < 0x7f800000u ? b : 0u));
+            }
+        }
+        if (i * 4 >= left) r = 0;
+        for (int o = 1; o < 8; o <<= 1) r = max(r, __shfl_xor_sync(0xffffffffu, r, o));
+        low = min(low, r - 1u);
+    }
+    return low;
 }
 
 // Work: an item is 128 rows of a sequence with one kv head, its tiles split
@@ -530,7 +556,7 @@ __device__ __forceinline__ unsigned long long tree_window(const TreeParams& p, i
     return (w & ones(len + n - p0)) | ones(len - p0);
 }
 
-// Groups whose nodes differ too much (rows_differ), position by position on the f32 units, as the softmax would have had
+// Groups whose nodes differ too much (far_apart), position by position on the f32 units, as the softmax would have had
 // them: `mine` holds the row's sums (columns as staged_at has them, by turn), m and *l their maximum and sum of weights.
 // Ends with what the row's place is to hold.
 template <int TYPE, int HD>
@@ -554,8 +580,10 @@ __device__ __noinline__ float add_apart(const MmaParams& mp, const TreeSpot& spo
             const auto* kr = reinterpret_cast<const typename E::T*>(p.kv.k + from);
             const auto* vr = reinterpret_cast<const typename E::T*>(p.kv.v + from);
             float s = 0.f;
-#pragma unroll 8
-            for (int d = 0; at >= 0 && d < HD; ++d) s = fmaf(q[d], E::load(kr[d]), s);
+            if (at >= 0) {
+#pragma unroll 32
+                for (int d = 0; d < HD; ++d) s = fmaf(q[d], E::load(kr[d]), s);
+            }
             s *= p.scale;
             const float mn = fmaxf(m, s), c = fmaxf(ex2(m - mn), least()), w = ex2(s - mn + 14.f);
             m = mn;
@@ -564,7 +592,7 @@ __device__ __noinline__ float add_apart(const MmaParams& mp, const TreeSpot& spo
                 const float x = at >= 0 ? E::load(vr[d]) : 0.f;
                 return fabsf(x) < INFINITY ? x : 0.f;
             };
-#pragma unroll 2
+#pragma unroll 4
             for (int d = 0; d < HD; d += 4) {
                 float4 f = mine[(d >> 2) ^ turn];
                 f.x = fmaf(w, v(d), f.x * c), f.y = fmaf(w, v(d + 1), f.y * c);
@@ -1095,7 +1123,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
 #pragma unroll
                     for (int i = 0; i < NX; ++i)
                         low = min(low, __float_as_uint(max3_abs_nan(max3_abs_nan(0.f, x[i].x, x[i].y), x[i].z, x[i].w)) - 1u);
-                    differ = rows_differ(mx, low);
+                    differ = far_apart<TYPE>(mx, low);
                     if (differ) note_apart(t);
                 }
                 const int a = scale_of(mx, isv ? 60 : 100);
@@ -1171,7 +1199,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                     return;
                 }
                 const bool nodes = NODES && (t0 + t) * T + (w + 1) * SH::RPW > len;
-                uint32_t low = 0xffffffffu;  // see rows_differ
+                uint32_t low = 0xffffffffu;  // see far_apart
                 auto largest = [&](bool finite, auto with_low) {
                     uint32_t b = 0, least = 0xffffffffu;  // two at once: bf16's magnitudes are ordered as 16-bit numbers
 #pragma unroll 1
@@ -1200,7 +1228,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) tree_mma_kernel(const __grid_c
                     mx = largest(true, std::integral_constant<bool, NODES>());
                     note_bad(t);
                 }
-                const bool differ = nodes && rows_differ(mx, low);
+                const bool differ = nodes && far_apart<TYPE>(mx, low) && far_apart<TYPE>(mx, lowest_row<PER, HD / 64, SH::COLS>(at, left));
                 if (differ) note_apart(t);
                 const int a = scale_of(mx, isv ? 60 : 100);
                 const float f = pow2(a);

@@ -121,3 +121,15 @@ def test_long_chains_with_outliers(gpu, kv, hd):
             page, off = at(i)
             v[:, page, off] *= 1e12
     check(gpu, kv, "tensor", hd, 1000, n, None, change, H=4, KV=2)
+
+
+@pytest.mark.parametrize("kv", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [7, 40])
+def test_channels_that_are_large_in_every_row(gpu, kv, hd, n):
+    """A few channels of K and V are 3e4 times the others, in all rows."""
+    def change(k, v, at):
+        k[..., 5] *= 3e4
+        v[..., 1] *= 3e4
+        v[..., hd - 3] *= 3e4
+    check(gpu, kv, "tensor", hd, 300, n, None, change, scale=1e-5)
