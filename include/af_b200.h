@@ -496,7 +496,8 @@ cudaError_t af_engine_prefill_batched(af_engine* e, const int32_t* h_tokens, int
  * token at a time; a chain (h_parents[i] = i-1) gives what
  * af_engine_prefill gives for each of its tokens, up to the rounding of the
  * batched linear layers (relative 2e-5 of a layer's output for n <= 32, 2e-4
- * above, which later layers may amplify).  One GPU. */
+ * above, which later layers may amplify).  These passes keep the numerics of
+ * the batched prompt pass where af_engine_set_q8_activations is on.  One GPU. */
 cudaError_t af_engine_step_tree(af_engine* e, const int32_t* h_tokens, const int32_t* h_parents, int n, int32_t pos0,
                                 float* h_logits, int32_t* h_next);
 /* Keep the nodes h_path[0..n_path) (rising) of the tree that was stepped at

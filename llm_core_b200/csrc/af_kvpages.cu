@@ -120,8 +120,8 @@ __device__ __forceinline__ bool store_place(const StoreParams& p, const StorePla
 // warp's first heads (U) are loaded before the row's place is known.  Bound by
 // memory, q, k, v once in, once out, and by a row's chain of loads (counts, then
 // table and rotation), hidden behind other rows': 8 sequences of up to 509 rows,
-// 16/2 heads of 128, bf16, 16.7 us a warp a row (4.1 TB/s), 20.5 a block of 8 warps,
-// 18.3 of 4; one row 2.7 us, a launch.  Measured and not taken: 2 to 8 rows a block with the next row's loads
+// 16/2 heads of 128, bf16, 17.5 us a warp a row (3.9 TB/s), 20.5 a block of 8 warps,
+// 18.3 of 4; one row 2.9 us, a launch.  Measured and not taken: 2 to 8 rows a block with the next row's loads
 // ahead, 27 us (64 registers, fewer blocks an SM).
 template <int TYPE, int HD, bool WARP>
 __global__ void __launch_bounds__(kStoreThreads, WARP ? 4 : 5) kv_store_vec_kernel(StoreParams p) {
@@ -498,8 +498,8 @@ constexpr int kCopyThreads = 256;
 
 // Block (i, layer, K or V): the rows of output i's partly filled page, one
 // contiguous range.  Bound by memory; 4 loads of 16 bytes a thread in flight:
-// 4 sequences of 8 beams, 32 layers of 32 heads of 128, bf16, 23.4 us with the
-// bookkeeping (110 MB, 4.7 TB/s); 4 beams over 22 layers 6.4 us, two launches.
+// 4 sequences of 8 beams, 32 layers of 32 heads of 128, bf16, 22.6 us with the
+// bookkeeping (110 MB, 4.9 TB/s); 4 beams over 22 layers 6.4 us, two launches.
 __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(KvView kv, const int4* copies) {
     pdl_wait();
     const int4 c = copies[blockIdx.x];
